@@ -206,6 +206,86 @@ int q38b_gemm_prefill_f16(q38b_ctx* ctx, uint32_t type, const void* W_dev, size_
                           long long ldx, int B, float* Y_dev, long long ldy, int accumulate, void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------
+ * The steps of a token between its products.  No counterpart among the reference interfaces above: the reference keeps
+ * them inside its attention preparation and its sampler.  Each call works on the context's device whatever device is
+ * current, enqueues on `stream`, allocates nothing and shares no work area: calls on several streams may overlap.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/* The query or the key heads of `rows` rows: element i of head h of row t at src + (t * src_row + h * src_head + i), strides in
+ * elements (>= 0; a projection that interleaves a gate with each head has src_head = 2 D), the same for dst. */
+typedef struct q38b_heads {
+    const void* src;
+    void* dst;
+    long long src_row, src_head, dst_row, dst_head;
+    const float* weight;   /* [D], or NULL: ones */
+    int n_heads;
+} q38b_heads;
+
+/* RMSNorm of each query and key head and the rotation by position, in one pass over the projections' outputs:
+ *   z = x / sqrt(mean(x^2) + eps) * weight
+ *   y_a = scale (z_a cos - z_b sin), y_b = scale (z_b cos + z_a sin) for the pairs (a, b) = (j, j + rot / 2), or (2j, 2j + 1) if
+ *   adjacent, j < rot / 2, angle = positions[t] * inv_freq[j]; elements from `rot` on are z.
+ * k may be NULL.  positions: int32 [rows], any sign; inv_freq: float64 [rot / 2], finite, radians per position (both may be NULL with
+ * rot = 0); the angle is exact to about |position| 2^-52 turns.  in_kind, out_kind: q38b_out_kind of src and dst.  D <= 1024, rot even and
+ * at most D.  dst may be src itself (same kind, same strides); otherwise the two must not overlap, nor may the query heads'
+ * elements be among the key heads'.  Sums in fp32, outputs rounded once. */
+int q38b_qk_norm_rope(q38b_ctx* ctx, const q38b_heads* q, const q38b_heads* k, int D, int rot, int adjacent, float eps, float scale,
+                      const int* positions_dev, const double* inv_freq_dev, int in_kind, int out_kind, int rows, void* stream);
+
+/* What shapes the logits of each row before the top-k; every part may be absent (NULL).  Lists of rows lie one behind the other, row r's
+ * entries at [begin[r], begin[r + 1]) (int64, n_rows + 1 of them).  Token ids outside the logits (negative ones too) are passed over. */
+typedef struct q38b_logit_rules {
+    const float* penalties;          /* [n_rows][3]: repetition (> 0, 1: none), frequency, presence; needs history */
+    const int* history;              /* token ids: prompt, then generated ones; needs penalties */
+    const long long* history_begin;
+    const int* prompt_len;           /* [n_rows] how many of a row's entries are its prompt; NULL: none */
+    const int* bias_ids;             /* token ids; the last entry of a token counts */
+    const float* bias_values;
+    const long long* bias_begin;
+    const uint32_t* masks;           /* bit v % 32 of word v / 32 set: token v is allowed; masks mask_ld words apart */
+    long long mask_ld;
+    const int* mask_of_row;          /* [n_rows] which mask, negative: none; NULL: mask r for row r */
+} q38b_logit_rules;
+
+/* y[r][i] from x[r][i] for n_rows rows (1..65535) of n logits, x_ld / y_ld floats apart, token id index_offset + i:
+ *   in history:            l = l > 0 ? l / repetition : l * repetition
+ *   generated c > 0 times: l = l - frequency * c - presence
+ *   biased:                l = l + bias
+ *   mask bit clear:        l = -infinity (whatever l was; a mask without a bit leaves a row of them)
+ * y may be x (then y_ld = x_ld); otherwise they must not overlap.  Same inputs, same bits. */
+int q38b_adjust_logits(q38b_ctx* ctx, const float* x_dev, long long x_ld, int n, int n_rows, int index_offset, const q38b_logit_rules* rules,
+                       float* y_dev, long long y_ld, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point (OCP MX: E2M1 elements, one E8M0 scale per 32), the block format that the tensor cores of
+ * sm_100a multiply as it is.  A matrix of `rows` rows of K values (K a multiple of 32):
+ *   codes   [rows][ld] bytes, two elements per byte (even one in the low four bits), ld >= K / 2 a multiple of 16, 16-byte aligned;
+ *   scales  q38b_mx4_scale_bytes(K, rows) bytes, 16-byte aligned: tiles of 128 rows x 4 blocks (512 bytes; block b of row r at
+ *           16 (r % 32) + 4 (r / 32) + b), tile (i, j) at (i * ceil(K / 128) + j) * 512; zeros behind the last row and block.
+ * ------------------------------------------------------------------------------------------------------------ */
+size_t q38b_mx4_scale_bytes(int K, int rows);
+/* x (x_kind, x_ld elements between rows) -> codes and scales: per 32 values 2^e, e = floor(log2 of the largest magnitude) - 2, at
+ * least -127; elements x / 2^e rounded half to even, at most 6 in magnitude.  A block with a NaN or an infinity gets the NaN scale 255. */
+int q38b_quantize_mx4(q38b_ctx* ctx, const void* x_dev, int x_kind, long long x_ld, int K, int rows, void* codes_dev, long long codes_ld,
+                      void* scales_dev, void* stream);
+/* Scale bytes of another producer, [rows][src_ld] with K / 32 of them in a row, into the tiles above. */
+int q38b_mx4_tile_scales(q38b_ctx* ctx, const void* src_dev, long long src_ld, int K, int rows, void* scales_dev, void* stream);
+/* The values that codes and scales stand for, exact in fp32, rounded once to fp16 / bf16. */
+int q38b_dequant_mx4(q38b_ctx* ctx, const void* codes_dev, long long codes_ld, const void* scales_dev, int K, int rows, void* out_dev,
+                     int out_kind, long long out_ld, void* stream);
+/* Y[t * ldy + r] (+)= sum_k X[t][k] W[r][k] for t < B, r < M over those values, on the block-scaled tensor-core instructions; fp32 sums
+ * in a fixed order, rounded once to y_kind (accumulate: added to Y in fp32 first).  How K is cut depends on B, M, K and the device's
+ * SM count: the same call gives the same bits on the same device.  Y must not overlap the operands. */
+int q38b_gemm_mx4(q38b_ctx* ctx, const void* W_codes, long long W_ld, const void* W_scales, int K, int M, const void* X_codes, long long X_ld,
+                  const void* X_scales, int B, void* Y_dev, int y_kind, long long ldy, int accumulate, void* stream);
+/* The same from activations as they are: x is quantized into `scratch_dev` (16-byte aligned, the caller's, at least
+ * q38b_gemm_mx4_scratch_bytes(K, B) bytes) and multiplied; results equal the two calls' bit for bit. */
+size_t q38b_gemm_mx4_scratch_bytes(int K, int B);
+int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W_codes, long long W_ld, const void* W_scales, int K, int M, const void* x_dev, int x_kind,
+                    long long x_ld, int B, void* Y_dev, int y_kind, long long ldy, int accumulate, void* scratch_dev, size_t scratch_bytes,
+                    void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
  * All-HBM planner.  Replaces the reference's residency planner and split upload (plan_residency,
  * src/runtime/planner.cpp:91-163; SplitMat / upload_split, src/runtime/engine.h:55-85, engine.cpp:594-629): every
  * matrix is resident in HBM, row-sharded over the ranks (one process per GPU): rank g of G owns rows

@@ -16,6 +16,7 @@ _LIB = None
 
 OUT_F32, OUT_F16, OUT_BF16 = 0, 1, 2
 _OUT_DTYPES = {OUT_F32: torch.float32, OUT_F16: torch.float16, OUT_BF16: torch.bfloat16}
+_OUT_KINDS = {d: k for k, d in _OUT_DTYPES.items()}
 
 
 class Q38BError(RuntimeError):
@@ -107,6 +108,17 @@ def load_library():
     lib.q38b_debug_set_one_cta.argtypes = [vp, i32]
     lib.q38b_debug_set_gemv_part_items.argtypes = [vp, ll]
     lib.q38b_gemv_group.argtypes = [vp, u32, i32, vp, sz, i32, vp, vp, vp, vp, vp]
+    lib.q38b_qk_norm_rope.argtypes = [vp, vp, vp, i32, i32, i32, C.c_float, C.c_float, vp, vp, i32, i32, i32, vp]
+    lib.q38b_adjust_logits.argtypes = [vp, vp, ll, i32, i32, i32, vp, vp, ll, vp]
+    lib.q38b_mx4_scale_bytes.argtypes = [i32, i32]
+    lib.q38b_mx4_scale_bytes.restype = sz
+    lib.q38b_quantize_mx4.argtypes = [vp, vp, i32, ll, i32, i32, vp, ll, vp, vp]
+    lib.q38b_mx4_tile_scales.argtypes = [vp, vp, ll, i32, i32, vp, vp]
+    lib.q38b_dequant_mx4.argtypes = [vp, vp, ll, vp, i32, i32, vp, i32, ll, vp]
+    lib.q38b_gemm_mx4.argtypes = [vp, vp, ll, vp, i32, i32, vp, ll, vp, i32, vp, i32, ll, i32, vp]
+    lib.q38b_gemm_mx4_scratch_bytes.argtypes = [i32, i32]
+    lib.q38b_gemm_mx4_scratch_bytes.restype = sz
+    lib.q38b_gemm_mx4_x.argtypes = [vp, vp, ll, vp, i32, i32, vp, i32, ll, i32, vp, i32, ll, i32, vp, sz, vp]
     _LIB = lib
     return lib
 
@@ -118,6 +130,38 @@ def status_string(status):
 def _stream():
     """The current stream's handle.  Asked for raw: torch.cuda.current_stream() builds a Stream object on every call."""
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+class _Heads(C.Structure):
+    """q38b_heads: the query or the key heads of a chunk of rows."""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_row", C.c_longlong), ("src_head", C.c_longlong), ("dst_row", C.c_longlong),
+                ("dst_head", C.c_longlong), ("weight", C.c_void_p), ("n_heads", C.c_int)]
+
+
+class _LogitRules(C.Structure):
+    """q38b_logit_rules: what shapes the logits before the top-k."""
+    _fields_ = [("penalties", C.c_void_p), ("history", C.c_void_p), ("history_begin", C.c_void_p), ("prompt_len", C.c_void_p),
+                ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p), ("bias_begin", C.c_void_p), ("masks", C.c_void_p),
+                ("mask_ld", C.c_longlong), ("mask_of_row", C.c_void_p)]
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+class Mx4:
+    """A matrix in microscaled 4-bit floating point: codes uint8 [rows, K / 2] (two elements a byte), scales uint8 in the library's tiles
+    (Context.quantize_mx4 makes both, Context.pack_mx4 takes another producer's)."""
+
+    def __init__(self, codes, scales):
+        _need(codes.dtype == scales.dtype == torch.uint8 and codes.dim() == 2 and codes.stride(1) == 1, "Mx4: uint8 codes [rows, K / 2] with packed rows, uint8 scales")
+        rows, half = codes.shape
+        _need(rows >= 1 and half >= 16 and half % 16 == 0, "Mx4: K a multiple of 32, at least one row")
+        _need(scales.is_contiguous() and scales.numel() == ((rows + 127) // 128) * ((half + 63) // 64) * 512, "Mx4: contiguous tiles of 128 rows x 4 blocks of scales")
+        _need(codes.device == scales.device, "Mx4: codes and scales on one device")
+        self.codes, self.scales, self.rows, self.K = codes, scales, rows, 2 * half
+        self.ld = codes.stride(0) if rows > 1 else half   # (the stride of a single row says nothing)
 
 
 class Context:
@@ -267,6 +311,133 @@ class Context:
         y = torch.empty(N, dtype=torch.float32, device=W.device)
         self._rc(self.lib.q38b_gemv_bf16(self.h, W.data_ptr(), K, N, x.data_ptr(), y.data_ptr(), _stream()), "q38b_gemv_bf16")
         return y
+
+    # ---- the steps of a token between its products --------------------------------------------
+    def _mine(self, what, *tensors):
+        for t in tensors:
+            if t is not None and t.device != self.device:
+                raise ValueError(f"{what}: tensors on {self.device}, the context's device")
+
+    def _stream(self):
+        return torch._C._cuda_getCurrentRawStream(self.device.index)
+
+    def qk_norm_rope(self, q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, adjacent=False, scale=1.0, kind=None, q_out=None, k_out=None):
+        """q [rows, heads, D], k [rows, heads, D] or None (fp32, fp16 or bf16, any row and head strides): RMSNorm of each head, rotation of its first
+        2 * len(inv_freq) elements by positions (int32 [rows]) times inv_freq (float64); weights fp32 [D].  kind: OUT_* of the results (that of
+        the inputs by default); returns (q_out, k_out), which may be q and k themselves."""
+        rows, _, D = q.shape
+        kind = _OUT_KINDS.get(q.dtype) if kind is None else kind
+        out_dtype = _OUT_DTYPES[kind] if q.dtype in _OUT_KINDS else None
+        _need(out_dtype is not None, "qk_norm_rope: fp32, fp16 or bf16 heads")
+        rot = 0 if inv_freq is None else 2 * inv_freq.shape[0]
+        if rot:
+            _need(positions is not None and positions.dtype == torch.int32 and positions.shape == (rows,) and (rows == 1 or positions.stride(0) == 1), "qk_norm_rope: int32 positions, one per row")
+            _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and rot <= D, "qk_norm_rope: float64 inv_freq, at most D / 2")
+            self._mine("qk_norm_rope", positions, inv_freq)
+        parts, outs = [], []
+        for x, w, out in ((q, q_weight, q_out), (k, k_weight, k_out)):
+            if x is None:
+                parts.append(None)
+                outs.append(None)
+                continue
+            _need(x.dim() == 3 and x.shape[0] == rows and x.shape[2] == D and x.dtype == q.dtype and (D == 1 or x.stride(2) == 1), "qk_norm_rope: heads [rows, heads, D] of one type, elements side by side")
+            _need(w is None or (w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous()), "qk_norm_rope: fp32 weights [D]")
+            if out is None:
+                out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+            _need(out.shape == x.shape and out.dtype == out_dtype and (D == 1 or out.stride(2) == 1), "qk_norm_rope: outputs shaped like the heads")
+            self._mine("qk_norm_rope", x, w, out)
+            parts.append(_Heads(x.data_ptr(), out.data_ptr(), x.stride(0), x.stride(1), out.stride(0), out.stride(1), None if w is None else w.data_ptr(), x.shape[1]))
+            outs.append(out)
+        self._rc(self.lib.q38b_qk_norm_rope(self.h, C.byref(parts[0]), None if k is None else C.byref(parts[1]), D, rot, int(bool(adjacent)), eps, scale,
+                                            positions.data_ptr() if rot else None, inv_freq.data_ptr() if rot else None, _OUT_KINDS[q.dtype], kind, rows,
+                                            self._stream()), "q38b_qk_norm_rope")
+        return outs[0], outs[1]
+
+    def logit_rules(self, rows, n, penalties=None, history=None, history_begin=None, prompt_len=None, bias_ids=None, bias_values=None, bias_begin=None,
+                    masks=None, mask_of_row=None, index_offset=0):
+        """q38b_logit_rules of checked device tensors: penalties fp32 [rows, 3] (repetition, frequency, presence), history int32 with int64 begins
+        [rows + 1] and int32 prompt lengths [rows]; bias_ids int32, bias_values fp32, int64 begins; masks int32 [*, words] of allowed-token
+        bits, mask_of_row int32 [rows]."""
+        flat = lambda t, dtype, *shape: t is None or (t.dtype == dtype and t.is_contiguous() and (not shape or t.shape == shape))   # noqa: E731
+        f32, i32, i64 = torch.float32, torch.int32, torch.int64
+        _need(flat(penalties, f32, rows, 3) and flat(history, i32) and flat(history_begin, i64, rows + 1) and flat(prompt_len, i32, rows), "adjust_logits: penalties, history")
+        _need(flat(bias_ids, i32) and flat(bias_values, f32) and flat(bias_begin, i64, rows + 1), "adjust_logits: biases")
+        _need(bias_ids is None or (bias_values is not None and bias_values.numel() == bias_ids.numel()), "adjust_logits: one value per bias")
+        _need(masks is None or (masks.dtype == i32 and masks.dim() == 2 and masks.stride(1) == 1 and masks.shape[1] * 32 >= index_offset + n and
+                                (masks.shape[0] >= rows or mask_of_row is not None)), "adjust_logits: masks int32 [masks, words], a bit for each token")
+        _need(flat(mask_of_row, i32, rows), "adjust_logits: mask_of_row int32 [rows]")
+        self._mine("adjust_logits", penalties, history, history_begin, prompt_len, bias_ids, bias_values, bias_begin, masks, mask_of_row)
+        ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+        # (an empty list has no address: no history then, which changes nothing)
+        gone = history is not None and history.numel() == 0
+        none = bias_ids is not None and bias_ids.numel() == 0
+        return _LogitRules(None if gone else ptr(penalties), None if gone else ptr(history), None if gone else ptr(history_begin), None if gone else ptr(prompt_len),
+                           None if none else ptr(bias_ids), None if none else ptr(bias_values), None if none else ptr(bias_begin), ptr(masks),
+                           0 if masks is None else masks.stride(0) if masks.shape[0] > 1 else masks.shape[1], ptr(mask_of_row))
+
+    def adjust_logits(self, logits, out=None, index_offset=0, **rules):
+        """logits fp32 [rows, n] (any row stride) -> penalised, biased, masked logits (`out`, which may be `logits`); the rules are those of
+        logit_rules.  Token v is column v - index_offset."""
+        _need(logits.dtype == torch.float32 and logits.dim() == 2 and (logits.shape[1] == 1 or logits.stride(1) == 1), "adjust_logits: fp32 logits [rows, n]")
+        rows, n = logits.shape
+        r = self.logit_rules(rows, n, index_offset=index_offset, **rules)
+        if out is None:
+            out = torch.empty((rows, n), dtype=torch.float32, device=logits.device)
+        _need(out.dtype == torch.float32 and out.shape == logits.shape and (n == 1 or out.stride(1) == 1), "adjust_logits: fp32 out of the logits' shape")
+        self._mine("adjust_logits", logits, out)
+        self._rc(self.lib.q38b_adjust_logits(self.h, logits.data_ptr(), logits.stride(0), n, rows, index_offset, C.byref(r), out.data_ptr(), out.stride(0),
+                                             self._stream()), "q38b_adjust_logits")
+        return out
+
+    # ---- microscaled 4-bit floating point -----------------------------------------------------
+    def quantize_mx4(self, x):
+        """x [rows, K] (fp32, fp16 or bf16, any row stride) -> Mx4."""
+        _need(x.dtype in _OUT_KINDS and x.dim() == 2 and x.stride(1) == 1, "quantize_mx4: fp32, fp16 or bf16 [rows, K]")
+        rows, K = x.shape
+        self._mine("quantize_mx4", x)
+        codes = torch.empty((rows, K // 2), dtype=torch.uint8, device=x.device)
+        scales = torch.empty(self.lib.q38b_mx4_scale_bytes(K, rows), dtype=torch.uint8, device=x.device)
+        self._rc(self.lib.q38b_quantize_mx4(self.h, x.data_ptr(), _OUT_KINDS[x.dtype], max(K, x.stride(0)) if rows == 1 else x.stride(0), K, rows,
+                                            codes.data_ptr(), K // 2, scales.data_ptr(), self._stream()), "q38b_quantize_mx4")
+        return Mx4(codes, scales)
+
+    def pack_mx4(self, codes, scales):
+        """Codes uint8 [rows, K / 2] and scale bytes uint8 [rows, K / 32] of another producer -> Mx4 (the codes are kept, not copied)."""
+        _need(scales.dtype == torch.uint8 and scales.dim() == 2 and scales.stride(1) == 1 and scales.shape == (codes.shape[0], codes.shape[1] // 16), "pack_mx4: uint8 scales [rows, K / 32]")
+        rows, K = codes.shape[0], 2 * codes.shape[1]
+        self._mine("pack_mx4", codes, scales)
+        tiles = torch.empty(self.lib.q38b_mx4_scale_bytes(K, rows), dtype=torch.uint8, device=codes.device)
+        self._rc(self.lib.q38b_mx4_tile_scales(self.h, scales.data_ptr(), max(scales.stride(0), K // 32), K, rows, tiles.data_ptr(), self._stream()), "q38b_mx4_tile_scales")
+        return Mx4(codes, tiles)
+
+    def dequant_mx4(self, m, kind=OUT_F32):
+        """The values of an Mx4: [rows, K]."""
+        self._mine("dequant_mx4", m.codes)
+        out = torch.empty((m.rows, m.K), dtype=_OUT_DTYPES[kind], device=m.codes.device)
+        self._rc(self.lib.q38b_dequant_mx4(self.h, m.codes.data_ptr(), m.ld, m.scales.data_ptr(), m.K, m.rows, out.data_ptr(), kind, m.K, self._stream()), "q38b_dequant_mx4")
+        return out
+
+    def gemm_mx4(self, W, X, kind=OUT_F32, out=None, accumulate=False):
+        """Y [B, W.rows] = X W^T for W an Mx4 and X an Mx4 or activations [B, K] (fp32, fp16 or bf16), which are quantized first.  kind: OUT_* of Y
+        where `out` is not given."""
+        B = X.rows if isinstance(X, Mx4) else X.shape[0]
+        if out is None:
+            out = torch.empty((B, W.rows), dtype=_OUT_DTYPES[kind], device=W.codes.device)
+        _need(out.shape == (B, W.rows) and out.dtype in _OUT_KINDS and (W.rows == 1 or out.stride(1) == 1), "gemm_mx4: out [B, W.rows]")
+        ldy = out.stride(0) if B > 1 else W.rows
+        if isinstance(X, Mx4):
+            _need(X.K == W.K, "gemm_mx4: operands of one K")
+            self._mine("gemm_mx4", W.codes, X.codes, out)
+            self._rc(self.lib.q38b_gemm_mx4(self.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), W.K, W.rows, X.codes.data_ptr(), X.ld, X.scales.data_ptr(), B,
+                                            out.data_ptr(), _OUT_KINDS[out.dtype], ldy, int(bool(accumulate)), self._stream()), "q38b_gemm_mx4")
+            return out
+        _need(X.dtype in _OUT_KINDS and X.dim() == 2 and X.stride(1) == 1 and X.shape[1] == W.K, "gemm_mx4: activations [B, K] of the weights' K")
+        self._mine("gemm_mx4", W.codes, X, out)
+        scratch = torch.empty(self.lib.q38b_gemm_mx4_scratch_bytes(W.K, B), dtype=torch.uint8, device=X.device)
+        self._rc(self.lib.q38b_gemm_mx4_x(self.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), W.K, W.rows, X.data_ptr(), _OUT_KINDS[X.dtype],
+                                          X.stride(0) if B > 1 else W.K, B, out.data_ptr(), _OUT_KINDS[out.dtype], ldy, int(bool(accumulate)), scratch.data_ptr(),
+                                          scratch.numel(), self._stream()), "q38b_gemm_mx4_x")
+        return out
 
     def topk(self, logits, k, index_offset=0):
         """The k largest of each row of `logits` [rows, n] (fp32, device): (values [rows, k], positions [rows, k] int32)."""

@@ -1,0 +1,504 @@
+// q38b_mx4.cu -- microscaled 4-bit floating point (OCP MX: E2M1 elements, one E8M0 scale per 32): quantizer, dequantizer
+// and the product of two such matrices on the block-scaled tensor-core instructions.
+//
+//   e = clamp(floor(log2 amax) - 2, -127, 127) over 32 values; code = x / 2^e rounded half to even to {0 .5 1 1.5 2 3 4 6}
+//   Y[t][r] (+)= sum_k X[t][k] W[r][k] over the values the codes and scales stand for
+//
+// A matrix is held as the tensor core reads it: codes [rows][K/2], two per byte (even element low), rows `ld` bytes apart;
+// scale bytes in tiles of 128 rows x 4 blocks (512 bytes: byte 16 (r % 32) + 4 (r / 32) + b), tile (i, j) at (i ceil(K/128) + j) 512,
+// which is what one copy into tensor memory takes; bytes behind the last row and block are zero.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "../../include/q38b200.h"
+#include "q38b_host.h"
+#include "q38b_internal.h"
+#include "q38b_pipe.cuh"
+#include "q38b_types.cuh"
+#include "q38b_umma.cuh"
+
+using namespace q38b;
+
+namespace {
+
+constexpr int MX_TILE = 512;   // scale bytes of 128 rows x 4 blocks
+
+__host__ __device__ inline long long mx_tiles_k(int K) { return (K + 127) / 128; }
+
+// Two values to two E2M1 codes (a in the low four bits): half to even, saturated at 6.
+__device__ __forceinline__ uint32_t e2m1_pair(float a, float b) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// The scale byte of a block whose largest magnitude has the bit pattern `top`, and the power of two its values are multiplied
+// with.  The byte is the exponent field less two (the exponent of 4, the largest power of two an element holds), never below 0;
+// a block that holds a NaN or an infinity gets 255, the scale that is NaN, and codes of its own zeros (0 times anything but NaN).
+__device__ __forceinline__ uint32_t mx_scale(uint32_t top, float& inv) {
+    const uint32_t field = top >> 23;
+    if (field == 255u) { inv = 0.0f; return 255u; }
+    const uint32_t byte = field > 2u ? field - 2u : 0u;
+    inv = __uint_as_float((254u - byte) << 23);
+    return byte;
+}
+
+// One warp per (row, 128 values): a lane takes four neighbours, eight lanes a block.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, long long x_ld, int K, int rows, uint8_t* codes, long long codes_ld, uint8_t* scales) {
+    const int lane = threadIdx.x & 31;
+    const long long kt = mx_tiles_k(K), rows_pad = (long long)(rows + 127) / 128 * 128;
+    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (item >= rows_pad * kt) return;
+    const long long row = item / kt;
+    const int j = (int)(item % kt), k = 128 * j + 4 * lane;
+    float v[4] = {};
+    if (row < rows && k < K) {
+        const T* p = x + row * x_ld + k;
+        if constexpr (VEC) {
+            if constexpr (sizeof(T) == 4) {
+                const float4 t = *(const float4*)p;
+                v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+            } else {
+                const uint2 t = *(const uint2*)p;
+                const T* e = (const T*)&t;
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = to_f32(e[i]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = to_f32(p[i]);
+        }
+    }
+    uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; i++) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+#pragma unroll
+    for (int s = 1; s < 8; s <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, s));
+    float inv;
+    uint32_t byte = mx_scale(top, inv);
+    const uint32_t code = e2m1_pair(v[0] * inv, v[1] * inv) | (e2m1_pair(v[2] * inv, v[3] * inv) << 8);
+    if (row < rows && k < K) *(uint16_t*)(codes + row * codes_ld + k / 2) = (uint16_t)code;
+    if (row >= rows || k >= K) byte = 0u;
+    if ((lane & 7) == 0)
+        scales[((row / 128) * kt + j) * MX_TILE + 16 * (row % 32) + 4 * (row % 128 / 32) + lane / 8] = (uint8_t)byte;
+}
+
+// Scale bytes of another producer, row by row, into the tiles.
+__global__ void __launch_bounds__(256) mx4_tile_kernel(const uint8_t* src, long long src_ld, int K, int rows, uint8_t* scales) {
+    const long long kt = mx_tiles_k(K), n = (long long)(rows + 127) / 128 * kt * MX_TILE;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    const int in = (int)(i % MX_TILE);
+    const long long row = i / MX_TILE / kt * 128 + in / 16 + 32 * (in % 16 / 4), block = i / MX_TILE % kt * 4 + in % 4;
+    scales[i] = row < rows && block < K / 32 ? src[row * src_ld + block] : (uint8_t)0;
+}
+
+__device__ __forceinline__ float mx_scale_value(uint32_t byte) {   // 2^(byte - 127); 255: NaN
+    return byte == 255u ? __uint_as_float(0x7FC00000u) : byte == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(byte << 23);
+}
+__device__ __forceinline__ float e2m1_value(uint32_t c) {   // sign, two exponent bits, one mantissa bit
+    const uint32_t m = c & 7u;
+    const float v = m < 2u ? 0.5f * (float)m : __uint_as_float((((m >> 1) + 126u) << 23) | ((m & 1u) << 22));
+    return c & 8u ? -v : v;
+}
+
+// One thread per eight values.
+template <typename T>
+__global__ void __launch_bounds__(256) mx4_dequant_kernel(const uint8_t* codes, long long codes_ld, const uint8_t* scales, int K, int rows, T* out, long long out_ld) {
+    const long long per = K / 8, i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= per * rows) return;
+    const long long row = i / per;
+    const int k = (int)(i % per) * 8;
+    const float s = mx_scale_value(scales[((row / 128) * mx_tiles_k(K) + k / 128) * MX_TILE + 16 * (row % 32) + 4 * (row % 128 / 32) + k % 128 / 32]);
+    const uint32_t c = *(const uint32_t*)(codes + row * codes_ld + k / 2);
+#pragma unroll
+    for (int e = 0; e < 8; e++) out[row * out_ld + k + e] = from_f32<T>(e2m1_value((c >> (4 * e)) & 15u) * s);
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// The product.  A CTA owns 128 weight rows (MMA M) and up to 256 tokens (MMA N).  One thread keeps a ring of stages of 256 K filled
+// (codes by tiled TMA with the 128-byte swizzle, scale tiles by bulk copies), one issues per stage the copies of the scale tiles into
+// tensor memory and the MMA (kind::mxf4, K = 64, one scale per 32), four warps store the accumulator.  Nothing is expanded: the
+// tensor core multiplies the codes and applies the scales.  Products of two elements are multiples of 1/4 up to 36 and the scales
+// are powers of two, so only the 32-bit sum rounds.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int MX_ROWS = 128, MX_MAX_N = 256, MX_K = 256;
+constexpr int MX_THREADS = 192, MX_MAX_STAGES = 8, MX_MAX_SPLITS = 8;
+constexpr int MX_A_BYTES = MX_ROWS * MX_K / 2, MX_SFA_BYTES = 2 * MX_TILE;
+
+struct MxArgs {
+    const uint8_t *w_scales, *x_scales;
+    void* Y;
+    long long ldy;
+    int* status;
+    int K, M, B, accumulate;
+    int n_tile, stages, splits, pdl;
+};
+__host__ __device__ constexpr int mx_groups(int n_tile) { return (n_tile + 127) / 128; }
+__host__ __device__ constexpr int mx_stage_bytes(int n_tile) { return MX_A_BYTES + n_tile * (MX_K / 2) + MX_SFA_BYTES * (1 + mx_groups(n_tile)); }
+// accumulator, then two buffers of a stage's scales: 4 columns per tile of 128 rows x 128 K
+__host__ __device__ constexpr int mx_acc_cols(int n_tile) { return (n_tile + 31) / 32 * 32; }
+__host__ __device__ constexpr int mx_scale_cols(int n_tile) { return 8 * (1 + mx_groups(n_tile)); }
+__host__ __device__ constexpr uint32_t mx_tmem_cols(int n_tile) {
+    const int n = mx_acc_cols(n_tile) + 2 * mx_scale_cols(n_tile);
+    return n <= 64 ? 64u : n <= 128 ? 128u : n <= 256 ? 256u : 512u;
+}
+
+__device__ __forceinline__ uint64_t umma_desc_flat(uint32_t smem_addr) {   // no swizzle, groups of eight 16-byte rows 128 bytes apart
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
+}
+// one scale tile (32 x 16 bytes) to four columns of tensor memory, repeated for the four quarters of the lanes
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(umma_desc_flat(smem_addr)) : "memory");
+}
+__device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+        "r"(sfa), "r"(sfb), "r"(add)
+        : "memory");
+}
+// E2M1 times E2M1, E8M0 scales, K-major; half: which two of a column's four scales (K 0..63 or 64..127 of a tile)
+__device__ __forceinline__ uint32_t mx_idesc(int n, int half) {
+    return ((uint32_t)(2 * half) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(MX_ROWS >> 4) << 24) |
+           ((uint32_t)(2 * half) << 29);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t* full = (uint64_t*)smem;
+    uint64_t* empty = full + MX_MAX_STAGES;
+    uint64_t* acc_done = empty + MX_MAX_STAGES;
+    uint32_t* tmem_slot = (uint32_t*)(acc_done + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    uint8_t* ring = smem + 1024;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = a.splits > 1 ? (int)cluster_rank() : 0;
+    const int row0 = (int)(blockIdx.x / (unsigned)a.splits) * MX_ROWS, tok0 = (int)blockIdx.y * a.n_tile;
+    const int n_tok = min(a.n_tile, a.B - tok0), n_mma = (n_tok + 15) / 16 * 16, groups = mx_groups(a.n_tile);
+    const int kt = (int)mx_tiles_k(a.K), steps = (a.K + MX_K - 1) / MX_K;
+    const int s_begin = (int)((long long)steps * rank / a.splits), s_end = (int)((long long)steps * (rank + 1) / a.splits);
+    const int stage_bytes = mx_stage_bytes(a.n_tile);
+    const uint32_t tmem_cols = mx_tmem_cols(a.n_tile);
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < a.stages; s++) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        mbar_init(smem_u32(acc_done), 1);
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+    if (a.pdl) pdl_wait_prior();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int st = 0;
+            uint32_t use = 0;
+            const uint8_t* wsc = a.w_scales + (size_t)(row0 / 128) * kt * MX_TILE;
+            for (int s = s_begin; s < s_end; s++) {
+                mbar_wait_bounded(smem_u32(&empty[st]), use ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
+                const uint32_t bar = smem_u32(&full[st]), at = smem_u32(ring + st * stage_bytes), scale_bytes = (uint32_t)min(2, kt - 2 * s) * MX_TILE;
+                const uint32_t sf = at + MX_A_BYTES + (uint32_t)a.n_tile * (MX_K / 2);
+                const int used = (n_tok + 127) / 128;   // groups of 128 tokens that hold any
+                mbar_arrive_expect_tx(bar, (uint32_t)(MX_A_BYTES + a.n_tile * (MX_K / 2)) + scale_bytes * (uint32_t)(1 + used));
+                tma_load_2d(at, &wmap, s * (MX_K / 2), row0, bar);
+                tma_load_2d(at + MX_A_BYTES, &xmap, s * (MX_K / 2), tok0, bar);
+                bulk_copy_g2s(sf, wsc + (size_t)s * MX_SFA_BYTES, scale_bytes, bar);
+                for (int g = 0; g < used; g++)
+                    bulk_copy_g2s(sf + (uint32_t)(1 + g) * MX_SFA_BYTES, a.x_scales + ((size_t)(tok0 / 128 + g) * kt + 2 * s) * MX_TILE, scale_bytes, bar);
+                if (++st == a.stages) { st = 0; use ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        int st = 0;
+        uint32_t use = 0;
+        const uint64_t desc0 = umma_desc_sw128(0);
+        const uint32_t sf_cols = tmem_base + (uint32_t)mx_acc_cols(a.n_tile);
+        for (int s = s_begin; s < s_end; s++) {
+            mbar_wait_bounded(smem_u32(&full[st]), use, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect_one()) {
+                const uint32_t at = smem_u32(ring + st * stage_bytes), sf = at + MX_A_BYTES + (uint32_t)a.n_tile * (MX_K / 2);
+                const uint64_t ad = desc0 + ((at & 0x3FFFFu) >> 4), bd = desc0 + (((at + MX_A_BYTES) & 0x3FFFFu) >> 4);
+                const uint32_t cols = sf_cols + (uint32_t)((s & 1) * mx_scale_cols(a.n_tile));
+                const int n_k = min(4, (a.K - s * MX_K + 63) / 64);   // MMA of 64 K; codes behind K are zero
+                for (int c = 0; 2 * c < n_k; c++) {
+                    tmem_copy_scales(cols + (uint32_t)(4 * c), sf + (uint32_t)(c * MX_TILE));
+                    for (int g = 0; g < groups; g++)
+                        tmem_copy_scales(cols + (uint32_t)(8 + 4 * (c * groups + g)), sf + (uint32_t)((1 + g) * MX_SFA_BYTES + c * MX_TILE));
+                }
+                for (int k = 0; k < n_k; k++)
+                    mma_mxf4(tmem_base, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), mx_idesc(n_mma, k & 1), cols + (uint32_t)(4 * (k >> 1)),
+                             cols + (uint32_t)(8 + 4 * (k >> 1) * groups), s > s_begin || k > 0 ? 1u : 0u);
+                umma_commit<false>(smem_u32(&empty[st]));
+                if (s == s_end - 1) umma_commit<false>(smem_u32(acc_done));
+            }
+            __syncwarp();
+            if (++st == a.stages) { st = 0; use ^= 1u; }
+        }
+    }
+
+    // ---------------- warps 2..5 store: lanes 32 (warp % 4) .. + 31 of the accumulator are 32 rows ----------------
+    const int n_chunks = (n_tok + 15) / 16, quad = warp & 3, row = row0 + 32 * quad + lane;
+    const uint32_t acc = tmem_base + ((uint32_t)(32 * quad) << 16);
+    T* Y = (T*)a.Y;
+    auto store = [&](int chunk, const float (&v)[16]) {
+        if (row >= a.M) return;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int t = 16 * chunk + j;
+            if (t < n_tok) {
+                T* y = Y + (size_t)(tok0 + t) * a.ldy + row;
+                *y = from_f32<T>(a.accumulate ? to_f32(*y) + v[j] : v[j]);
+            }
+        }
+    };
+    if (warp >= 2) {
+        mbar_wait_bounded(smem_u32(acc_done), 0u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+    if (a.splits == 1) {
+        if (warp >= 2)
+            for (int chunk = 0; chunk < n_chunks; chunk++) {
+                uint32_t v[16];
+                float f[16];
+                tmem_ld16(acc + (uint32_t)(16 * chunk), v);
+#pragma unroll
+                for (int j = 0; j < 16; j++) f[j] = __uint_as_float(v[j]);
+                store(chunk, f);
+            }
+    } else {
+        // Chunk c of the tile is finished by rank c % splits: the others put their sums of it into that CTA's ring, idle by then,
+        // [source][c / splits][16 tokens][128 rows]; sums are added in rank order.
+        const int own_chunks = (n_chunks + a.splits - 1) / a.splits;
+        const uint32_t box = smem_u32(ring);
+        __syncwarp();
+        cluster_sync_all();
+        if (warp >= 2)
+            for (int chunk = 0; chunk < n_chunks; chunk++) {
+                const int owner = chunk % a.splits;
+                if (owner == rank) continue;
+                uint32_t v[16];
+                tmem_ld16(acc + (uint32_t)(16 * chunk), v);
+                const int src = rank - (rank > owner ? 1 : 0);
+                const uint32_t to = peer_smem(box + (uint32_t)((src * own_chunks + chunk / a.splits) * (16 * MX_ROWS) + 32 * quad + lane) * 4u, (uint32_t)owner);
+#pragma unroll
+                for (int j = 0; j < 16; j++) st_peer_f32(to + (uint32_t)(j * MX_ROWS * 4), v[j]);
+            }
+        cluster_sync_all();   // all sums have arrived; nobody touches another CTA's memory after this
+        if (warp >= 2)
+            for (int own = 0; own * a.splits + rank < n_chunks; own++) {
+                uint32_t v[16];
+                float f[16] = {};
+                tmem_ld16(acc + (uint32_t)(16 * (own * a.splits + rank)), v);
+                for (int r = 0; r < a.splits; r++) {
+                    const float* in = (const float*)ring + (size_t)((r - (r > rank ? 1 : 0)) * own_chunks + own) * (16 * MX_ROWS) + 32 * quad + lane;
+#pragma unroll
+                    for (int j = 0; j < 16; j++) f[j] += r == rank ? __uint_as_float(v[j]) : in[j * MX_ROWS];
+                }
+                store(own * a.splits + rank, f);
+            }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols) : "memory");
+    }
+}
+
+// How a product is cut: tokens in tiles of n_tile (one tile, or several of 128 or 256: a tile starts on a scale tile's border), K in
+// `splits` parts.
+struct MxCut { int n_tile, stages, splits; };
+
+int exchange_bytes(const MxCut& c) {
+    const int chunks = c.n_tile / 16;
+    return (c.splits - 1) * ((chunks + c.splits - 1) / c.splits) * 16 * MX_ROWS * 4;
+}
+
+MxCut mx_cut(int sm_count, int smem_optin, int K, int M, int B) {
+    MxCut c;
+    c.n_tile = B <= MX_MAX_N ? (B + 15) / 16 * 16 : MX_MAX_N;
+    const int steps = (K + MX_K - 1) / MX_K;
+    const long long tiles = (long long)((M + MX_ROWS - 1) / MX_ROWS) * ((B + c.n_tile - 1) / c.n_tile);
+    c.splits = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(MX_MAX_SPLITS, sm_count / tiles), steps / 4));
+    c.stages = std::min(MX_MAX_STAGES, (smem_optin - 1024) / mx_stage_bytes(c.n_tile));
+    while (c.splits > 1 && exchange_bytes(c) > c.stages * mx_stage_bytes(c.n_tile)) c.splits--;
+    return c;
+}
+
+size_t kind_size(int kind) { return kind == Q38B_OUT_F32 ? 4 : 2; }
+bool known_kind(int kind) { return kind == Q38B_OUT_F32 || kind == Q38B_OUT_F16 || kind == Q38B_OUT_BF16; }
+bool mx_shape(int K, int rows) { return K >= 32 && K % 32 == 0 && rows >= 1; }
+
+template <typename T>
+int quantize_as(q38b_ctx* ctx, const void* x, long long x_ld, int K, int rows, uint8_t* codes, long long codes_ld, uint8_t* scales, cudaStream_t st) {
+    const long long items = (long long)(rows + 127) / 128 * 128 * mx_tiles_k(K);
+    const unsigned grid = (unsigned)((items + 7) / 8);
+    const bool vec = ((uintptr_t)x | (uintptr_t)(x_ld * (long long)sizeof(T))) % (4 * sizeof(T)) == 0;
+    if (vec) mx4_quantize_kernel<T, true><<<grid, 256, 0, st>>>((const T*)x, x_ld, K, rows, codes, codes_ld, scales);
+    else mx4_quantize_kernel<T, false><<<grid, 256, 0, st>>>((const T*)x, x_ld, K, rows, codes, codes_ld, scales);
+    return launch_status(ctx, cudaSuccess);
+}
+
+template <typename T>
+int dequant_as(q38b_ctx* ctx, const uint8_t* codes, long long codes_ld, const uint8_t* scales, int K, int rows, void* out, long long out_ld, cudaStream_t st) {
+    const long long n = (long long)(K / 8) * rows;
+    mx4_dequant_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(codes, codes_ld, scales, K, rows, (T*)out, out_ld);
+    return launch_status(ctx, cudaSuccess);
+}
+
+bool encode_codes(CUtensorMap* map, const void* codes, long long ld, int K, int rows, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)K / 2, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld};
+    const cuuint32_t box[2] = {MX_K / 2, (cuuint32_t)box_rows}, estr[2] = {1, 1};
+    EncodeTiledFn enc = encode_fn();
+    return enc && enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, (void*)codes, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T>
+int gemm_as(q38b_ctx* ctx, const MxArgs& a, const CUtensorMap& wmap, const CUtensorMap& xmap, cudaStream_t st) {
+    auto kern = mx4_gemm_kernel<T>;
+    const int rc = q38b_ensure_kernel_smem(ctx, (const void*)kern, ctx->smem_optin, false);
+    if (rc != Q38B_OK) return rc;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)((a.M + MX_ROWS - 1) / MX_ROWS * a.splits), (unsigned)((a.B + a.n_tile - 1) / a.n_tile));
+    cfg.blockDim = dim3(MX_THREADS);
+    cfg.dynamicSmemBytes = (size_t)(1024 + a.stages * mx_stage_bytes(a.n_tile));
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    if (a.splits > 1) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = (unsigned)a.splits;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        n++;
+    }
+    if (a.pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        n++;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = (unsigned)n;
+    return launch_status(ctx, cudaLaunchKernelEx(&cfg, kern, a, wmap, xmap));
+}
+
+// arguments of one operand
+int check_operand(const void* codes, long long ld, const void* scales, int K, int rows) {
+    if (!codes || !scales || !mx_shape(K, rows) || ld < K / 2) return Q38B_ERR_ARG;
+    return ((uintptr_t)codes & 15) || (ld & 15) || ((uintptr_t)scales & 15) ? Q38B_ERR_ALIGN : Q38B_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t q38b_mx4_scale_bytes(int K, int rows) { return mx_shape(K, rows) ? (size_t)((rows + 127) / 128) * (size_t)mx_tiles_k(K) * MX_TILE : 0; }
+
+int q38b_quantize_mx4(q38b_ctx* ctx, const void* x, int x_kind, long long x_ld, int K, int rows, void* codes, long long codes_ld, void* scales, void* stream) {
+    if (!ctx || !x || !known_kind(x_kind) || x_ld < K) return Q38B_ERR_ARG;
+    const int rc = check_operand(codes, codes_ld, scales, K, rows);
+    if (rc != Q38B_OK) return rc;
+    if ((uintptr_t)x % kind_size(x_kind)) return Q38B_ERR_ALIGN;
+    DeviceGuard on(ctx);
+    cudaStream_t st = (cudaStream_t)stream;
+    uint8_t *c = (uint8_t*)codes, *s = (uint8_t*)scales;
+    return x_kind == Q38B_OUT_F32 ? quantize_as<float>(ctx, x, x_ld, K, rows, c, codes_ld, s, st)
+         : x_kind == Q38B_OUT_F16 ? quantize_as<__half>(ctx, x, x_ld, K, rows, c, codes_ld, s, st)
+                                  : quantize_as<__nv_bfloat16>(ctx, x, x_ld, K, rows, c, codes_ld, s, st);
+}
+
+int q38b_mx4_tile_scales(q38b_ctx* ctx, const void* src, long long src_ld, int K, int rows, void* scales, void* stream) {
+    if (!ctx || !src || !scales || !mx_shape(K, rows) || src_ld < K / 32) return Q38B_ERR_ARG;
+    if ((uintptr_t)scales & 15) return Q38B_ERR_ALIGN;
+    DeviceGuard on(ctx);
+    const size_t n = q38b_mx4_scale_bytes(K, rows);
+    mx4_tile_kernel<<<(unsigned)((n + 255) / 256), 256, 0, (cudaStream_t)stream>>>((const uint8_t*)src, src_ld, K, rows, (uint8_t*)scales);
+    return launch_status(ctx, cudaSuccess);
+}
+
+int q38b_dequant_mx4(q38b_ctx* ctx, const void* codes, long long codes_ld, const void* scales, int K, int rows, void* out, int out_kind, long long out_ld,
+                     void* stream) {
+    if (!ctx || !out || !known_kind(out_kind) || out_ld < K) return Q38B_ERR_ARG;
+    const int rc = check_operand(codes, codes_ld, scales, K, rows);
+    if (rc != Q38B_OK) return rc;
+    if ((uintptr_t)out % kind_size(out_kind)) return Q38B_ERR_ALIGN;
+    DeviceGuard on(ctx);
+    cudaStream_t st = (cudaStream_t)stream;
+    const uint8_t *c = (const uint8_t*)codes, *s = (const uint8_t*)scales;
+    return out_kind == Q38B_OUT_F32 ? dequant_as<float>(ctx, c, codes_ld, s, K, rows, out, out_ld, st)
+         : out_kind == Q38B_OUT_F16 ? dequant_as<__half>(ctx, c, codes_ld, s, K, rows, out, out_ld, st)
+                                    : dequant_as<__nv_bfloat16>(ctx, c, codes_ld, s, K, rows, out, out_ld, st);
+}
+
+int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales, int K, int M, const void* X, long long X_ld, const void* X_scales, int B,
+                    void* Y, int y_kind, long long ldy, int accumulate, void* stream, bool behind_quantizer) {
+    if (!ctx || !Y || !known_kind(y_kind) || ldy < M) return Q38B_ERR_ARG;
+    int rc = check_operand(W, W_ld, W_scales, K, M);
+    if (rc == Q38B_OK) rc = check_operand(X, X_ld, X_scales, K, B);
+    if (rc != Q38B_OK) return rc;
+    if ((uintptr_t)Y % kind_size(y_kind)) return Q38B_ERR_ALIGN;
+    DeviceGuard on(ctx);
+    const MxCut cut = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B);
+    if ((B + cut.n_tile - 1) / cut.n_tile > 65535) return Q38B_ERR_UNSUPPORTED;
+    CUtensorMap wmap, xmap;
+    if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS) || !encode_codes(&xmap, X, X_ld, K, B, cut.n_tile)) return Q38B_ERR_ARG;
+    MxArgs a;
+    a.w_scales = (const uint8_t*)W_scales;
+    a.x_scales = (const uint8_t*)X_scales;
+    a.Y = Y;
+    a.ldy = ldy;
+    a.status = ctx->d_status;
+    a.K = K;
+    a.M = M;
+    a.B = B;
+    a.accumulate = accumulate ? 1 : 0;
+    a.n_tile = cut.n_tile;
+    a.stages = cut.stages;
+    a.splits = cut.splits;
+    a.pdl = behind_quantizer ? 1 : 0;
+    cudaStream_t st = (cudaStream_t)stream;
+    return y_kind == Q38B_OUT_F32 ? gemm_as<float>(ctx, a, wmap, xmap, st) : y_kind == Q38B_OUT_F16 ? gemm_as<__half>(ctx, a, wmap, xmap, st)
+                                                                                                    : gemm_as<__nv_bfloat16>(ctx, a, wmap, xmap, st);
+}
+
+int q38b_gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales, int K, int M, const void* X, long long X_ld, const void* X_scales, int B,
+                  void* Y, int y_kind, long long ldy, int accumulate, void* stream) {
+    return gemm_mx4(ctx, W, W_ld, W_scales, K, M, X, X_ld, X_scales, B, Y, y_kind, ldy, accumulate, stream, false);
+}
+
+size_t q38b_gemm_mx4_scratch_bytes(int K, int B) { return mx_shape(K, B) ? (size_t)B * (K / 2) + q38b_mx4_scale_bytes(K, B) + 16 : 0; }
+
+int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales, int K, int M, const void* x, int x_kind, long long x_ld, int B, void* Y,
+                    int y_kind, long long ldy, int accumulate, void* scratch, size_t scratch_bytes, void* stream) {
+    if (!ctx || !scratch || !mx_shape(K, B)) return Q38B_ERR_ARG;
+    if ((uintptr_t)scratch & 15) return Q38B_ERR_ALIGN;
+    if (scratch_bytes < q38b_gemm_mx4_scratch_bytes(K, B)) return Q38B_ERR_NOMEM;
+    uint8_t* scales = (uint8_t*)scratch;
+    uint8_t* codes = scales + q38b_mx4_scale_bytes(K, B);
+    if (!Y || !known_kind(y_kind) || ldy < M) return Q38B_ERR_ARG;
+    int rc = check_operand(W, W_ld, W_scales, K, M);
+    if (rc == Q38B_OK) rc = q38b_quantize_mx4(ctx, x, x_kind, x_ld, K, B, codes, K / 2, scales, stream);
+    if (rc != Q38B_OK) return rc;
+    return gemm_mx4(ctx, W, W_ld, W_scales, K, M, codes, K / 2, scales, B, Y, y_kind, ldy, accumulate, stream, true);
+}
+
+}  // extern "C"
