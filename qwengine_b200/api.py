@@ -118,6 +118,7 @@ def load_library():
     lib.q38b_gemm_mx4.argtypes = [vp, vp, ll, vp, i32, i32, vp, ll, vp, i32, vp, i32, ll, i32, vp]
     lib.q38b_gemm_mx4_scratch_bytes.argtypes = [i32, i32]
     lib.q38b_gemm_mx4_scratch_bytes.restype = sz
+    lib.q38b_debug_set_mx4_pairs.argtypes = [vp, i32]
     lib.q38b_gemm_mx4_x.argtypes = [vp, vp, ll, vp, i32, i32, vp, i32, ll, i32, vp, i32, ll, i32, vp, sz, vp]
     _LIB = lib
     return lib
@@ -225,6 +226,10 @@ class Context:
     def debug_set_gemv_part_items(self, items):
         """Test hook: the multi-column kernel's K-part scratch area counts as `items` (tile, part) sums (0: its real size)."""
         self._rc(self.lib.q38b_debug_set_gemv_part_items(self.h, int(items)), "q38b_debug_set_gemv_part_items")
+
+    def debug_set_mx4_pairs(self, mode):
+        """Test hook: 4-bit products in pairs of CTAs never (-1), with tiles of `mode` tokens, by the rule (0)."""
+        self._rc(self.lib.q38b_debug_set_mx4_pairs(self.h, int(mode)), "q38b_debug_set_mx4_pairs")
 
     def set_wait_budget_cycles(self, cycles):
         self._rc(self.lib.q38b_ctx_set_wait_budget_cycles(self.h, int(cycles)), "q38b_ctx_set_wait_budget_cycles")

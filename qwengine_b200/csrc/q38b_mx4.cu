@@ -140,11 +140,11 @@ struct MxArgs {
 };
 __host__ __device__ constexpr int mx_groups(int n_tile) { return (n_tile + 127) / 128; }
 __host__ __device__ constexpr int mx_stage_bytes(int n_tile) { return MX_A_BYTES + n_tile * (MX_K / 2) + MX_SFA_BYTES * (1 + mx_groups(n_tile)); }
-// accumulator, then two buffers of a stage's scales: 4 columns per tile of 128 rows x 128 K
+// accumulator, then the scales of each stage (a stage's columns are free when its shared memory is): 4 columns per tile of 128 rows x 128 K
 __host__ __device__ constexpr int mx_acc_cols(int n_tile) { return (n_tile + 31) / 32 * 32; }
 __host__ __device__ constexpr int mx_scale_cols(int n_tile) { return 8 * (1 + mx_groups(n_tile)); }
-__host__ __device__ constexpr uint32_t mx_tmem_cols(int n_tile) {
-    const int n = mx_acc_cols(n_tile) + 2 * mx_scale_cols(n_tile);
+__host__ __device__ constexpr uint32_t mx_tmem_cols(int n_tile, int stages) {
+    const int n = mx_acc_cols(n_tile) + stages * mx_scale_cols(n_tile);
     return n <= 64 ? 64u : n <= 128 ? 128u : n <= 256 ? 256u : 512u;
 }
 
@@ -152,23 +152,57 @@ __device__ __forceinline__ uint64_t umma_desc_flat(uint32_t smem_addr) {   // no
     return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);
 }
 // one scale tile (32 x 16 bytes) to four columns of tensor memory, repeated for the four quarters of the lanes
+// (of a pair: in each CTA from its own shared memory)
+template <bool PAIR>
 __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(umma_desc_flat(smem_addr)) : "memory");
+    if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(umma_desc_flat(smem_addr)) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(umma_desc_flat(smem_addr)) : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t add) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-        "r"(sfa), "r"(sfb), "r"(add)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+            "r"(sfa), "r"(sfb), "r"(add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+            "r"(sfa), "r"(sfb), "r"(add)
+            : "memory");
 }
-// E2M1 times E2M1, E8M0 scales, K-major; half: which two of a column's four scales (K 0..63 or 64..127 of a tile)
-__device__ __forceinline__ uint32_t mx_idesc(int n, int half) {
-    return ((uint32_t)(2 * half) << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(MX_ROWS >> 4) << 24) |
-           ((uint32_t)(2 * half) << 29);
+// E2M1 times E2M1, E8M0 scales, K-major; the first two of a column's four scales (K 0..63 of a tile; 2 in both scale fields: K 64..127)
+__device__ __forceinline__ uint32_t mx_idesc(int m, int n) { return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24); }
+
+// What the tensor core does with a stage that is there: NK steps of 64 K (four but for the last stage).  The counts are constants and the
+// addresses come from outside the elected branch, the same in every lane: in uniform registers a step issues in tens of clocks, out of
+// vector registers in a hundred and more (with loops over run-time counts a stage took some 1200 clocks whatever its tokens: 2048 x
+// 17408 x 5120 110 us).
+template <bool PAIR, int GROUPS, int NK>
+__device__ __forceinline__ void mx_issue(uint32_t d, uint64_t ad, uint64_t bd, uint32_t sf, uint32_t cols, uint32_t first_col, uint32_t idesc, uint32_t add) {
+#pragma unroll
+    for (int c = 0; 2 * c < NK; c++) {
+        tmem_copy_scales<PAIR>(cols + (uint32_t)(4 * c), sf + (uint32_t)(c * MX_TILE));
+#pragma unroll
+        for (int g = 0; g < GROUPS; g++)
+            tmem_copy_scales<PAIR>(cols + (uint32_t)(8 + 4 * (c * GROUPS + g)), sf + (uint32_t)((1 + g) * MX_SFA_BYTES + c * MX_TILE));
+    }
+#pragma unroll
+    for (int k = 0; k < NK; k++)
+        mma_mxf4<PAIR>(d, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), idesc + (k & 1 ? (2u << 4) | (2u << 29) : 0u), cols + (uint32_t)(4 * (k >> 1)),
+                       cols + first_col + (uint32_t)(4 * (k >> 1) * GROUPS), k > 0 ? 1u : add);
+}
+template <bool PAIR, int GROUPS>
+__device__ __forceinline__ void mx_issue_stage(int n_k, uint32_t d, uint64_t ad, uint64_t bd, uint32_t sf, uint32_t cols, uint32_t first_col, uint32_t idesc, uint32_t add) {
+    if (n_k >= 4) mx_issue<PAIR, GROUPS, 4>(d, ad, bd, sf, cols, first_col, idesc, add);
+    else if (n_k == 3) mx_issue<PAIR, GROUPS, 3>(d, ad, bd, sf, cols, first_col, idesc, add);
+    else if (n_k == 2) mx_issue<PAIR, GROUPS, 2>(d, ad, bd, sf, cols, first_col, idesc, add);
+    else mx_issue<PAIR, GROUPS, 1>(d, ad, bd, sf, cols, first_col, idesc, add);
 }
 
-template <typename T>
+template <typename T, int GROUPS>
 __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* full = (uint64_t*)smem;
@@ -180,11 +214,11 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = a.splits > 1 ? (int)cluster_rank() : 0;
     const int row0 = (int)(blockIdx.x / (unsigned)a.splits) * MX_ROWS, tok0 = (int)blockIdx.y * a.n_tile;
-    const int n_tok = min(a.n_tile, a.B - tok0), n_mma = (n_tok + 15) / 16 * 16, groups = mx_groups(a.n_tile);
+    const int n_tok = min(a.n_tile, a.B - tok0), n_mma = (n_tok + 15) / 16 * 16;
     const int kt = (int)mx_tiles_k(a.K), steps = (a.K + MX_K - 1) / MX_K;
     const int s_begin = (int)((long long)steps * rank / a.splits), s_end = (int)((long long)steps * (rank + 1) / a.splits);
     const int stage_bytes = mx_stage_bytes(a.n_tile);
-    const uint32_t tmem_cols = mx_tmem_cols(a.n_tile);
+    const uint32_t tmem_cols = mx_tmem_cols(a.n_tile, a.stages);
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -228,23 +262,15 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
         int st = 0;
         uint32_t use = 0;
         const uint64_t desc0 = umma_desc_sw128(0);
-        const uint32_t sf_cols = tmem_base + (uint32_t)mx_acc_cols(a.n_tile);
+        const uint32_t sf_cols = tmem_base + (uint32_t)mx_acc_cols(a.n_tile), ring_at = smem_u32(ring), idesc = mx_idesc(MX_ROWS, n_mma);
         for (int s = s_begin; s < s_end; s++) {
             mbar_wait_bounded(smem_u32(&full[st]), use, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t at = ring_at + (uint32_t)(st * stage_bytes), sf = at + MX_A_BYTES + (uint32_t)a.n_tile * (MX_K / 2);
+            const uint32_t cols = sf_cols + (uint32_t)(st * mx_scale_cols(a.n_tile));
+            const int n_k = (a.K - s * MX_K + 63) / 64;   // steps of 64 K that hold any; codes behind K are zero
             if (elect_one()) {
-                const uint32_t at = smem_u32(ring + st * stage_bytes), sf = at + MX_A_BYTES + (uint32_t)a.n_tile * (MX_K / 2);
-                const uint64_t ad = desc0 + ((at & 0x3FFFFu) >> 4), bd = desc0 + (((at + MX_A_BYTES) & 0x3FFFFu) >> 4);
-                const uint32_t cols = sf_cols + (uint32_t)((s & 1) * mx_scale_cols(a.n_tile));
-                const int n_k = min(4, (a.K - s * MX_K + 63) / 64);   // MMA of 64 K; codes behind K are zero
-                for (int c = 0; 2 * c < n_k; c++) {
-                    tmem_copy_scales(cols + (uint32_t)(4 * c), sf + (uint32_t)(c * MX_TILE));
-                    for (int g = 0; g < groups; g++)
-                        tmem_copy_scales(cols + (uint32_t)(8 + 4 * (c * groups + g)), sf + (uint32_t)((1 + g) * MX_SFA_BYTES + c * MX_TILE));
-                }
-                for (int k = 0; k < n_k; k++)
-                    mma_mxf4(tmem_base, ad + (uint64_t)(2 * k), bd + (uint64_t)(2 * k), mx_idesc(n_mma, k & 1), cols + (uint32_t)(4 * (k >> 1)),
-                             cols + (uint32_t)(8 + 4 * (k >> 1) * groups), s > s_begin || k > 0 ? 1u : 0u);
+                mx_issue_stage<false, GROUPS>(n_k, tmem_base, desc0 + (at >> 4), desc0 + ((at + MX_A_BYTES) >> 4), sf, cols, 8u, idesc, s > s_begin ? 1u : 0u);
                 umma_commit<false>(smem_u32(&empty[st]));
                 if (s == s_end - 1) umma_commit<false>(smem_u32(acc_done));
             }
@@ -322,6 +348,161 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
     }
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// Many tokens: two CTAs (a cluster of two on neighbouring SMs) multiply as one, M = 256: each holds 128 weight rows and half of
+// the tokens' codes, so that a stage costs an SM 16 + 16 KB of codes for 256 x 256 instead of 16 + 32 for 128 x 256.  The pairs
+// stay and walk the tiles (tokens fastest: neighbours read the same weights out of L2), the ring runs on across tiles, and eight warps
+// bring the accumulator to registers and hand it back before they store: the tensor core goes on meanwhile.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int MXP_THREADS = 320, MXP_EPI_WARPS = 8;
+
+struct MxPairArgs {
+    void* Y;
+    long long ldy;
+    int* status;
+    int K, M, B, accumulate;
+    int n_tile, stages, n_acc, tok_tiles, n_tiles, pdl;
+};
+__host__ __device__ constexpr int mxp_stage_bytes(int n_tile) { return MX_A_BYTES + n_tile / 2 * (MX_K / 2) + MX_SFA_BYTES * (1 + mx_groups(n_tile)); }
+
+template <typename T, int GROUPS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MXP_THREADS, 1)
+mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wsmap,
+                const __grid_constant__ CUtensorMap xsmap) {
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t* full = (uint64_t*)smem;                // CTA 0's: the bytes of both CTAs
+    uint64_t* empty = full + MX_MAX_STAGES;          // each CTA's
+    uint64_t* acc_full = empty + MX_MAX_STAGES;      // [2] each CTA's
+    uint64_t* acc_empty = acc_full + 2;              // [2] CTA 0's: the storing warps of both
+    uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    uint8_t* ring = smem + 1024;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, side = (int)cluster_rank();
+    const int pair = (int)(blockIdx.x >> 1), n_pairs = (int)(gridDim.x >> 1);
+    const int steps = (a.K + MX_K - 1) / MX_K;
+    const int stage_bytes = mxp_stage_bytes(a.n_tile);
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        for (int s = 0; s < a.stages; s++) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(smem_u32(&acc_full[i]), 1);
+            mbar_init(smem_u32(&acc_empty[i]), 2 * MXP_EPI_WARPS);
+        }
+        mbar_fence_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync_all();   // the other CTA's barriers are initialised
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *tmem_slot;
+    if (a.pdl) pdl_wait_prior();
+
+    if (warp == 0) {
+        if (lane == 0) {
+            int st = 0;
+            uint32_t use = 0;
+            for (int tile = pair; tile < a.n_tiles; tile += n_pairs) {
+                const int row0 = tile / a.tok_tiles * 256 + side * MX_ROWS, tok0 = tile % a.tok_tiles * a.n_tile;
+                const int n_mma = (min(a.n_tile, a.B - tok0) + 31) / 32 * 32;
+                for (int s = 0; s < steps; s++) {
+                    mbar_wait_bounded(smem_u32(&empty[st]), use ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
+                    const uint32_t bar = peer_smem(smem_u32(&full[st]), 0u), at = smem_u32(ring + st * stage_bytes);
+                    const uint32_t sf = at + MX_A_BYTES + (uint32_t)(a.n_tile / 2) * (MX_K / 2);
+                    if (side == 0) mbar_arrive_expect_tx(smem_u32(&full[st]), 2u * (uint32_t)stage_bytes);
+                    tma_load_2d_pair(at, &wmap, s * (MX_K / 2), row0, bar);
+                    tma_load_2d_pair(at + MX_A_BYTES, &xmap, s * (MX_K / 2), tok0 + side * (n_mma / 2), bar);
+                    tma_load_3d_pair(sf, &wsmap, 0, 2 * s, row0 / 128, bar);
+                    tma_load_3d_pair(sf + MX_SFA_BYTES, &xsmap, 0, 2 * s, tok0 / 128, bar);
+                    if (++st == a.stages) { st = 0; use ^= 1u; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (side == 0) {
+            int st = 0, acc = 0;
+            uint32_t use = 0, acc_use = 0;
+            const uint64_t desc0 = umma_desc_sw128(0);
+            const uint32_t sf_cols = tmem_base + (uint32_t)(a.n_acc * mx_acc_cols(a.n_tile)), ring_at = smem_u32(ring);
+            for (int tile = pair; tile < a.n_tiles; tile += n_pairs) {
+                const int tok0 = tile % a.tok_tiles * a.n_tile, n_mma = (min(a.n_tile, a.B - tok0) + 31) / 32 * 32;
+                const uint32_t first_col = (uint32_t)(8 + (tok0 & 127) / 32), d = tmem_base + (uint32_t)(acc * mx_acc_cols(a.n_tile)), idesc = mx_idesc(256, n_mma);
+                mbar_wait_bounded(smem_u32(&acc_empty[acc]), acc_use ^ 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                for (int s = 0; s < steps; s++) {
+                    mbar_wait_bounded(smem_u32(&full[st]), use, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t at = ring_at + (uint32_t)(st * stage_bytes), sf = at + MX_A_BYTES + (uint32_t)(a.n_tile / 2) * (MX_K / 2);
+                    const uint32_t cols = sf_cols + (uint32_t)(st * mx_scale_cols(a.n_tile));
+                    const int n_k = (a.K - s * MX_K + 63) / 64;
+                    if (elect_one()) {
+                        mx_issue_stage<true, GROUPS>(n_k, d, desc0 + (at >> 4), desc0 + ((at + MX_A_BYTES) >> 4), sf, cols, first_col, idesc, s > 0 ? 1u : 0u);
+                        umma_commit<true>(smem_u32(&empty[st]));
+                        if (s == steps - 1) umma_commit<true>(smem_u32(&acc_full[acc]));
+                    }
+                    __syncwarp();
+                    if (++st == a.stages) { st = 0; use ^= 1u; }
+                }
+                if (++acc == a.n_acc) { acc = 0; acc_use ^= 1u; }
+            }
+        }
+    } else {
+        // a warp reads the 16-token chunks 2 i + part of its quarter of the rows
+        const int quad = warp & 3, part = (warp - 2) >> 2;
+        int acc = 0;
+        uint32_t acc_use = 0;
+        T* Y = (T*)a.Y;
+        for (int tile = pair; tile < a.n_tiles; tile += n_pairs) {
+            const int row = tile / a.tok_tiles * 256 + side * MX_ROWS + 32 * quad + lane, tok0 = tile % a.tok_tiles * a.n_tile, n_tok = min(a.n_tile, a.B - tok0);
+            mbar_wait_bounded(smem_u32(&acc_full[acc]), acc_use, abort_flag, a.status, ST_TMEM_TIMEOUT);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t from = tmem_base + ((uint32_t)(32 * quad) << 16) + (uint32_t)(acc * mx_acc_cols(a.n_tile) + 16 * part);
+            uint32_t v[8][16] = {};
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                if (16 * (2 * i + part) < n_tok) tmem_ld16_start(from + (uint32_t)(32 * i), v[i]);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 8; i++) tmem_ld_arrived(v[i]);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                if (side == 0) mbar_arrive(smem_u32(&acc_empty[acc]));
+                else mbar_arrive_peer(peer_smem(smem_u32(&acc_empty[acc]), 0u));
+            }
+            if (++acc == a.n_acc) { acc = 0; acc_use ^= 1u; }
+            if (row < a.M) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const int t = 16 * (2 * i + part) + j;
+                        if (t < n_tok) {
+                            T* y = Y + (size_t)(tok0 + t) * a.ldy + row;
+                            const float f = __uint_as_float(v[i][j]);
+                            *y = from_f32<T>(a.accumulate ? to_f32(*y) + f : f);
+                        }
+                    }
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    cluster_sync_all();   // both CTAs have read their accumulators, and nothing is on its way to the other's barriers
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+    }
+    cluster_sync_all();   // neither CTA leaves before both have given it back
+}
+
 // How a product is cut: tokens in tiles of n_tile (one tile, or several of 128 or 256: a tile starts on a scale tile's border), K in
 // `splits` parts.
 struct MxCut { int n_tile, stages, splits; };
@@ -340,6 +521,32 @@ MxCut mx_cut(int sm_count, int smem_optin, int K, int M, int B) {
     c.stages = std::min(MX_MAX_STAGES, (smem_optin - 1024) / mx_stage_bytes(c.n_tile));
     while (c.splits > 1 && exchange_bytes(c) > c.stages * mx_stage_bytes(c.n_tile)) c.splits--;
     return c;
+}
+
+// Tiles of a product in pairs: 64, 128, 192 or 256 tokens (a tile starts on half a scale tile).
+struct MxPairCut { int n_tile, stages, n_acc, tok_tiles, n_tiles; };
+MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int forced) {
+    MxPairCut best = {};
+    double best_cost = 0.0;
+    const int row_tiles = (M + 255) / 256, steps = (K + MX_K - 1) / MX_K;
+    for (int n = 64; n <= 256; n += 64) {
+        if (forced && n != forced) continue;
+        MxPairCut c;
+        c.n_tile = n;
+        c.tok_tiles = (B + n - 1) / n;
+        c.n_tiles = row_tiles * c.tok_tiles;
+        c.stages = std::min(MX_MAX_STAGES, (smem_optin - 1024) / mxp_stage_bytes(n));
+        c.n_acc = 1;
+        const int two = (512 - 2 * mx_acc_cols(n)) / mx_scale_cols(n);   // stages whose scales fit beside two accumulators
+        if (two >= 4) {
+            c.n_acc = 2;
+            c.stages = std::min(c.stages, two);
+        }
+        const int pairs = sm_count / 2;
+        const double cost = (double)((c.n_tiles + pairs - 1) / pairs) * (steps * 2.0 * n + (c.n_acc == 2 ? 200.0 : 1200.0));
+        if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
+    }
+    return best;
 }
 
 size_t kind_size(int kind) { return kind == Q38B_OUT_F32 ? 4 : 2; }
@@ -372,9 +579,39 @@ bool encode_codes(CUtensorMap* map, const void* codes, long long ld, int K, int 
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// the scale tiles of a matrix as they lie: 512 bytes x K tiles x row tiles
+bool encode_scales(CUtensorMap* map, const void* scales, int K, int rows, int groups) {
+    const cuuint64_t kt = (cuuint64_t)mx_tiles_k(K);
+    const cuuint64_t dims[3] = {MX_TILE / 4, kt, (cuuint64_t)((rows + 127) / 128)};
+    const cuuint64_t strides[2] = {MX_TILE, kt * MX_TILE};
+    const cuuint32_t box[3] = {MX_TILE / 4, 2, (cuuint32_t)groups}, estr[3] = {1, 1, 1};
+    EncodeTiledFn enc = encode_fn();
+    return enc && enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, (void*)scales, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T>
+int pair_as(q38b_ctx* ctx, const MxPairArgs& a, const CUtensorMap& wmap, const CUtensorMap& xmap, const CUtensorMap& wsmap, const CUtensorMap& xsmap, cudaStream_t st) {
+    auto kern = mx_groups(a.n_tile) == 1 ? mx4_pair_kernel<T, 1> : mx4_pair_kernel<T, 2>;
+    const int rc = q38b_ensure_kernel_smem(ctx, (const void*)kern, ctx->smem_optin, false);
+    if (rc != Q38B_OK) return rc;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(2u * (unsigned)std::min(ctx->sm_count / 2, a.n_tiles));
+    cfg.blockDim = dim3(MXP_THREADS);
+    cfg.dynamicSmemBytes = (size_t)(1024 + a.stages * mxp_stage_bytes(a.n_tile));
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.pdl ? 1 : 0;
+    return launch_status(ctx, cudaLaunchKernelEx(&cfg, kern, a, wmap, xmap, wsmap, xsmap));
+}
+
 template <typename T>
 int gemm_as(q38b_ctx* ctx, const MxArgs& a, const CUtensorMap& wmap, const CUtensorMap& xmap, cudaStream_t st) {
-    auto kern = mx4_gemm_kernel<T>;
+    auto kern = mx_groups(a.n_tile) == 1 ? mx4_gemm_kernel<T, 1> : mx4_gemm_kernel<T, 2>;
     const int rc = q38b_ensure_kernel_smem(ctx, (const void*)kern, ctx->smem_optin, false);
     if (rc != Q38B_OK) return rc;
     cudaLaunchConfig_t cfg;
@@ -457,6 +694,18 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
     if (rc != Q38B_OK) return rc;
     if ((uintptr_t)Y % kind_size(y_kind)) return Q38B_ERR_ALIGN;
     DeviceGuard on(ctx);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (ctx->mx4_pairs > 0 || (ctx->mx4_pairs == 0 && B > 128 && M > MX_ROWS)) {
+        const MxPairCut cut = mx_pair_cut(ctx->sm_count, ctx->smem_optin, K, M, B, ctx->mx4_pairs);
+        CUtensorMap wmap, xmap, wsmap, xsmap;
+        if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS) || !encode_codes(&xmap, X, X_ld, K, B, cut.n_tile / 2) || !encode_scales(&wsmap, W_scales, K, M, 1) ||
+            !encode_scales(&xsmap, X_scales, K, B, mx_groups(cut.n_tile)))
+            return Q38B_ERR_ARG;
+        const MxPairArgs a = {Y, ldy, ctx->d_status, K, M, B, accumulate ? 1 : 0, cut.n_tile, cut.stages, cut.n_acc, cut.tok_tiles, cut.n_tiles, behind_quantizer ? 1 : 0};
+        return y_kind == Q38B_OUT_F32 ? pair_as<float>(ctx, a, wmap, xmap, wsmap, xsmap, st)
+             : y_kind == Q38B_OUT_F16 ? pair_as<__half>(ctx, a, wmap, xmap, wsmap, xsmap, st)
+                                      : pair_as<__nv_bfloat16>(ctx, a, wmap, xmap, wsmap, xsmap, st);
+    }
     const MxCut cut = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B);
     if ((B + cut.n_tile - 1) / cut.n_tile > 65535) return Q38B_ERR_UNSUPPORTED;
     CUtensorMap wmap, xmap;
@@ -475,7 +724,6 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
     a.stages = cut.stages;
     a.splits = cut.splits;
     a.pdl = behind_quantizer ? 1 : 0;
-    cudaStream_t st = (cudaStream_t)stream;
     return y_kind == Q38B_OUT_F32 ? gemm_as<float>(ctx, a, wmap, xmap, st) : y_kind == Q38B_OUT_F16 ? gemm_as<__half>(ctx, a, wmap, xmap, st)
                                                                                                     : gemm_as<__nv_bfloat16>(ctx, a, wmap, xmap, st);
 }
@@ -499,6 +747,13 @@ int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_
     if (rc == Q38B_OK) rc = q38b_quantize_mx4(ctx, x, x_kind, x_ld, K, B, codes, K / 2, scales, stream);
     if (rc != Q38B_OK) return rc;
     return gemm_mx4(ctx, W, W_ld, W_scales, K, M, codes, K / 2, scales, B, Y, y_kind, ldy, accumulate, stream, true);
+}
+
+// Test hook (not in the public header): products in pairs of CTAs never (-1), with tiles of `mode` tokens (64, 128, 192, 256), by the rule (0).
+int q38b_debug_set_mx4_pairs(q38b_ctx* ctx, int mode) {
+    if (!ctx || mode < -1 || mode > 256 || (mode > 0 && mode % 64)) return Q38B_ERR_ARG;
+    ctx->mx4_pairs = mode;
+    return Q38B_OK;
 }
 
 }  // extern "C"

@@ -139,6 +139,46 @@ def test_product(ctx, B, M, K):
     ctx.check()
 
 
+@pytest.mark.parametrize("tile", [64, 128, 192, 256])
+@pytest.mark.parametrize("B,M,K", [(1, 1, 32), (5, 130, 96), (200, 257, 352), (65, 300, 2080), (449, 700, 1024), (1030, 256, 288)])
+def test_products_in_pairs_of_every_tile(ctx, B, M, K, tile):
+    """Tiles that start on half a scale tile, a last tile of any length, one K tile in the last stage, more tiles than pairs below."""
+    x, w = rand(B, K, B + K), rand(M, K, M + K + 1)
+    xv, wv = mx_values(x.double().numpy())[0], mx_values(w.double().numpy())[0]
+    W, X = ctx.quantize_mx4(w.cuda()), ctx.quantize_mx4(x.cuda())
+    try:
+        ctx.debug_set_mx4_pairs(tile)
+        for kind in ("f32", "bf16"):
+            whole = torch.full((B + 2, M + 5), 3.0, dtype=DTYPES[kind], device="cuda")
+            out = whole[1:B + 1, 2:M + 2]
+            ctx.gemm_mx4(W, X, out=out)
+            ctx.check()
+            check_product(out, xv, wv, K, kind)
+            keep = out.clone()
+            ctx.gemm_mx4(W, X, out=out, accumulate=True)
+            assert torch.equal(out, (keep.float() + ctx.gemm_mx4(W, X)).to(DTYPES[kind]))
+            out.fill_(3.0)
+            assert (whole == 3.0).all()
+    finally:
+        ctx.debug_set_mx4_pairs(0)
+
+
+@pytest.mark.parametrize("tile", [64, 128, 192, 256])
+def test_a_pair_walks_many_tiles(ctx, tile):
+    B, M, K = 1500, 4000, 544                     # 16 x 6 .. 24 tiles for 74 pairs, whole-number sums
+    g = np.random.default_rng(tile)
+    x, w = (torch.from_numpy(g.choice([0.0, 1, -1, 2, -2, 4, -4], (n, K)).astype(np.float32)).cuda() for n in (B, M))
+    x[:, ::32], w[:, ::32] = 4, -4
+    W, X = ctx.quantize_mx4(w), ctx.quantize_mx4(x)
+    try:
+        ctx.debug_set_mx4_pairs(tile)
+        y = ctx.gemm_mx4(W, X)
+        ctx.check()
+    finally:
+        ctx.debug_set_mx4_pairs(0)
+    assert torch.equal(y.double(), x.double() @ w.double().t())
+
+
 @pytest.mark.parametrize("B,M,K", [(1, 200, 4096), (9, 130, 992), (300, 260, 512)])
 def test_whole_number_products_are_exact(ctx, B, M, K):
     """Elements 0, +-1, +-2, +-4 (and one 4 a block, so that every scale is 1): sums are whole numbers below 2^24, which fp32 holds."""
