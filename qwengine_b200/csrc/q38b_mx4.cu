@@ -352,23 +352,27 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
 // Many tokens: two CTAs (a cluster of two on neighbouring SMs) multiply as one, M = 256: each holds 128 weight rows and half of
 // the tokens' codes, so that a stage costs an SM 16 + 16 KB of codes for 256 x 256 instead of 16 + 32 for 128 x 256.  The pairs
 // stay and walk the tiles (tokens fastest: neighbours read the same weights out of L2), the ring runs on across tiles, and eight warps
-// bring the accumulator to registers and hand it back before they store: the tensor core goes on meanwhile.
+// bring the accumulator to registers and hand it back before they store: the tensor core goes on meanwhile.  Outputs leave through
+// shared memory and TMA stores (a token's 128 rows are one piece of 256 or 512 bytes) where Y's base and row stride are multiples of 16
+// bytes; plain stores, 64 bytes of a token a warp in 16 bits, stood in the way of the loads: 2048 x 17408 x 5120 76 us, 61 without them.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int MXP_THREADS = 320, MXP_EPI_WARPS = 8;
+constexpr int MXP_OUT_BYTES = 4096;   // one TMA store: 16 tokens (8 in 32 bits) x 128 rows; two halves of the storing warps with two buffers each
+constexpr int MXP_FIXED_SMEM = 1024 + 4 * MXP_OUT_BYTES;
 
 struct MxPairArgs {
     void* Y;
     long long ldy;
     int* status;
     int K, M, B, accumulate;
-    int n_tile, stages, n_acc, tok_tiles, n_tiles, pdl;
+    int n_tile, stages, n_acc, tok_tiles, n_tiles, pdl, tma_out;
 };
 __host__ __device__ constexpr int mxp_stage_bytes(int n_tile) { return MX_A_BYTES + n_tile / 2 * (MX_K / 2) + MX_SFA_BYTES * (1 + mx_groups(n_tile)); }
 
 template <typename T, int GROUPS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MXP_THREADS, 1)
 mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wsmap,
-                const __grid_constant__ CUtensorMap xsmap) {
+                const __grid_constant__ CUtensorMap xsmap, const __grid_constant__ CUtensorMap ymap) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* full = (uint64_t*)smem;                // CTA 0's: the bytes of both CTAs
     uint64_t* empty = full + MX_MAX_STAGES;          // each CTA's
@@ -376,7 +380,7 @@ mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, co
     uint64_t* acc_empty = acc_full + 2;              // [2] CTA 0's: the storing warps of both
     uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-    uint8_t* ring = smem + 1024;
+    uint8_t* ring = smem + MXP_FIXED_SMEM;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, side = (int)cluster_rank();
     const int pair = (int)(blockIdx.x >> 1), n_pairs = (int)(gridDim.x >> 1);
     const int steps = (a.K + MX_K - 1) / MX_K;
@@ -456,11 +460,14 @@ mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, co
     } else {
         // a warp reads the 16-token chunks 2 i + part of its quarter of the rows
         const int quad = warp & 3, part = (warp - 2) >> 2;
-        int acc = 0;
+        constexpr int OUT_TOK = MXP_OUT_BYTES / (MX_ROWS * (int)sizeof(T));
+        uint8_t* out = smem + 1024 + part * 2 * MXP_OUT_BYTES;
+        const bool storer = quad == 0 && lane == 0;
+        int acc = 0, buf = 0;
         uint32_t acc_use = 0;
         T* Y = (T*)a.Y;
         for (int tile = pair; tile < a.n_tiles; tile += n_pairs) {
-            const int row = tile / a.tok_tiles * 256 + side * MX_ROWS + 32 * quad + lane, tok0 = tile % a.tok_tiles * a.n_tile, n_tok = min(a.n_tile, a.B - tok0);
+            const int row0 = tile / a.tok_tiles * 256 + side * MX_ROWS, row = row0 + 32 * quad + lane, tok0 = tile % a.tok_tiles * a.n_tile, n_tok = min(a.n_tile, a.B - tok0);
             mbar_wait_bounded(smem_u32(&acc_full[acc]), acc_use, abort_flag, a.status, ST_TMEM_TIMEOUT);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t from = tmem_base + ((uint32_t)(32 * quad) << 16) + (uint32_t)(acc * mx_acc_cols(a.n_tile) + 16 * part);
@@ -478,20 +485,44 @@ mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, co
                 else mbar_arrive_peer(peer_smem(smem_u32(&acc_empty[acc]), 0u));
             }
             if (++acc == a.n_acc) { acc = 0; acc_use ^= 1u; }
-            if (row < a.M) {
+            auto value = [&](int i, int j) {
+                const float f = __uint_as_float(v[i][j]);
+                if (!a.accumulate) return from_f32<T>(f);
+                const int t = 16 * (2 * i + part) + j;
+                return row < a.M && t < n_tok ? from_f32<T>(to_f32(Y[(size_t)(tok0 + t) * a.ldy + row]) + f) : from_f32<T>(f);
+            };
+            // (a store is clipped in whole 16-byte units only: a last tile that ends inside one goes by plain stores)
+            if (a.tma_out && (row0 + MX_ROWS <= a.M || a.M % (16 / (int)sizeof(T)) == 0)) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (16 * (2 * i + part) >= n_tok) break;
+#pragma unroll
+                    for (int h = 0; h < 16 / OUT_TOK; h++) {
+                        if (storer) tma_store_wait_read<1>();
+                        named_bar_sync(1 + part, 128);   // the buffer of two stores before is free
+                        T* to = (T*)(out + buf * MXP_OUT_BYTES) + 32 * quad + lane;
+#pragma unroll
+                        for (int j = 0; j < OUT_TOK; j++) to[j * MX_ROWS] = value(i, OUT_TOK * h + j);
+                        fence_proxy_async();
+                        named_bar_sync(1 + part, 128);
+                        if (storer) {
+                            tma_store_2d(&ymap, smem_u32(out + buf * MXP_OUT_BYTES), row0, tok0 + 16 * (2 * i + part) + OUT_TOK * h);
+                            tma_store_commit();
+                        }
+                        buf ^= 1;
+                    }
+                }
+            } else if (row < a.M) {
 #pragma unroll
                 for (int i = 0; i < 8; i++)
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
                         const int t = 16 * (2 * i + part) + j;
-                        if (t < n_tok) {
-                            T* y = Y + (size_t)(tok0 + t) * a.ldy + row;
-                            const float f = __uint_as_float(v[i][j]);
-                            *y = from_f32<T>(a.accumulate ? to_f32(*y) + f : f);
-                        }
+                        if (t < n_tok) Y[(size_t)(tok0 + t) * a.ldy + row] = value(i, j);
                     }
             }
         }
+        if (storer) tma_store_wait_all();
     }
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -535,7 +566,7 @@ MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int for
         c.n_tile = n;
         c.tok_tiles = (B + n - 1) / n;
         c.n_tiles = row_tiles * c.tok_tiles;
-        c.stages = std::min(MX_MAX_STAGES, (smem_optin - 1024) / mxp_stage_bytes(n));
+        c.stages = std::min(MX_MAX_STAGES, (smem_optin - MXP_FIXED_SMEM) / mxp_stage_bytes(n));
         c.n_acc = 1;
         const int two = (512 - 2 * mx_acc_cols(n)) / mx_scale_cols(n);   // stages whose scales fit beside two accumulators
         if (two >= 4) {
@@ -590,8 +621,22 @@ bool encode_scales(CUtensorMap* map, const void* scales, int K, int rows, int gr
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// the outputs, stored in pieces of MXP_OUT_BYTES; false: they go there by plain stores
+bool encode_out(CUtensorMap* map, void* Y, int kind, long long ldy, int M, int B) {
+    const int size = kind == Q38B_OUT_F32 ? 4 : 2;
+    if (((uintptr_t)Y & 15) || (ldy * size) % 16) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)M, (cuuint64_t)B};
+    const cuuint64_t strides[1] = {(cuuint64_t)ldy * size};
+    const cuuint32_t box[2] = {MX_ROWS, (cuuint32_t)(MXP_OUT_BYTES / (MX_ROWS * size))}, estr[2] = {1, 1};
+    EncodeTiledFn enc = encode_fn();
+    return enc && enc(map, kind == Q38B_OUT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kind == Q38B_OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, Y,
+                      dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T>
-int pair_as(q38b_ctx* ctx, const MxPairArgs& a, const CUtensorMap& wmap, const CUtensorMap& xmap, const CUtensorMap& wsmap, const CUtensorMap& xsmap, cudaStream_t st) {
+int pair_as(q38b_ctx* ctx, const MxPairArgs& a, const CUtensorMap& wmap, const CUtensorMap& xmap, const CUtensorMap& wsmap, const CUtensorMap& xsmap, const CUtensorMap& ymap,
+            cudaStream_t st) {
     auto kern = mx_groups(a.n_tile) == 1 ? mx4_pair_kernel<T, 1> : mx4_pair_kernel<T, 2>;
     const int rc = q38b_ensure_kernel_smem(ctx, (const void*)kern, ctx->smem_optin, false);
     if (rc != Q38B_OK) return rc;
@@ -599,14 +644,14 @@ int pair_as(q38b_ctx* ctx, const MxPairArgs& a, const CUtensorMap& wmap, const C
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(2u * (unsigned)std::min(ctx->sm_count / 2, a.n_tiles));
     cfg.blockDim = dim3(MXP_THREADS);
-    cfg.dynamicSmemBytes = (size_t)(1024 + a.stages * mxp_stage_bytes(a.n_tile));
+    cfg.dynamicSmemBytes = (size_t)(MXP_FIXED_SMEM + a.stages * mxp_stage_bytes(a.n_tile));
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = a.pdl ? 1 : 0;
-    return launch_status(ctx, cudaLaunchKernelEx(&cfg, kern, a, wmap, xmap, wsmap, xsmap));
+    return launch_status(ctx, cudaLaunchKernelEx(&cfg, kern, a, wmap, xmap, wsmap, xsmap, ymap));
 }
 
 template <typename T>
@@ -697,14 +742,16 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
     cudaStream_t st = (cudaStream_t)stream;
     if (ctx->mx4_pairs > 0 || (ctx->mx4_pairs == 0 && B > 128 && M > MX_ROWS)) {
         const MxPairCut cut = mx_pair_cut(ctx->sm_count, ctx->smem_optin, K, M, B, ctx->mx4_pairs);
-        CUtensorMap wmap, xmap, wsmap, xsmap;
+        CUtensorMap wmap, xmap, wsmap, xsmap, ymap;
+        memset(&ymap, 0, sizeof(ymap));
+        const int tma_out = encode_out(&ymap, Y, y_kind, ldy, M, B) ? 1 : 0;
         if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS) || !encode_codes(&xmap, X, X_ld, K, B, cut.n_tile / 2) || !encode_scales(&wsmap, W_scales, K, M, 1) ||
             !encode_scales(&xsmap, X_scales, K, B, mx_groups(cut.n_tile)))
             return Q38B_ERR_ARG;
-        const MxPairArgs a = {Y, ldy, ctx->d_status, K, M, B, accumulate ? 1 : 0, cut.n_tile, cut.stages, cut.n_acc, cut.tok_tiles, cut.n_tiles, behind_quantizer ? 1 : 0};
-        return y_kind == Q38B_OUT_F32 ? pair_as<float>(ctx, a, wmap, xmap, wsmap, xsmap, st)
-             : y_kind == Q38B_OUT_F16 ? pair_as<__half>(ctx, a, wmap, xmap, wsmap, xsmap, st)
-                                      : pair_as<__nv_bfloat16>(ctx, a, wmap, xmap, wsmap, xsmap, st);
+        const MxPairArgs a = {Y, ldy, ctx->d_status, K, M, B, accumulate ? 1 : 0, cut.n_tile, cut.stages, cut.n_acc, cut.tok_tiles, cut.n_tiles, behind_quantizer ? 1 : 0, tma_out};
+        return y_kind == Q38B_OUT_F32 ? pair_as<float>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st)
+             : y_kind == Q38B_OUT_F16 ? pair_as<__half>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st)
+                                      : pair_as<__nv_bfloat16>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st);
     }
     const MxCut cut = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B);
     if ((B + cut.n_tile - 1) / cut.n_tile > 65535) return Q38B_ERR_UNSUPPORTED;

@@ -140,7 +140,7 @@ def test_product(ctx, B, M, K):
 
 
 @pytest.mark.parametrize("tile", [64, 128, 192, 256])
-@pytest.mark.parametrize("B,M,K", [(1, 1, 32), (5, 130, 96), (200, 257, 352), (65, 300, 2080), (449, 700, 1024), (1030, 256, 288)])
+@pytest.mark.parametrize("B,M,K", [(1, 1, 32), (5, 130, 96), (200, 257, 352), (65, 300, 2080), (449, 700, 1024), (130, 136, 64), (1030, 256, 288)])
 def test_products_in_pairs_of_every_tile(ctx, B, M, K, tile):
     """Tiles that start on half a scale tile, a last tile of any length, one K tile in the last stage, more tiles than pairs below."""
     x, w = rand(B, K, B + K), rand(M, K, M + K + 1)
@@ -148,9 +148,9 @@ def test_products_in_pairs_of_every_tile(ctx, B, M, K, tile):
     W, X = ctx.quantize_mx4(w.cuda()), ctx.quantize_mx4(x.cuda())
     try:
         ctx.debug_set_mx4_pairs(tile)
-        for kind in ("f32", "bf16"):
-            whole = torch.full((B + 2, M + 5), 3.0, dtype=DTYPES[kind], device="cuda")
-            out = whole[1:B + 1, 2:M + 2]
+        for kind, left, wide in (("f32", 2, M + 5), ("bf16", 2, M + 5), ("f32", 4, (M + 15) // 8 * 8), ("bf16", 8, (M + 23) // 8 * 8)):   # plain stores, TMA stores
+            whole = torch.full((B + 2, wide), 3.0, dtype=DTYPES[kind], device="cuda")
+            out = whole[1:B + 1, left:M + left]
             ctx.gemm_mx4(W, X, out=out)
             ctx.check()
             check_product(out, xv, wv, K, kind)
