@@ -76,10 +76,16 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
 // ---------------------------------------------------------------------------------------------------------------
 // Logits.  count_v: times token v occurs among the generated tokens of the row, seen_v: in prompt or generated ones.
 //   seen: l = l > 0 ? l / rep : l * rep;  l -= freq * count_v;  count_v > 0: l -= pres;  l += bias_v;  mask bit clear: l = -inf
-// A CTA owns LG_CHUNK logits of a row, counts the row's tokens that fall into them in shared memory (whole numbers, so the
-// order of the atomics does not matter), notes the last bias entry of each, and passes over its logits once.
+// A CTA owns CHUNK logits of a row.  They pass through the mask first (neighbours in a warp, so any alignment and stride will do; in place
+// nothing passes through, only masked logits are written).  Then it counts the row's tokens that fall among them in shared memory (whole
+// numbers, so the order of the atomics does not matter) and mends the logits that occur: few, packed 32 at a time so that no warp computes
+// for one lane.  Biases come last, the last entry of each token found in the same shared words.
+// Every CTA of a row reads the whole text, which costs as much as the logits do once texts are long; so a CTA takes as many logits as leaves
+// three to an SM, and an id costs four instructions (difference, comparison, address, predicated atomic).  Clusters that share a text by
+// atomics in each other's memory were slower at every size (128 rows of 248320 with 20000-token texts: 111 us in twos, 161 in eights, 101
+// alone, all with 8192 logits a CTA): their CTAs stream and count in step.  So 92 us = 2.9 TB/s; without texts 63 us.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int LG_CHUNK = 4096, LG_THREADS = 512;
+constexpr int LG_THREADS = 512, LG_WARPS = LG_THREADS / 32;
 constexpr uint32_t LG_PROMPT = 0x80000000u;   // seen in the prompt; the other bits count generated tokens
 
 struct LogitsArgs {
@@ -90,51 +96,158 @@ struct LogitsArgs {
     int n, index_offset;
 };
 
-__global__ void __launch_bounds__(LG_THREADS) logits_kernel(const LogitsArgs a) {
-    __shared__ uint32_t seen[LG_CHUNK], last[LG_CHUNK];
-    const int row = blockIdx.y, c0 = blockIdx.x * LG_CHUNK, n = min(LG_CHUNK, a.n - c0), first = a.index_offset + c0;
-    const bool counts = a.r.history && a.r.penalties, biases = a.r.bias_ids != nullptr;
-    for (int i = threadIdx.x; i < LG_CHUNK; i += LG_THREADS) {
-        seen[i] = 0u;
-        last[i] = 0u;
+// Counts those of ids[0, len) that are among the n logits from `first` on: in the prompt (a flag) or generated (a count).
+// (Unsigned: ids below the first and negative ones fall out with those behind the last.)
+template <bool GENERATED>
+__device__ __forceinline__ void count_id(uint32_t words, int id, uint32_t first, uint32_t n) {
+    const uint32_t at = (uint32_t)id - first;
+    if constexpr (GENERATED)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %0, %1;\n\t@p red.shared.add.u32 [%2], 1;\n\t}" ::"r"(at), "r"(n), "r"(words + 4u * at) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %0, %1;\n\t@p red.shared.or.b32 [%2], %3;\n\t}" ::"r"(at), "r"(n), "r"(words + 4u * at), "r"(LG_PROMPT) : "memory");
+}
+template <bool GENERATED>
+__device__ __forceinline__ void count_ids(uint32_t words, const int* ids, long long len, uint32_t first, uint32_t n) {
+    if (len <= 0) return;
+    const int tid = threadIdx.x;
+    // four ids a load, two loads of a thread ahead of their atomics; the ends that are no whole 16 bytes by themselves
+    const int head = (int)min(len, (long long)((16 - ((uintptr_t)ids & 15)) & 15) / 4);
+    const long long quads = (len - head) / 4;
+    const int4* q = (const int4*)(ids + head) + tid;
+    long long k = tid;
+    for (; k + LG_THREADS < quads; k += 2 * LG_THREADS, q += 2 * LG_THREADS) {
+        const int4 a = __ldg(q), b = __ldg(q + LG_THREADS);
+        count_id<GENERATED>(words, a.x, first, n);
+        count_id<GENERATED>(words, a.y, first, n);
+        count_id<GENERATED>(words, a.z, first, n);
+        count_id<GENERATED>(words, a.w, first, n);
+        count_id<GENERATED>(words, b.x, first, n);
+        count_id<GENERATED>(words, b.y, first, n);
+        count_id<GENERATED>(words, b.z, first, n);
+        count_id<GENERATED>(words, b.w, first, n);
     }
-    __syncthreads();
+    if (k < quads) {
+        const int4 a = __ldg(q);
+        count_id<GENERATED>(words, a.x, first, n);
+        count_id<GENERATED>(words, a.y, first, n);
+        count_id<GENERATED>(words, a.z, first, n);
+        count_id<GENERATED>(words, a.w, first, n);
+    }
+    if (tid < head) count_id<GENERATED>(words, ids[tid], first, n);
+    if (tid < 4 && head + 4 * quads + tid < len) count_id<GENERATED>(words, ids[head + 4 * quads + tid], first, n);
+}
+
+template <int CHUNK>
+__global__ void __launch_bounds__(LG_THREADS, 3) logits_kernel(const LogitsArgs a) {
+    constexpr int UN = CHUNK / LG_THREADS < 16 ? CHUNK / LG_THREADS : 16;   // logits of a thread on their way at a time
+    extern __shared__ __align__(16) uint32_t seen[];                        // [CHUNK], where there are texts or biases
+    __shared__ uint16_t packed[LG_WARPS][64];
+    const int row = blockIdx.y, c0 = blockIdx.x * CHUNK, n = min(CHUNK, a.n - c0), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t first = (uint32_t)(a.index_offset + c0);
+    const bool counts = a.r.history != nullptr, in_place = a.x == a.y;
+    const float* x = a.x + row * a.x_ld + c0;
+    float* y = a.y + row * a.y_ld + c0;
+    // what the later parts need, on its way before the logits: the text's and the biases' ends, a thread's first bias
+    long long text = 0, text_len = 0, prompt = 0, bias0 = 0, n_bias = 0;
     if (counts) {
-        const long long b = a.r.history_begin[row], e = a.r.history_begin[row + 1], made = b + (a.r.prompt_len ? a.r.prompt_len[row] : 0);
-        for (long long i = b + threadIdx.x; i < e; i += LG_THREADS) {
-            const unsigned at = (unsigned)a.r.history[i] - (unsigned)first;
-            if (a.r.history[i] >= 0 && at < (unsigned)n) {
-                if (i < made) atomicOr(&seen[at], LG_PROMPT);
-                else atomicAdd(&seen[at], 1u);
+        text = a.r.history_begin[row];
+        text_len = a.r.history_begin[row + 1] - text;
+        prompt = a.r.prompt_len ? min(max((long long)a.r.prompt_len[row], 0LL), max(text_len, 0LL)) : 0;
+    }
+    if (a.r.bias_ids) {
+        bias0 = a.r.bias_begin[row];
+        n_bias = a.r.bias_begin[row + 1] - bias0;
+    }
+    const int m = !a.r.masks ? -1 : a.r.mask_of_row ? a.r.mask_of_row[row] : row;
+    const uint32_t* mask = a.r.masks + (m >= 0 ? m * a.r.mask_ld : 0);
+    const uint32_t mask_end = (uint32_t)(a.index_offset + a.n - 1) >> 5;
+    auto allowed = [&](uint32_t at) { return m < 0 || (mask[(first + at) >> 5] >> ((first + at) & 31u) & 1u); };
+    if (!in_place || m >= 0) {
+#pragma unroll 1
+        for (int c = 0; c < CHUNK && c < n; c += LG_THREADS * UN) {
+            float v[UN];
+            if (!in_place) {
+#pragma unroll
+                for (int u = 0; u < UN; u++) v[u] = c + LG_THREADS * u + tid < n ? x[c + LG_THREADS * u + tid] : 0.0f;
+            }
+            // the mask bits of the warp's logits: lane u has those of its 32 neighbours c + LG_THREADS * u + 32 * warp ..
+            uint32_t bits = 0xFFFFFFFFu;
+            if (m >= 0 && lane < UN && c + LG_THREADS * lane + 32 * warp < n) {
+                const uint32_t at = first + (uint32_t)(c + LG_THREADS * lane + 32 * warp);
+                bits = __funnelshift_r(mask[at >> 5], mask[min((at >> 5) + 1u, mask_end)], at & 31u);
+            }
+#pragma unroll
+            for (int u = 0; u < UN; u++) {
+                const int i = c + LG_THREADS * u + tid;
+                const bool keep = __shfl_sync(0xffffffffu, bits, u) >> lane & 1u;
+                if (i < n) {
+                    if (!keep) y[i] = __int_as_float(0xFF800000);
+                    else if (!in_place) y[i] = v[u];
+                }
             }
         }
     }
-    long long bias0 = 0;
-    if (biases) {
-        bias0 = a.r.bias_begin[row];
-        const long long e = a.r.bias_begin[row + 1];
-        for (long long i = bias0 + threadIdx.x; i < e; i += LG_THREADS) {
-            const unsigned at = (unsigned)a.r.bias_ids[i] - (unsigned)first;
-            if (a.r.bias_ids[i] >= 0 && at < (unsigned)n) atomicMax(&last[at], (uint32_t)(i - bias0) + 1u);
+    if (!counts && !a.r.bias_ids) return;
+    uint32_t bias_at = 0xFFFFFFFFu;
+    if (tid < n_bias) bias_at = (uint32_t)a.r.bias_ids[bias0 + tid] - first;
+    const int* ids = a.r.bias_ids + bias0;
+    auto each = [&](auto&& f) {   // f(entry, place) for this thread's biases among the block's logits
+        if (bias_at < (uint32_t)n) f((uint32_t)tid, bias_at);
+        for (long long j = tid + LG_THREADS; j < n_bias; j += LG_THREADS) {
+            const uint32_t at = (uint32_t)ids[j] - first;
+            if (at < (uint32_t)n) f((uint32_t)j, at);
         }
+    };
+    bool any = false;
+    each([&](uint32_t, uint32_t) { any = true; });
+    if (counts)
+        for (int i = 4 * tid; i < CHUNK; i += 4 * LG_THREADS) *(uint4*)(seen + i) = make_uint4(0, 0, 0, 0);
+    any = __syncthreads_or(any);   // (and every logit is through)
+    if (counts) {
+        count_ids<false>(smem_u32(seen), a.r.history + text, prompt, first, (uint32_t)n);
+        count_ids<true>(smem_u32(seen), a.r.history + text + prompt, text_len - prompt, first, (uint32_t)n);
+        const float repetition = a.r.penalties[3 * row], frequency = a.r.penalties[3 * row + 1], presence = a.r.penalties[3 * row + 2];
+        __syncthreads();
+        // a warp's share of the words, 32 at a time; places of those that count are packed and mended 32 at a time
+        uint16_t* mine = packed[warp];
+        int waiting = 0;
+        auto mend = [&](int k) {   // the warp's lanes below k
+            if (lane < k) {
+                const uint32_t at = mine[lane], s = seen[at], times = s & ~LG_PROMPT;
+                if (allowed(at)) {
+                    float l = y[at];
+                    l = l > 0.0f ? __fdiv_rn(l, repetition) : l * repetition;
+                    if (times) l = l - frequency * (float)times - presence;
+                    y[at] = l;
+                }
+            }
+        };
+        for (int i = 32 * warp; i < n; i += LG_THREADS) {
+            const uint32_t hit = __ballot_sync(0xffffffffu, seen[i + lane] != 0u);
+            if (!hit) continue;
+            if (hit >> lane & 1u) mine[waiting + __popc(hit & ((1u << lane) - 1u))] = (uint16_t)(i + lane);
+            waiting += __popc(hit);
+            __syncwarp();
+            if (waiting >= 32) {
+                mend(32);
+                const uint16_t rest = lane < waiting - 32 ? mine[32 + lane] : (uint16_t)0;
+                __syncwarp();
+                mine[lane] = rest;
+                waiting -= 32;
+                __syncwarp();
+            }
+        }
+        mend(waiting);
     }
+    if (!any) return;
     __syncthreads();
-    const float rep = counts ? a.r.penalties[3 * row] : 1.0f, freq = counts ? a.r.penalties[3 * row + 1] : 0.0f, pres = counts ? a.r.penalties[3 * row + 2] : 0.0f;
-    const int m = !a.r.masks ? -1 : a.r.mask_of_row ? a.r.mask_of_row[row] : row;
-    const uint32_t* mask = m >= 0 ? a.r.masks + m * a.r.mask_ld : nullptr;
-    for (int i = threadIdx.x; i < n; i += LG_THREADS) {
-        float v = a.x[row * a.x_ld + c0 + i];
-        const uint32_t s = seen[i];
-        if (s) {
-            v = v > 0.0f ? __fdiv_rn(v, rep) : v * rep;
-            const uint32_t count = s & ~LG_PROMPT;
-            if (count) v = v - freq * (float)count - pres;
-        }
-        if (last[i]) v += a.r.bias_values[bias0 + last[i] - 1];
-        const int id = first + i;
-        if (mask && !((mask[id >> 5] >> (id & 31)) & 1u)) v = __int_as_float(0xFF800000);
-        a.y[row * a.y_ld + c0 + i] = v;
-    }
+    each([&](uint32_t, uint32_t at) { seen[at] = 0u; });
+    __syncthreads();
+    each([&](uint32_t j, uint32_t at) { atomicMax(&seen[at], j + 1u); });
+    __syncthreads();
+    each([&](uint32_t j, uint32_t at) {
+        if (seen[at] == j + 1u && allowed(at)) y[at] += a.r.bias_values[bias0 + j];
+    });
 }
 
 bool known_kind(int kind) { return kind == Q38B_OUT_F32 || kind == Q38B_OUT_F16 || kind == Q38B_OUT_BF16; }
@@ -149,6 +262,15 @@ int heads_as(q38b_ctx* ctx, const HeadsArgs& a, cudaStream_t st) {
 template <typename Tin>
 int heads_from(q38b_ctx* ctx, const HeadsArgs& a, int out_kind, cudaStream_t st) {
     return out_kind == Q38B_OUT_F32 ? heads_as<Tin, float>(ctx, a, st) : out_kind == Q38B_OUT_F16 ? heads_as<Tin, __half>(ctx, a, st) : heads_as<Tin, __nv_bfloat16>(ctx, a, st);
+}
+
+template <int CHUNK>
+int logits_as(q38b_ctx* ctx, const LogitsArgs& a, int n_rows, cudaStream_t st) {
+    const int rc = q38b_ensure_kernel_smem(ctx, (const void*)logits_kernel<CHUNK>, CHUNK * 4, false);
+    if (rc != Q38B_OK) return rc;
+    const size_t smem = a.r.history || a.r.bias_ids ? CHUNK * sizeof(uint32_t) : 0;
+    logits_kernel<CHUNK><<<dim3((unsigned)((a.n + CHUNK - 1) / CHUNK), (unsigned)n_rows), LG_THREADS, smem, st>>>(a);
+    return launch_status(ctx, cudaSuccess);
 }
 
 }  // namespace
@@ -208,8 +330,11 @@ int q38b_adjust_logits(q38b_ctx* ctx, const float* x, long long x_ld, int n, int
     a.n = n;
     a.index_offset = index_offset;
     DeviceGuard on(ctx);
-    logits_kernel<<<dim3((unsigned)((n + LG_CHUNK - 1) / LG_CHUNK), (unsigned)n_rows), LG_THREADS, 0, (cudaStream_t)stream>>>(a);
-    return launch_status(ctx, cudaSuccess);
+    cudaStream_t st = (cudaStream_t)stream;
+    // as many logits a CTA as still leaves three CTAs to every SM, or the fewest
+    const auto fills = [&](int chunk) { return (long long)n_rows * ((n + chunk - 1) / chunk) >= 3 * ctx->sm_count; };
+    return fills(16384) ? logits_as<16384>(ctx, a, n_rows, st) : fills(8192) ? logits_as<8192>(ctx, a, n_rows, st)
+         : fills(4096)  ? logits_as<4096>(ctx, a, n_rows, st) : logits_as<2048>(ctx, a, n_rows, st);
 }
 
 }  // extern "C"
