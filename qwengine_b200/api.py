@@ -6,6 +6,7 @@ src/cuda/prefill.cuh:17-28): weights are uint8 tensors holding GGUF blocks row b
 """
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -133,17 +134,11 @@ def _stream():
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
-class _Heads(C.Structure):
-    """q38b_heads: the query or the key heads of a chunk of rows."""
-    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_row", C.c_longlong), ("src_head", C.c_longlong), ("dst_row", C.c_longlong),
-                ("dst_head", C.c_longlong), ("weight", C.c_void_p), ("n_heads", C.c_int)]
-
-
-class _LogitRules(C.Structure):
-    """q38b_logit_rules: what shapes the logits before the top-k."""
-    _fields_ = [("penalties", C.c_void_p), ("history", C.c_void_p), ("history_begin", C.c_void_p), ("prompt_len", C.c_void_p),
-                ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p), ("bias_begin", C.c_void_p), ("masks", C.c_void_p),
-                ("mask_ld", C.c_longlong), ("mask_of_row", C.c_void_p)]
+# q38b_heads and q38b_logit_rules as bytes: a call costs a host microsecond less than with ctypes structures
+_pack_heads = struct.Struct("@PPqqqqPi4x").pack      # src, dst, src_row, src_head, dst_row, dst_head, weight, n_heads
+_pack_rules = struct.Struct("@PPPPPPPPqP").pack      # penalties .. bias_begin, masks, mask_ld, mask_of_row
+_empty = torch.empty_strided
+_current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
 def _need(ok, what):
@@ -154,15 +149,17 @@ def _need(ok, what):
 class Mx4:
     """A matrix in microscaled 4-bit floating point: codes uint8 [rows, K / 2] (two elements a byte), scales uint8 in the library's tiles
     (Context.quantize_mx4 makes both, Context.pack_mx4 takes another producer's)."""
+    __slots__ = ("codes", "scales", "rows", "K", "ld")
 
     def __init__(self, codes, scales):
-        _need(codes.dtype == scales.dtype == torch.uint8 and codes.dim() == 2 and codes.stride(1) == 1, "Mx4: uint8 codes [rows, K / 2] with packed rows, uint8 scales")
         rows, half = codes.shape
+        ld, one = codes.stride()
+        _need(codes.dtype == scales.dtype == torch.uint8 and one == 1, "Mx4: uint8 codes [rows, K / 2] with packed rows, uint8 scales")
         _need(rows >= 1 and half >= 16 and half % 16 == 0, "Mx4: K a multiple of 32, at least one row")
         _need(scales.is_contiguous() and scales.numel() == ((rows + 127) // 128) * ((half + 63) // 64) * 512, "Mx4: contiguous tiles of 128 rows x 4 blocks of scales")
-        _need(codes.device == scales.device, "Mx4: codes and scales on one device")
+        _need(codes.get_device() == scales.get_device(), "Mx4: codes and scales on one device")
         self.codes, self.scales, self.rows, self.K = codes, scales, rows, 2 * half
-        self.ld = codes.stride(0) if rows > 1 else half   # (the stride of a single row says nothing)
+        self.ld = ld if rows > 1 else half   # (the stride of a single row says nothing)
 
 
 class Context:
@@ -318,130 +315,179 @@ class Context:
         return y
 
     # ---- the steps of a token between its products --------------------------------------------
-    def _mine(self, what, *tensors):
-        for t in tensors:
-            if t is not None and t.device != self.device:
-                raise ValueError(f"{what}: tensors on {self.device}, the context's device")
-
     def _stream(self):
-        return torch._C._cuda_getCurrentRawStream(self.device.index)
+        """The current stream of the context's device (whatever device is current)."""
+        return _current_stream(self.device.index)
 
     def qk_norm_rope(self, q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, adjacent=False, scale=1.0, kind=None, q_out=None, k_out=None):
         """q [rows, heads, D], k [rows, heads, D] or None (fp32, fp16 or bf16, any row and head strides): RMSNorm of each head, rotation of its first
         2 * len(inv_freq) elements by positions (int32 [rows]) times inv_freq (float64); weights fp32 [D].  kind: OUT_* of the results (that of
         the inputs by default); returns (q_out, k_out), which may be q and k themselves."""
         rows, _, D = q.shape
-        kind = _OUT_KINDS.get(q.dtype) if kind is None else kind
-        out_dtype = _OUT_DTYPES[kind] if q.dtype in _OUT_KINDS else None
-        _need(out_dtype is not None, "qk_norm_rope: fp32, fp16 or bf16 heads")
-        rot = 0 if inv_freq is None else 2 * inv_freq.shape[0]
-        if rot:
-            _need(positions is not None and positions.dtype == torch.int32 and positions.shape == (rows,) and (rows == 1 or positions.stride(0) == 1), "qk_norm_rope: int32 positions, one per row")
+        dtype = q.dtype
+        in_kind = _OUT_KINDS.get(dtype)
+        _need(in_kind is not None, "qk_norm_rope: fp32, fp16 or bf16 heads")
+        if kind is None:
+            kind = in_kind
+        out_dtype, dev, rot, pos_ptr, freq_ptr = _OUT_DTYPES[kind], self.device.index, 0, None, None
+        if inv_freq is not None and inv_freq.numel():
+            rot = 2 * inv_freq.shape[0]
+            _need(positions is not None and positions.dtype == torch.int32 and positions.shape == (rows,) and positions.is_contiguous(), "qk_norm_rope: int32 positions, one per row")
             _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and rot <= D, "qk_norm_rope: float64 inv_freq, at most D / 2")
-            self._mine("qk_norm_rope", positions, inv_freq)
+            _need(positions.get_device() == dev and inv_freq.get_device() == dev, "qk_norm_rope: tensors on the context's device")
+            pos_ptr, freq_ptr = positions.data_ptr(), inv_freq.data_ptr()
         parts, outs = [], []
         for x, w, out in ((q, q_weight, q_out), (k, k_weight, k_out)):
             if x is None:
                 parts.append(None)
                 outs.append(None)
                 continue
-            _need(x.dim() == 3 and x.shape[0] == rows and x.shape[2] == D and x.dtype == q.dtype and (D == 1 or x.stride(2) == 1), "qk_norm_rope: heads [rows, heads, D] of one type, elements side by side")
-            _need(w is None or (w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous()), "qk_norm_rope: fp32 weights [D]")
+            n, heads, d = x.shape
+            row, head, one = x.stride()
+            _need(n == rows and d == D and x.dtype == dtype and (one == 1 or D == 1), "qk_norm_rope: heads [rows, heads, D] of one type, elements side by side")
+            _need(x.get_device() == dev, "qk_norm_rope: tensors on the context's device")
             if out is None:
-                out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-            _need(out.shape == x.shape and out.dtype == out_dtype and (D == 1 or out.stride(2) == 1), "qk_norm_rope: outputs shaped like the heads")
-            self._mine("qk_norm_rope", x, w, out)
-            parts.append(_Heads(x.data_ptr(), out.data_ptr(), x.stride(0), x.stride(1), out.stride(0), out.stride(1), None if w is None else w.data_ptr(), x.shape[1]))
+                out_row, out_head = heads * D, D
+                out = _empty((rows, heads, D), (out_row, D, 1), dtype=out_dtype, device=self.device)
+            else:
+                out_row, out_head, one = out.stride()
+                _need(out.shape == x.shape and out.dtype == out_dtype and (one == 1 or D == 1), "qk_norm_rope: outputs shaped like the heads")
+                _need(out.get_device() == dev, "qk_norm_rope: tensors on the context's device")
+            w_ptr = 0
+            if w is not None:
+                _need(w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous() and w.get_device() == dev, "qk_norm_rope: fp32 weights [D] on the context's device")
+                w_ptr = w.data_ptr()
+            parts.append(_pack_heads(x.data_ptr(), out.data_ptr(), row, head, out_row, out_head, w_ptr, heads))
             outs.append(out)
-        self._rc(self.lib.q38b_qk_norm_rope(self.h, C.byref(parts[0]), None if k is None else C.byref(parts[1]), D, rot, int(bool(adjacent)), eps, scale,
-                                            positions.data_ptr() if rot else None, inv_freq.data_ptr() if rot else None, _OUT_KINDS[q.dtype], kind, rows,
-                                            self._stream()), "q38b_qk_norm_rope")
+        rc = self.lib.q38b_qk_norm_rope(self.h, parts[0], parts[1], D, rot, 1 if adjacent else 0, eps, scale, pos_ptr, freq_ptr, in_kind, kind, rows, self._stream())
+        if rc:
+            self._rc(rc, "q38b_qk_norm_rope")
         return outs[0], outs[1]
+
+    def _list(self, what, t, dtype, shape=None):
+        """Address of an optional contiguous tensor of the context's device (0: none, or nothing in it)."""
+        if t is None:
+            return 0
+        _need(t.dtype == dtype and t.is_contiguous() and t.get_device() == self.device.index and (shape is None or t.shape == shape), what)
+        return t.data_ptr()
 
     def logit_rules(self, rows, n, penalties=None, history=None, history_begin=None, prompt_len=None, bias_ids=None, bias_values=None, bias_begin=None,
                     masks=None, mask_of_row=None, index_offset=0):
-        """q38b_logit_rules of checked device tensors: penalties fp32 [rows, 3] (repetition, frequency, presence), history int32 with int64 begins
-        [rows + 1] and int32 prompt lengths [rows]; bias_ids int32, bias_values fp32, int64 begins; masks int32 [*, words] of allowed-token
-        bits, mask_of_row int32 [rows]."""
-        flat = lambda t, dtype, *shape: t is None or (t.dtype == dtype and t.is_contiguous() and (not shape or t.shape == shape))   # noqa: E731
-        f32, i32, i64 = torch.float32, torch.int32, torch.int64
-        _need(flat(penalties, f32, rows, 3) and flat(history, i32) and flat(history_begin, i64, rows + 1) and flat(prompt_len, i32, rows), "adjust_logits: penalties, history")
-        _need(flat(bias_ids, i32) and flat(bias_values, f32) and flat(bias_begin, i64, rows + 1), "adjust_logits: biases")
-        _need(bias_ids is None or (bias_values is not None and bias_values.numel() == bias_ids.numel()), "adjust_logits: one value per bias")
-        _need(masks is None or (masks.dtype == i32 and masks.dim() == 2 and masks.stride(1) == 1 and masks.shape[1] * 32 >= index_offset + n and
-                                (masks.shape[0] >= rows or mask_of_row is not None)), "adjust_logits: masks int32 [masks, words], a bit for each token")
-        _need(flat(mask_of_row, i32, rows), "adjust_logits: mask_of_row int32 [rows]")
-        self._mine("adjust_logits", penalties, history, history_begin, prompt_len, bias_ids, bias_values, bias_begin, masks, mask_of_row)
-        ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
-        # (an empty list has no address: no history then, which changes nothing)
-        gone = history is not None and history.numel() == 0
-        none = bias_ids is not None and bias_ids.numel() == 0
-        return _LogitRules(None if gone else ptr(penalties), None if gone else ptr(history), None if gone else ptr(history_begin), None if gone else ptr(prompt_len),
-                           None if none else ptr(bias_ids), None if none else ptr(bias_values), None if none else ptr(bias_begin), ptr(masks),
-                           0 if masks is None else masks.stride(0) if masks.shape[0] > 1 else masks.shape[1], ptr(mask_of_row))
+        """The bytes of a q38b_logit_rules of checked device tensors: penalties fp32 [rows, 3] (repetition, frequency, presence), history int32 with int64
+        begins [rows + 1] and int32 prompt lengths [rows]; bias_ids int32, bias_values fp32, int64 begins; masks int32 [*, words] of
+        allowed-token bits, mask_of_row int32 [rows]."""
+        f32, i32, i64, address = torch.float32, torch.int32, torch.int64, self._list
+        p = h = hb = pl = bi = bv = bb = mk = mr = ld = 0
+        if penalties is not None or history is not None or history_begin is not None or prompt_len is not None:
+            p = address("adjust_logits: fp32 penalties [rows, 3]", penalties, f32, (rows, 3))
+            h = address("adjust_logits: int32 history", history, i32)
+            hb = address("adjust_logits: int64 history_begin [rows + 1]", history_begin, i64, (rows + 1,))
+            pl = address("adjust_logits: int32 prompt_len [rows]", prompt_len, i32, (rows,))
+            if history is not None and history.numel() == 0:
+                p = h = hb = pl = 0   # no token at all: nothing to penalise
+        if bias_ids is not None or bias_values is not None or bias_begin is not None:
+            bi = address("adjust_logits: int32 bias_ids", bias_ids, i32)
+            bv = address("adjust_logits: fp32 bias_values", bias_values, f32)
+            bb = address("adjust_logits: int64 bias_begin [rows + 1]", bias_begin, i64, (rows + 1,))
+            if bias_ids is not None:
+                _need(bias_values is not None and bias_values.numel() == bias_ids.numel(), "adjust_logits: one value per bias")
+                if bias_ids.numel() == 0:
+                    bi = bv = bb = 0
+        if masks is not None:
+            count, words = masks.shape
+            ld, one = masks.stride()
+            _need(masks.dtype == i32 and one == 1 and masks.get_device() == self.device.index and words * 32 >= index_offset + n and
+                  (count >= rows or mask_of_row is not None), "adjust_logits: masks int32 [masks, words], a bit for each token")
+            mk, ld = masks.data_ptr(), ld if count > 1 else words
+        if mask_of_row is not None:
+            mr = address("adjust_logits: mask_of_row int32 [rows]", mask_of_row, i32, (rows,))
+        return _pack_rules(p, h, hb, pl, bi, bv, bb, mk, ld, mr)
 
     def adjust_logits(self, logits, out=None, index_offset=0, **rules):
         """logits fp32 [rows, n] (any row stride) -> penalised, biased, masked logits (`out`, which may be `logits`); the rules are those of
         logit_rules.  Token v is column v - index_offset."""
-        _need(logits.dtype == torch.float32 and logits.dim() == 2 and (logits.shape[1] == 1 or logits.stride(1) == 1), "adjust_logits: fp32 logits [rows, n]")
         rows, n = logits.shape
+        ld, one = logits.stride()
+        dev = self.device.index
+        _need(logits.dtype == torch.float32 and (one == 1 or n == 1) and logits.get_device() == dev, "adjust_logits: fp32 logits [rows, n] on the context's device")
         r = self.logit_rules(rows, n, index_offset=index_offset, **rules)
         if out is None:
-            out = torch.empty((rows, n), dtype=torch.float32, device=logits.device)
-        _need(out.dtype == torch.float32 and out.shape == logits.shape and (n == 1 or out.stride(1) == 1), "adjust_logits: fp32 out of the logits' shape")
-        self._mine("adjust_logits", logits, out)
-        self._rc(self.lib.q38b_adjust_logits(self.h, logits.data_ptr(), logits.stride(0), n, rows, index_offset, C.byref(r), out.data_ptr(), out.stride(0),
-                                             self._stream()), "q38b_adjust_logits")
+            out_ld = n
+            out = _empty((rows, n), (n, 1), dtype=torch.float32, device=self.device)
+        else:
+            out_ld, one = out.stride()
+            _need(out.dtype == torch.float32 and out.shape == logits.shape and (one == 1 or n == 1) and out.get_device() == dev, "adjust_logits: fp32 out of the logits' shape")
+        rc = self.lib.q38b_adjust_logits(self.h, logits.data_ptr(), ld, n, rows, index_offset, r, out.data_ptr(), out_ld, self._stream())
+        if rc:
+            self._rc(rc, "q38b_adjust_logits")
         return out
 
     # ---- microscaled 4-bit floating point -----------------------------------------------------
     def quantize_mx4(self, x):
         """x [rows, K] (fp32, fp16 or bf16, any row stride) -> Mx4."""
-        _need(x.dtype in _OUT_KINDS and x.dim() == 2 and x.stride(1) == 1, "quantize_mx4: fp32, fp16 or bf16 [rows, K]")
         rows, K = x.shape
-        self._mine("quantize_mx4", x)
-        codes = torch.empty((rows, K // 2), dtype=torch.uint8, device=x.device)
-        scales = torch.empty(self.lib.q38b_mx4_scale_bytes(K, rows), dtype=torch.uint8, device=x.device)
-        self._rc(self.lib.q38b_quantize_mx4(self.h, x.data_ptr(), _OUT_KINDS[x.dtype], max(K, x.stride(0)) if rows == 1 else x.stride(0), K, rows,
-                                            codes.data_ptr(), K // 2, scales.data_ptr(), self._stream()), "q38b_quantize_mx4")
+        ld, one = x.stride()
+        kind = _OUT_KINDS.get(x.dtype)
+        _need(kind is not None and one == 1 and x.get_device() == self.device.index, "quantize_mx4: fp32, fp16 or bf16 [rows, K] on the context's device")
+        if K % 32 or K == 0 or rows == 0:
+            raise Q38BError(-1, "q38b_quantize_mx4")
+        half, tiles = K // 2, ((rows + 127) // 128) * ((K + 127) // 128) * 512
+        codes = _empty((rows, half), (half, 1), dtype=torch.uint8, device=self.device)
+        scales = _empty((tiles,), (1,), dtype=torch.uint8, device=self.device)
+        rc = self.lib.q38b_quantize_mx4(self.h, x.data_ptr(), kind, ld if rows > 1 else K, K, rows, codes.data_ptr(), half, scales.data_ptr(), self._stream())
+        if rc:
+            self._rc(rc, "q38b_quantize_mx4")
         return Mx4(codes, scales)
 
     def pack_mx4(self, codes, scales):
         """Codes uint8 [rows, K / 2] and scale bytes uint8 [rows, K / 32] of another producer -> Mx4 (the codes are kept, not copied)."""
-        _need(scales.dtype == torch.uint8 and scales.dim() == 2 and scales.stride(1) == 1 and scales.shape == (codes.shape[0], codes.shape[1] // 16), "pack_mx4: uint8 scales [rows, K / 32]")
-        rows, K = codes.shape[0], 2 * codes.shape[1]
-        self._mine("pack_mx4", codes, scales)
-        tiles = torch.empty(self.lib.q38b_mx4_scale_bytes(K, rows), dtype=torch.uint8, device=codes.device)
-        self._rc(self.lib.q38b_mx4_tile_scales(self.h, scales.data_ptr(), max(scales.stride(0), K // 32), K, rows, tiles.data_ptr(), self._stream()), "q38b_mx4_tile_scales")
+        rows, half = codes.shape
+        _need(scales.dtype == torch.uint8 and scales.shape == (rows, half // 16) and half % 16 == 0 and scales.stride(1) == 1, "pack_mx4: uint8 scales [rows, K / 32]")
+        _need(codes.get_device() == self.device.index and scales.get_device() == self.device.index, "pack_mx4: tensors on the context's device")
+        K = 2 * half
+        tiles = torch.empty(self.lib.q38b_mx4_scale_bytes(K, rows), dtype=torch.uint8, device=self.device)
+        self._rc(self.lib.q38b_mx4_tile_scales(self.h, scales.data_ptr(), scales.stride(0) if rows > 1 else K // 32, K, rows, tiles.data_ptr(), self._stream()), "q38b_mx4_tile_scales")
         return Mx4(codes, tiles)
 
     def dequant_mx4(self, m, kind=OUT_F32):
         """The values of an Mx4: [rows, K]."""
-        self._mine("dequant_mx4", m.codes)
-        out = torch.empty((m.rows, m.K), dtype=_OUT_DTYPES[kind], device=m.codes.device)
-        self._rc(self.lib.q38b_dequant_mx4(self.h, m.codes.data_ptr(), m.ld, m.scales.data_ptr(), m.K, m.rows, out.data_ptr(), kind, m.K, self._stream()), "q38b_dequant_mx4")
+        _need(m.codes.get_device() == self.device.index, "dequant_mx4: a matrix on the context's device")
+        out = _empty((m.rows, m.K), (m.K, 1), dtype=_OUT_DTYPES[kind], device=self.device)
+        rc = self.lib.q38b_dequant_mx4(self.h, m.codes.data_ptr(), m.ld, m.scales.data_ptr(), m.K, m.rows, out.data_ptr(), kind, m.K, self._stream())
+        if rc:
+            self._rc(rc, "q38b_dequant_mx4")
         return out
 
     def gemm_mx4(self, W, X, kind=OUT_F32, out=None, accumulate=False):
         """Y [B, W.rows] = X W^T for W an Mx4 and X an Mx4 or activations [B, K] (fp32, fp16 or bf16), which are quantized first.  kind: OUT_* of Y
         where `out` is not given."""
-        B = X.rows if isinstance(X, Mx4) else X.shape[0]
+        K, M, dev, mx = W.K, W.rows, self.device.index, isinstance(X, Mx4)
+        B = X.rows if mx else X.shape[0]
+        _need(W.codes.get_device() == dev and (X.codes if mx else X).get_device() == dev, "gemm_mx4: operands on the context's device")
         if out is None:
-            out = torch.empty((B, W.rows), dtype=_OUT_DTYPES[kind], device=W.codes.device)
-        _need(out.shape == (B, W.rows) and out.dtype in _OUT_KINDS and (W.rows == 1 or out.stride(1) == 1), "gemm_mx4: out [B, W.rows]")
-        ldy = out.stride(0) if B > 1 else W.rows
-        if isinstance(X, Mx4):
-            _need(X.K == W.K, "gemm_mx4: operands of one K")
-            self._mine("gemm_mx4", W.codes, X.codes, out)
-            self._rc(self.lib.q38b_gemm_mx4(self.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), W.K, W.rows, X.codes.data_ptr(), X.ld, X.scales.data_ptr(), B,
-                                            out.data_ptr(), _OUT_KINDS[out.dtype], ldy, int(bool(accumulate)), self._stream()), "q38b_gemm_mx4")
+            ldy = M
+            out = _empty((B, M), (M, 1), dtype=_OUT_DTYPES[kind], device=self.device)
+        else:
+            kind = _OUT_KINDS.get(out.dtype)
+            _need(kind is not None and out.shape == (B, M) and (M == 1 or out.stride(1) == 1) and out.get_device() == dev, "gemm_mx4: out [B, W.rows]")
+            ldy = out.stride(0) if B > 1 else M
+        if mx:
+            _need(X.K == K, "gemm_mx4: operands of one K")
+            rc = self.lib.q38b_gemm_mx4(self.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), K, M, X.codes.data_ptr(), X.ld, X.scales.data_ptr(), B, out.data_ptr(), kind,
+                                        ldy, 1 if accumulate else 0, self._stream())
+            if rc:
+                self._rc(rc, "q38b_gemm_mx4")
             return out
-        _need(X.dtype in _OUT_KINDS and X.dim() == 2 and X.stride(1) == 1 and X.shape[1] == W.K, "gemm_mx4: activations [B, K] of the weights' K")
-        self._mine("gemm_mx4", W.codes, X, out)
-        scratch = torch.empty(self.lib.q38b_gemm_mx4_scratch_bytes(W.K, B), dtype=torch.uint8, device=X.device)
-        self._rc(self.lib.q38b_gemm_mx4_x(self.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), W.K, W.rows, X.data_ptr(), _OUT_KINDS[X.dtype],
-                                          X.stride(0) if B > 1 else W.K, B, out.data_ptr(), _OUT_KINDS[out.dtype], ldy, int(bool(accumulate)), scratch.data_ptr(),
-                                          scratch.numel(), self._stream()), "q38b_gemm_mx4_x")
+        x_kind = _OUT_KINDS.get(X.dtype)
+        B, k = X.shape
+        ld, one = X.stride()
+        _need(x_kind is not None and one == 1 and k == K and B > 0, "gemm_mx4: activations [B, K] of the weights' K")
+        need = B * (K // 2) + ((B + 127) // 128) * ((K + 127) // 128) * 512 + 16   # q38b_gemm_mx4_scratch_bytes
+        scratch = _empty((need,), (1,), dtype=torch.uint8, device=self.device)
+        rc = self.lib.q38b_gemm_mx4_x(self.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), K, M, X.data_ptr(), x_kind, ld if B > 1 else K, B, out.data_ptr(), kind, ldy,
+                                      1 if accumulate else 0, scratch.data_ptr(), need, self._stream())
+        if rc:
+            self._rc(rc, "q38b_gemm_mx4_x")
         return out
 
     def topk(self, logits, k, index_offset=0):

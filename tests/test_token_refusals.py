@@ -16,11 +16,28 @@ P, ODD = 0x10000, 0x10002               # addresses that are only compared and c
 ARG, UNSUPPORTED, ALIGN, NOMEM = -1, -2, -3, -6
 
 
+class Heads(C.Structure):
+    """q38b_heads"""
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_row", C.c_longlong), ("src_head", C.c_longlong), ("dst_row", C.c_longlong),
+                ("dst_head", C.c_longlong), ("weight", C.c_void_p), ("n_heads", C.c_int)]
+
+
+class Rules(C.Structure):
+    """q38b_logit_rules"""
+    _fields_ = [(n, C.c_void_p) for n in ("penalties", "history", "history_begin", "prompt_len", "bias_ids", "bias_values", "bias_begin", "masks")] + \
+               [("mask_ld", C.c_longlong), ("mask_of_row", C.c_void_p)]
+
+
 def heads(**kw):
-    from qwengine_b200.api import _Heads
     v = dict(src=P, dst=P + 4096, src_row=512, src_head=64, dst_row=512, dst_head=64, weight=P, n_heads=8)
     v.update(kw)
-    return _Heads(**v)
+    return Heads(**v)
+
+
+def test_the_wrappers_bytes_are_the_structures():
+    from qwengine_b200 import api
+    assert api._pack_heads(1, 2, 3, 4, 5, 6, 7, 8) == bytes(Heads(1, 2, 3, 4, 5, 6, 7, 8))
+    assert api._pack_rules(*range(1, 11)) == bytes(Rules(*range(1, 11)))
 
 
 @pytest.mark.parametrize("change,status", [
@@ -54,10 +71,9 @@ def test_heads_null(lib):
     ({}, dict(bias_ids=P, bias_values=P, bias_begin=P + 4), ALIGN),
 ])
 def test_logits(lib, change, rules, status):
-    from qwengine_b200.api import _LogitRules
     a = dict(x=P, x_ld=100, n=100, rows=2, off=0, y=P + 65536, y_ld=100)
     a.update(change)
-    r = _LogitRules(**rules)
+    r = Rules(**rules)
     assert lib.q38b_adjust_logits(CTX, a["x"], a["x_ld"], a["n"], a["rows"], a["off"], C.byref(r), a["y"], a["y_ld"], None) == status
     assert lib.q38b_adjust_logits(CTX, P, 100, 100, 2, 0, None, P + 65536, 100, None) == ARG
 
