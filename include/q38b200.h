@@ -279,7 +279,8 @@ int q38b_dequant_mx4(q38b_ctx* ctx, const void* codes_dev, long long codes_ld, c
 int q38b_gemm_mx4(q38b_ctx* ctx, const void* W_codes, long long W_ld, const void* W_scales, int K, int M, const void* X_codes, long long X_ld,
                   const void* X_scales, int B, void* Y_dev, int y_kind, long long ldy, int accumulate, void* stream);
 /* The same from activations as they are: x is quantized into `scratch_dev` (16-byte aligned, the caller's, at least
- * q38b_gemm_mx4_scratch_bytes(K, B) bytes) and multiplied; results equal the two calls' bit for bit. */
+ * q38b_gemm_mx4_scratch_bytes(K, B) bytes; 0 for few tokens and K, which the product's kernel quantizes itself: then it may be NULL) and
+ * multiplied; results equal the two calls' bit for bit. */
 size_t q38b_gemm_mx4_scratch_bytes(int K, int B);
 int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W_codes, long long W_ld, const void* W_scales, int K, int M, const void* x_dev, int x_kind,
                     long long x_ld, int B, void* Y_dev, int y_kind, long long ldy, int accumulate, void* scratch_dev, size_t scratch_bytes,

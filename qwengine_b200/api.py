@@ -120,6 +120,7 @@ def load_library():
     lib.q38b_gemm_mx4_scratch_bytes.argtypes = [i32, i32]
     lib.q38b_gemm_mx4_scratch_bytes.restype = sz
     lib.q38b_debug_set_mx4_pairs.argtypes = [vp, i32]
+    lib.q38b_debug_set_mx4_two_launches.argtypes = [vp, i32]
     lib.q38b_gemm_mx4_x.argtypes = [vp, vp, ll, vp, i32, i32, vp, i32, ll, i32, vp, i32, ll, i32, vp, sz, vp]
     _LIB = lib
     return lib
@@ -482,10 +483,12 @@ class Context:
         B, k = X.shape
         ld, one = X.stride()
         _need(x_kind is not None and one == 1 and k == K and B > 0, "gemm_mx4: activations [B, K] of the weights' K")
-        need = B * (K // 2) + ((B + 127) // 128) * ((K + 127) // 128) * 512 + 16   # q38b_gemm_mx4_scratch_bytes
-        scratch = _empty((need,), (1,), dtype=torch.uint8, device=self.device)
+        scratch, need = None, 0
+        if B > 1 or K > 8192:   # q38b_gemm_mx4_scratch_bytes
+            need = B * (K // 2) + ((B + 127) // 128) * ((K + 127) // 128) * 512 + 16
+            scratch = _empty((need,), (1,), dtype=torch.uint8, device=self.device)
         rc = self.lib.q38b_gemm_mx4_x(self.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), K, M, X.data_ptr(), x_kind, ld if B > 1 else K, B, out.data_ptr(), kind, ldy,
-                                      1 if accumulate else 0, scratch.data_ptr(), need, self._stream())
+                                      1 if accumulate else 0, None if scratch is None else scratch.data_ptr(), need, self._stream())
         if rc:
             self._rc(rc, "q38b_gemm_mx4_x")
         return out

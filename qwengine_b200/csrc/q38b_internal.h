@@ -16,7 +16,7 @@ struct q38b_ctx {
     int check_occupancy = 0, occupancy_shortfalls = 0;   // test hook q38b_debug_occupancy_shortfalls
     int cols_route = 0;        // test hook q38b_debug_set_cols_route: 1 never, 2 always (where there is a plan) by granules
     int prefill_tiles = 0, prefill_splits = 0;   // test hook q38b_debug_set_prefill_cut
-    int mx4_pairs = 0;         // test hook q38b_debug_set_mx4_pairs
+    int mx4_pairs = 0, mx4_two_launches = 0;   // test hooks q38b_debug_set_mx4_pairs, q38b_debug_set_mx4_two_launches
     int uniform_columns = 0;   // 1: single-column calls also run the tensor-core kernel (bit-identical to columns of wider calls)
     long long wait_budget_cycles = 4000000000LL;   // bounded waits on other GPUs (q38b_ctx_set_wait_budget_cycles)
     int* d_status = nullptr;

@@ -92,6 +92,7 @@ template <typename T> __device__ __forceinline__ uint32_t raw8_top(const Raw8<T>
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, long long x_ld, int K, int rows, uint8_t* codes, long long codes_ld, uint8_t* scales) {
+    pdl_launch_dependents();   // (a product behind it brings its first weights meanwhile)
     MxWalk w;
     if (!mx_walk(K, rows, w)) return;
     const int lane = threadIdx.x & 31;
@@ -204,7 +205,9 @@ __global__ void __launch_bounds__(256) mx4_dequant_kernel(const uint8_t* codes, 
 // are powers of two, so only the 32-bit sum rounds.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int MX_ROWS = 128, MX_MAX_N = 256, MX_K = 256;
-constexpr int MX_THREADS = 192, MX_MAX_STAGES = 8, MX_MAX_SPLITS = 8;
+constexpr int MX_THREADS = 320, MX_MAX_STAGES = 12, MX_MAX_SPLITS = 8;
+constexpr int MX_FUSE_MAX_B = 1;      // up to so many tokens every CTA quantizes its part of the activations itself
+constexpr int MX_FUSE_MAX_K = 8192;   // ... of at most so many K
 constexpr int MX_A_BYTES = MX_ROWS * MX_K / 2, MX_SFA_BYTES = 2 * MX_TILE;
 
 struct MxArgs {
@@ -214,9 +217,15 @@ struct MxArgs {
     int* status;
     int K, M, B, accumulate;
     int n_tile, stages, splits, pdl;
+    const void* x;          // FUSED: the activations as they are
+    long long x_ld;
+    int x_kind, x_steps;    // x_steps: stages of K a CTA holds, at most
 };
 __host__ __device__ constexpr int mx_groups(int n_tile) { return (n_tile + 127) / 128; }
 __host__ __device__ constexpr int mx_stage_bytes(int n_tile) { return MX_A_BYTES + n_tile * (MX_K / 2) + MX_SFA_BYTES * (1 + mx_groups(n_tile)); }
+// FUSED: a stage is weights only; the activations' codes (16 rows) and scales of every stage lie in front of the ring
+constexpr int MX_FUSED_STAGE = MX_A_BYTES + MX_SFA_BYTES, MX_FUSED_X = 16 * (MX_K / 2);
+__host__ __device__ constexpr int mx_fused_x_bytes(int steps) { return steps * (MX_FUSED_X + MX_SFA_BYTES); }
 // accumulator, then the scales of each stage (a stage's columns are free when its shared memory is): 4 columns per tile of 128 rows x 128 K
 __host__ __device__ constexpr int mx_acc_cols(int n_tile) { return (n_tile + 31) / 32 * 32; }
 __host__ __device__ constexpr int mx_scale_cols(int n_tile) { return 8 * (1 + mx_groups(n_tile)); }
@@ -258,13 +267,13 @@ __device__ __forceinline__ uint32_t mx_idesc(int m, int n) { return (1u << 7) | 
 // vector registers in a hundred and more (with loops over run-time counts a stage took some 1200 clocks whatever its tokens: 2048 x
 // 17408 x 5120 110 us).
 template <bool PAIR, int GROUPS, int NK>
-__device__ __forceinline__ void mx_issue(uint32_t d, uint64_t ad, uint64_t bd, uint32_t sf, uint32_t cols, uint32_t first_col, uint32_t idesc, uint32_t add) {
+__device__ __forceinline__ void mx_issue(uint32_t d, uint64_t ad, uint64_t bd, uint32_t sfa, uint32_t sfb, uint32_t cols, uint32_t first_col, uint32_t idesc, uint32_t add) {
 #pragma unroll
     for (int c = 0; 2 * c < NK; c++) {
-        tmem_copy_scales<PAIR>(cols + (uint32_t)(4 * c), sf + (uint32_t)(c * MX_TILE));
+        tmem_copy_scales<PAIR>(cols + (uint32_t)(4 * c), sfa + (uint32_t)(c * MX_TILE));
 #pragma unroll
         for (int g = 0; g < GROUPS; g++)
-            tmem_copy_scales<PAIR>(cols + (uint32_t)(8 + 4 * (c * GROUPS + g)), sf + (uint32_t)((1 + g) * MX_SFA_BYTES + c * MX_TILE));
+            tmem_copy_scales<PAIR>(cols + (uint32_t)(8 + 4 * (c * GROUPS + g)), sfb + (uint32_t)(g * MX_SFA_BYTES + c * MX_TILE));
     }
 #pragma unroll
     for (int k = 0; k < NK; k++)
@@ -272,31 +281,79 @@ __device__ __forceinline__ void mx_issue(uint32_t d, uint64_t ad, uint64_t bd, u
                        cols + first_col + (uint32_t)(4 * (k >> 1) * GROUPS), k > 0 ? 1u : add);
 }
 template <bool PAIR, int GROUPS>
-__device__ __forceinline__ void mx_issue_stage(int n_k, uint32_t d, uint64_t ad, uint64_t bd, uint32_t sf, uint32_t cols, uint32_t first_col, uint32_t idesc, uint32_t add) {
-    if (n_k >= 4) mx_issue<PAIR, GROUPS, 4>(d, ad, bd, sf, cols, first_col, idesc, add);
-    else if (n_k == 3) mx_issue<PAIR, GROUPS, 3>(d, ad, bd, sf, cols, first_col, idesc, add);
-    else if (n_k == 2) mx_issue<PAIR, GROUPS, 2>(d, ad, bd, sf, cols, first_col, idesc, add);
-    else mx_issue<PAIR, GROUPS, 1>(d, ad, bd, sf, cols, first_col, idesc, add);
+__device__ __forceinline__ void mx_issue_stage(int n_k, uint32_t d, uint64_t ad, uint64_t bd, uint32_t sfa, uint32_t sfb, uint32_t cols, uint32_t first_col, uint32_t idesc, uint32_t add) {
+    if (n_k >= 4) mx_issue<PAIR, GROUPS, 4>(d, ad, bd, sfa, sfb, cols, first_col, idesc, add);
+    else if (n_k == 3) mx_issue<PAIR, GROUPS, 3>(d, ad, bd, sfa, sfb, cols, first_col, idesc, add);
+    else if (n_k == 2) mx_issue<PAIR, GROUPS, 2>(d, ad, bd, sfa, sfb, cols, first_col, idesc, add);
+    else mx_issue<PAIR, GROUPS, 1>(d, ad, bd, sfa, sfb, cols, first_col, idesc, add);
 }
 
-template <typename T, int GROUPS>
+// Eight neighbours of a row of activations, of whatever kind and alignment
+__device__ __forceinline__ void load_x8(const void* x, int kind, long long at, bool vec, float (&v)[8]) {
+    if (kind == Q38B_OUT_F32) {
+        const float* p = (const float*)x + at;
+        if (vec) {
+            const float4 a = *(const float4*)p, b = *(const float4*)(p + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = p[i];
+        }
+        return;
+    }
+    const uint16_t* p = (const uint16_t*)x + at;
+    uint16_t h[8];
+    if (vec) {
+        *(uint4*)h = *(const uint4*)p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) h[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = kind == Q38B_OUT_F16 ? __half2float(__ushort_as_half(h[i])) : __uint_as_float((uint32_t)h[i] << 16);
+}
+
+// FUSED (one token): warps 2..9 quantize the activations of this CTA's K into operand B and its scales while the first weights are on
+// their way; one launch instead of two: 17408 x 5120 12.2 us against 13.4, 5120 x 17408 14.6 against 15.2.  (With two tokens 13.6 and 13.4,
+// with eight 18.5 and 13.5: every CTA quantizes what one kernel does once, and the weights' ring stands full meanwhile.)
+// The weights of the first stages are asked for before anything else, also before the quantizer's kernel in front has ended.
+template <typename T, int GROUPS, bool FUSED>
 __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* full = (uint64_t*)smem;
     uint64_t* empty = full + MX_MAX_STAGES;
     uint64_t* acc_done = empty + MX_MAX_STAGES;
-    uint32_t* tmem_slot = (uint32_t*)(acc_done + 1);
+    uint64_t* x_there = acc_done + 1;
+    uint32_t* tmem_slot = (uint32_t*)(x_there + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-    uint8_t* ring = smem + 1024;
+    uint8_t* x_codes = smem + 1024;                                                       // FUSED: [steps][16 rows x 128 bytes], swizzled
+    uint8_t* x_sf = x_codes + (FUSED ? a.x_steps * MX_FUSED_X : 0);                       // FUSED: [steps][two scale tiles]
+    uint8_t* ring = smem + 1024 + (FUSED ? mx_fused_x_bytes(a.x_steps) : 0);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = a.splits > 1 ? (int)cluster_rank() : 0;
     const int row0 = (int)(blockIdx.x / (unsigned)a.splits) * MX_ROWS, tok0 = (int)blockIdx.y * a.n_tile;
     const int n_tok = min(a.n_tile, a.B - tok0), n_mma = (n_tok + 15) / 16 * 16;
     const int kt = (int)mx_tiles_k(a.K), steps = (a.K + MX_K - 1) / MX_K;
     const int s_begin = (int)((long long)steps * rank / a.splits), s_end = (int)((long long)steps * (rank + 1) / a.splits);
-    const int stage_bytes = mx_stage_bytes(a.n_tile);
+    const int stage_bytes = FUSED ? MX_FUSED_STAGE : mx_stage_bytes(a.n_tile), sf_at = FUSED ? MX_A_BYTES : MX_A_BYTES + a.n_tile * (MX_K / 2);
     const uint32_t tmem_cols = mx_tmem_cols(a.n_tile, a.stages);
+    const int used = (n_tok + 127) / 128;   // groups of 128 tokens that hold any
+    const uint8_t* wsc = a.w_scales + (size_t)(row0 / 128) * kt * MX_TILE;
+    auto scale_bytes = [&](int s) { return (uint32_t)min(2, kt - 2 * s) * MX_TILE; };
+    auto ask_weights = [&](int s, int st) {   // and what the stage waits for altogether
+        const uint32_t bar = smem_u32(&full[st]), at = smem_u32(ring + st * stage_bytes);
+        mbar_arrive_expect_tx(bar, (uint32_t)(FUSED ? MX_A_BYTES : sf_at) + scale_bytes(s) * (uint32_t)(FUSED ? 1 : 1 + used));
+        tma_load_2d(at, &wmap, s * (MX_K / 2), row0, bar);
+        bulk_copy_g2s(at + (uint32_t)sf_at, wsc + (size_t)s * MX_SFA_BYTES, scale_bytes(s), bar);
+    };
+    auto ask_tokens = [&](int s, int st) {
+        const uint32_t bar = smem_u32(&full[st]), at = smem_u32(ring + st * stage_bytes);
+        tma_load_2d(at + MX_A_BYTES, &xmap, s * (MX_K / 2), tok0, bar);
+        for (int g = 0; g < used; g++)
+            bulk_copy_g2s(at + (uint32_t)(sf_at + (1 + g) * MX_SFA_BYTES), a.x_scales + ((size_t)(tok0 / 128 + g) * kt + 2 * s) * MX_TILE, scale_bytes(s), bar);
+    };
 
+    const int ahead = min(a.stages, s_end - s_begin);   // stages that need no waiting for
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < a.stages; s++) {
@@ -304,7 +361,10 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
             mbar_init(smem_u32(&empty[s]), 1);
         }
         mbar_init(smem_u32(acc_done), 1);
+        mbar_init(smem_u32(x_there), 8);
         mbar_fence_init();
+        fence_proxy_async();
+        for (int i = 0; i < ahead; i++) ask_weights(s_begin + i, i);
     }
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(tmem_cols) : "memory");
@@ -318,20 +378,14 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
 
     if (warp == 0) {
         if (lane == 0) {
+            if constexpr (!FUSED)
+                for (int i = 0; i < ahead; i++) ask_tokens(s_begin + i, i);
             int st = 0;
             uint32_t use = 0;
-            const uint8_t* wsc = a.w_scales + (size_t)(row0 / 128) * kt * MX_TILE;
-            for (int s = s_begin; s < s_end; s++) {
-                mbar_wait_bounded(smem_u32(&empty[st]), use ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
-                const uint32_t bar = smem_u32(&full[st]), at = smem_u32(ring + st * stage_bytes), scale_bytes = (uint32_t)min(2, kt - 2 * s) * MX_TILE;
-                const uint32_t sf = at + MX_A_BYTES + (uint32_t)a.n_tile * (MX_K / 2);
-                const int used = (n_tok + 127) / 128;   // groups of 128 tokens that hold any
-                mbar_arrive_expect_tx(bar, (uint32_t)(MX_A_BYTES + a.n_tile * (MX_K / 2)) + scale_bytes * (uint32_t)(1 + used));
-                tma_load_2d(at, &wmap, s * (MX_K / 2), row0, bar);
-                tma_load_2d(at + MX_A_BYTES, &xmap, s * (MX_K / 2), tok0, bar);
-                bulk_copy_g2s(sf, wsc + (size_t)s * MX_SFA_BYTES, scale_bytes, bar);
-                for (int g = 0; g < used; g++)
-                    bulk_copy_g2s(sf + (uint32_t)(1 + g) * MX_SFA_BYTES, a.x_scales + ((size_t)(tok0 / 128 + g) * kt + 2 * s) * MX_TILE, scale_bytes, bar);
+            for (int s = s_begin + ahead; s < s_end; s++) {
+                mbar_wait_bounded(smem_u32(&empty[st]), use, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
+                ask_weights(s, st);
+                if constexpr (!FUSED) ask_tokens(s, st);
                 if (++st == a.stages) { st = 0; use ^= 1u; }
             }
         }
@@ -340,23 +394,72 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
         uint32_t use = 0;
         const uint64_t desc0 = umma_desc_sw128(0);
         const uint32_t sf_cols = tmem_base + (uint32_t)mx_acc_cols(a.n_tile), ring_at = smem_u32(ring), idesc = mx_idesc(MX_ROWS, n_mma);
+        uint32_t xc = smem_u32(x_codes), xs = smem_u32(x_sf);
+        if constexpr (FUSED) mbar_wait_bounded(smem_u32(x_there), 0u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
         for (int s = s_begin; s < s_end; s++) {
             mbar_wait_bounded(smem_u32(&full[st]), use, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t at = ring_at + (uint32_t)(st * stage_bytes), sf = at + MX_A_BYTES + (uint32_t)a.n_tile * (MX_K / 2);
+            const uint32_t at = ring_at + (uint32_t)(st * stage_bytes), sfa = at + (uint32_t)sf_at;
+            const uint32_t b_at = FUSED ? xc : at + MX_A_BYTES, sfb = FUSED ? xs : sfa + MX_SFA_BYTES;
             const uint32_t cols = sf_cols + (uint32_t)(st * mx_scale_cols(a.n_tile));
             const int n_k = (a.K - s * MX_K + 63) / 64;   // steps of 64 K that hold any; codes behind K are zero
             if (elect_one()) {
-                mx_issue_stage<false, GROUPS>(n_k, tmem_base, desc0 + (at >> 4), desc0 + ((at + MX_A_BYTES) >> 4), sf, cols, 8u, idesc, s > s_begin ? 1u : 0u);
+                mx_issue_stage<false, GROUPS>(n_k, tmem_base, desc0 + (at >> 4), desc0 + (b_at >> 4), sfa, sfb, cols, 8u, idesc, s > s_begin ? 1u : 0u);
                 umma_commit<false>(smem_u32(&empty[st]));
                 if (s == s_end - 1) umma_commit<false>(smem_u32(acc_done));
             }
             __syncwarp();
+            xc += MX_FUSED_X;
+            xs += MX_SFA_BYTES;
             if (++st == a.stages) { st = 0; use ^= 1u; }
         }
+    } else if constexpr (FUSED) {
+        // units of eight values of a row, four lanes a block; behind K zeros as far as the last step of 64 K reaches
+        const int k0 = s_begin * MX_K, span = min(s_end * MX_K, (a.K + 63) / 64 * 64) - k0, per_row = span / 8, units = a.B * per_row;
+        const bool vec = (((uintptr_t)a.x | (uintptr_t)(a.x_ld * (a.x_kind == Q38B_OUT_F32 ? 4 : 2))) & 15) == 0;
+        constexpr int AHEAD = 4;   // units of a lane on their way at a time
+        for (int u0 = 32 * (warp - 2); u0 < units; u0 += 256 * AHEAD) {
+            float v[AHEAD][8];
+            int row[AHEAD], at[AHEAD];
+#pragma unroll
+            for (int g = 0; g < AHEAD; g++) {
+                const int u = u0 + 256 * g + lane;
+                row[g] = u / per_row;
+                at[g] = (u - row[g] * per_row) * 8;
+                if (u < units && k0 + at[g] < a.K) {
+                    load_x8(a.x, a.x_kind, (long long)row[g] * a.x_ld + k0 + at[g], vec, v[g]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[g][i] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < AHEAD; g++) {
+                if (u0 + 256 * g >= units) break;   // (the whole warp)
+                uint32_t top = 0u;
+#pragma unroll
+                for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[g][i]) & 0x7FFFFFFFu);
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                float inv;
+                const uint32_t byte = mx_scale(top, inv);
+                uint32_t code = 0u;
+#pragma unroll
+                for (int i = 0; i < 4; i++) code |= e2m1_pair(v[g][2 * i] * inv, v[g][2 * i + 1] * inv) << (8 * i);
+                if (u0 + 256 * g + lane < units) {   // 128 bytes of a row hold 256 K; 16-byte piece c at c ^ (row & 7) (128-byte swizzle)
+                    const int s = at[g] / MX_K, b = at[g] % MX_K / 2, r = row[g];
+                    *(uint32_t*)(x_codes + s * MX_FUSED_X + r * 128 + 16 * ((b / 16) ^ (r & 7)) + b % 16) = code;
+                    if (lane % 4 == 0) x_sf[s * MX_SFA_BYTES + b / 64 * MX_TILE + 16 * r + b / 16 % 4] = (uint8_t)byte;
+                }
+            }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(x_there));
     }
 
-    // ---------------- warps 2..5 store: lanes 32 (warp % 4) .. + 31 of the accumulator are 32 rows ----------------
+    // ---------------- warps 2..9 store: lanes 32 (warp % 4) .. + 31 of the accumulator are 32 rows; two warps share their tokens ----------------
+    const int part = (warp - 2) >> 2;
     const int n_chunks = (n_tok + 15) / 16, quad = warp & 3, row = row0 + 32 * quad + lane;
     const uint32_t acc = tmem_base + ((uint32_t)(32 * quad) << 16);
     T* Y = (T*)a.Y;
@@ -377,7 +480,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
     }
     if (a.splits == 1) {
         if (warp >= 2)
-            for (int chunk = 0; chunk < n_chunks; chunk++) {
+            for (int chunk = part; chunk < n_chunks; chunk += 2) {
                 uint32_t v[16];
                 float f[16];
                 tmem_ld16(acc + (uint32_t)(16 * chunk), v);
@@ -393,7 +496,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
         __syncwarp();
         cluster_sync_all();
         if (warp >= 2)
-            for (int chunk = 0; chunk < n_chunks; chunk++) {
+            for (int chunk = part; chunk < n_chunks; chunk += 2) {
                 const int owner = chunk % a.splits;
                 if (owner == rank) continue;
                 uint32_t v[16];
@@ -405,7 +508,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
             }
         cluster_sync_all();   // all sums have arrived; nobody touches another CTA's memory after this
         if (warp >= 2)
-            for (int own = 0; own * a.splits + rank < n_chunks; own++) {
+            for (int own = part; own * a.splits + rank < n_chunks; own += 2) {
                 uint32_t v[16];
                 float f[16] = {};
                 tmem_ld16(acc + (uint32_t)(16 * (own * a.splits + rank)), v);
@@ -524,7 +627,7 @@ mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, co
                     const uint32_t cols = sf_cols + (uint32_t)(st * mx_scale_cols(a.n_tile));
                     const int n_k = (a.K - s * MX_K + 63) / 64;
                     if (elect_one()) {
-                        mx_issue_stage<true, GROUPS>(n_k, d, desc0 + (at >> 4), desc0 + ((at + MX_A_BYTES) >> 4), sf, cols, first_col, idesc, s > 0 ? 1u : 0u);
+                        mx_issue_stage<true, GROUPS>(n_k, d, desc0 + (at >> 4), desc0 + ((at + MX_A_BYTES) >> 4), sf, sf + MX_SFA_BYTES, cols, first_col, idesc, s > 0 ? 1u : 0u);
                         umma_commit<true>(smem_u32(&empty[st]));
                         if (s == steps - 1) umma_commit<true>(smem_u32(&acc_full[acc]));
                     }
@@ -620,20 +723,32 @@ int exchange_bytes(const MxCut& c) {
     return (c.splits - 1) * ((chunks + c.splits - 1) / c.splits) * 16 * MX_ROWS * 4;
 }
 
-MxCut mx_cut(int sm_count, int smem_optin, int K, int M, int B) {
+// ... by their time in SM clocks: rounds of CTAs, each stage 600 clocks and 5 a token (2048 x 17408 x 5120 174 us in tiles of 256), what starts
+// and drains a CTA, and the exchange of split sums.  (Clusters of three and more leave some SMs unused.)
+MxCut mx_cut(int sm_count, int smem_optin, int K, int M, int B, double* cost_of) {
+    MxCut best = {};
+    double best_cost = 0.0;
+    const int steps = (K + MX_K - 1) / MX_K;
     MxCut c;
     c.n_tile = B <= MX_MAX_N ? (B + 15) / 16 * 16 : MX_MAX_N;
-    const int steps = (K + MX_K - 1) / MX_K;
     const long long tiles = (long long)((M + MX_ROWS - 1) / MX_ROWS) * ((B + c.n_tile - 1) / c.n_tile);
-    c.splits = (int)std::max<long long>(1, std::min<long long>(std::min<long long>(MX_MAX_SPLITS, sm_count / tiles), steps / 4));
     c.stages = std::min(MX_MAX_STAGES, (smem_optin - 1024) / mx_stage_bytes(c.n_tile));
-    while (c.splits > 1 && exchange_bytes(c) > c.stages * mx_stage_bytes(c.n_tile)) c.splits--;
-    return c;
+    c.stages = std::min(c.stages, (512 - mx_acc_cols(c.n_tile)) / mx_scale_cols(c.n_tile));
+    for (c.splits = 1; c.splits <= std::min(MX_MAX_SPLITS, steps); c.splits++) {
+        if (c.splits > 1 && exchange_bytes(c) > c.stages * mx_stage_bytes(c.n_tile)) break;
+        const long long slots = c.splits <= 2 ? sm_count : sm_count * 9 / 10 / c.splits * c.splits, ctas = tiles * c.splits;
+        const double cost = (double)((ctas + slots - 1) / slots) * ((steps + c.splits - 1) / c.splits * (600.0 + 5.0 * c.n_tile) + 4000.0 + (c.splits > 1 ? 1500.0 + 10.0 * c.n_tile : 0.0));
+        if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
+    }
+    if (cost_of) *cost_of = best_cost;
+    return best;
 }
 
-// Tiles of a product in pairs: 64, 128, 192 or 256 tokens (a tile starts on half a scale tile).
+// Tiles of a product in pairs: 64, 128, 192 or 256 tokens (a tile starts on half a scale tile), by their time in SM clocks: rounds of
+// tiles over the pairs, each stage 500 clocks and 1.45 a token (measured at 128, 192 and 256 tokens of 2048 x 17408 x 5120: 109, 85 and 73 us;
+// 333 x 16384 x 5120: 27, 21 and 26 us, with 64 tokens 50), and what starts and drains a tile, less where two accumulators take turns.
 struct MxPairCut { int n_tile, stages, n_acc, tok_tiles, n_tiles; };
-MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int forced) {
+MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int forced, double* cost_of) {
     MxPairCut best = {};
     double best_cost = 0.0;
     const int row_tiles = (M + 255) / 256, steps = (K + MX_K - 1) / MX_K;
@@ -651,9 +766,10 @@ MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int for
             c.stages = std::min(c.stages, two);
         }
         const int pairs = sm_count / 2;
-        const double cost = (double)((c.n_tiles + pairs - 1) / pairs) * (steps * 2.0 * n + (c.n_acc == 2 ? 200.0 : 1200.0));
+        const double cost = (double)((c.n_tiles + pairs - 1) / pairs) * (steps * (500.0 + 1.45 * n) + (c.n_acc == 2 ? 1700.0 : 2700.0));
         if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
     }
+    if (cost_of) *cost_of = best_cost + 4000.0;
     return best;
 }
 
@@ -735,16 +851,16 @@ int pair_as(q38b_ctx* ctx, const MxPairArgs& a, const CUtensorMap& wmap, const C
     return launch_status(ctx, cudaLaunchKernelEx(&cfg, kern, a, wmap, xmap, wsmap, xsmap, ymap));
 }
 
-template <typename T>
+template <typename T, int GROUPS, bool FUSED>
 int gemm_as(q38b_ctx* ctx, const MxArgs& a, const CUtensorMap& wmap, const CUtensorMap& xmap, cudaStream_t st) {
-    auto kern = mx_groups(a.n_tile) == 1 ? mx4_gemm_kernel<T, 1> : mx4_gemm_kernel<T, 2>;
+    auto kern = mx4_gemm_kernel<T, GROUPS, FUSED>;
     const int rc = q38b_ensure_kernel_smem(ctx, (const void*)kern, ctx->smem_optin, false);
     if (rc != Q38B_OK) return rc;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)((a.M + MX_ROWS - 1) / MX_ROWS * a.splits), (unsigned)((a.B + a.n_tile - 1) / a.n_tile));
     cfg.blockDim = dim3(MX_THREADS);
-    cfg.dynamicSmemBytes = (size_t)(1024 + a.stages * mx_stage_bytes(a.n_tile));
+    cfg.dynamicSmemBytes = (size_t)(1024 + (FUSED ? mx_fused_x_bytes(a.x_steps) + a.stages * MX_FUSED_STAGE : a.stages * mx_stage_bytes(a.n_tile)));
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     int n = 0;
@@ -762,6 +878,29 @@ int gemm_as(q38b_ctx* ctx, const MxArgs& a, const CUtensorMap& wmap, const CUten
     cfg.attrs = attr;
     cfg.numAttrs = (unsigned)n;
     return launch_status(ctx, cudaLaunchKernelEx(&cfg, kern, a, wmap, xmap));
+}
+template <int GROUPS, bool FUSED>
+int gemm_kind(q38b_ctx* ctx, const MxArgs& a, const CUtensorMap& wmap, const CUtensorMap& xmap, int y_kind, cudaStream_t st) {
+    return y_kind == Q38B_OUT_F32 ? gemm_as<float, GROUPS, FUSED>(ctx, a, wmap, xmap, st)
+         : y_kind == Q38B_OUT_F16 ? gemm_as<__half, GROUPS, FUSED>(ctx, a, wmap, xmap, st)
+                                  : gemm_as<__nv_bfloat16, GROUPS, FUSED>(ctx, a, wmap, xmap, st);
+}
+
+MxArgs mx_args(q38b_ctx* ctx, const MxCut& cut, const void* W_scales, int K, int M, int B, void* Y, long long ldy, int accumulate) {
+    MxArgs a;
+    memset(&a, 0, sizeof(a));
+    a.w_scales = (const uint8_t*)W_scales;
+    a.Y = Y;
+    a.ldy = ldy;
+    a.status = ctx->d_status;
+    a.K = K;
+    a.M = M;
+    a.B = B;
+    a.accumulate = accumulate ? 1 : 0;
+    a.n_tile = cut.n_tile;
+    a.stages = cut.stages;
+    a.splits = cut.splits;
+    return a;
 }
 
 // arguments of one operand
@@ -821,8 +960,10 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
     if ((uintptr_t)Y % kind_size(y_kind)) return Q38B_ERR_ALIGN;
     DeviceGuard on(ctx);
     cudaStream_t st = (cudaStream_t)stream;
-    if (ctx->mx4_pairs > 0 || (ctx->mx4_pairs == 0 && B > 128 && M > MX_ROWS)) {
-        const MxPairCut cut = mx_pair_cut(ctx->sm_count, ctx->smem_optin, K, M, B, ctx->mx4_pairs);
+    double cost = 0.0, pair_cost = 0.0;
+    const MxCut one = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B, &cost);
+    const MxPairCut cut = mx_pair_cut(ctx->sm_count, ctx->smem_optin, K, M, B, ctx->mx4_pairs > 0 ? ctx->mx4_pairs : 0, &pair_cost);
+    if (ctx->mx4_pairs > 0 || (ctx->mx4_pairs == 0 && B > 32 && M > MX_ROWS && pair_cost < cost)) {
         CUtensorMap wmap, xmap, wsmap, xsmap, ymap;
         memset(&ymap, 0, sizeof(ymap));
         const int tma_out = encode_out(&ymap, Y, y_kind, ldy, M, B) ? 1 : 0;
@@ -834,26 +975,13 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
              : y_kind == Q38B_OUT_F16 ? pair_as<__half>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st)
                                       : pair_as<__nv_bfloat16>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st);
     }
-    const MxCut cut = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B);
-    if ((B + cut.n_tile - 1) / cut.n_tile > 65535) return Q38B_ERR_UNSUPPORTED;
+    if ((B + one.n_tile - 1) / one.n_tile > 65535) return Q38B_ERR_UNSUPPORTED;
     CUtensorMap wmap, xmap;
-    if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS) || !encode_codes(&xmap, X, X_ld, K, B, cut.n_tile)) return Q38B_ERR_ARG;
-    MxArgs a;
-    a.w_scales = (const uint8_t*)W_scales;
+    if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS) || !encode_codes(&xmap, X, X_ld, K, B, one.n_tile)) return Q38B_ERR_ARG;
+    MxArgs a = mx_args(ctx, one, W_scales, K, M, B, Y, ldy, accumulate);
     a.x_scales = (const uint8_t*)X_scales;
-    a.Y = Y;
-    a.ldy = ldy;
-    a.status = ctx->d_status;
-    a.K = K;
-    a.M = M;
-    a.B = B;
-    a.accumulate = accumulate ? 1 : 0;
-    a.n_tile = cut.n_tile;
-    a.stages = cut.stages;
-    a.splits = cut.splits;
     a.pdl = behind_quantizer ? 1 : 0;
-    return y_kind == Q38B_OUT_F32 ? gemm_as<float>(ctx, a, wmap, xmap, st) : y_kind == Q38B_OUT_F16 ? gemm_as<__half>(ctx, a, wmap, xmap, st)
-                                                                                                    : gemm_as<__nv_bfloat16>(ctx, a, wmap, xmap, st);
+    return mx_groups(a.n_tile) == 1 ? gemm_kind<1, false>(ctx, a, wmap, xmap, y_kind, st) : gemm_kind<2, false>(ctx, a, wmap, xmap, y_kind, st);
 }
 
 int q38b_gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales, int K, int M, const void* X, long long X_ld, const void* X_scales, int B,
@@ -861,18 +989,44 @@ int q38b_gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_sc
     return gemm_mx4(ctx, W, W_ld, W_scales, K, M, X, X_ld, X_scales, B, Y, y_kind, ldy, accumulate, stream, false);
 }
 
-size_t q38b_gemm_mx4_scratch_bytes(int K, int B) { return mx_shape(K, B) ? (size_t)B * (K / 2) + q38b_mx4_scale_bytes(K, B) + 16 : 0; }
+size_t q38b_gemm_mx4_scratch_bytes(int K, int B) {
+    if (!mx_shape(K, B) || (B <= MX_FUSE_MAX_B && K <= MX_FUSE_MAX_K)) return 0;
+    return (size_t)B * (K / 2) + q38b_mx4_scale_bytes(K, B) + 16;
+}
 
 int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales, int K, int M, const void* x, int x_kind, long long x_ld, int B, void* Y,
                     int y_kind, long long ldy, int accumulate, void* scratch, size_t scratch_bytes, void* stream) {
-    if (!ctx || !scratch || !mx_shape(K, B)) return Q38B_ERR_ARG;
+    if (!ctx || !x || !Y || !known_kind(x_kind) || !known_kind(y_kind) || x_ld < K || B < 1) return Q38B_ERR_ARG;
+    int rc = check_operand(W, W_ld, W_scales, K, M);
+    if (rc != Q38B_OK) return rc;
+    if (ldy < M) return Q38B_ERR_ARG;
+    if ((uintptr_t)x % kind_size(x_kind) || (uintptr_t)Y % kind_size(y_kind)) return Q38B_ERR_ALIGN;
+    const size_t need = q38b_gemm_mx4_scratch_bytes(K, B);
+    if (need && !scratch) return Q38B_ERR_ARG;
     if ((uintptr_t)scratch & 15) return Q38B_ERR_ALIGN;
-    if (scratch_bytes < q38b_gemm_mx4_scratch_bytes(K, B)) return Q38B_ERR_NOMEM;
+    if (scratch_bytes < need) return Q38B_ERR_NOMEM;
+    if (B <= MX_FUSE_MAX_B && ctx->mx4_pairs <= 0 && !ctx->mx4_two_launches) {
+        MxCut cut = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B, nullptr);   // (the same cut as of the two calls: the same sums)
+        const int steps = (K + MX_K - 1) / MX_K, x_steps = (steps + cut.splits - 1) / cut.splits;
+        if (x_steps * MX_K <= MX_FUSE_MAX_K) {
+            DeviceGuard on(ctx);
+            cut.stages = std::min(MX_MAX_STAGES, (ctx->smem_optin - 1024 - mx_fused_x_bytes(x_steps)) / MX_FUSED_STAGE);
+            CUtensorMap wmap, none;
+            memset(&none, 0, sizeof(none));
+            if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS)) return Q38B_ERR_ARG;
+            MxArgs a = mx_args(ctx, cut, W_scales, K, M, B, Y, ldy, accumulate);
+            a.x = x;
+            a.x_ld = x_ld;
+            a.x_kind = x_kind;
+            a.x_steps = x_steps;
+            return gemm_kind<1, true>(ctx, a, wmap, none, y_kind, (cudaStream_t)stream);
+        }
+    }
+    if (!scratch) return Q38B_ERR_ARG;
     uint8_t* scales = (uint8_t*)scratch;
     uint8_t* codes = scales + q38b_mx4_scale_bytes(K, B);
-    if (!Y || !known_kind(y_kind) || ldy < M) return Q38B_ERR_ARG;
-    int rc = check_operand(W, W_ld, W_scales, K, M);
-    if (rc == Q38B_OK) rc = q38b_quantize_mx4(ctx, x, x_kind, x_ld, K, B, codes, K / 2, scales, stream);
+    if (scratch_bytes < (size_t)(codes - scales) + (size_t)B * (K / 2)) return Q38B_ERR_NOMEM;
+    rc = q38b_quantize_mx4(ctx, x, x_kind, x_ld, K, B, codes, K / 2, scales, stream);
     if (rc != Q38B_OK) return rc;
     return gemm_mx4(ctx, W, W_ld, W_scales, K, M, codes, K / 2, scales, B, Y, y_kind, ldy, accumulate, stream, true);
 }
@@ -881,6 +1035,13 @@ int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_
 int q38b_debug_set_mx4_pairs(q38b_ctx* ctx, int mode) {
     if (!ctx || mode < -1 || mode > 256 || (mode > 0 && mode % 64)) return Q38B_ERR_ARG;
     ctx->mx4_pairs = mode;
+    return Q38B_OK;
+}
+
+// Test hook (not in the public header): q38b_gemm_mx4_x quantizes in a launch of its own whatever the tokens.
+int q38b_debug_set_mx4_two_launches(q38b_ctx* ctx, int enabled) {
+    if (!ctx) return Q38B_ERR_ARG;
+    ctx->mx4_two_launches = enabled ? 1 : 0;
     return Q38B_OK;
 }
 

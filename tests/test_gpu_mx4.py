@@ -218,6 +218,29 @@ def test_product_adds_to_what_is_there_and_writes_no_more(ctx):
         assert (whole == 3.0).all()
 
 
+@pytest.mark.parametrize("B,M,K", [(1, 128, 256), (1, 200, 32), (3, 129, 96), (1, 300, 5120), (7, 640, 2080), (1, 1000, 8192), (1, 128, 8224), (1, 18000, 8224), (1, 256, 17408), (1, 70, 992)])
+@pytest.mark.parametrize("dtype,pad", [("f32", 0), ("bf16", 0), ("f16", 3)])
+def test_few_tokens_are_quantized_by_the_product(ctx, B, M, K, dtype, pad):
+    """One launch or two, with blocks of NaN and zeros, any row stride: the same bits."""
+    x = torch.randn((B, K + pad), generator=torch.Generator().manual_seed(K + B)).to(DTYPES[dtype]).cuda()[:, :K]
+    x[0, 0:32] = 0
+    if B > 2:
+        x[2, K - 1] = float("nan")
+    W = ctx.quantize_mx4(rand(M, K, 7).cuda())
+    one = ctx.gemm_mx4(W, x)
+    try:
+        ctx.lib.q38b_debug_set_mx4_two_launches(ctx.h, 1)
+        scratch = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+        two = torch.empty_like(one)
+        assert ctx.lib.q38b_gemm_mx4_x(ctx.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), K, M, x.data_ptr(), KIND[dtype], K + pad, B, two.data_ptr(), 0, M, 0,
+                                       scratch.data_ptr(), scratch.numel(), ctx._stream()) == 0
+    finally:
+        ctx.lib.q38b_debug_set_mx4_two_launches(ctx.h, 0)
+    ctx.check()
+    assert torch.equal(one.view(torch.int32), two.view(torch.int32)) and torch.equal(torch.isnan(one).all(1).cpu(), torch.arange(B) == 2)
+    assert torch.equal(one.nan_to_num(), ctx.gemm_mx4(W, ctx.quantize_mx4(x)).nan_to_num())
+
+
 def test_nan_block_reaches_its_row_and_column_only(ctx):
     B, M, K = 20, 140, 256
     x, w = rand(B, K, 1), rand(M, K, 2)

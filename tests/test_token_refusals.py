@@ -102,9 +102,10 @@ def test_mx4_sizes_and_scratch(lib):
     assert lib.q38b_mx4_scale_bytes(32, 1) == 512 and lib.q38b_mx4_scale_bytes(5120, 129) == 2 * 40 * 512 and lib.q38b_mx4_scale_bytes(160, 128) == 2 * 512
     assert lib.q38b_mx4_scale_bytes(48, 1) == 0 and lib.q38b_mx4_scale_bytes(64, 0) == 0
     assert lib.q38b_mx4_scale_bytes(1 << 20, 1 << 20) == (1 << 13) * (1 << 13) * 512      # past 32 bits
-    need = lib.q38b_gemm_mx4_scratch_bytes(96, 3)
-    assert need >= 3 * 48 + 512
-    x = lambda **kw: lib.q38b_gemm_mx4_x(CTX, P, 48, P, 96, 200, *[{**dict(x=P, kind=0, ld=96, B=3, Y=P, yk=0, ldy=200, acc=0, s=P, n=need), **kw}[k]   # noqa: E731
+    assert lib.q38b_gemm_mx4_scratch_bytes(96, 1) == 0 == lib.q38b_gemm_mx4_scratch_bytes(8192, 1)      # quantized by the product's kernel
+    need = lib.q38b_gemm_mx4_scratch_bytes(96, 9)
+    assert need >= 9 * 48 + 512 and lib.q38b_gemm_mx4_scratch_bytes(8224, 1) >= 4112 + 65 * 512
+    x = lambda **kw: lib.q38b_gemm_mx4_x(CTX, P, 48, P, 96, 200, *[{**dict(x=P, kind=0, ld=96, B=9, Y=P, yk=0, ldy=200, acc=0, s=P, n=need), **kw}[k]   # noqa: E731
                                                                   for k in ("x", "kind", "ld", "B", "Y", "yk", "ldy", "acc", "s", "n")], None)
-    assert x(n=need - 1) == NOMEM and x(s=P + 8) == ALIGN and x(s=None) == ARG
+    assert x(n=need - 1) == NOMEM and x(s=P + 8) == ALIGN and x(s=None) == ARG and x(x=P + 2) == ALIGN and x(Y=P + 2) == ALIGN and x(B=1, s=P + 4, n=0) == ALIGN
     assert [x(x=None), x(kind=5), x(ld=95), x(B=0), x(Y=None), x(yk=4), x(ldy=100)] == [ARG] * 7
