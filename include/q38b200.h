@@ -334,6 +334,21 @@ int q38b_pass_op_gemv_local(q38b_pass* pass, int matrix, int src_q8k, int dst_f3
 /* The k best of n logits of buffer src_f32 (from float offset off) per column: dst_f32 gets k values followed by k
  * positions (int32 bit patterns), so that a run can return 8 k bytes per column instead of all logits. */
 int q38b_pass_op_topk(q38b_pass* pass, int src_f32, int off, int n, int k, int dst_f32);
+/* q38b_qk_norm_rope between two steps of a pass, on fp32 buffers: a column is a row; offsets and strides in floats of a column.  The heads may
+ * be mended in place (same buffer, offset and stride); otherwise no range that is written may overlap another.  The device arrays
+ * (positions: one int32 for each of max_nb columns) belong to the caller and are read at every run. */
+typedef struct q38b_pass_heads {
+    int src, src_off, src_head;    /* buffer, first element of head 0, distance of two heads */
+    int dst, dst_off, dst_head;
+    int n_heads;
+    const float* weight;           /* [D], or NULL: ones */
+} q38b_pass_heads;
+int q38b_pass_op_qk_norm_rope(q38b_pass* pass, const q38b_pass_heads* q, const q38b_pass_heads* k, int D, int rot, int adjacent, float eps,
+                              float scale, const int* positions_dev, const double* inv_freq_dev);
+/* q38b_adjust_logits on n logits of buffer src_f32 (from float offset off), a column is a row, into dst_f32 from dst_off on (which may be the
+ * same place).  The rules' device arrays (of max_nb rows) belong to the caller and are read at every run: a host gives each row room for its
+ * text, filled with -1, which is passed over, and appends a token by writing it over the first of them. */
+int q38b_pass_op_adjust_logits(q38b_pass* pass, int src_f32, int off, int n, const q38b_logit_rules* rules, int dst_f32, int dst_off);
 /* After q38b_peer_connect the fp32 buffers of a pass live in the arena and matvec steps push their outputs to every
  * peer; q38b_pass_op_barrier then makes them usable on all ranks.  One barrier may cover several matvecs. */
 int q38b_pass_op_barrier(q38b_pass* pass);

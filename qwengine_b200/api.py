@@ -111,6 +111,8 @@ def load_library():
     lib.q38b_gemv_group.argtypes = [vp, u32, i32, vp, sz, i32, vp, vp, vp, vp, vp]
     lib.q38b_qk_norm_rope.argtypes = [vp, vp, vp, i32, i32, i32, C.c_float, C.c_float, vp, vp, i32, i32, i32, vp]
     lib.q38b_adjust_logits.argtypes = [vp, vp, ll, i32, i32, i32, vp, vp, ll, vp]
+    lib.q38b_pass_op_qk_norm_rope.argtypes = [vp, vp, vp, i32, i32, i32, C.c_float, C.c_float, vp, vp]
+    lib.q38b_pass_op_adjust_logits.argtypes = [vp, i32, i32, i32, vp, i32, i32]
     lib.q38b_mx4_scale_bytes.argtypes = [i32, i32]
     lib.q38b_mx4_scale_bytes.restype = sz
     lib.q38b_quantize_mx4.argtypes = [vp, vp, i32, ll, i32, i32, vp, ll, vp, vp]
@@ -138,6 +140,7 @@ def _stream():
 # q38b_heads and q38b_logit_rules as bytes: a call costs a host microsecond less than with ctypes structures
 _pack_heads = struct.Struct("@PPqqqqPi4x").pack      # src, dst, src_row, src_head, dst_row, dst_head, weight, n_heads
 _pack_rules = struct.Struct("@PPPPPPPPqP").pack      # penalties .. bias_begin, masks, mask_ld, mask_of_row
+_pack_pass_heads = struct.Struct("@7i4xP").pack      # q38b_pass_heads: src, src_off, src_head, dst, dst_off, dst_head, n_heads, weight
 _empty = torch.empty_strided
 _current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
@@ -646,6 +649,29 @@ class Pass:
 
     def topk(self, src, off, n, k, dst):
         self.ctx._rc(self.lib.q38b_pass_op_topk(self.h, src, off, n, k, dst), "q38b_pass_op_topk")
+
+    def qk_norm_rope(self, q, k, D, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, adjacent=False, scale=1.0):
+        """q, k (or None): dicts of buf, n_heads and, if need be, off (0), head (D), dst (buf: in place), dst_off, dst_head.  positions int32
+        [max_nb], inv_freq float64 and weights fp32 [D] are device tensors, kept by the pass and read at every run."""
+        for t, dtype, shape in ((positions, torch.int32, (self.max_nb,)), (inv_freq, torch.float64, None), (q_weight, torch.float32, (D,)), (k_weight, torch.float32, (D,))):
+            _need(t is None or (t.dtype == dtype and t.is_contiguous() and t.device == self.ctx.device and (shape is None or t.shape == shape)), "qk_norm_rope: device tensors of the pass")
+        def pack(h, w):
+            off, head, dst = h.get("off", 0), h.get("head", D), h.get("dst", h["buf"])
+            here = dst == h["buf"]
+            return _pack_pass_heads(h["buf"], off, head, dst, h.get("dst_off", off if here else 0), h.get("dst_head", head if here else D), h["n_heads"], 0 if w is None else w.data_ptr())
+        rot = 0 if inv_freq is None else 2 * inv_freq.numel()
+        self.ctx._rc(self.lib.q38b_pass_op_qk_norm_rope(self.h, pack(q, q_weight), None if k is None else pack(k, k_weight), D, rot, int(bool(adjacent)), eps, scale,
+                                                        positions.data_ptr() if rot else None, inv_freq.data_ptr() if rot else None), "q38b_pass_op_qk_norm_rope")
+        self._keep += [positions, inv_freq, q_weight, k_weight]
+
+    def adjust_logits(self, src, off, n, dst=None, dst_off=None, **rules):
+        """The rules of Context.logit_rules on n logits of buffer src (in place where dst is not given); the rules' tensors have max_nb rows, are
+        kept by the pass and read at every run."""
+        dst = src if dst is None else dst
+        dst_off = (off if dst == src else 0) if dst_off is None else dst_off
+        packed = self.ctx.logit_rules(self.max_nb, n, **rules)
+        self.ctx._rc(self.lib.q38b_pass_op_adjust_logits(self.h, src, off, n, packed, dst, dst_off), "q38b_pass_op_adjust_logits")
+        self._keep += [t for t in rules.values() if isinstance(t, torch.Tensor)]
 
     def barrier(self):
         self.ctx._rc(self.lib.q38b_pass_op_barrier(self.h), "q38b_pass_op_barrier")

@@ -51,9 +51,12 @@ Nccl& nccl() {
 }
 constexpr int NCCL_FLOAT = 7;
 
-enum OpKind { OP_QUANT, OP_GEMV, OP_SWIGLU, OP_GATHER, OP_BARRIER, OP_TOPK };
+enum OpKind { OP_QUANT, OP_GEMV, OP_SWIGLU, OP_GATHER, OP_BARRIER, OP_TOPK, OP_HEADS, OP_LOGITS };
 struct Op { int kind, a, b, c, d, n, off; };
 struct Buf { void* ptr; int n; bool q8k; void* peer[8]; int n_peer_ranks; bool in_arena; };
+// q38b_pass_op_qk_norm_rope, q38b_pass_op_adjust_logits: what an Op has no room for (Op::a is their number)
+struct HeadsStep { q38b_pass_heads t[2]; int n_tensors, D, rot, adjacent; float eps, scale; const int* positions; const double* inv_freq; };
+struct LogitsStep { q38b_logit_rules rules; };
 struct Mat { uint32_t type; const void* W; size_t row_bytes; int K, M; bool owned; };
 
 struct PeerPtrs { uint32_t* p[8]; };
@@ -81,6 +84,8 @@ struct q38b_pass {
     std::vector<Buf> bufs;
     std::vector<Mat> mats;
     std::vector<Op> ops;
+    std::vector<HeadsStep> heads;
+    std::vector<LogitsStep> logits;
     cudaGraphExec_t graphs[9] = {};
     size_t arena_mark = (size_t)-1;
     int peer_store = 1;
@@ -374,6 +379,23 @@ int enqueue_ops(q38b_pass* p, int nb, cudaStream_t st) {
                 rc = q38b_topk(ctx, (const float*)s.ptr + o.off, s.n, o.n, nb, o.d, 0, (float*)d.ptr, (int*)d.ptr + o.d, d.n, st);
                 break;
             }
+            case OP_HEADS: {
+                const HeadsStep& s = p->heads[o.a];
+                q38b_heads t[2];
+                for (int i = 0; i < s.n_tensors; i++) {
+                    const q38b_pass_heads& h = s.t[i];
+                    const Buf &from = p->bufs[h.src], &to = p->bufs[h.dst];
+                    t[i] = {(const float*)from.ptr + h.src_off, (float*)to.ptr + h.dst_off, from.n, h.src_head, to.n, h.dst_head, h.weight, h.n_heads};
+                }
+                rc = q38b_qk_norm_rope(ctx, &t[0], s.n_tensors > 1 ? &t[1] : nullptr, s.D, s.rot, s.adjacent, s.eps, s.scale, s.positions, s.inv_freq, Q38B_OUT_F32,
+                                       Q38B_OUT_F32, nb, st);
+                break;
+            }
+            case OP_LOGITS: {   // a: which rules, b: source, off: first logit, n: how many, c: destination, d: its first logit
+                const Buf &from = p->bufs[o.b], &to = p->bufs[o.c];
+                rc = q38b_adjust_logits(ctx, (const float*)from.ptr + o.off, from.n, o.n, nb, 0, &p->logits[o.a].rules, (float*)to.ptr + o.d, to.n, st);
+                break;
+            }
             case OP_BARRIER: {
                 if (n_barriers == 0) break;
                 if (ctx->pending_sync_seq >= 0) {   // two barriers in a row: the earlier one runs by itself
@@ -612,6 +634,44 @@ int q38b_pass_op_topk(q38b_pass* p, int src, int off, int n, int k, int dst) {
         return Q38B_ERR_ARG;
     if ((n + 1023) / 1024 > 384) return Q38B_ERR_UNSUPPORTED;
     p->ops.push_back({OP_TOPK, src, dst, 0, k, n, off});
+    return Q38B_OK;
+}
+
+int q38b_pass_op_qk_norm_rope(q38b_pass* p, const q38b_pass_heads* q, const q38b_pass_heads* k, int D, int rot, int adjacent, float eps, float scale,
+                              const int* positions, const double* inv_freq) {
+    if (!p || !q || D < 1 || D > 1024 || rot < 0 || rot > D || rot % 2 || (rot > 0 && (!positions || !inv_freq))) return Q38B_ERR_ARG;
+    if (((uintptr_t)positions & 3) || ((uintptr_t)inv_freq & 7)) return Q38B_ERR_ALIGN;
+    HeadsStep s = {{*q, k ? *k : q38b_pass_heads{}}, k ? 2 : 1, D, rot, adjacent, eps, scale, positions, inv_freq};
+    struct Span { int buf; long long lo, hi; bool written; int of; };
+    std::vector<Span> spans;
+    for (int i = 0; i < s.n_tensors; i++) {
+        const q38b_pass_heads& t = s.t[i];
+        if (!is_f32(p, t.src) || !is_f32(p, t.dst) || t.n_heads < 1 || t.src_off < 0 || t.dst_off < 0 || t.src_head < 0) return Q38B_ERR_ARG;
+        if (t.n_heads > 1 && t.dst_head < D) return Q38B_ERR_ARG;
+        if ((uintptr_t)t.weight & 3) return Q38B_ERR_ALIGN;
+        const long long src_end = t.src_off + (long long)(t.n_heads - 1) * t.src_head + D, dst_end = t.dst_off + (long long)(t.n_heads - 1) * t.dst_head + D;
+        if (src_end > p->bufs[t.src].n || dst_end > p->bufs[t.dst].n) return Q38B_ERR_ARG;
+        const bool in_place = t.src == t.dst && t.src_off == t.dst_off && (t.n_heads == 1 || t.src_head == t.dst_head);
+        if (!in_place) spans.push_back({t.src, t.src_off, src_end, false, i});
+        spans.push_back({t.dst, t.dst_off, dst_end, true, i});
+    }
+    // what is written lies apart from everything else that is read or written (but for heads mended in place)
+    for (const Span& w : spans)
+        for (const Span& o : spans)
+            if (w.written && &w != &o && w.buf == o.buf && w.lo < o.hi && o.lo < w.hi) return Q38B_ERR_ARG;
+    p->heads.push_back(s);
+    p->ops.push_back({OP_HEADS, (int)p->heads.size() - 1, 0, 0, 0, 0, 0});
+    return Q38B_OK;
+}
+
+int q38b_pass_op_adjust_logits(q38b_pass* p, int src, int off, int n, const q38b_logit_rules* rules, int dst, int dst_off) {
+    if (!p || !rules || !is_f32(p, src) || !is_f32(p, dst) || off < 0 || dst_off < 0 || n < 1 || off + (long long)n > p->bufs[src].n || dst_off + (long long)n > p->bufs[dst].n)
+        return Q38B_ERR_ARG;
+    if (src == dst && off != dst_off && off < dst_off + (long long)n && dst_off < off + (long long)n) return Q38B_ERR_ARG;
+    const int rc = q38b_logit_rules_check(rules, n, 0);
+    if (rc != Q38B_OK) return rc;
+    p->logits.push_back({*rules});
+    p->ops.push_back({OP_LOGITS, (int)p->logits.size() - 1, src, dst, dst_off, n, off});
     return Q38B_OK;
 }
 

@@ -20,6 +20,7 @@ from . import formats as F
 
 HIDDEN, FF, INNER, VOCAB = 5120, 17408, 6144, 248320
 N_LAYERS = 64
+HEAD_DIM = 256     # 24 query heads beside their gates, 4 key heads; the first 64 elements of a head rotate
 TOPK = 32          # candidates the sampler takes from the head (TK of the reference, src/cuda/ops.cu:821)
 # fp16 super-scale magnitudes at which a matvec of uniformly random (zero-mean, see synth.ZERO_MEAN_DMIN) blocks has
 # a gain near 1, so that the 64 chained layers of the synthetic pass stay inside the fp32 range
@@ -63,7 +64,7 @@ def total_weight_bytes(n_layers=N_LAYERS, head=True):
     return sum(m.nbytes for m in all_specs(n_layers, head))
 
 
-def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather="peer", replicate_small=True):
+def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather="peer", replicate_small=True, heads=None, rules=None):
     """Records the pass on `ps` (qwengine_b200.Pass).
 
     make_matrix(spec, rows) -> matrix id for this rank's shard of `rows` rows (rows = spec.M // world);
@@ -77,6 +78,9 @@ def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather
     rank and computed by every rank: streaming 65 MB costs a GPU about 11 us, sharding them over N GPUs saves at most
     (1 - 1/N) of that and costs two cross-GPU exchanges of 4-5 us each per layer.  The FFN (115 MB per layer) and the
     head (1 GB) are row-sharded.  Bit-identical either way: a row's result does not depend on who computes it.
+    heads: dict(positions, inv_freq, q_weight, k_weight, eps) of device tensors (Pass.qk_norm_rope): the attention layers then norm and rotate their
+    query heads (24 of 256, beside their gates) and key heads (4 of 256) in place, as the reference does before its attention.
+    rules: dict of Context.logit_rules' tensors: the head's logits are penalised, biased and masked in place before the top-k.
     Returns dict(in_buf, out_buf, out_len, topk_buf, topk_k).
     """
     x_in = ps.buffer_f32(HIDDEN)           # the token's hidden state: read by layer 0 only, never written, so that
@@ -122,6 +126,8 @@ def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather
             matvec(mats[0], xq, big, 0, shard=not whole)
             proj_out = mats[1]
         sync(not whole)
+        if attn and heads is not None:
+            ps.qk_norm_rope(dict(buf=big, n_heads=12288 // (2 * HEAD_DIM), head=2 * HEAD_DIM), dict(buf=kv, n_heads=1024 // HEAD_DIM), HEAD_DIM, **heads)
         ps.quantize(big, 0, INNER, iq)
         matvec(proj_out, iq, x, 0, shard=not whole)
         sync(not whole)
@@ -142,6 +148,8 @@ def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather
         ps.quantize(x, 0, HIDDEN, xq)
         matvec(MatSpec("lm_head", "Q6_K", VOCAB, HIDDEN), xq, logits, 0)
         sync()
+        if rules is not None:
+            ps.adjust_logits(logits, 0, VOCAB, **rules)
         if hasattr(ps, "topk"):
             # what the sampler needs from the head (Engine::decode_batch's top-k, src/runtime/engine.cpp:1680 of the
             # reference project): TOPK values and positions per column instead of 248320 logits
