@@ -174,14 +174,17 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, 6) heads4_kernel(const Heads
 // ---------------------------------------------------------------------------------------------------------------
 // Logits.  count_v: times token v occurs among the generated tokens of the row, seen_v: in prompt or generated ones.
 //   seen: l = l > 0 ? l / rep : l * rep;  l -= freq * count_v;  count_v > 0: l -= pres;  l += bias_v;  mask bit clear: l = -inf
-// A CTA owns CHUNK logits of a row.  They pass through the mask first (neighbours in a warp, so any alignment and stride will do; in place
-// nothing passes through, only masked logits are written).  Then it counts the row's tokens that fall among them in shared memory (whole
-// numbers, so the order of the atomics does not matter) and mends the logits that occur: few, packed 32 at a time so that no warp computes
-// for one lane.  Biases come last, the last entry of each token found in the same shared words.
-// Every CTA of a row reads the whole text, which costs as much as the logits do once texts are long; so a CTA takes as many logits as leaves
-// three to an SM, and an id costs four instructions (difference, comparison, address, predicated atomic).  Clusters that share a text by
-// atomics in each other's memory were slower at every size (128 rows of 248320 with 20000-token texts: 111 us in twos, 161 in eights, 101
-// alone, all with 8192 logits a CTA): their CTAs stream and count in step.  So 92 us = 2.9 TB/s; without texts 63 us.
+// A CTA owns CHUNK logits of a row.  Their loads are issued first (four neighbours a lane where rows are aligned to 16 bytes, else one: any
+// stride will do; in place nothing is loaded and only masked logits are written).  While they are on their way the CTA counts the row's tokens
+// that fall among them in shared memory (whole numbers, so the order of the atomics does not matter); then the logits pass through the
+// mask, and those that occur, few, are mended where they were written, packed 32 at a time so that no warp computes for one lane.  Biases
+// come last, the last entry of each token found in the same shared words.
+// Every CTA of a row reads the whole text, so a CTA takes as many logits as leaves three to an SM (two are there at a time), and an id costs
+// four instructions (difference, comparison, address, predicated atomic).  128 rows of 248320: nothing but the counting of one token each
+// 50 us = 5.1 TB/s, texts of 4000 to 16000 tokens 75, with masks, generated tokens and biases 91 = 2.9 TB/s.  What was slower there: clusters that
+// share a text by atomics in each other's memory (101 alone, 111 in twos, 161 in eights, all with 8192 logits a CTA); CTAs that stay and bring
+// the next piece's logits ahead (138); half of the warps counting a piece ahead of the others (112 mending in memory, 156 in registers): a warp
+// then waits too often for too few others.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int LG_THREADS = 512, LG_WARPS = LG_THREADS / 32;
 constexpr uint32_t LG_PROMPT = 0x80000000u;   // seen in the prompt; the other bits count generated tokens
@@ -205,9 +208,8 @@ __device__ __forceinline__ void count_id(uint32_t words, int id, uint32_t first,
         asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %0, %1;\n\t@p red.shared.or.b32 [%2], %3;\n\t}" ::"r"(at), "r"(n), "r"(words + 4u * at), "r"(LG_PROMPT) : "memory");
 }
 template <bool GENERATED>
-__device__ __forceinline__ void count_ids(uint32_t words, const int* ids, long long len, uint32_t first, uint32_t n) {
+__device__ __forceinline__ void count_ids(uint32_t words, const int* ids, long long len, uint32_t first, uint32_t n, int tid) {
     if (len <= 0) return;
-    const int tid = threadIdx.x;
     // four ids a load, two loads of a thread ahead of their atomics; the ends that are no whole 16 bytes by themselves
     const int head = (int)min(len, (long long)((16 - ((uintptr_t)ids & 15)) & 15) / 4);
     const long long quads = (len - head) / 4;
@@ -235,22 +237,25 @@ __device__ __forceinline__ void count_ids(uint32_t words, const int* ids, long l
     if (tid < 4 && head + 4 * quads + tid < len) count_id<GENERATED>(words, ids[head + 4 * quads + tid], first, n);
 }
 
-template <int CHUNK>
-__global__ void __launch_bounds__(LG_THREADS, 3) logits_kernel(const LogitsArgs a) {
-    constexpr int UN = CHUNK / LG_THREADS < 16 ? CHUNK / LG_THREADS : 16;   // logits of a thread on their way at a time
-    extern __shared__ __align__(16) uint32_t seen[];                        // [CHUNK], where there are texts or biases
-    __shared__ uint16_t packed[LG_WARPS][64];
+// VEC: rows of x and y are aligned to 16 bytes, a lane has four neighbours at a time.
+template <int CHUNK, bool VEC>
+__global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kernel(const LogitsArgs a) {
+    constexpr int E = VEC ? 4 : 1, WARP = 32 * E, STEP = LG_THREADS * E;   // logits of a lane, a warp, the block at a time
+    constexpr int UN = CHUNK / STEP;                                       // ... of a lane altogether
+    extern __shared__ __align__(16) uint32_t seen[];                       // [CHUNK], where there are texts or biases
+    __shared__ uint16_t packed[LG_WARPS][32 + WARP];
     const int row = blockIdx.y, c0 = blockIdx.x * CHUNK, n = min(CHUNK, a.n - c0), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t first = (uint32_t)(a.index_offset + c0);
     const bool counts = a.r.history != nullptr, in_place = a.x == a.y;
     const float* x = a.x + row * a.x_ld + c0;
     float* y = a.y + row * a.y_ld + c0;
-    // what the later parts need, on its way before the logits: the text's and the biases' ends, a thread's first bias
-    long long text = 0, text_len = 0, prompt = 0, bias0 = 0, n_bias = 0;
+    // what the later parts need, on its way before the logits
+    long long text = 0, text_len = 0, bias0 = 0, n_bias = 0;
+    int prompt = 0;
     if (counts) {
         text = a.r.history_begin[row];
         text_len = a.r.history_begin[row + 1] - text;
-        prompt = a.r.prompt_len ? min(max((long long)a.r.prompt_len[row], 0LL), max(text_len, 0LL)) : 0;
+        if (a.r.prompt_len) prompt = (int)max(0LL, min((long long)a.r.prompt_len[row], text_len));
     }
     if (a.r.bias_ids) {
         bias0 = a.r.bias_begin[row];
@@ -260,58 +265,73 @@ __global__ void __launch_bounds__(LG_THREADS, 3) logits_kernel(const LogitsArgs 
     const uint32_t* mask = a.r.masks + (m >= 0 ? m * a.r.mask_ld : 0);
     const uint32_t mask_end = (uint32_t)(a.index_offset + a.n - 1) >> 5;
     auto allowed = [&](uint32_t at) { return m < 0 || (mask[(first + at) >> 5] >> ((first + at) & 31u) & 1u); };
+    // the logits on their way
+    float v[UN][E];
+    if (!in_place) {
+#pragma unroll
+        for (int u = 0; u < UN; u++) {
+            const int i = STEP * u + E * tid;
+            if constexpr (VEC) {
+                const float4 q = i + 3 < n ? *(const float4*)(x + i)   // (or the row's last one to three)
+                                           : make_float4(i < n ? x[i] : 0.0f, i + 1 < n ? x[i + 1] : 0.0f, i + 2 < n ? x[i + 2] : 0.0f, 0.0f);
+                v[u][0] = q.x; v[u][1] = q.y; v[u][2] = q.z; v[u][3] = q.w;
+            } else {
+                v[u][0] = i < n ? x[i] : 0.0f;
+            }
+        }
+    }
+    // the mask bits of the warp's logits: lane E u + k has those of the k-th 32 of its u-th WARP
+    uint32_t bits = 0xFFFFFFFFu;
+    const int masked_at = STEP * (lane / E) + WARP * warp + 32 * (lane % E);
+    if (m >= 0 && lane < E * UN && masked_at < n) {
+        const uint32_t at = first + (uint32_t)masked_at;
+        bits = __funnelshift_r(mask[at >> 5], mask[min((at >> 5) + 1u, mask_end)], at & 31u);
+    }
+    // biases among the block's logits; a thread keeps its first one's place
+    const uint32_t bias_at = tid < n_bias ? (uint32_t)a.r.bias_ids[bias0 + tid] - first : 0xFFFFFFFFu;
+    bool any = bias_at < (uint32_t)n;
+    for (long long j = tid + LG_THREADS; j < n_bias; j += LG_THREADS) any |= (uint32_t)a.r.bias_ids[bias0 + j] - first < (uint32_t)n;
+    if (counts)
+        for (int i = 4 * tid; i < CHUNK; i += 4 * LG_THREADS) *(uint4*)(seen + i) = make_uint4(0, 0, 0, 0);
+    if (counts) {
+        __syncthreads();
+        count_ids<false>(smem_u32(seen), a.r.history + text, prompt, first, (uint32_t)n, tid);
+        count_ids<true>(smem_u32(seen), a.r.history + text + prompt, text_len - prompt, first, (uint32_t)n, tid);
+    }
+    // ... and through
     if (!in_place || m >= 0) {
-#pragma unroll 1
-        for (int c = 0; c < CHUNK && c < n; c += LG_THREADS * UN) {
-            float v[UN];
-            if (!in_place) {
+        const float minus_inf = __int_as_float(0xFF800000);
 #pragma unroll
-                for (int u = 0; u < UN; u++) v[u] = c + LG_THREADS * u + tid < n ? x[c + LG_THREADS * u + tid] : 0.0f;
-            }
-            // the mask bits of the warp's logits: lane u has those of its 32 neighbours c + LG_THREADS * u + 32 * warp ..
-            uint32_t bits = 0xFFFFFFFFu;
-            if (m >= 0 && lane < UN && c + LG_THREADS * lane + 32 * warp < n) {
-                const uint32_t at = first + (uint32_t)(c + LG_THREADS * lane + 32 * warp);
-                bits = __funnelshift_r(mask[at >> 5], mask[min((at >> 5) + 1u, mask_end)], at & 31u);
-            }
+        for (int u = 0; u < UN; u++) {
+            const int i = STEP * u + E * tid;
+            const uint32_t keep = __shfl_sync(0xffffffffu, bits, E * u + E * lane / 32) >> (E * lane % 32);
+            if constexpr (VEC) {
+                if (i + 3 < n && !in_place) {
+                    *(float4*)(y + i) = make_float4(keep & 1u ? v[u][0] : minus_inf, keep & 2u ? v[u][1] : minus_inf, keep & 4u ? v[u][2] : minus_inf, keep & 8u ? v[u][3] : minus_inf);
+                } else {   // in place, and the row's last one to three
 #pragma unroll
-            for (int u = 0; u < UN; u++) {
-                const int i = c + LG_THREADS * u + tid;
-                const bool keep = __shfl_sync(0xffffffffu, bits, u) >> lane & 1u;
-                if (i < n) {
-                    if (!keep) y[i] = __int_as_float(0xFF800000);
-                    else if (!in_place) y[i] = v[u];
+                    for (int k = 0; k < 4; k++) {
+                        if (i + k >= n) break;
+                        if (!(keep >> k & 1u)) y[i + k] = minus_inf;
+                        else if (!in_place) y[i + k] = v[u][k];
+                    }
                 }
+            } else if (i < n) {
+                if (!(keep & 1u)) y[i] = minus_inf;
+                else if (!in_place) y[i] = v[u][0];
             }
         }
     }
     if (!counts && !a.r.bias_ids) return;
-    uint32_t bias_at = 0xFFFFFFFFu;
-    if (tid < n_bias) bias_at = (uint32_t)a.r.bias_ids[bias0 + tid] - first;
-    const int* ids = a.r.bias_ids + bias0;
-    auto each = [&](auto&& f) {   // f(entry, place) for this thread's biases among the block's logits
-        if (bias_at < (uint32_t)n) f((uint32_t)tid, bias_at);
-        for (long long j = tid + LG_THREADS; j < n_bias; j += LG_THREADS) {
-            const uint32_t at = (uint32_t)ids[j] - first;
-            if (at < (uint32_t)n) f((uint32_t)j, at);
-        }
-    };
-    bool any = false;
-    each([&](uint32_t, uint32_t) { any = true; });
-    if (counts)
-        for (int i = 4 * tid; i < CHUNK; i += 4 * LG_THREADS) *(uint4*)(seen + i) = make_uint4(0, 0, 0, 0);
-    any = __syncthreads_or(any);   // (and every logit is through)
+    any = __syncthreads_or(any);   // (every id is counted, and every logit through)
     if (counts) {
-        count_ids<false>(smem_u32(seen), a.r.history + text, prompt, first, (uint32_t)n);
-        count_ids<true>(smem_u32(seen), a.r.history + text + prompt, text_len - prompt, first, (uint32_t)n);
         const float repetition = a.r.penalties[3 * row], frequency = a.r.penalties[3 * row + 1], presence = a.r.penalties[3 * row + 2];
-        __syncthreads();
-        // a warp's share of the words, 32 at a time; places of those that count are packed and mended 32 at a time
+        // a warp looks through its share of the words; places of those that count are packed and mended 32 at a time
         uint16_t* mine = packed[warp];
         int waiting = 0;
-        auto mend = [&](int k) {   // the warp's lanes below k
+        auto mend = [&](int from, int k) {   // k of the packed places
             if (lane < k) {
-                const uint32_t at = mine[lane], s = seen[at], times = s & ~LG_PROMPT;
+                const uint32_t at = mine[from + lane], times = seen[at] & ~LG_PROMPT;
                 if (allowed(at)) {
                     float l = y[at];
                     l = l > 0.0f ? __fdiv_rn(l, repetition) : l * repetition;
@@ -320,31 +340,47 @@ __global__ void __launch_bounds__(LG_THREADS, 3) logits_kernel(const LogitsArgs 
                 }
             }
         };
-        for (int i = 32 * warp; i < n; i += LG_THREADS) {
-            const uint32_t hit = __ballot_sync(0xffffffffu, seen[i + lane] != 0u);
-            if (!hit) continue;
-            if (hit >> lane & 1u) mine[waiting + __popc(hit & ((1u << lane) - 1u))] = (uint16_t)(i + lane);
-            waiting += __popc(hit);
+        for (int i = WARP * warp; i < n; i += STEP) {
+            uint32_t w[E];
+            if constexpr (VEC) {
+                const uint4 q = *(const uint4*)(seen + i + 4 * lane);
+                w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+                if (!__any_sync(0xffffffffu, (q.x | q.y | q.z | q.w) != 0u)) continue;
+            } else {
+                w[0] = seen[i + lane];
+            }
+#pragma unroll
+            for (int k = 0; k < E; k++) {
+                const uint32_t hit = __ballot_sync(0xffffffffu, w[k] != 0u);
+                if (w[k]) mine[waiting + __popc(hit & ((1u << lane) - 1u))] = (uint16_t)(i + E * lane + k);
+                waiting += __popc(hit);
+            }
             __syncwarp();
-            if (waiting >= 32) {
-                mend(32);
-                const uint16_t rest = lane < waiting - 32 ? mine[32 + lane] : (uint16_t)0;
-                __syncwarp();
-                mine[lane] = rest;
+            while (waiting >= 32) {   // the last 32
                 waiting -= 32;
+                mend(waiting, 32);
                 __syncwarp();
             }
         }
-        mend(waiting);
+        mend(0, waiting);
     }
     if (!any) return;
+    const long long biases = a.r.bias_begin[row], count_b = a.r.bias_begin[row + 1] - biases;   // (again, not kept in registers)
+    const int* ids = a.r.bias_ids + biases;
+    auto each = [&](auto&& f) {   // f(entry, place) for this thread's biases among the block's logits
+        if (bias_at < (uint32_t)n) f((uint32_t)tid, bias_at);
+        for (long long j = tid + LG_THREADS; j < count_b; j += LG_THREADS) {
+            const uint32_t at = (uint32_t)ids[j] - first;
+            if (at < (uint32_t)n) f((uint32_t)j, at);
+        }
+    };
     __syncthreads();
     each([&](uint32_t, uint32_t at) { seen[at] = 0u; });
     __syncthreads();
     each([&](uint32_t j, uint32_t at) { atomicMax(&seen[at], j + 1u); });
     __syncthreads();
     each([&](uint32_t j, uint32_t at) {
-        if (seen[at] == j + 1u && allowed(at)) y[at] += a.r.bias_values[bias0 + j];
+        if (seen[at] == j + 1u && allowed(at)) y[at] += a.r.bias_values[biases + j];
     });
 }
 
@@ -388,13 +424,20 @@ int heads_from(q38b_ctx* ctx, const HeadsArgs& a, int out_kind, cudaStream_t st)
     return out_kind == Q38B_OUT_F32 ? heads_as<Tin, float>(ctx, a, st) : out_kind == Q38B_OUT_F16 ? heads_as<Tin, __half>(ctx, a, st) : heads_as<Tin, __nv_bfloat16>(ctx, a, st);
 }
 
-template <int CHUNK>
+template <int CHUNK, bool VEC>
 int logits_as(q38b_ctx* ctx, const LogitsArgs& a, int n_rows, cudaStream_t st) {
-    const int rc = q38b_ensure_kernel_smem(ctx, (const void*)logits_kernel<CHUNK>, CHUNK * 4, false);
+    const int rc = q38b_ensure_kernel_smem(ctx, (const void*)logits_kernel<CHUNK, VEC>, CHUNK * 4, false);
     if (rc != Q38B_OK) return rc;
-    const size_t smem = a.r.history || a.r.bias_ids ? CHUNK * sizeof(uint32_t) : 0;
-    logits_kernel<CHUNK><<<dim3((unsigned)((a.n + CHUNK - 1) / CHUNK), (unsigned)n_rows), LG_THREADS, smem, st>>>(a);
+    const size_t smem = a.r.history || a.r.bias_ids ? CHUNK * 4 : 0;
+    logits_kernel<CHUNK, VEC><<<dim3((unsigned)((a.n + CHUNK - 1) / CHUNK), (unsigned)n_rows), LG_THREADS, smem, st>>>(a);
     return launch_status(ctx, cudaSuccess);
+}
+template <bool VEC>
+int logits_in(q38b_ctx* ctx, const LogitsArgs& a, int n_rows, cudaStream_t st) {
+    // as many logits a CTA as still leaves three CTAs to every SM, or the fewest
+    const auto fills = [&](int chunk) { return (long long)n_rows * ((a.n + chunk - 1) / chunk) >= 3 * ctx->sm_count; };
+    return fills(16384) ? logits_as<16384, VEC>(ctx, a, n_rows, st) : fills(8192) ? logits_as<8192, VEC>(ctx, a, n_rows, st)
+         : fills(4096)  ? logits_as<4096, VEC>(ctx, a, n_rows, st) : logits_as<2048, VEC>(ctx, a, n_rows, st);
 }
 
 }  // namespace
@@ -461,10 +504,8 @@ int q38b_adjust_logits(q38b_ctx* ctx, const float* x, long long x_ld, int n, int
     a.index_offset = index_offset;
     DeviceGuard on(ctx);
     cudaStream_t st = (cudaStream_t)stream;
-    // as many logits a CTA as still leaves three CTAs to every SM, or the fewest
-    const auto fills = [&](int chunk) { return (long long)n_rows * ((n + chunk - 1) / chunk) >= 3 * ctx->sm_count; };
-    return fills(16384) ? logits_as<16384>(ctx, a, n_rows, st) : fills(8192) ? logits_as<8192>(ctx, a, n_rows, st)
-         : fills(4096)  ? logits_as<4096>(ctx, a, n_rows, st) : logits_as<2048>(ctx, a, n_rows, st);
+    const bool vec = (((uintptr_t)x | (uintptr_t)y) & 15) == 0 && (n_rows == 1 || ((x_ld | y_ld) & 3) == 0);
+    return vec ? logits_in<true>(ctx, a, n_rows, st) : logits_in<false>(ctx, a, n_rows, st);
 }
 
 }  // extern "C"

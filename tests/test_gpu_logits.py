@@ -157,6 +157,34 @@ def test_row_strides_offsets_and_in_place(ctx, pad, start):
     assert (flat == 123.0).all()
 
 
+@pytest.mark.parametrize("rows,n,hist,nbias,n_masks,off", [(40, 248320, 3000, 40, 7, 0), (300, 20011, 900, 5, 300, 0), (41, 130000, 30000, 700, 3, 77), (640, 8192, 50, 0, 0, 31),
+                                                           (641, 8193, 0, 3, 2, 0), (1200, 4099, 300, 20, 1200, 0)])
+def test_four_at_a_time_give_the_bits_of_one(ctx, rows, n, hist, nbias, n_masks, off):
+    """Rows that are aligned (contiguous ones) or not (an odd distance), every size of a CTA's piece."""
+    g = np.random.default_rng(rows)
+    x = torch.randn((rows, n + 3), generator=torch.Generator(device="cuda").manual_seed(rows), device="cuda")[:, 1:n + 1]
+    length = g.integers(0, hist + 1, rows)
+    begin = np.concatenate([[0], np.cumsum(length)])
+    dev = lambda v, dtype: torch.from_numpy(np.ascontiguousarray(v)).to(dtype).cuda()   # noqa: E731
+    rules = dict(masks=dev(g.integers(-2 ** 31, 2 ** 31, (max(n_masks, 1), (off + n + 31) // 32)), torch.int32), mask_of_row=dev(g.integers(-1, n_masks, rows), torch.int32)) if n_masks else {}
+    if hist:
+        rules.update(penalties=dev(np.stack([0.8 + g.random(rows), g.random(rows) - 0.2, g.random(rows)], 1), torch.float32), history_begin=dev(begin, torch.int64),
+                     history=dev(np.exp(g.random(begin[-1]) * np.log(off + n + 9)).astype(np.int64) - 2, torch.int32), prompt_len=dev(g.integers(-3, hist + 9, rows), torch.int32))
+    if nbias:
+        rules.update(bias_ids=dev(g.integers(-2, off + n + 2, rows * nbias), torch.int32), bias_values=dev(g.standard_normal(rows * nbias), torch.float32), bias_begin=dev(np.arange(rows + 1) * nbias, torch.int64))
+    got = ctx.adjust_logits(x, index_offset=off, **rules)
+    wide = torch.empty((rows, (n + 7) // 4 * 4), device="cuda")
+    aligned = torch.empty_like(wide)[:, :n]
+    wide[:, :n] = x
+    want = ctx.adjust_logits(wide[:, :n], index_offset=off, out=aligned, **rules)
+    assert torch.equal(got.view(torch.int32), want.contiguous().view(torch.int32))
+    want = want.contiguous()
+    assert torch.equal(ctx.adjust_logits(wide[:, :n], index_offset=off, out=wide[:, :n], **rules).contiguous().view(torch.int32), want.view(torch.int32))
+    here = ctx.adjust_logits(x, index_offset=off, out=x, **rules)
+    assert torch.equal(here.contiguous().view(torch.int32), want.view(torch.int32))
+    ctx.check()
+
+
 def test_long_histories_give_the_same_bits_each_time(ctx):
     x, rules = case(6, 50000, 60000, 100, 2)
     a = run(ctx, x, **rules)
