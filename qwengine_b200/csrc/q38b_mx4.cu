@@ -57,15 +57,15 @@ struct MxWalk {
     int k;           // this lane's first value
     long long tile;  // the scales' first K tile of the warp, in tiles
 };
-__host__ __device__ inline long long mx_walk_warps(int K, int rows) { return (long long)(rows + 127) / 128 * 32 * ((K + 255) / 256); }
-__device__ __forceinline__ bool mx_walk(int K, int rows, MxWalk& w) {
-    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), kc = (K + 255) / 256;
-    if (item >= mx_walk_warps(K, rows)) return false;
+__host__ __device__ inline long long mx_walk_warps(int K, int rows, int span) { return (long long)(rows + 127) / 128 * 32 * ((K + span - 1) / span); }
+__device__ __forceinline__ bool mx_walk(int K, int rows, int span, MxWalk& w) {   // span: the warp's values of a row, a multiple of 256
+    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), kc = (K + span - 1) / span;
+    if (item >= mx_walk_warps(K, rows, span)) return false;
     // the eight warps of a block: neighbouring rows, so that their scales are one piece of 128 bytes
     const long long group = item / 8, at = group / kc, c = group % kc;
     w.row = at / 4 * 128 + at % 4 * 8 + (item & 7);
-    w.k = (int)c * 256 + 8 * (int)(threadIdx.x & 31);
-    w.tile = at / 4 * mx_tiles_k(K) + 2 * c;
+    w.k = (int)c * span + 8 * (int)(threadIdx.x & 31);
+    w.tile = at / 4 * mx_tiles_k(K) + span / 128 * c;
     return true;
 }
 
@@ -76,60 +76,83 @@ template <typename T> __device__ __forceinline__ void raw8_values(const Raw8<T>&
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = to_f32(e[i]);
 }
-// the bit pattern of the largest magnitude; a NaN's exceeds them all
-template <typename T> __device__ __forceinline__ uint32_t raw8_top(const Raw8<T>& r, const float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {   // two at a time: magnitudes of 16-bit floats compare like their bits
-        const uint32_t m = __vmaxu2(__vmaxu2(r.q[0].x & 0x7FFF7FFFu, r.q[0].y & 0x7FFF7FFFu), __vmaxu2(r.q[0].z & 0x7FFF7FFFu, r.q[0].w & 0x7FFF7FFFu));
-        const unsigned short top = (unsigned short)max(m & 0xFFFFu, m >> 16);
-        return __float_as_uint(to_f32(*(const T*)&top));
-    } else {
-        uint32_t top = 0u;
-#pragma unroll
-        for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-        return top;
-    }
+// 16-bit types: the largest magnitudes of the even and of the odd four (magnitudes compare like their bits, a NaN's exceeds them all)
+template <typename T> __device__ __forceinline__ uint32_t raw8_top16(const Raw8<T>& r) {
+    return __vmaxu2(__vmaxu2(r.q[0].x & 0x7FFF7FFFu, r.q[0].y & 0x7FFF7FFFu), __vmaxu2(r.q[0].z & 0x7FFF7FFFu, r.q[0].w & 0x7FFF7FFFu));
 }
 
+constexpr __host__ __device__ int mx_quantize_span(size_t size) { return size == 2 ? 512 : 256; }   // values of a row a warp takes, all on their way at once
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, long long x_ld, int K, int rows, uint8_t* codes, long long codes_ld, uint8_t* scales) {
     pdl_launch_dependents();   // (a product behind it brings its first weights meanwhile)
     MxWalk w;
-    if (!mx_walk(K, rows, w)) return;
+    constexpr int SPANS = mx_quantize_span(sizeof(T)) / 256;
+    if (!mx_walk(K, rows, 256 * SPANS, w)) return;
     const int lane = threadIdx.x & 31;
-    Raw8<T> raw[4] = {};
+    Raw8<T> ahead[SPANS][4] = {};
+#pragma unroll
+    for (int p = 0; p < SPANS; p++)
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (w.row + 32 * j < rows && w.k < K) {
-            const T* p = x + (w.row + 32 * j) * x_ld + w.k;
+        if (w.row + 32 * j < rows && w.k + 256 * p < K) {
+            const T* from = x + (w.row + 32 * j) * x_ld + w.k + 256 * p;
             if constexpr (VEC) {
-                raw[j] = *(const Raw8<T>*)p;
+                ahead[p][j] = *(const Raw8<T>*)from;
             } else {
                 T e[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) e[i] = p[i];
-                memcpy(&raw[j], e, sizeof(e));
+                for (int i = 0; i < 8; i++) e[i] = from[i];
+                memcpy(&ahead[p][j], e, sizeof(e));
             }
         }
-    uint32_t word[4];
+#pragma unroll
+    for (int p = 0; p < SPANS; p++, w.k += 256, w.tile += 2) {
+    const Raw8<T>(&raw)[4] = ahead[p];
+    // the largest magnitudes of the four rows' blocks (16-bit types: two rows a word, which compare and travel together)
+    uint32_t top[4];
+    if constexpr (sizeof(T) == 2) {
+        uint32_t pair[2];
+#pragma unroll
+        for (int p = 0; p < 2; p++) {
+            const uint32_t a = raw8_top16<T>(raw[2 * p]), b = raw8_top16<T>(raw[2 * p + 1]);
+            pair[p] = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+            pair[p] = __vmaxu2(pair[p], __shfl_xor_sync(0xffffffffu, pair[p], 1));
+            pair[p] = __vmaxu2(pair[p], __shfl_xor_sync(0xffffffffu, pair[p], 2));
+            const unsigned short lo = (unsigned short)(pair[p] & 0xFFFFu), hi = (unsigned short)(pair[p] >> 16);
+            top[2 * p] = __float_as_uint(to_f32(*(const T*)&lo));
+            top[2 * p + 1] = __float_as_uint(to_f32(*(const T*)&hi));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float* v = (const float*)raw[j].q;
+            top[j] = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; i++) top[j] = max(top[j], __float_as_uint(v[i]) & 0x7FFFFFFFu);
+            top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));
+            top[j] = max(top[j], __shfl_xor_sync(0xffffffffu, top[j], 2));
+        }
+    }
+    uint32_t bytes = 0u;   // of the four rows' blocks here
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        float v[8];
+        float v[8], inv;
         raw8_values<T>(raw[j], v);
-        uint32_t top = raw8_top<T>(raw[j], v);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        float inv;
-        const uint32_t byte = mx_scale(top, inv);   // (zeros behind the last row and block: byte 0)
+        bytes |= mx_scale(top[j], inv) << (8 * j);   // (zeros behind the last row and block: byte 0)
         uint32_t code = 0u;
 #pragma unroll
         for (int i = 0; i < 4; i++) code |= e2m1_pair(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
         if (w.row + 32 * j < rows && w.k < K) *(uint32_t*)(codes + (w.row + 32 * j) * codes_ld + w.k / 2) = code;
-        word[j] = byte << (8 * (lane / 4 % 4));     // the K tile's four bytes of this row meet in every one of its lanes
-        word[j] |= __shfl_xor_sync(0xffffffffu, word[j], 4);
-        word[j] |= __shfl_xor_sync(0xffffffffu, word[j], 8);
     }
-    if (lane % 16 == 0 && w.k < K)
-        *(uint4*)(scales + (w.tile + lane / 16) * MX_TILE + 16 * (w.row % 32)) = make_uint4(word[0], word[1], word[2], word[3]);
+    // four rows of this block to four blocks of a row: a transposition of 4 x 4 bytes between the K tile's four blocks
+    const int q = lane / 4 % 4;
+    uint32_t other = __shfl_xor_sync(0xffffffffu, bytes, 4);
+    bytes = __byte_perm(bytes, other, q & 1 ? 0x3715 : 0x6240);
+    other = __shfl_xor_sync(0xffffffffu, bytes, 8);
+    bytes = __byte_perm(bytes, other, q & 2 ? 0x3276 : 0x5410);
+    if (lane % 4 == 0 && w.k - 8 * (lane % 16) < K)   // (the K tile is there)
+        *(uint32_t*)(scales + (w.tile + lane / 16) * MX_TILE + 16 * (w.row % 32) + 4 * q) = bytes;
+    }
 }
 
 // Scale bytes of another producer, row by row, into the tiles.
@@ -159,7 +182,7 @@ __global__ void __launch_bounds__(256) mx4_dequant_kernel(const uint8_t* codes, 
     constexpr int E = 16 / (int)sizeof(T), PARTS = 256 / (32 * E);
     using Code = typename std::conditional<E == 8, uint32_t, uint16_t>::type;
     MxWalk w;
-    if (!mx_walk(K, rows, w)) return;
+    if (!mx_walk(K, rows, 256, w)) return;
     const int lane = threadIdx.x & 31;
     w.k = w.k - 8 * lane + E * lane;
     uint32_t code[PARTS][4], word[PARTS][4];
@@ -779,7 +802,7 @@ bool mx_shape(int K, int rows) { return K >= 32 && K % 32 == 0 && rows >= 1; }
 
 template <typename T>
 int quantize_as(q38b_ctx* ctx, const void* x, long long x_ld, int K, int rows, uint8_t* codes, long long codes_ld, uint8_t* scales, cudaStream_t st) {
-    const long long blocks = (mx_walk_warps(K, rows) + 7) / 8;
+    const long long blocks = (mx_walk_warps(K, rows, mx_quantize_span(sizeof(T))) + 7) / 8;
     if (blocks > 0x7FFFFFFF) return Q38B_ERR_UNSUPPORTED;
     const unsigned grid = (unsigned)blocks;
     const bool vec = (((uintptr_t)x | (uintptr_t)(x_ld * (long long)sizeof(T))) & 15) == 0;
@@ -790,7 +813,7 @@ int quantize_as(q38b_ctx* ctx, const void* x, long long x_ld, int K, int rows, u
 
 template <typename T>
 int dequant_as(q38b_ctx* ctx, const uint8_t* codes, long long codes_ld, const uint8_t* scales, int K, int rows, void* out, long long out_ld, cudaStream_t st) {
-    const long long blocks = (mx_walk_warps(K, rows) + 7) / 8;
+    const long long blocks = (mx_walk_warps(K, rows, 256) + 7) / 8;
     if (blocks > 0x7FFFFFFF) return Q38B_ERR_UNSUPPORTED;
     const bool vec = (((uintptr_t)out | (uintptr_t)(out_ld * (long long)sizeof(T))) & 15) == 0;
     if (vec) mx4_dequant_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(codes, codes_ld, scales, K, rows, (T*)out, out_ld);
