@@ -51,21 +51,21 @@ __device__ __forceinline__ uint32_t mx_scale(uint32_t top, float& inv) {
 // Quantizer and dequantizer walk a matrix alike: a warp owns 256 values (two K tiles) of the four rows r, r + 32, r + 64, r + 96 whose
 // scales lie together in a tile, 16 bytes for each K tile, so that scales move in whole pieces; a lane has eight neighbours of each row
 // (four lanes are a block) and all four rows' loads in flight.  Bound by memory: what is read and written once.  17408 x 5120 bf16 122 ->
-// 45 us (5.0 TB/s; fp32 58 us, 7.0 TB/s), back to bf16 179 -> 37 us (6.1 TB/s), against one row and four values a lane with a byte store per block.
+// 44 us (5.1 TB/s; fp32 58 us, 7.0 TB/s), back to bf16 179 -> 37 us (6.1 TB/s), against one row and four values a lane with a byte store per block.
 struct MxWalk {
     long long row;   // the first of the four rows
     int k;           // this lane's first value
     long long tile;  // the scales' first K tile of the warp, in tiles
 };
-__host__ __device__ inline long long mx_walk_warps(int K, int rows, int span) { return (long long)(rows + 127) / 128 * 32 * ((K + span - 1) / span); }
-__device__ __forceinline__ bool mx_walk(int K, int rows, int span, MxWalk& w) {   // span: the warp's values of a row, a multiple of 256
-    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), kc = (K + span - 1) / span;
-    if (item >= mx_walk_warps(K, rows, span)) return false;
+__host__ __device__ inline long long mx_walk_warps(int K, int rows) { return (long long)(rows + 127) / 128 * 32 * ((K + 255) / 256); }
+__device__ __forceinline__ bool mx_walk(int K, int rows, MxWalk& w) {
+    const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5), kc = (K + 255) / 256;
+    if (item >= mx_walk_warps(K, rows)) return false;
     // the eight warps of a block: neighbouring rows, so that their scales are one piece of 128 bytes
     const long long group = item / 8, at = group / kc, c = group % kc;
     w.row = at / 4 * 128 + at % 4 * 8 + (item & 7);
-    w.k = (int)c * span + 8 * (int)(threadIdx.x & 31);
-    w.tile = at / 4 * mx_tiles_k(K) + span / 128 * c;
+    w.k = (int)c * 256 + 8 * (int)(threadIdx.x & 31);
+    w.tile = at / 4 * mx_tiles_k(K) + 2 * c;
     return true;
 }
 
@@ -81,33 +81,26 @@ template <typename T> __device__ __forceinline__ uint32_t raw8_top16(const Raw8<
     return __vmaxu2(__vmaxu2(r.q[0].x & 0x7FFF7FFFu, r.q[0].y & 0x7FFF7FFFu), __vmaxu2(r.q[0].z & 0x7FFF7FFFu, r.q[0].w & 0x7FFF7FFFu));
 }
 
-constexpr __host__ __device__ int mx_quantize_span(size_t size) { return size == 2 ? 512 : 256; }   // values of a row a warp takes, all on their way at once
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, long long x_ld, int K, int rows, uint8_t* codes, long long codes_ld, uint8_t* scales) {
     pdl_launch_dependents();   // (a product behind it brings its first weights meanwhile)
     MxWalk w;
-    constexpr int SPANS = mx_quantize_span(sizeof(T)) / 256;
-    if (!mx_walk(K, rows, 256 * SPANS, w)) return;
+    if (!mx_walk(K, rows, w)) return;
     const int lane = threadIdx.x & 31;
-    Raw8<T> ahead[SPANS][4] = {};
-#pragma unroll
-    for (int p = 0; p < SPANS; p++)
+    Raw8<T> raw[4] = {};
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (w.row + 32 * j < rows && w.k + 256 * p < K) {
-            const T* from = x + (w.row + 32 * j) * x_ld + w.k + 256 * p;
+        if (w.row + 32 * j < rows && w.k < K) {
+            const T* p = x + (w.row + 32 * j) * x_ld + w.k;
             if constexpr (VEC) {
-                ahead[p][j] = *(const Raw8<T>*)from;
+                raw[j] = *(const Raw8<T>*)p;
             } else {
                 T e[8];
 #pragma unroll
-                for (int i = 0; i < 8; i++) e[i] = from[i];
-                memcpy(&ahead[p][j], e, sizeof(e));
+                for (int i = 0; i < 8; i++) e[i] = p[i];
+                memcpy(&raw[j], e, sizeof(e));
             }
         }
-#pragma unroll
-    for (int p = 0; p < SPANS; p++, w.k += 256, w.tile += 2) {
-    const Raw8<T>(&raw)[4] = ahead[p];
     // the largest magnitudes of the four rows' blocks (16-bit types: two rows a word, which compare and travel together)
     uint32_t top[4];
     if constexpr (sizeof(T) == 2) {
@@ -152,7 +145,6 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, long long
     bytes = __byte_perm(bytes, other, q & 2 ? 0x3276 : 0x5410);
     if (lane % 4 == 0 && w.k - 8 * (lane % 16) < K)   // (the K tile is there)
         *(uint32_t*)(scales + (w.tile + lane / 16) * MX_TILE + 16 * (w.row % 32) + 4 * q) = bytes;
-    }
 }
 
 // Scale bytes of another producer, row by row, into the tiles.
@@ -182,7 +174,7 @@ __global__ void __launch_bounds__(256) mx4_dequant_kernel(const uint8_t* codes, 
     constexpr int E = 16 / (int)sizeof(T), PARTS = 256 / (32 * E);
     using Code = typename std::conditional<E == 8, uint32_t, uint16_t>::type;
     MxWalk w;
-    if (!mx_walk(K, rows, 256, w)) return;
+    if (!mx_walk(K, rows, w)) return;
     const int lane = threadIdx.x & 31;
     w.k = w.k - 8 * lane + E * lane;
     uint32_t code[PARTS][4], word[PARTS][4];
@@ -802,7 +794,7 @@ bool mx_shape(int K, int rows) { return K >= 32 && K % 32 == 0 && rows >= 1; }
 
 template <typename T>
 int quantize_as(q38b_ctx* ctx, const void* x, long long x_ld, int K, int rows, uint8_t* codes, long long codes_ld, uint8_t* scales, cudaStream_t st) {
-    const long long blocks = (mx_walk_warps(K, rows, mx_quantize_span(sizeof(T))) + 7) / 8;
+    const long long blocks = (mx_walk_warps(K, rows) + 7) / 8;
     if (blocks > 0x7FFFFFFF) return Q38B_ERR_UNSUPPORTED;
     const unsigned grid = (unsigned)blocks;
     const bool vec = (((uintptr_t)x | (uintptr_t)(x_ld * (long long)sizeof(T))) & 15) == 0;
@@ -813,7 +805,7 @@ int quantize_as(q38b_ctx* ctx, const void* x, long long x_ld, int K, int rows, u
 
 template <typename T>
 int dequant_as(q38b_ctx* ctx, const uint8_t* codes, long long codes_ld, const uint8_t* scales, int K, int rows, void* out, long long out_ld, cudaStream_t st) {
-    const long long blocks = (mx_walk_warps(K, rows, 256) + 7) / 8;
+    const long long blocks = (mx_walk_warps(K, rows) + 7) / 8;
     if (blocks > 0x7FFFFFFF) return Q38B_ERR_UNSUPPORTED;
     const bool vec = (((uintptr_t)out | (uintptr_t)(out_ld * (long long)sizeof(T))) & 15) == 0;
     if (vec) mx4_dequant_kernel<T, true><<<(unsigned)blocks, 256, 0, st>>>(codes, codes_ld, scales, K, rows, (T*)out, out_ld);
