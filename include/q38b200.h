@@ -228,7 +228,7 @@ typedef struct q38b_heads {
  * k may be NULL.  positions: int32 [rows], any sign; inv_freq: float64 [rot / 2], finite, radians per position (both may be NULL with
  * rot = 0); the angle is exact to about |position| 2^-52 turns.  in_kind, out_kind: q38b_out_kind of src and dst.  D <= 1024, rot even and
  * at most D.  dst may be src itself (same kind, same strides); otherwise the two must not overlap, nor may the query heads'
- * elements be among the key heads'.  Sums in fp32, outputs rounded once. */
+ * elements be among the key heads'.  In dst rows lie outside heads (dst_row at least a row's extent) or heads outside rows.  Sums in fp32, outputs rounded once. */
 int q38b_qk_norm_rope(q38b_ctx* ctx, const q38b_heads* q, const q38b_heads* k, int D, int rot, int adjacent, float eps, float scale,
                       const int* positions_dev, const double* inv_freq_dev, int in_kind, int out_kind, int rows, void* stream);
 
@@ -252,7 +252,8 @@ typedef struct q38b_logit_rules {
  *   generated c > 0 times: l = l - frequency * c - presence
  *   biased:                l = l + bias
  *   mask bit clear:        l = -infinity (whatever l was; a mask without a bit leaves a row of them)
- * y may be x (then y_ld = x_ld); otherwise they must not overlap.  Same inputs, same bits. */
+ * y may be x (then y_ld = x_ld); otherwise they must not overlap.  n <= 2^30.  A number in mask_of_row must be that of a mask there is.
+ * Same inputs, same bits. */
 int q38b_adjust_logits(q38b_ctx* ctx, const float* x_dev, long long x_ld, int n, int n_rows, int index_offset, const q38b_logit_rules* rules,
                        float* y_dev, long long y_ld, void* stream);
 
@@ -265,7 +266,8 @@ int q38b_adjust_logits(q38b_ctx* ctx, const float* x_dev, long long x_ld, int n,
  * ------------------------------------------------------------------------------------------------------------ */
 size_t q38b_mx4_scale_bytes(int K, int rows);
 /* x (x_kind, x_ld elements between rows) -> codes and scales: per 32 values 2^e, e = floor(log2 of the largest magnitude) - 2, at
- * least -127; elements x / 2^e rounded half to even, at most 6 in magnitude.  A block with a NaN or an infinity gets the NaN scale 255. */
+ * least -127; elements x / 2^e rounded half to even, at most 6 in magnitude.  A block with a NaN or an infinity gets the NaN scale 255.
+ * x, codes and scales must not overlap; K and rows at most 2^30. */
 int q38b_quantize_mx4(q38b_ctx* ctx, const void* x_dev, int x_kind, long long x_ld, int K, int rows, void* codes_dev, long long codes_ld,
                       void* scales_dev, void* stream);
 /* Scale bytes of another producer, [rows][src_ld] with K / 32 of them in a row, into the tiles above. */

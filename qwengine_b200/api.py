@@ -142,6 +142,7 @@ _pack_heads = struct.Struct("@PPqqqqPi4x").pack      # src, dst, src_row, src_he
 _pack_rules = struct.Struct("@PPPPPPPPqP").pack      # penalties .. bias_begin, masks, mask_ld, mask_of_row
 _pack_pass_heads = struct.Struct("@7i4xP").pack      # q38b_pass_heads: src, src_off, src_head, dst, dst_off, dst_head, n_heads, weight
 _empty = torch.empty_strided
+_F32, _F64, _I32, _I64, _U8 = torch.float32, torch.float64, torch.int32, torch.int64, torch.uint8
 _current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
@@ -158,10 +159,14 @@ class Mx4:
     def __init__(self, codes, scales):
         rows, half = codes.shape
         ld, one = codes.stride()
-        _need(codes.dtype == scales.dtype == torch.uint8 and one == 1, "Mx4: uint8 codes [rows, K / 2] with packed rows, uint8 scales")
-        _need(rows >= 1 and half >= 16 and half % 16 == 0, "Mx4: K a multiple of 32, at least one row")
-        _need(scales.is_contiguous() and scales.numel() == ((rows + 127) // 128) * ((half + 63) // 64) * 512, "Mx4: contiguous tiles of 128 rows x 4 blocks of scales")
-        _need(codes.get_device() == scales.get_device(), "Mx4: codes and scales on one device")
+        if codes.dtype != _U8 or scales.dtype != _U8 or one != 1:
+            raise ValueError("Mx4: uint8 codes [rows, K / 2] with packed rows, uint8 scales")
+        if rows < 1 or half < 16 or half % 16:
+            raise ValueError("Mx4: K a multiple of 32, at least one row")
+        if not scales.is_contiguous() or scales.numel() != ((rows + 127) // 128) * ((half + 63) // 64) * 512:
+            raise ValueError("Mx4: contiguous tiles of 128 rows x 4 blocks of scales")
+        if codes.get_device() != scales.get_device():
+            raise ValueError("Mx4: codes and scales on one device")
         self.codes, self.scales, self.rows, self.K = codes, scales, rows, 2 * half
         self.ld = ld if rows > 1 else half   # (the stride of a single row says nothing)
 
@@ -173,7 +178,7 @@ class Context:
         self.lib = load_library()
         if not torch.cuda.is_available():
             raise RuntimeError("no CUDA device: this library has no CPU path")
-        self.device = torch.device("cuda", device)
+        self.device, self._index = torch.device("cuda", device), device
         h = C.c_void_p()
         rc = self.lib.q38b_ctx_create(device, C.byref(h))
         if rc:
@@ -321,58 +326,66 @@ class Context:
     # ---- the steps of a token between its products --------------------------------------------
     def _stream(self):
         """The current stream of the context's device (whatever device is current)."""
-        return _current_stream(self.device.index)
+        return _current_stream(self._index)
 
     def qk_norm_rope(self, q, k, positions, inv_freq, q_weight=None, k_weight=None, eps=1e-6, adjacent=False, scale=1.0, kind=None, q_out=None, k_out=None):
         """q [rows, heads, D], k [rows, heads, D] or None (fp32, fp16 or bf16, any row and head strides): RMSNorm of each head, rotation of its first
         2 * len(inv_freq) elements by positions (int32 [rows]) times inv_freq (float64); weights fp32 [D].  kind: OUT_* of the results (that of
         the inputs by default); returns (q_out, k_out), which may be q and k themselves."""
         rows, _, D = q.shape
-        dtype = q.dtype
+        dtype, dev = q.dtype, self._index
         in_kind = _OUT_KINDS.get(dtype)
-        _need(in_kind is not None, "qk_norm_rope: fp32, fp16 or bf16 heads")
+        if in_kind is None:
+            raise ValueError("qk_norm_rope: fp32, fp16 or bf16 heads")
         if kind is None:
             kind = in_kind
-        out_dtype, dev, rot, pos_ptr, freq_ptr = _OUT_DTYPES[kind], self.device.index, 0, None, None
+        out_dtype, rot, pos_ptr, freq_ptr = _OUT_DTYPES[kind], 0, None, None
         if inv_freq is not None and inv_freq.numel():
-            rot = 2 * inv_freq.shape[0]
-            _need(positions is not None and positions.dtype == torch.int32 and positions.shape == (rows,) and positions.is_contiguous(), "qk_norm_rope: int32 positions, one per row")
-            _need(inv_freq.dtype == torch.float64 and inv_freq.dim() == 1 and inv_freq.is_contiguous() and rot <= D, "qk_norm_rope: float64 inv_freq, at most D / 2")
-            _need(positions.get_device() == dev and inv_freq.get_device() == dev, "qk_norm_rope: tensors on the context's device")
+            rot = 2 * inv_freq.numel()
+            if positions is None or positions.dtype != _I32 or positions.numel() != rows or not positions.is_contiguous():
+                raise ValueError("qk_norm_rope: int32 positions, one per row")
+            if inv_freq.dtype != _F64 or not inv_freq.is_contiguous() or rot > D:
+                raise ValueError("qk_norm_rope: float64 inv_freq, at most D / 2")
+            if positions.get_device() != dev or inv_freq.get_device() != dev:
+                raise ValueError("qk_norm_rope: tensors on the context's device")
             pos_ptr, freq_ptr = positions.data_ptr(), inv_freq.data_ptr()
-        parts, outs = [], []
-        for x, w, out in ((q, q_weight, q_out), (k, k_weight, k_out)):
-            if x is None:
-                parts.append(None)
-                outs.append(None)
-                continue
-            n, heads, d = x.shape
-            row, head, one = x.stride()
-            _need(n == rows and d == D and x.dtype == dtype and (one == 1 or D == 1), "qk_norm_rope: heads [rows, heads, D] of one type, elements side by side")
-            _need(x.get_device() == dev, "qk_norm_rope: tensors on the context's device")
-            if out is None:
-                out_row, out_head = heads * D, D
-                out = _empty((rows, heads, D), (out_row, D, 1), dtype=out_dtype, device=self.device)
-            else:
-                out_row, out_head, one = out.stride()
-                _need(out.shape == x.shape and out.dtype == out_dtype and (one == 1 or D == 1), "qk_norm_rope: outputs shaped like the heads")
-                _need(out.get_device() == dev, "qk_norm_rope: tensors on the context's device")
-            w_ptr = 0
-            if w is not None:
-                _need(w.dtype == torch.float32 and w.shape == (D,) and w.is_contiguous() and w.get_device() == dev, "qk_norm_rope: fp32 weights [D] on the context's device")
-                w_ptr = w.data_ptr()
-            parts.append(_pack_heads(x.data_ptr(), out.data_ptr(), row, head, out_row, out_head, w_ptr, heads))
-            outs.append(out)
-        rc = self.lib.q38b_qk_norm_rope(self.h, parts[0], parts[1], D, rot, 1 if adjacent else 0, eps, scale, pos_ptr, freq_ptr, in_kind, kind, rows, self._stream())
+        q_out, q_part = self._heads(q, q_weight, q_out, rows, D, dtype, out_dtype, dev)
+        k_part = None
+        if k is not None:
+            k_out, k_part = self._heads(k, k_weight, k_out, rows, D, dtype, out_dtype, dev)
+        rc = self.lib.q38b_qk_norm_rope(self.h, q_part, k_part, D, rot, 1 if adjacent else 0, eps, scale, pos_ptr, freq_ptr, in_kind, kind, rows, _current_stream(dev))
         if rc:
             self._rc(rc, "q38b_qk_norm_rope")
-        return outs[0], outs[1]
+        return q_out, k_out if k is not None else None
+
+    def _heads(self, x, w, out, rows, D, dtype, out_dtype, dev):
+        """Checks one tensor of heads: its output, and the bytes of its q38b_heads."""
+        n, heads, d = x.shape
+        row, head, one = x.stride()
+        if n != rows or d != D or x.dtype != dtype or (one != 1 and D != 1):
+            raise ValueError("qk_norm_rope: heads [rows, heads, D] of one type, elements side by side")
+        if out is None:
+            out_row, out_head = heads * D, D
+            out = _empty((rows, heads, D), (out_row, D, 1), dtype=out_dtype, device=self.device)
+        else:
+            out_row, out_head, one = out.stride()
+            if out.shape != x.shape or out.dtype != out_dtype or (one != 1 and D != 1):
+                raise ValueError("qk_norm_rope: outputs shaped like the heads")
+        if x.get_device() != dev or out.get_device() != dev:
+            raise ValueError("qk_norm_rope: tensors on the context's device")
+        w_ptr = 0
+        if w is not None:
+            if w.dtype != _F32 or w.numel() != D or not w.is_contiguous() or w.get_device() != dev:
+                raise ValueError("qk_norm_rope: fp32 weights [D] on the context's device")
+            w_ptr = w.data_ptr()
+        return out, _pack_heads(x.data_ptr(), out.data_ptr(), row, head, out_row, out_head, w_ptr, heads)
 
     def _list(self, what, t, dtype, shape=None):
         """Address of an optional contiguous tensor of the context's device (0: none, or nothing in it)."""
         if t is None:
             return 0
-        _need(t.dtype == dtype and t.is_contiguous() and t.get_device() == self.device.index and (shape is None or t.shape == shape), what)
+        if t.dtype != dtype or not t.is_contiguous() or t.get_device() != self._index or (shape is not None and t.shape != shape):
+            raise ValueError(what)
         return t.data_ptr()
 
     def logit_rules(self, rows, n, penalties=None, history=None, history_begin=None, prompt_len=None, bias_ids=None, bias_values=None, bias_begin=None,
@@ -380,7 +393,7 @@ class Context:
         """The bytes of a q38b_logit_rules of checked device tensors: penalties fp32 [rows, 3] (repetition, frequency, presence), history int32 with int64
         begins [rows + 1] and int32 prompt lengths [rows]; bias_ids int32, bias_values fp32, int64 begins; masks int32 [*, words] of
         allowed-token bits, mask_of_row int32 [rows]."""
-        f32, i32, i64, address = torch.float32, torch.int32, torch.int64, self._list
+        f32, i32, i64, address = _F32, _I32, _I64, self._list
         p = h = hb = pl = bi = bv = bb = mk = mr = ld = 0
         if penalties is not None or history is not None or history_begin is not None or prompt_len is not None:
             p = address("adjust_logits: fp32 penalties [rows, 3]", penalties, f32, (rows, 3))
@@ -400,7 +413,7 @@ class Context:
         if masks is not None:
             count, words = masks.shape
             ld, one = masks.stride()
-            _need(masks.dtype == i32 and one == 1 and masks.get_device() == self.device.index and words * 32 >= index_offset + n and
+            _need(masks.dtype == i32 and one == 1 and masks.get_device() == self._index and words * 32 >= index_offset + n and
                   (count >= rows or mask_of_row is not None), "adjust_logits: masks int32 [masks, words], a bit for each token")
             mk, ld = masks.data_ptr(), ld if count > 1 else words
         if mask_of_row is not None:
@@ -412,8 +425,9 @@ class Context:
         logit_rules.  Token v is column v - index_offset."""
         rows, n = logits.shape
         ld, one = logits.stride()
-        dev = self.device.index
-        _need(logits.dtype == torch.float32 and (one == 1 or n == 1) and logits.get_device() == dev, "adjust_logits: fp32 logits [rows, n] on the context's device")
+        dev = self._index
+        if logits.dtype != _F32 or (one != 1 and n != 1) or logits.get_device() != dev:
+            raise ValueError("adjust_logits: fp32 logits [rows, n] on the context's device")
         r = self.logit_rules(rows, n, index_offset=index_offset, **rules)
         if out is None:
             out_ld = n
@@ -421,7 +435,7 @@ class Context:
         else:
             out_ld, one = out.stride()
             _need(out.dtype == torch.float32 and out.shape == logits.shape and (one == 1 or n == 1) and out.get_device() == dev, "adjust_logits: fp32 out of the logits' shape")
-        rc = self.lib.q38b_adjust_logits(self.h, logits.data_ptr(), ld, n, rows, index_offset, r, out.data_ptr(), out_ld, self._stream())
+        rc = self.lib.q38b_adjust_logits(self.h, logits.data_ptr(), ld, n, rows, index_offset, r, out.data_ptr(), out_ld, _current_stream(dev))
         if rc:
             self._rc(rc, "q38b_adjust_logits")
         return out
@@ -432,7 +446,7 @@ class Context:
         rows, K = x.shape
         ld, one = x.stride()
         kind = _OUT_KINDS.get(x.dtype)
-        _need(kind is not None and one == 1 and x.get_device() == self.device.index, "quantize_mx4: fp32, fp16 or bf16 [rows, K] on the context's device")
+        _need(kind is not None and one == 1 and x.get_device() == self._index, "quantize_mx4: fp32, fp16 or bf16 [rows, K] on the context's device")
         if K % 32 or K == 0 or rows == 0:
             raise Q38BError(-1, "q38b_quantize_mx4")
         half, tiles = K // 2, ((rows + 127) // 128) * ((K + 127) // 128) * 512
@@ -447,7 +461,7 @@ class Context:
         """Codes uint8 [rows, K / 2] and scale bytes uint8 [rows, K / 32] of another producer -> Mx4 (the codes are kept, not copied)."""
         rows, half = codes.shape
         _need(scales.dtype == torch.uint8 and scales.shape == (rows, half // 16) and half % 16 == 0 and scales.stride(1) == 1, "pack_mx4: uint8 scales [rows, K / 32]")
-        _need(codes.get_device() == self.device.index and scales.get_device() == self.device.index, "pack_mx4: tensors on the context's device")
+        _need(codes.get_device() == self._index and scales.get_device() == self._index, "pack_mx4: tensors on the context's device")
         K = 2 * half
         tiles = torch.empty(self.lib.q38b_mx4_scale_bytes(K, rows), dtype=torch.uint8, device=self.device)
         self._rc(self.lib.q38b_mx4_tile_scales(self.h, scales.data_ptr(), scales.stride(0) if rows > 1 else K // 32, K, rows, tiles.data_ptr(), self._stream()), "q38b_mx4_tile_scales")
@@ -455,7 +469,7 @@ class Context:
 
     def dequant_mx4(self, m, kind=OUT_F32):
         """The values of an Mx4: [rows, K]."""
-        _need(m.codes.get_device() == self.device.index, "dequant_mx4: a matrix on the context's device")
+        _need(m.codes.get_device() == self._index, "dequant_mx4: a matrix on the context's device")
         out = _empty((m.rows, m.K), (m.K, 1), dtype=_OUT_DTYPES[kind], device=self.device)
         rc = self.lib.q38b_dequant_mx4(self.h, m.codes.data_ptr(), m.ld, m.scales.data_ptr(), m.K, m.rows, out.data_ptr(), kind, m.K, self._stream())
         if rc:
@@ -465,9 +479,10 @@ class Context:
     def gemm_mx4(self, W, X, kind=OUT_F32, out=None, accumulate=False):
         """Y [B, W.rows] = X W^T for W an Mx4 and X an Mx4 or activations [B, K] (fp32, fp16 or bf16), which are quantized first.  kind: OUT_* of Y
         where `out` is not given."""
-        K, M, dev, mx = W.K, W.rows, self.device.index, isinstance(X, Mx4)
+        K, M, dev, mx = W.K, W.rows, self._index, isinstance(X, Mx4)
         B = X.rows if mx else X.shape[0]
-        _need(W.codes.get_device() == dev and (X.codes if mx else X).get_device() == dev, "gemm_mx4: operands on the context's device")
+        if W.codes.get_device() != dev or (X.codes if mx else X).get_device() != dev:
+            raise ValueError("gemm_mx4: operands on the context's device")
         if out is None:
             ldy = M
             out = _empty((B, M), (M, 1), dtype=_OUT_DTYPES[kind], device=self.device)
@@ -485,7 +500,8 @@ class Context:
         x_kind = _OUT_KINDS.get(X.dtype)
         B, k = X.shape
         ld, one = X.stride()
-        _need(x_kind is not None and one == 1 and k == K and B > 0, "gemm_mx4: activations [B, K] of the weights' K")
+        if x_kind is None or one != 1 or k != K or B == 0:
+            raise ValueError("gemm_mx4: activations [B, K] of the weights' K")
         scratch, need = None, 0
         if B > 1 or K > 8192:   # q38b_gemm_mx4_scratch_bytes
             need = B * (K // 2) + ((B + 127) // 128) * ((K + 127) // 128) * 512 + 16

@@ -772,6 +772,7 @@ MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int for
         MxPairCut c;
         c.n_tile = n;
         c.tok_tiles = (B + n - 1) / n;
+        if ((long long)row_tiles * c.tok_tiles > 0x7FFFFFFF) continue;
         c.n_tiles = row_tiles * c.tok_tiles;
         c.stages = std::min(MX_MAX_STAGES, (smem_optin - MXP_FIXED_SMEM) / mxp_stage_bytes(n));
         c.n_acc = 1;
@@ -790,7 +791,8 @@ MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int for
 
 size_t kind_size(int kind) { return kind == Q38B_OUT_F32 ? 4 : 2; }
 bool known_kind(int kind) { return kind == Q38B_OUT_F32 || kind == Q38B_OUT_F16 || kind == Q38B_OUT_BF16; }
-bool mx_shape(int K, int rows) { return K >= 32 && K % 32 == 0 && rows >= 1; }
+// (sizes that leave room for rounding up in 32 bits)
+bool mx_shape(int K, int rows) { return K >= 32 && K % 32 == 0 && K <= 1 << 30 && rows >= 1 && rows <= 1 << 30; }
 
 template <typename T>
 int quantize_as(q38b_ctx* ctx, const void* x, long long x_ld, int K, int rows, uint8_t* codes, long long codes_ld, uint8_t* scales, cudaStream_t st) {
@@ -978,7 +980,9 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
     double cost = 0.0, pair_cost = 0.0;
     const MxCut one = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B, &cost);
     const MxPairCut cut = mx_pair_cut(ctx->sm_count, ctx->smem_optin, K, M, B, ctx->mx4_pairs > 0 ? ctx->mx4_pairs : 0, &pair_cost);
-    if (ctx->mx4_pairs > 0 || (ctx->mx4_pairs == 0 && B > 32 && M > MX_ROWS && pair_cost < cost)) {
+    const bool too_many = (B + one.n_tile - 1) / one.n_tile > 65535;   // token tiles, for a grid's second dimension
+    if (ctx->mx4_pairs > 0 || (ctx->mx4_pairs == 0 && (too_many || (B > 32 && M > MX_ROWS && pair_cost < cost)))) {
+        if (!cut.n_tile) return Q38B_ERR_UNSUPPORTED;
         CUtensorMap wmap, xmap, wsmap, xsmap, ymap;
         memset(&ymap, 0, sizeof(ymap));
         const int tma_out = encode_out(&ymap, Y, y_kind, ldy, M, B) ? 1 : 0;
@@ -990,7 +994,7 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
              : y_kind == Q38B_OUT_F16 ? pair_as<__half>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st)
                                       : pair_as<__nv_bfloat16>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st);
     }
-    if ((B + one.n_tile - 1) / one.n_tile > 65535) return Q38B_ERR_UNSUPPORTED;
+    if (too_many) return Q38B_ERR_UNSUPPORTED;
     CUtensorMap wmap, xmap;
     if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS) || !encode_codes(&xmap, X, X_ld, K, B, one.n_tile)) return Q38B_ERR_ARG;
     MxArgs a = mx_args(ctx, one, W_scales, K, M, B, Y, ldy, accumulate);

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, 6) heads4_kernel(const Heads
 // the next piece's logits ahead (138); half of the warps counting a piece ahead of the others (112 mending in memory, 156 in registers): a warp
 // then waits too often for too few others.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int LG_THREADS = 512, LG_WARPS = LG_THREADS / 32;
+constexpr int LG_THREADS = 512, LG_WARPS = LG_THREADS / 32, LG_MAX_N = 1 << 30;
 constexpr uint32_t LG_PROMPT = 0x80000000u;   // seen in the prompt; the other bits count generated tokens
 
 struct LogitsArgs {
@@ -393,7 +393,7 @@ bool heads_by_four(const HeadsArgs& a, uintptr_t in_size, uintptr_t out_size) {
     for (const q38b_heads& t : a.t) {
         if (!t.n_heads) continue;
         if ((uintptr_t)t.src % (4 * in_size) || (uintptr_t)t.dst % (4 * out_size) || (uintptr_t)t.weight % 16) return false;
-        if ((t.src_row | t.src_head | t.dst_row | t.dst_head) % 4) return false;
+        if ((t.src_head | t.dst_head) % 4 || (a.rows > 1 && (t.src_row | t.dst_row) % 4)) return false;
     }
     return true;
 }
@@ -465,8 +465,10 @@ int q38b_qk_norm_rope(q38b_ctx* ctx, const q38b_heads* q, const q38b_heads* k, i
     for (int i = 0; i < (k ? 2 : 1); i++) {
         const q38b_heads& t = a.t[i];
         if (!t.src || !t.dst || t.n_heads < 1 || t.src_head < 0 || t.dst_head < 0 || t.src_row < 0 || t.dst_row < 0) return Q38B_ERR_ARG;
-        // two heads, or two rows, of one destination must not share elements
+        // no two heads of one destination share elements: rows lie outside heads, or heads outside rows
+        const long long in_row = (t.n_heads - 1) * t.dst_head + D, in_head = (rows - 1) * t.dst_row + D;
         if ((t.n_heads > 1 && t.dst_head < D) || (rows > 1 && t.dst_row < D)) return Q38B_ERR_ARG;
+        if (t.n_heads > 1 && rows > 1 && t.dst_row < in_row && t.dst_head < in_head) return Q38B_ERR_ARG;
         if ((uintptr_t)t.src % kind_size(in_kind) || (uintptr_t)t.dst % kind_size(out_kind) || ((uintptr_t)t.weight & 3)) return Q38B_ERR_ALIGN;
         // in place only element over element
         if (t.src == t.dst && (in_kind != out_kind || t.src_head != t.dst_head || t.src_row != t.dst_row)) return Q38B_ERR_ARG;
@@ -489,6 +491,7 @@ int q38b_qk_norm_rope(q38b_ctx* ctx, const q38b_heads* q, const q38b_heads* k, i
 int q38b_adjust_logits(q38b_ctx* ctx, const float* x, long long x_ld, int n, int n_rows, int index_offset, const q38b_logit_rules* rules, float* y, long long y_ld,
                        void* stream) {
     if (!ctx || !x || !y || !rules || n < 1 || n_rows < 1 || n_rows > 65535 || index_offset < 0 || index_offset > 0x7FFFFFFF - n) return Q38B_ERR_ARG;
+    if (n > LG_MAX_N) return Q38B_ERR_UNSUPPORTED;
     if (n_rows > 1 && (x_ld < n || y_ld < n)) return Q38B_ERR_ARG;
     if (x == y && n_rows > 1 && x_ld != y_ld) return Q38B_ERR_ARG;
     if (((uintptr_t)x | (uintptr_t)y) & 3) return Q38B_ERR_ALIGN;

@@ -45,6 +45,7 @@ def test_the_wrappers_bytes_are_the_structures():
     (dict(out_kind=-1), ARG), (dict(positions=None), ARG), (dict(inv_freq=None), ARG), (dict(positions=P + 2), ALIGN), (dict(inv_freq=P + 4), ALIGN),
     (dict(q=heads(src=None)), ARG), (dict(q=heads(dst=None)), ARG), (dict(q=heads(n_heads=0)), ARG), (dict(q=heads(src_head=-64)), ARG),
     (dict(q=heads(dst_head=63)), ARG), (dict(q=heads(dst_row=63)), ARG), (dict(q=heads(src=P + 2)), ALIGN), (dict(q=heads(weight=P + 1)), ALIGN),
+    (dict(q=heads(dst_row=64)), ARG), (dict(q=heads(dst_row=511)), ARG), (dict(q=heads(dst_row=64, dst_head=191)), ARG),   # rows among heads
     (dict(k=heads(dst=None)), ARG), (dict(k=heads(dst_row=0)), ARG),
     (dict(q=heads(dst=P, dst_head=65)), ARG),                        # in place, but not element over element
     (dict(q=heads(dst=P), out_kind=2), ARG),
@@ -64,7 +65,7 @@ def test_heads_null(lib):
 
 @pytest.mark.parametrize("change,rules,status", [
     (dict(x=None), {}, ARG), (dict(y=None), {}, ARG), (dict(n=0), {}, ARG), (dict(rows=0), {}, ARG), (dict(rows=65536), {}, ARG), (dict(x_ld=99), {}, ARG),
-    (dict(y_ld=99), {}, ARG), (dict(off=-1), {}, ARG), (dict(off=0x7FFFFFFF), {}, ARG), (dict(y=P, y_ld=104), {}, ARG), (dict(x=P + 2), {}, ALIGN),
+    (dict(y_ld=99), {}, ARG), (dict(off=-1), {}, ARG), (dict(off=0x7FFFFFFF), {}, ARG), (dict(n=(1 << 30) + 1, x_ld=1 << 31, y_ld=1 << 31), {}, UNSUPPORTED), (dict(y=P, y_ld=104), {}, ARG), (dict(x=P + 2), {}, ALIGN),
     ({}, dict(penalties=P), ARG), ({}, dict(history=P, history_begin=P), ARG), ({}, dict(penalties=P, history=P), ARG), ({}, dict(prompt_len=P), ARG),
     ({}, dict(bias_ids=P, bias_values=P), ARG), ({}, dict(bias_begin=P), ARG), ({}, dict(mask_of_row=P), ARG), ({}, dict(masks=P, mask_ld=3), ARG),
     (dict(off=29), dict(masks=P, mask_ld=4), ARG), ({}, dict(masks=ODD, mask_ld=4), ALIGN), ({}, dict(penalties=P, history=P, history_begin=P + 4), ALIGN),
@@ -89,7 +90,7 @@ def test_mx4(lib):
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(W=None), ARG), (dict(Ws=None), ARG), (dict(X=None), ARG), (dict(Xs=None), ARG), (dict(Y=None), ARG), (dict(K=100), ARG), (dict(M=0), ARG), (dict(B=0), ARG),
+    (dict(W=None), ARG), (dict(Ws=None), ARG), (dict(X=None), ARG), (dict(Xs=None), ARG), (dict(Y=None), ARG), (dict(K=100), ARG), (dict(M=0), ARG), (dict(M=(1 << 30) + 1, ldy=1 << 31), ARG), (dict(B=0), ARG),
     (dict(kind=3), ARG), (dict(ldy=199), ARG), (dict(W_ld=16), ARG), (dict(X_ld=16), ARG), (dict(W=P + 8), ALIGN), (dict(X_ld=56), ALIGN), (dict(Xs=P + 8), ALIGN),
     (dict(Y=P + 2), ALIGN)])
 def test_mx4_product(lib, change, status):
