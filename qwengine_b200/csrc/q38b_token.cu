@@ -76,8 +76,8 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
 // Heads of up to 256 elements whose rows allow it move four elements a lane at a time.  A CTA has one row (its sines and cosines are computed
 // once, into shared memory) and up to HEADS_BATCH heads a warp, whose loads are all issued first; a head's L lanes add its squares by
 // shuffles and swap partners of the rotation through shared memory.  Bound by memory: 8192 rows of 24 + 4 heads of 256, fp32 to bf16, 68 us =
-// 5.1 TB/s (four heads a warp and three CTAs an SM 77) against 114 us element by element, where every head's warp computed its own angles.
-constexpr int HEADS_BATCH = 2, HEADS_WARPS = 8, HEADS_MAX_D = 256;
+// 5.2 TB/s (four heads a warp, eight warps a CTA, three CTAs an SM 77) against 114 us element by element, where every head's warp computed its own angles.
+constexpr int HEADS_BATCH = 2, HEADS_WARPS = 4, HEADS_MAX_D = 256;
 
 template <typename T> __device__ __forceinline__ float4 load4(const T* p) {
     if constexpr (sizeof(T) == 4) return *(const float4*)p;
@@ -99,7 +99,7 @@ template <typename T> __device__ __forceinline__ void store4(T* p, float4 v) {
 
 // L lanes a head (two heads a warp where 16 do), NV vectors of four elements a lane
 template <typename Tin, typename Tout, int L, int NV>
-__global__ void __launch_bounds__(32 * HEADS_WARPS, 6) heads4_kernel(const HeadsArgs a, int heads_per_cta, int ctas_per_row) {
+__global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const HeadsArgs a, int heads_per_cta, int ctas_per_row) {
     constexpr int SUB = 32 / L;
     __shared__ float cs[HEADS_MAX_D / 2], sn[HEADS_MAX_D / 2];
     __shared__ float4 swap[HEADS_WARPS][32 * NV];
