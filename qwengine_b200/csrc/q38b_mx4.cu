@@ -30,10 +30,12 @@ constexpr int MX_TILE = 512;   // scale bytes of 128 rows x 4 blocks
 
 __host__ __device__ inline long long mx_tiles_k(int K) { return (K + 127) / 128; }
 
-// Two values to two E2M1 codes (a in the low four bits): half to even, saturated at 6.
-__device__ __forceinline__ uint32_t e2m1_pair(float a, float b) {
+// Eight values to E2M1 codes in a word, the first in its low four bits: half to even, saturated at 6 (one block: the conversions then merge their bytes themselves)
+__device__ __forceinline__ uint32_t e2m1_eight(const float (&v)[8]) {
     uint32_t r;
-    asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %2, %1;\n\tcvt.u32.u8 %0, t;\n\t}" : "=r"(r) : "f"(a), "f"(b));
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tcvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
 
@@ -51,7 +53,7 @@ __device__ __forceinline__ uint32_t mx_scale(uint32_t top, float& inv) {
 // Quantizer and dequantizer walk a matrix alike: a warp owns 256 values (two K tiles) of the four rows r, r + 32, r + 64, r + 96 whose
 // scales lie together in a tile, 16 bytes for each K tile, so that scales move in whole pieces; a lane has eight neighbours of each row
 // (four lanes are a block) and all four rows' loads in flight.  Bound by memory: what is read and written once.  17408 x 5120 bf16 122 ->
-// 44 us (5.1 TB/s; fp32 58 us, 7.0 TB/s), back to bf16 179 -> 37 us (6.1 TB/s), against one row and four values a lane with a byte store per block.
+// 40 us (5.7 TB/s; fp32 58 us, 7.0 TB/s), back to bf16 179 -> 37 us (6.1 TB/s), against one row and four values a lane with a byte store per block.
 struct MxWalk {
     long long row;   // the first of the four rows
     int k;           // this lane's first value
@@ -86,12 +88,13 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, long long
     pdl_launch_dependents();   // (a product behind it brings its first weights meanwhile)
     MxWalk w;
     if (!mx_walk(K, rows, w)) return;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, here = w.k < K ? (int)min(4LL, (rows - w.row + 31) / 32) : 0;   // of the four rows, those that are there
+    const T* p = x + w.row * x_ld + w.k;
+    uint8_t* to = codes + w.row * codes_ld + w.k / 2;
     Raw8<T> raw[4] = {};
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (w.row + 32 * j < rows && w.k < K) {
-            const T* p = x + (w.row + 32 * j) * x_ld + w.k;
+    for (int j = 0; j < 4; j++, p += 32 * x_ld)
+        if (j < here) {
             if constexpr (VEC) {
                 raw[j] = *(const Raw8<T>*)p;
             } else {
@@ -128,14 +131,13 @@ __global__ void __launch_bounds__(256) mx4_quantize_kernel(const T* x, long long
     }
     uint32_t bytes = 0u;   // of the four rows' blocks here
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
+    for (int j = 0; j < 4; j++, to += 32 * codes_ld) {
         float v[8], inv;
         raw8_values<T>(raw[j], v);
         bytes |= mx_scale(top[j], inv) << (8 * j);   // (zeros behind the last row and block: byte 0)
-        uint32_t code = 0u;
 #pragma unroll
-        for (int i = 0; i < 4; i++) code |= e2m1_pair(v[2 * i] * inv, v[2 * i + 1] * inv) << (8 * i);
-        if (w.row + 32 * j < rows && w.k < K) *(uint32_t*)(codes + (w.row + 32 * j) * codes_ld + w.k / 2) = code;
+        for (int i = 0; i < 8; i++) v[i] *= inv;
+        if (j < here) *(uint32_t*)to = e2m1_eight(v);
     }
     // four rows of this block to four blocks of a row: a transposition of 4 x 4 bytes between the K tile's four blocks
     const int q = lane / 4 % 4;
@@ -458,9 +460,9 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
                 top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 float inv;
                 const uint32_t byte = mx_scale(top, inv);
-                uint32_t code = 0u;
 #pragma unroll
-                for (int i = 0; i < 4; i++) code |= e2m1_pair(v[g][2 * i] * inv, v[g][2 * i + 1] * inv) << (8 * i);
+                for (int i = 0; i < 8; i++) v[g][i] *= inv;
+                const uint32_t code = e2m1_eight(v[g]);
                 if (u0 + 256 * g + lane < units) {   // 128 bytes of a row hold 256 K; 16-byte piece c at c ^ (row & 7) (128-byte swizzle)
                     const int s = at[g] / MX_K, b = at[g] % MX_K / 2, r = row[g];
                     *(uint32_t*)(x_codes + s * MX_FUSED_X + r * 128 + 16 * ((b / 16) ^ (r & 7)) + b % 16) = code;

@@ -27,7 +27,7 @@ struct HeadsArgs {
     const int* positions;
     const double* inv_freq;
     int D, rot, adjacent, rows;
-    float eps, scale;
+    float eps, scale, inv_d;
 };
 
 __device__ __forceinline__ unsigned long long turn_fraction(double inv_freq) {
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
     }
 #pragma unroll
     for (int s = 16; s; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
-    const float r = rsqrtf(ss / (float)a.D + a.eps);
+    const float r = rsqrtf(ss * a.inv_d + a.eps);
     const int half = a.rot / 2;
     for (int j = lane; j < half; j += 32) {
         const int ia = a.adjacent ? 2 * j : j, ib = a.adjacent ? 2 * j + 1 : j + half;
@@ -75,8 +75,8 @@ __global__ void __launch_bounds__(256) heads_kernel(const HeadsArgs a) {
 
 // Heads of up to 256 elements whose rows allow it move four elements a lane at a time.  A CTA has one row (its sines and cosines are computed
 // once, into shared memory) and up to HEADS_BATCH heads a warp, whose loads are all issued first; a head's L lanes add its squares by
-// shuffles and swap partners of the rotation through shared memory.  Bound by memory: 8192 rows of 24 + 4 heads of 256, fp32 to bf16, 68 us =
-// 5.2 TB/s (four heads a warp, eight warps a CTA, three CTAs an SM 77) against 114 us element by element, where every head's warp computed its own angles.
+// shuffles and swap partners of the rotation through shared memory.  Bound by memory: 8192 rows of 24 + 4 heads of 256, fp32 to bf16, 62 us =
+// 5.7 TB/s (four heads a warp, eight warps a CTA, three CTAs an SM 77) against 114 us element by element, where every head's warp computed its own angles.
 constexpr int HEADS_BATCH = 2, HEADS_WARPS = 4, HEADS_MAX_D = 256;
 
 template <typename T> __device__ __forceinline__ float4 load4(const T* p) {
@@ -97,43 +97,43 @@ template <typename T> __device__ __forceinline__ void store4(T* p, float4 v) {
     }
 }
 
-// L lanes a head (two heads a warp where 16 do), NV vectors of four elements a lane
+// L lanes a head (two heads a warp where 16 do), NV vectors of four elements a lane.  A CTA has heads of one tensor: its pointers and weights
+// are the same for all of them (with heads of both in a CTA 68 us, bound by the issue of instructions: 232 a head, 74 % of the slots).
 template <typename Tin, typename Tout, int L, int NV>
-__global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const HeadsArgs a, int heads_per_cta, int ctas_per_row) {
-    constexpr int SUB = 32 / L;
+__global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const HeadsArgs a, int heads_per_cta, int q_ctas, int ctas_per_row) {
+    constexpr int SUB = 32 / L, STEP = HEADS_WARPS * SUB;
     __shared__ float cs[HEADS_MAX_D / 2], sn[HEADS_MAX_D / 2];
     __shared__ float4 swap[HEADS_WARPS][32 * NV];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l = lane % L, half = a.rot / 2, nq = a.t[0].n_heads;
-    const int row = (int)(blockIdx.x / (unsigned)ctas_per_row), h0 = (int)(blockIdx.x % (unsigned)ctas_per_row) * heads_per_cta;
-    const int h_end = min(nq + a.t[1].n_heads, h0 + heads_per_cta), h_mine = h0 + warp * SUB + lane / L;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, l = lane % L, half = a.rot / 2;
+    const int row = (int)(blockIdx.x / (unsigned)ctas_per_row), c = (int)(blockIdx.x % (unsigned)ctas_per_row);
+    const q38b_heads& t = a.t[c >= q_ctas];
+    const int h0 = (c >= q_ctas ? c - q_ctas : c) * heads_per_cta, h_end = min(t.n_heads, h0 + heads_per_cta), h_mine = h0 + warp * SUB + lane / L;
+    const Tin* src = (const Tin*)t.src + row * t.src_row + h_mine * t.src_head + 4 * l;
     float4 x[HEADS_BATCH][NV];
 #pragma unroll
-    for (int b = 0; b < HEADS_BATCH; b++) {
-        const int h = h_mine + b * HEADS_WARPS * SUB;
-        const q38b_heads& t = a.t[h >= nq];
-        const Tin* src = (const Tin*)t.src + row * t.src_row + (h >= nq ? h - nq : h) * t.src_head;
+    for (int b = 0; b < HEADS_BATCH; b++)
 #pragma unroll
-        for (int i = 0; i < NV; i++) x[b][i] = h < h_end && 4 * (l + L * i) < a.D ? load4(src + 4 * (l + L * i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
+        for (int i = 0; i < NV; i++)
+            x[b][i] = h_mine + b * STEP < h_end && 4 * (l + L * i) < a.D ? load4(src + b * STEP * t.src_head + 4 * L * i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (tid < half) turn_sincos(turn_fraction(a.inv_freq[tid]), a.positions[row], a.scale, sn[tid], cs[tid]);
+    float4 w[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) w[i] = t.weight && 4 * (l + L * i) < a.D ? __ldg((const float4*)(t.weight + 4 * (l + L * i))) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+    Tout* dst = (Tout*)t.dst + row * t.dst_row + h_mine * t.dst_head + 4 * l;
     __syncthreads();
 #pragma unroll
     for (int b = 0; b < HEADS_BATCH; b++) {
-        const int h = h_mine + b * HEADS_WARPS * SUB;
-        if (h0 + warp * SUB + b * HEADS_WARPS * SUB >= h_end) break;   // (the whole warp)
-        const q38b_heads& t = a.t[h >= nq];
+        if (h0 + warp * SUB + b * STEP >= h_end) break;   // (the whole warp)
         float ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; i++) ss += x[b][i].x * x[b][i].x + x[b][i].y * x[b][i].y + x[b][i].z * x[b][i].z + x[b][i].w * x[b][i].w;
 #pragma unroll
         for (int s = L / 2; s; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
-        const float r = rsqrtf(ss / (float)a.D + a.eps);
+        const float r = rsqrtf(ss * a.inv_d + a.eps);
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int e = 4 * (l + L * i);
-            const float4 w = t.weight && e < a.D ? __ldg((const float4*)(t.weight + e)) : make_float4(1.0f, 1.0f, 1.0f, 1.0f);
             float4& z = x[b][i];
-            z = make_float4(z.x * r * w.x, z.y * r * w.y, z.z * r * w.z, z.w * r * w.w);
+            z = make_float4(z.x * r * w[i].x, z.y * r * w[i].y, z.z * r * w[i].z, z.w * r * w[i].w);
         }
         if (a.adjacent) {
 #pragma unroll
@@ -146,27 +146,28 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const Head
         } else if (half) {
             float4* mine = swap[warp] + lane / L * L * NV;
 #pragma unroll
-            for (int i = 0; i < NV; i++) mine[l + L * i] = x[b][i];
+            for (int i = 0; i < NV; i++)
+                if (4 * (l + L * i) < a.rot) mine[l + L * i] = x[b][i];
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const int e = 4 * (l + L * i);
                 if (e < a.rot) {
                     const bool second = e >= half;
-                    const int j = second ? e - half : e;
-                    const float4 o = mine[(second ? e - half : e + half) / 4], c = *(const float4*)(cs + j), n = *(const float4*)(sn + j);
+                    const int other = second ? e - half : e + half, j = second ? other : e;
+                    const float4 o = mine[other / 4], cj = *(const float4*)(cs + j);
+                    float4 n = *(const float4*)(sn + j);
+                    if (!second) n = make_float4(-n.x, -n.y, -n.z, -n.w);
                     float4& z = x[b][i];
-                    z = second ? make_float4(z.x * c.x + o.x * n.x, z.y * c.y + o.y * n.y, z.z * c.z + o.z * n.z, z.w * c.w + o.w * n.w)
-                               : make_float4(z.x * c.x - o.x * n.x, z.y * c.y - o.y * n.y, z.z * c.z - o.z * n.z, z.w * c.w - o.w * n.w);
+                    z = make_float4(z.x * cj.x + o.x * n.x, z.y * cj.y + o.y * n.y, z.z * cj.z + o.z * n.z, z.w * cj.w + o.w * n.w);
                 }
             }
             __syncwarp();
         }
-        if (h < h_end) {
-            Tout* dst = (Tout*)t.dst + row * t.dst_row + (h >= nq ? h - nq : h) * t.dst_head;
+        if (h_mine + b * STEP < h_end) {
 #pragma unroll
             for (int i = 0; i < NV; i++)
-                if (4 * (l + L * i) < a.D) store4(dst + 4 * (l + L * i), x[b][i]);
+                if (4 * (l + L * i) < a.D) store4(dst + b * STEP * t.dst_head + 4 * L * i, x[b][i]);
         }
     }
 }
@@ -405,13 +406,14 @@ int heads_as(q38b_ctx* ctx, const HeadsArgs& a, cudaStream_t st) {
         // as many heads a CTA as its warps take at once, fewer where rows alone leave SMs idle
         const int once = HEADS_WARPS * (a.D <= 64 ? 2 : 1);
         int per = once * HEADS_BATCH;
-        while (per > once && (long long)a.rows * ((n_heads + per - 1) / per) < 2 * ctx->sm_count) per -= once;
-        const int ctas = (n_heads + per - 1) / per;
-        const long long grid = (long long)a.rows * ctas;
+        const auto ctas = [&](int n, int of) { return (n + of - 1) / of; };
+        while (per > once && (long long)a.rows * (ctas(a.t[0].n_heads, per) + ctas(a.t[1].n_heads, per)) < 2 * ctx->sm_count) per -= once;
+        const int q = ctas(a.t[0].n_heads, per), all = q + ctas(a.t[1].n_heads, per);
+        const long long grid = (long long)a.rows * all;
         if (grid > 0x7FFFFFFF) return Q38B_ERR_UNSUPPORTED;
-        if (a.D <= 64) heads4_kernel<Tin, Tout, 16, 1><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, ctas);
-        else if (a.D <= 128) heads4_kernel<Tin, Tout, 32, 1><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, ctas);
-        else heads4_kernel<Tin, Tout, 32, 2><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, ctas);
+        if (a.D <= 64) heads4_kernel<Tin, Tout, 16, 1><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, q, all);
+        else if (a.D <= 128) heads4_kernel<Tin, Tout, 32, 1><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, q, all);
+        else heads4_kernel<Tin, Tout, 32, 2><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, q, all);
         return launch_status(ctx, cudaSuccess);
     }
     const long long blocks = ((long long)a.rows * n_heads + 7) / 8;
@@ -480,6 +482,7 @@ int q38b_qk_norm_rope(q38b_ctx* ctx, const q38b_heads* q, const q38b_heads* k, i
     a.rows = rows;
     a.eps = eps;
     a.scale = scale;
+    a.inv_d = 1.0f / (float)D;
     a.positions = positions;
     a.inv_freq = inv_freq;
     DeviceGuard on(ctx);
