@@ -237,6 +237,7 @@ struct MxArgs {
     const void* x;          // FUSED: the activations as they are
     long long x_ld;
     int x_kind, x_steps;    // x_steps: stages of K a CTA holds, at most
+    int box_at;             // splits: where the others' sums come in shared memory; 0: over the ring
 };
 __host__ __device__ constexpr int mx_groups(int n_tile) { return (n_tile + 127) / 128; }
 __host__ __device__ constexpr int mx_stage_bytes(int n_tile) { return MX_A_BYTES + n_tile * (MX_K / 2) + MX_SFA_BYTES * (1 + mx_groups(n_tile)); }
@@ -391,6 +392,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *tmem_slot;
+    if (a.box_at) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");   // (this CTA has started; waited for in front of the exchange)
     if (a.pdl) pdl_wait_prior();
 
     if (warp == 0) {
@@ -506,12 +508,15 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
                 store(chunk, f);
             }
     } else {
-        // Chunk c of the tile is finished by rank c % splits: the others put their sums of it into that CTA's ring, idle by then,
-        // [source][c / splits][16 tokens][128 rows]; sums are added in rank order.
+        // Chunk c of the tile is finished by rank c % splits: the others put their sums of it into that CTA's shared memory,
+        // [source][c / splits][16 tokens][128 rows]; sums are added in rank order.  Few tokens have a place of their own there; more go over
+        // the ring, which every CTA's tensor core has read by then.
         const int own_chunks = (n_chunks + a.splits - 1) / a.splits;
-        const uint32_t box = smem_u32(ring);
+        const uint8_t* boxes = a.box_at ? smem + a.box_at : ring;
+        const uint32_t box = smem_u32(boxes);
         __syncwarp();
-        cluster_sync_all();
+        if (a.box_at) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+        else cluster_sync_all();
         if (warp >= 2)
             for (int chunk = part; chunk < n_chunks; chunk += 2) {
                 const int owner = chunk % a.splits;
@@ -530,7 +535,7 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
                 float f[16] = {};
                 tmem_ld16(acc + (uint32_t)(16 * (own * a.splits + rank)), v);
                 for (int r = 0; r < a.splits; r++) {
-                    const float* in = (const float*)ring + (size_t)((r - (r > rank ? 1 : 0)) * own_chunks + own) * (16 * MX_ROWS) + 32 * quad + lane;
+                    const float* in = (const float*)boxes + (size_t)((r - (r > rank ? 1 : 0)) * own_chunks + own) * (16 * MX_ROWS) + 32 * quad + lane;
 #pragma unroll
                     for (int j = 0; j < 16; j++) f[j] += r == rank ? __uint_as_float(v[j]) : in[j * MX_ROWS];
                 }
@@ -733,7 +738,7 @@ mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, co
 
 // How a product is cut: tokens in tiles of n_tile (one tile, or several of 128 or 256: a tile starts on a scale tile's border), K in
 // `splits` parts.
-struct MxCut { int n_tile, stages, splits; };
+struct MxCut { int n_tile, stages, splits, box; };   // box: bytes of shared memory for the others' sums (0: over the ring)
 
 int exchange_bytes(const MxCut& c) {
     const int chunks = c.n_tile / 16;
@@ -749,10 +754,10 @@ MxCut mx_cut(int sm_count, int smem_optin, int K, int M, int B, double* cost_of)
     MxCut c;
     c.n_tile = B <= MX_MAX_N ? (B + 15) / 16 * 16 : MX_MAX_N;
     const long long tiles = (long long)((M + MX_ROWS - 1) / MX_ROWS) * ((B + c.n_tile - 1) / c.n_tile);
-    c.stages = std::min(MX_MAX_STAGES, (smem_optin - 1024) / mx_stage_bytes(c.n_tile));
-    c.stages = std::min(c.stages, (512 - mx_acc_cols(c.n_tile)) / mx_scale_cols(c.n_tile));
     for (c.splits = 1; c.splits <= std::min(MX_MAX_SPLITS, steps); c.splits++) {
-        if (c.splits > 1 && exchange_bytes(c) > c.stages * mx_stage_bytes(c.n_tile)) break;
+        c.box = c.splits > 1 && c.n_tile <= 32 ? exchange_bytes(c) : 0;
+        c.stages = std::min(std::min(MX_MAX_STAGES, (smem_optin - 1024 - c.box) / mx_stage_bytes(c.n_tile)), (512 - mx_acc_cols(c.n_tile)) / mx_scale_cols(c.n_tile));
+        if (c.splits > 1 && !c.box && exchange_bytes(c) > c.stages * mx_stage_bytes(c.n_tile)) break;
         const long long slots = c.splits <= 2 ? sm_count : sm_count * 9 / 10 / c.splits * c.splits, ctas = tiles * c.splits;
         const double cost = (double)((ctas + slots - 1) / slots) * ((steps + c.splits - 1) / c.splits * (600.0 + 5.0 * c.n_tile) + 4000.0 + (c.splits > 1 ? 1500.0 + 10.0 * c.n_tile : 0.0));
         if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
@@ -870,8 +875,11 @@ int pair_as(q38b_ctx* ctx, const MxPairArgs& a, const CUtensorMap& wmap, const C
     return launch_status(ctx, cudaLaunchKernelEx(&cfg, kern, a, wmap, xmap, wsmap, xsmap, ymap));
 }
 
+// where the shared memory behind the ring begins
+template <bool FUSED> int mx_box_at(const MxArgs& a) { return 1024 + (FUSED ? mx_fused_x_bytes(a.x_steps) + a.stages * MX_FUSED_STAGE : a.stages * mx_stage_bytes(a.n_tile)); }
+
 template <typename T, int GROUPS, bool FUSED>
-int gemm_as(q38b_ctx* ctx, const MxArgs& a, const CUtensorMap& wmap, const CUtensorMap& xmap, cudaStream_t st) {
+int gemm_as(q38b_ctx* ctx, const MxArgs& a, int box, const CUtensorMap& wmap, const CUtensorMap& xmap, cudaStream_t st) {
     auto kern = mx4_gemm_kernel<T, GROUPS, FUSED>;
     const int rc = q38b_ensure_kernel_smem(ctx, (const void*)kern, ctx->smem_optin, false);
     if (rc != Q38B_OK) return rc;
@@ -879,7 +887,7 @@ int gemm_as(q38b_ctx* ctx, const MxArgs& a, const CUtensorMap& wmap, const CUten
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)((a.M + MX_ROWS - 1) / MX_ROWS * a.splits), (unsigned)((a.B + a.n_tile - 1) / a.n_tile));
     cfg.blockDim = dim3(MX_THREADS);
-    cfg.dynamicSmemBytes = (size_t)(1024 + (FUSED ? mx_fused_x_bytes(a.x_steps) + a.stages * MX_FUSED_STAGE : a.stages * mx_stage_bytes(a.n_tile)));
+    cfg.dynamicSmemBytes = (size_t)mx_box_at<FUSED>(a) + box;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     int n = 0;
@@ -899,10 +907,11 @@ int gemm_as(q38b_ctx* ctx, const MxArgs& a, const CUtensorMap& wmap, const CUten
     return launch_status(ctx, cudaLaunchKernelEx(&cfg, kern, a, wmap, xmap));
 }
 template <int GROUPS, bool FUSED>
-int gemm_kind(q38b_ctx* ctx, const MxArgs& a, const CUtensorMap& wmap, const CUtensorMap& xmap, int y_kind, cudaStream_t st) {
-    return y_kind == Q38B_OUT_F32 ? gemm_as<float, GROUPS, FUSED>(ctx, a, wmap, xmap, st)
-         : y_kind == Q38B_OUT_F16 ? gemm_as<__half, GROUPS, FUSED>(ctx, a, wmap, xmap, st)
-                                  : gemm_as<__nv_bfloat16, GROUPS, FUSED>(ctx, a, wmap, xmap, st);
+int gemm_kind(q38b_ctx* ctx, MxArgs a, int box, const CUtensorMap& wmap, const CUtensorMap& xmap, int y_kind, cudaStream_t st) {
+    a.box_at = box ? mx_box_at<FUSED>(a) : 0;
+    return y_kind == Q38B_OUT_F32 ? gemm_as<float, GROUPS, FUSED>(ctx, a, box, wmap, xmap, st)
+         : y_kind == Q38B_OUT_F16 ? gemm_as<__half, GROUPS, FUSED>(ctx, a, box, wmap, xmap, st)
+                                  : gemm_as<__nv_bfloat16, GROUPS, FUSED>(ctx, a, box, wmap, xmap, st);
 }
 
 MxArgs mx_args(q38b_ctx* ctx, const MxCut& cut, const void* W_scales, int K, int M, int B, void* Y, long long ldy, int accumulate) {
@@ -1002,7 +1011,7 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
     MxArgs a = mx_args(ctx, one, W_scales, K, M, B, Y, ldy, accumulate);
     a.x_scales = (const uint8_t*)X_scales;
     a.pdl = behind_quantizer ? 1 : 0;
-    return mx_groups(a.n_tile) == 1 ? gemm_kind<1, false>(ctx, a, wmap, xmap, y_kind, st) : gemm_kind<2, false>(ctx, a, wmap, xmap, y_kind, st);
+    return mx_groups(a.n_tile) == 1 ? gemm_kind<1, false>(ctx, a, one.box, wmap, xmap, y_kind, st) : gemm_kind<2, false>(ctx, a, one.box, wmap, xmap, y_kind, st);
 }
 
 int q38b_gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales, int K, int M, const void* X, long long X_ld, const void* X_scales, int B,
@@ -1031,7 +1040,7 @@ int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_
         const int steps = (K + MX_K - 1) / MX_K, x_steps = (steps + cut.splits - 1) / cut.splits;
         if (x_steps * MX_K <= MX_FUSE_MAX_K) {
             DeviceGuard on(ctx);
-            cut.stages = std::min(MX_MAX_STAGES, (ctx->smem_optin - 1024 - mx_fused_x_bytes(x_steps)) / MX_FUSED_STAGE);
+            cut.stages = std::min(MX_MAX_STAGES, (ctx->smem_optin - 1024 - cut.box - mx_fused_x_bytes(x_steps)) / MX_FUSED_STAGE);
             CUtensorMap wmap, none;
             memset(&none, 0, sizeof(none));
             if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS)) return Q38B_ERR_ARG;
@@ -1040,7 +1049,7 @@ int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_
             a.x_ld = x_ld;
             a.x_kind = x_kind;
             a.x_steps = x_steps;
-            return gemm_kind<1, true>(ctx, a, wmap, none, y_kind, (cudaStream_t)stream);
+            return gemm_kind<1, true>(ctx, a, cut.box, wmap, none, y_kind, (cudaStream_t)stream);
         }
     }
     if (!scratch) return Q38B_ERR_ARG;
