@@ -446,16 +446,19 @@ class Context:
         rows, K = x.shape
         ld, one = x.stride()
         kind = _OUT_KINDS.get(x.dtype)
-        _need(kind is not None and one == 1 and x.get_device() == self._index, "quantize_mx4: fp32, fp16 or bf16 [rows, K] on the context's device")
+        if kind is None or one != 1 or x.get_device() != self._index:
+            raise ValueError("quantize_mx4: fp32, fp16 or bf16 [rows, K] on the context's device")
         if K % 32 or K == 0 or rows == 0:
             raise Q38BError(-1, "q38b_quantize_mx4")
         half, tiles = K // 2, ((rows + 127) // 128) * ((K + 127) // 128) * 512
         codes = _empty((rows, half), (half, 1), dtype=torch.uint8, device=self.device)
         scales = _empty((tiles,), (1,), dtype=torch.uint8, device=self.device)
-        rc = self.lib.q38b_quantize_mx4(self.h, x.data_ptr(), kind, ld if rows > 1 else K, K, rows, codes.data_ptr(), half, scales.data_ptr(), self._stream())
+        rc = self.lib.q38b_quantize_mx4(self.h, x.data_ptr(), kind, ld if rows > 1 else K, K, rows, codes.data_ptr(), half, scales.data_ptr(), _current_stream(self._index))
         if rc:
             self._rc(rc, "q38b_quantize_mx4")
-        return Mx4(codes, scales)
+        m = Mx4.__new__(Mx4)   # (made here: nothing to check)
+        m.codes, m.scales, m.rows, m.K, m.ld = codes, scales, rows, K, half
+        return m
 
     def pack_mx4(self, codes, scales):
         """Codes uint8 [rows, K / 2] and scale bytes uint8 [rows, K / 32] of another producer -> Mx4 (the codes are kept, not copied)."""
@@ -469,9 +472,11 @@ class Context:
 
     def dequant_mx4(self, m, kind=OUT_F32):
         """The values of an Mx4: [rows, K]."""
-        _need(m.codes.get_device() == self._index, "dequant_mx4: a matrix on the context's device")
-        out = _empty((m.rows, m.K), (m.K, 1), dtype=_OUT_DTYPES[kind], device=self.device)
-        rc = self.lib.q38b_dequant_mx4(self.h, m.codes.data_ptr(), m.ld, m.scales.data_ptr(), m.K, m.rows, out.data_ptr(), kind, m.K, self._stream())
+        codes, rows, K = m.codes, m.rows, m.K
+        if codes.get_device() != self._index:
+            raise ValueError("dequant_mx4: a matrix on the context's device")
+        out = _empty((rows, K), (K, 1), dtype=_OUT_DTYPES[kind], device=self.device)
+        rc = self.lib.q38b_dequant_mx4(self.h, codes.data_ptr(), m.ld, m.scales.data_ptr(), K, rows, out.data_ptr(), kind, K, _current_stream(self._index))
         if rc:
             self._rc(rc, "q38b_dequant_mx4")
         return out
