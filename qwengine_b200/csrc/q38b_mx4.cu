@@ -223,8 +223,7 @@ __global__ void __launch_bounds__(256) mx4_dequant_kernel(const uint8_t* codes, 
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int MX_ROWS = 128, MX_MAX_N = 256, MX_K = 256;
 constexpr int MX_THREADS = 320, MX_MAX_STAGES = 12, MX_MAX_SPLITS = 8;
-constexpr int MX_FUSE_MAX_B = 1;      // up to so many tokens every CTA quantizes its part of the activations itself
-constexpr int MX_FUSE_MAX_K = 8192;   // ... of at most so many K
+constexpr int MX_FUSE_MAX_K = 8192;   // one token: every CTA quantizes its part of the activations itself, of at most so many K
 constexpr int MX_A_BYTES = MX_ROWS * MX_K / 2, MX_SFA_BYTES = 2 * MX_TILE;
 
 struct MxArgs {
@@ -234,8 +233,7 @@ struct MxArgs {
     int* status;
     int K, M, B, accumulate;
     int n_tile, stages, splits, pdl;
-    const void* x;          // FUSED: the activations as they are
-    long long x_ld;
+    const void* x;          // FUSED: the token's activations as they are
     int x_kind, x_steps;    // x_steps: stages of K a CTA holds, at most
     int box_at;             // splits: where the others' sums come in shared memory; 0: over the ring
 };
@@ -320,7 +318,7 @@ __device__ __forceinline__ void load_x8(const void* x, int kind, long long at, b
         return;
     }
     const uint16_t* p = (const uint16_t*)x + at;
-    uint16_t h[8];
+    alignas(16) uint16_t h[8];
     if (vec) {
         *(uint4*)h = *(const uint4*)p;
     } else {
@@ -433,28 +431,21 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
             if (++st == a.stages) { st = 0; use ^= 1u; }
         }
     } else if constexpr (FUSED) {
-        // units of eight values of a row, four lanes a block; behind K zeros as far as the last step of 64 K reaches
-        const int k0 = s_begin * MX_K, span = min(s_end * MX_K, (a.K + 63) / 64 * 64) - k0, per_row = span / 8, units = a.B * per_row;
-        const bool vec = (((uintptr_t)a.x | (uintptr_t)(a.x_ld * (a.x_kind == Q38B_OUT_F32 ? 4 : 2))) & 15) == 0;
-        constexpr int AHEAD = 4;   // units of a lane on their way at a time
+        // units of eight values, four lanes a block; behind K zeros as far as the last step of 64 K reaches
+        const int k0 = s_begin * MX_K, units = (min(s_end * MX_K, (a.K + 63) / 64 * 64) - k0) / 8;
+        const bool vec = ((uintptr_t)a.x & 15) == 0;
+        constexpr int AHEAD = 3;   // units of a lane on their way at a time (5120 K: all of them)
         for (int u0 = 32 * (warp - 2); u0 < units; u0 += 256 * AHEAD) {
-            float v[AHEAD][8];
-            int row[AHEAD], at[AHEAD];
+            float v[AHEAD][8] = {};
 #pragma unroll
             for (int g = 0; g < AHEAD; g++) {
-                const int u = u0 + 256 * g + lane;
-                row[g] = u / per_row;
-                at[g] = (u - row[g] * per_row) * 8;
-                if (u < units && k0 + at[g] < a.K) {
-                    load_x8(a.x, a.x_kind, (long long)row[g] * a.x_ld + k0 + at[g], vec, v[g]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) v[g][i] = 0.0f;
-                }
+                const int k = 8 * (u0 + 256 * g + lane);
+                if (k < 8 * units && k0 + k < a.K) load_x8(a.x, a.x_kind, k0 + k, vec, v[g]);
             }
 #pragma unroll
             for (int g = 0; g < AHEAD; g++) {
                 if (u0 + 256 * g >= units) break;   // (the whole warp)
+                const int k = 8 * (u0 + 256 * g + lane);
                 uint32_t top = 0u;
 #pragma unroll
                 for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[g][i]) & 0x7FFFFFFFu);
@@ -465,10 +456,10 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
 #pragma unroll
                 for (int i = 0; i < 8; i++) v[g][i] *= inv;
                 const uint32_t code = e2m1_eight(v[g]);
-                if (u0 + 256 * g + lane < units) {   // 128 bytes of a row hold 256 K; 16-byte piece c at c ^ (row & 7) (128-byte swizzle)
-                    const int s = at[g] / MX_K, b = at[g] % MX_K / 2, r = row[g];
-                    *(uint32_t*)(x_codes + s * MX_FUSED_X + r * 128 + 16 * ((b / 16) ^ (r & 7)) + b % 16) = code;
-                    if (lane % 4 == 0) x_sf[s * MX_SFA_BYTES + b / 64 * MX_TILE + 16 * r + b / 16 % 4] = (uint8_t)byte;
+                if (k < 8 * units) {   // row 0 of operand B: 128 bytes a stage hold 256 K, in order (the swizzle moves rows 1 to 7)
+                    const int s = k / MX_K, b = k % MX_K / 2;
+                    *(uint32_t*)(x_codes + s * MX_FUSED_X + b) = code;
+                    if (lane % 4 == 0) x_sf[s * MX_SFA_BYTES + b / 64 * MX_TILE + b / 16 % 4] = (uint8_t)byte;
                 }
             }
         }
@@ -961,6 +952,7 @@ int q38b_mx4_tile_scales(q38b_ctx* ctx, const void* src, long long src_ld, int K
     if ((uintptr_t)scales & 15) return Q38B_ERR_ALIGN;
     DeviceGuard on(ctx);
     const size_t n = q38b_mx4_scale_bytes(K, rows);
+    if ((n + 255) / 256 > 0x7FFFFFFF) return Q38B_ERR_UNSUPPORTED;
     mx4_tile_kernel<<<(unsigned)((n + 255) / 256), 256, 0, (cudaStream_t)stream>>>((const uint8_t*)src, src_ld, K, rows, (uint8_t*)scales);
     return launch_status(ctx, cudaSuccess);
 }
@@ -1020,7 +1012,7 @@ int q38b_gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_sc
 }
 
 size_t q38b_gemm_mx4_scratch_bytes(int K, int B) {
-    if (!mx_shape(K, B) || (B <= MX_FUSE_MAX_B && K <= MX_FUSE_MAX_K)) return 0;
+    if (!mx_shape(K, B) || (B == 1 && K <= MX_FUSE_MAX_K)) return 0;
     return (size_t)B * (K / 2) + q38b_mx4_scale_bytes(K, B) + 16;
 }
 
@@ -1035,7 +1027,7 @@ int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_
     if (need && !scratch) return Q38B_ERR_ARG;
     if ((uintptr_t)scratch & 15) return Q38B_ERR_ALIGN;
     if (scratch_bytes < need) return Q38B_ERR_NOMEM;
-    if (B <= MX_FUSE_MAX_B && ctx->mx4_pairs <= 0 && !ctx->mx4_two_launches) {
+    if (B == 1 && ctx->mx4_pairs <= 0 && !ctx->mx4_two_launches) {
         MxCut cut = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B, nullptr);   // (the same cut as of the two calls: the same sums)
         const int steps = (K + MX_K - 1) / MX_K, x_steps = (steps + cut.splits - 1) / cut.splits;
         if (x_steps * MX_K <= MX_FUSE_MAX_K) {
@@ -1046,7 +1038,6 @@ int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_
             if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS)) return Q38B_ERR_ARG;
             MxArgs a = mx_args(ctx, cut, W_scales, K, M, B, Y, ldy, accumulate);
             a.x = x;
-            a.x_ld = x_ld;
             a.x_kind = x_kind;
             a.x_steps = x_steps;
             return gemm_kind<1, true>(ctx, a, cut.box, wmap, none, y_kind, (cudaStream_t)stream);

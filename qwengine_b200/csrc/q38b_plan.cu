@@ -642,8 +642,9 @@ int q38b_pass_op_qk_norm_rope(q38b_pass* p, const q38b_pass_heads* q, const q38b
     if (!p || !q || D < 1 || D > 1024 || rot < 0 || rot > D || rot % 2 || (rot > 0 && (!positions || !inv_freq))) return Q38B_ERR_ARG;
     if (((uintptr_t)positions & 3) || ((uintptr_t)inv_freq & 7)) return Q38B_ERR_ALIGN;
     HeadsStep s = {{*q, k ? *k : q38b_pass_heads{}}, k ? 2 : 1, D, rot, adjacent, eps, scale, positions, inv_freq};
-    struct Span { int buf; long long lo, hi; bool written; int of; };
-    std::vector<Span> spans;
+    struct Span { int buf; long long lo, hi; bool written; };
+    Span spans[4];
+    int n_spans = 0;
     for (int i = 0; i < s.n_tensors; i++) {
         const q38b_pass_heads& t = s.t[i];
         if (!is_f32(p, t.src) || !is_f32(p, t.dst) || t.n_heads < 1 || t.src_off < 0 || t.dst_off < 0 || t.src_head < 0) return Q38B_ERR_ARG;
@@ -652,15 +653,19 @@ int q38b_pass_op_qk_norm_rope(q38b_pass* p, const q38b_pass_heads* q, const q38b
         const long long src_end = t.src_off + (long long)(t.n_heads - 1) * t.src_head + D, dst_end = t.dst_off + (long long)(t.n_heads - 1) * t.dst_head + D;
         if (src_end > p->bufs[t.src].n || dst_end > p->bufs[t.dst].n) return Q38B_ERR_ARG;
         const bool in_place = t.src == t.dst && t.src_off == t.dst_off && (t.n_heads == 1 || t.src_head == t.dst_head);
-        if (!in_place) spans.push_back({t.src, t.src_off, src_end, false, i});
-        spans.push_back({t.dst, t.dst_off, dst_end, true, i});
+        if (!in_place) spans[n_spans++] = {t.src, t.src_off, src_end, false};
+        spans[n_spans++] = {t.dst, t.dst_off, dst_end, true};
     }
     // what is written lies apart from everything else that is read or written (but for heads mended in place)
-    for (const Span& w : spans)
-        for (const Span& o : spans)
-            if (w.written && &w != &o && w.buf == o.buf && w.lo < o.hi && o.lo < w.hi) return Q38B_ERR_ARG;
-    p->heads.push_back(s);
-    p->ops.push_back({OP_HEADS, (int)p->heads.size() - 1, 0, 0, 0, 0, 0});
+    for (int i = 0; i < n_spans; i++)
+        for (int j = 0; j < n_spans; j++)
+            if (spans[i].written && i != j && spans[i].buf == spans[j].buf && spans[i].lo < spans[j].hi && spans[j].lo < spans[i].hi) return Q38B_ERR_ARG;
+    try {
+        p->heads.push_back(s);
+        p->ops.push_back({OP_HEADS, (int)p->heads.size() - 1, 0, 0, 0, 0, 0});
+    } catch (...) {
+        return Q38B_ERR_NOMEM;
+    }
     return Q38B_OK;
 }
 
@@ -670,8 +675,12 @@ int q38b_pass_op_adjust_logits(q38b_pass* p, int src, int off, int n, const q38b
     if (src == dst && off != dst_off && off < dst_off + (long long)n && dst_off < off + (long long)n) return Q38B_ERR_ARG;
     const int rc = q38b_logit_rules_check(rules, n, 0);
     if (rc != Q38B_OK) return rc;
-    p->logits.push_back({*rules});
-    p->ops.push_back({OP_LOGITS, (int)p->logits.size() - 1, src, dst, dst_off, n, off});
+    try {
+        p->logits.push_back({*rules});
+        p->ops.push_back({OP_LOGITS, (int)p->logits.size() - 1, src, dst, dst_off, n, off});
+    } catch (...) {
+        return Q38B_ERR_NOMEM;
+    }
     return Q38B_OK;
 }
 

@@ -366,11 +366,11 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
         mend(0, waiting);
     }
     if (!any) return;
-    const long long biases = a.r.bias_begin[row], count_b = a.r.bias_begin[row + 1] - biases;   // (again, not kept in registers)
-    const int* ids = a.r.bias_ids + biases;
+    const long long from = a.r.bias_begin[row], count = a.r.bias_begin[row + 1] - from;   // (again: not kept in registers)
+    const int* ids = a.r.bias_ids + from;
     auto each = [&](auto&& f) {   // f(entry, place) for this thread's biases among the block's logits
         if (bias_at < (uint32_t)n) f((uint32_t)tid, bias_at);
-        for (long long j = tid + LG_THREADS; j < count_b; j += LG_THREADS) {
+        for (long long j = tid + LG_THREADS; j < count; j += LG_THREADS) {
             const uint32_t at = (uint32_t)ids[j] - first;
             if (at < (uint32_t)n) f((uint32_t)j, at);
         }
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
     each([&](uint32_t j, uint32_t at) { atomicMax(&seen[at], j + 1u); });
     __syncthreads();
     each([&](uint32_t j, uint32_t at) {
-        if (seen[at] == j + 1u && allowed(at)) y[at] += a.r.bias_values[biases + j];
+        if (seen[at] == j + 1u && allowed(at)) y[at] += a.r.bias_values[from + j];
     });
 }
 
