@@ -545,7 +545,9 @@ __global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a,
 // Many tokens: two CTAs (a cluster of two on neighbouring SMs) multiply as one, M = 256: each holds 128 weight rows and half of
 // the tokens' codes, so that a stage costs an SM 16 + 16 KB of codes for 256 x 256 instead of 16 + 32 for 128 x 256.  The pairs
 // stay and walk the tiles (tokens fastest: neighbours read the same weights out of L2), the ring runs on across tiles, and eight warps
-// bring the accumulator to registers and hand it back before they store: the tensor core goes on meanwhile.  Outputs leave through
+// bring the accumulator to registers and hand it back before they store: the tensor core goes on meanwhile.  Bound by shared memory: a
+// stage of 256 tokens writes 35 KB there and the tensor cores of both SMs read 48 KB of it, 650 clocks at 128 bytes, of which the MMA need 512;
+// it takes 870 (2048 x 17408 x 5120 in 73 us = 5.0 PFLOP/s; without stores 61, loads alone 44).  Outputs leave through
 // shared memory and TMA stores (a token's 128 rows are one piece of 256 or 512 bytes) where Y's base and row stride are multiples of 16
 // bytes; plain stores, 64 bytes of a token a warp in 16 bits, stood in the way of the loads: 2048 x 17408 x 5120 76 us, 61 without them.
 // ---------------------------------------------------------------------------------------------------------------
@@ -603,23 +605,26 @@ mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, co
     if (a.pdl) pdl_wait_prior();
 
     if (warp == 0) {
-        if (lane == 0) {
-            int st = 0;
-            uint32_t use = 0;
-            for (int tile = pair; tile < a.n_tiles; tile += n_pairs) {
-                const int row0 = tile / a.tok_tiles * 256 + side * MX_ROWS, tok0 = tile % a.tok_tiles * a.n_tile;
-                const int n_mma = (min(a.n_tile, a.B - tok0) + 31) / 32 * 32;
-                for (int s = 0; s < steps; s++) {
-                    mbar_wait_bounded(smem_u32(&empty[st]), use ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
-                    const uint32_t bar = peer_smem(smem_u32(&full[st]), 0u), at = smem_u32(ring + st * stage_bytes);
-                    const uint32_t sf = at + MX_A_BYTES + (uint32_t)(a.n_tile / 2) * (MX_K / 2);
+        // The whole warp walks and one elected lane issues, as for the MMA: the addresses stay in uniform registers (under `if (lane == 0)`
+        // four copies and a wait took some 700 clocks a stage: 2048 x 17408 x 5120 in tiles of 192 tokens 85 -> 78 us, 128 tokens 107 -> 93).
+        int st = 0;
+        uint32_t use = 0;
+        const uint32_t ring_at = smem_u32(ring), full_at = peer_smem(smem_u32(full), 0u);
+        for (int tile = pair; tile < a.n_tiles; tile += n_pairs) {
+            const int row0 = tile / a.tok_tiles * 256 + side * MX_ROWS, tok0 = tile % a.tok_tiles * a.n_tile;
+            const int tok = tok0 + side * ((min(a.n_tile, a.B - tok0) + 31) / 32 * 16);
+            for (int s = 0; s < steps; s++) {
+                mbar_wait_bounded(smem_u32(&empty[st]), use ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
+                const uint32_t bar = full_at + 8u * (uint32_t)st, at = ring_at + (uint32_t)(st * stage_bytes), sf = at + MX_A_BYTES + (uint32_t)(a.n_tile / 2) * (MX_K / 2);
+                if (elect_one()) {
                     if (side == 0) mbar_arrive_expect_tx(smem_u32(&full[st]), 2u * (uint32_t)stage_bytes);
                     tma_load_2d_pair(at, &wmap, s * (MX_K / 2), row0, bar);
-                    tma_load_2d_pair(at + MX_A_BYTES, &xmap, s * (MX_K / 2), tok0 + side * (n_mma / 2), bar);
+                    tma_load_2d_pair(at + MX_A_BYTES, &xmap, s * (MX_K / 2), tok, bar);
                     tma_load_3d_pair(sf, &wsmap, 0, 2 * s, row0 / 128, bar);
                     tma_load_3d_pair(sf + MX_SFA_BYTES, &xsmap, 0, 2 * s, tok0 / 128, bar);
-                    if (++st == a.stages) { st = 0; use ^= 1u; }
                 }
+                __syncwarp();
+                if (++st == a.stages) { st = 0; use ^= 1u; }
             }
         }
     } else if (warp == 1) {
@@ -758,8 +763,8 @@ MxCut mx_cut(int sm_count, int smem_optin, int K, int M, int B, double* cost_of)
 }
 
 // Tiles of a product in pairs: 64, 128, 192 or 256 tokens (a tile starts on half a scale tile), by their time in SM clocks: rounds of
-// tiles over the pairs, each stage 500 clocks and 1.45 a token (measured at 128, 192 and 256 tokens of 2048 x 17408 x 5120: 109, 85 and 73 us;
-// 333 x 16384 x 5120: 27, 21 and 26 us, with 64 tokens 50), and what starts and drains a tile, less where two accumulators take turns.
+// tiles over the pairs, each stage 350 clocks and 2 a token (measured at 128, 192 and 256 tokens of 2048 x 17408 x 5120: 93, 78 and 74 us;
+// 333 x 16384 x 5120: 22, 21 and 26 us), and what starts and drains a tile, less where two accumulators take turns.
 struct MxPairCut { int n_tile, stages, n_acc, tok_tiles, n_tiles; };
 MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int forced, double* cost_of) {
     MxPairCut best = {};
@@ -780,7 +785,7 @@ MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int for
             c.stages = std::min(c.stages, two);
         }
         const int pairs = sm_count / 2;
-        const double cost = (double)((c.n_tiles + pairs - 1) / pairs) * (steps * (500.0 + 1.45 * n) + (c.n_acc == 2 ? 1700.0 : 2700.0));
+        const double cost = (double)((c.n_tiles + pairs - 1) / pairs) * (steps * (350.0 + 2.0 * n) + (c.n_acc == 2 ? 1700.0 : 2700.0));
         if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
     }
     if (cost_of) *cost_of = best_cost + 4000.0;
