@@ -188,7 +188,6 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const Head
 // then waits too often for too few others.
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int LG_THREADS = 512, LG_WARPS = LG_THREADS / 32, LG_MAX_N = 1 << 30;
-constexpr uint32_t LG_PROMPT = 0x80000000u;   // seen in the prompt; the other bits count generated tokens
 
 struct LogitsArgs {
     const float* x;
@@ -198,18 +197,18 @@ struct LogitsArgs {
     int n, index_offset;
 };
 
-// Counts those of ids[0, len) that are among the n logits from `first` on: in the prompt (a flag) or generated (a count).
+// Counts those of ids[0, len) that are among the n logits from `first` on: a bit for each that occurs, a count for each generated one.
 // (Unsigned: ids below the first and negative ones fall out with those behind the last.)
 template <bool GENERATED>
-__device__ __forceinline__ void count_id(uint32_t words, int id, uint32_t first, uint32_t n) {
-    const uint32_t at = (uint32_t)id - first;
+__device__ __forceinline__ void count_id(uint32_t words, uint32_t occurs, int id, uint32_t first, uint32_t n) {
+    const uint32_t at = (uint32_t)id - first, word = occurs + at % LG_THREADS * 4u, bit = 1u << (at / LG_THREADS & 31u);
     if constexpr (GENERATED)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %0, %1;\n\t@p red.shared.add.u32 [%2], 1;\n\t}" ::"r"(at), "r"(n), "r"(words + 4u * at) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %0, %1;\n\t@p red.shared.or.b32 [%2], %3;\n\t@p red.shared.add.u32 [%4], 1;\n\t}" ::"r"(at), "r"(n), "r"(word), "r"(bit), "r"(words + 4u * at) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %0, %1;\n\t@p red.shared.or.b32 [%2], %3;\n\t}" ::"r"(at), "r"(n), "r"(words + 4u * at), "r"(LG_PROMPT) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %0, %1;\n\t@p red.shared.or.b32 [%2], %3;\n\t}" ::"r"(at), "r"(n), "r"(word), "r"(bit) : "memory");
 }
 template <bool GENERATED>
-__device__ __forceinline__ void count_ids(uint32_t words, const int* ids, long long len, uint32_t first, uint32_t n, int tid) {
+__device__ __forceinline__ void count_ids(uint32_t words, uint32_t occurs, const int* ids, long long len, uint32_t first, uint32_t n, int tid) {
     if (len <= 0) return;
     // four ids a load, two loads of a thread ahead of their atomics; the ends that are no whole 16 bytes by themselves
     const int head = (int)min(len, (long long)((16 - ((uintptr_t)ids & 15)) & 15) / 4);
@@ -218,24 +217,24 @@ __device__ __forceinline__ void count_ids(uint32_t words, const int* ids, long l
     long long k = tid;
     for (; k + LG_THREADS < quads; k += 2 * LG_THREADS, q += 2 * LG_THREADS) {
         const int4 a = __ldg(q), b = __ldg(q + LG_THREADS);
-        count_id<GENERATED>(words, a.x, first, n);
-        count_id<GENERATED>(words, a.y, first, n);
-        count_id<GENERATED>(words, a.z, first, n);
-        count_id<GENERATED>(words, a.w, first, n);
-        count_id<GENERATED>(words, b.x, first, n);
-        count_id<GENERATED>(words, b.y, first, n);
-        count_id<GENERATED>(words, b.z, first, n);
-        count_id<GENERATED>(words, b.w, first, n);
+        count_id<GENERATED>(words, occurs, a.x, first, n);
+        count_id<GENERATED>(words, occurs, a.y, first, n);
+        count_id<GENERATED>(words, occurs, a.z, first, n);
+        count_id<GENERATED>(words, occurs, a.w, first, n);
+        count_id<GENERATED>(words, occurs, b.x, first, n);
+        count_id<GENERATED>(words, occurs, b.y, first, n);
+        count_id<GENERATED>(words, occurs, b.z, first, n);
+        count_id<GENERATED>(words, occurs, b.w, first, n);
     }
     if (k < quads) {
         const int4 a = __ldg(q);
-        count_id<GENERATED>(words, a.x, first, n);
-        count_id<GENERATED>(words, a.y, first, n);
-        count_id<GENERATED>(words, a.z, first, n);
-        count_id<GENERATED>(words, a.w, first, n);
+        count_id<GENERATED>(words, occurs, a.x, first, n);
+        count_id<GENERATED>(words, occurs, a.y, first, n);
+        count_id<GENERATED>(words, occurs, a.z, first, n);
+        count_id<GENERATED>(words, occurs, a.w, first, n);
     }
-    if (tid < head) count_id<GENERATED>(words, ids[tid], first, n);
-    if (tid < 4 && head + 4 * quads + tid < len) count_id<GENERATED>(words, ids[head + 4 * quads + tid], first, n);
+    if (tid < head) count_id<GENERATED>(words, occurs, ids[tid], first, n);
+    if (tid < 4 && head + 4 * quads + tid < len) count_id<GENERATED>(words, occurs, ids[head + 4 * quads + tid], first, n);
 }
 
 // VEC: rows of x and y are aligned to 16 bytes, a lane has four neighbours at a time.
@@ -243,8 +242,9 @@ template <int CHUNK, bool VEC>
 __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kernel(const LogitsArgs a) {
     constexpr int E = VEC ? 4 : 1, WARP = 32 * E, STEP = LG_THREADS * E;   // logits of a lane, a warp, the block at a time
     constexpr int UN = CHUNK / STEP;                                       // ... of a lane altogether
-    extern __shared__ __align__(16) uint32_t seen[];                       // [CHUNK], where there are texts or biases
-    __shared__ uint16_t packed[LG_WARPS][32 + WARP];
+    extern __shared__ __align__(16) uint32_t times[];                      // [CHUNK] of generated tokens, where there are texts or biases
+    __shared__ uint32_t occurs[LG_THREADS];                                // bit b: the token of logit 512 b + the thread occurs
+    __shared__ uint16_t packed[LG_WARPS][64];
     const int row = blockIdx.y, c0 = blockIdx.x * CHUNK, n = min(CHUNK, a.n - c0), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t first = (uint32_t)(a.index_offset + c0);
     const bool counts = a.r.history != nullptr, in_place = a.x == a.y;
@@ -293,11 +293,12 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
     bool any = bias_at < (uint32_t)n;
     for (long long j = tid + LG_THREADS; j < n_bias; j += LG_THREADS) any |= (uint32_t)a.r.bias_ids[bias0 + j] - first < (uint32_t)n;
     if (counts)
-        for (int i = 4 * tid; i < CHUNK; i += 4 * LG_THREADS) *(uint4*)(seen + i) = make_uint4(0, 0, 0, 0);
+        for (int i = 4 * tid; i < CHUNK; i += 4 * LG_THREADS) *(uint4*)(times + i) = make_uint4(0, 0, 0, 0);
     if (counts) {
+        occurs[tid] = 0u;
         __syncthreads();
-        count_ids<false>(smem_u32(seen), a.r.history + text, prompt, first, (uint32_t)n, tid);
-        count_ids<true>(smem_u32(seen), a.r.history + text + prompt, text_len - prompt, first, (uint32_t)n, tid);
+        count_ids<false>(smem_u32(times), smem_u32(occurs), a.r.history + text, prompt, first, (uint32_t)n, tid);
+        count_ids<true>(smem_u32(times), smem_u32(occurs), a.r.history + text + prompt, text_len - prompt, first, (uint32_t)n, tid);
     }
     // ... and through
     if (!in_place || m >= 0) {
@@ -327,40 +328,30 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
     any = __syncthreads_or(any);   // (every id is counted, and every logit through)
     if (counts) {
         const float repetition = a.r.penalties[3 * row], frequency = a.r.penalties[3 * row + 1], presence = a.r.penalties[3 * row + 2];
-        // a warp looks through its share of the words; places of those that count are packed and mended 32 at a time
+        // a lane has the bits of 32 logits and gives one at a time; places are packed and mended 32 at a time
         uint16_t* mine = packed[warp];
         int waiting = 0;
         auto mend = [&](int from, int k) {   // k of the packed places
             if (lane < k) {
-                const uint32_t at = mine[from + lane], times = seen[at] & ~LG_PROMPT;
+                const uint32_t at = mine[from + lane], generated = times[at];
                 if (allowed(at)) {
                     float l = y[at];
                     l = l > 0.0f ? __fdiv_rn(l, repetition) : l * repetition;
-                    if (times) l = l - frequency * (float)times - presence;
+                    if (generated) l = l - frequency * (float)generated - presence;
                     y[at] = l;
                 }
             }
-        };
-        for (int i = WARP * warp; i < n; i += STEP) {
-            uint32_t w[E];
-            if constexpr (VEC) {
-                const uint4 q = *(const uint4*)(seen + i + 4 * lane);
-                w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
-                if (!__any_sync(0xffffffffu, (q.x | q.y | q.z | q.w) != 0u)) continue;
-            } else {
-                w[0] = seen[i + lane];
-            }
-#pragma unroll
-            for (int k = 0; k < E; k++) {
-                const uint32_t hit = __ballot_sync(0xffffffffu, w[k] != 0u);
-                if (w[k]) mine[waiting + __popc(hit & ((1u << lane) - 1u))] = (uint16_t)(i + E * lane + k);
-                waiting += __popc(hit);
-            }
             __syncwarp();
-            while (waiting >= 32) {   // the last 32
+        };
+        uint32_t left = occurs[tid];
+        while (const uint32_t giving = __ballot_sync(0xffffffffu, left != 0u)) {
+            if (left) mine[waiting + __popc(giving & ((1u << lane) - 1u))] = (uint16_t)(LG_THREADS * (__ffs(left) - 1) + tid);
+            left &= left - 1u;
+            waiting += __popc(giving);
+            __syncwarp();
+            if (waiting >= 32) {   // the last 32
                 waiting -= 32;
                 mend(waiting, 32);
-                __syncwarp();
             }
         }
         mend(0, waiting);
@@ -376,12 +367,12 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
         }
     };
     __syncthreads();
-    each([&](uint32_t, uint32_t at) { seen[at] = 0u; });
+    each([&](uint32_t, uint32_t at) { times[at] = 0u; });
     __syncthreads();
-    each([&](uint32_t j, uint32_t at) { atomicMax(&seen[at], j + 1u); });
+    each([&](uint32_t j, uint32_t at) { atomicMax(&times[at], j + 1u); });
     __syncthreads();
     each([&](uint32_t j, uint32_t at) {
-        if (seen[at] == j + 1u && allowed(at)) y[at] += a.r.bias_values[from + j];
+        if (times[at] == j + 1u && allowed(at)) y[at] += a.r.bias_values[from + j];
     });
 }
 
