@@ -177,15 +177,19 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const Head
 //   seen: l = l > 0 ? l / rep : l * rep;  l -= freq * count_v;  count_v > 0: l -= pres;  l += bias_v;  mask bit clear: l = -inf
 // A CTA owns CHUNK logits of a row.  Their loads are issued first (four neighbours a lane where rows are aligned to 16 bytes, else one: any
 // stride will do; in place nothing is loaded and only masked logits are written).  While they are on their way the CTA counts the row's tokens
-// that fall among them in shared memory (whole numbers, so the order of the atomics does not matter); then the logits pass through the
-// mask, and those that occur, few, are mended where they were written, packed 32 at a time so that no warp computes for one lane.  Biases
+// that fall among them in shared memory (whole numbers, so the order of the atomics does not matter): a bit for each that occurs, a count for
+// each generated one.  Then the logits pass through the mask, and those that occur, few, are mended from where they were read: a lane has the bits of
+// the logits 512 apart, so that a warp's share of a bit is 32 neighbours, and places are packed so that no warp computes for one lane.  Biases
 // come last, the last entry of each token found in the same shared words.
 // Every CTA of a row reads the whole text, so a CTA takes as many logits as leaves three to an SM (two are there at a time), and an id costs
-// four instructions (difference, comparison, address, predicated atomic).  128 rows of 248320: nothing but the counting of one token each
-// 50 us = 5.1 TB/s, texts of 4000 to 16000 tokens 75, with masks, generated tokens and biases 91 = 2.9 TB/s.  What was slower there: clusters that
+// six instructions (difference, comparison, address, bit, predicated atomics).  128 rows of 248320: nothing but the counting of one token each
+// 43.5 us = 5.8 TB/s, 16000 tokens of prompt 61, 4000 generated ones 53, both with masks and 32 biases 77.5 = 3.3 TB/s.  Without the bits, every word of
+// the counts looked through, 49, 76, 62 and 90; bits of 32 neighbours to a lane, whose 32 places at a time lie in 32 lines, 44, 76, 63 and 93; 32 places
+// mended at a time instead of 64, read back from where they were written, 44, 63, 53 and 79.5.  What was slower there: clusters that
 // share a text by atomics in each other's memory (101 alone, 111 in twos, 161 in eights, all with 8192 logits a CTA); CTAs that stay and bring
 // the next piece's logits ahead (138); half of the warps counting a piece ahead of the others (112 mending in memory, 156 in registers): a warp
-// then waits too often for too few others.
+// then waits too often for too few others; logits mended in registers before their only store, which then waits (95); logits read after
+// the counting, with three CTAs to an SM (81 to 86); text of the next step on its way during this one's counting (89, registers spilled).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int LG_THREADS = 512, LG_WARPS = LG_THREADS / 32, LG_MAX_N = 1 << 30;
 
@@ -244,7 +248,7 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
     constexpr int UN = CHUNK / STEP;                                       // ... of a lane altogether
     extern __shared__ __align__(16) uint32_t times[];                      // [CHUNK] of generated tokens, where there are texts or biases
     __shared__ uint32_t occurs[LG_THREADS];                                // bit b: the token of logit 512 b + the thread occurs
-    __shared__ uint16_t packed[LG_WARPS][64];
+    __shared__ uint16_t packed[LG_WARPS][96];
     const int row = blockIdx.y, c0 = blockIdx.x * CHUNK, n = min(CHUNK, a.n - c0), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t first = (uint32_t)(a.index_offset + c0);
     const bool counts = a.r.history != nullptr, in_place = a.x == a.y;
@@ -328,17 +332,26 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
     any = __syncthreads_or(any);   // (every id is counted, and every logit through)
     if (counts) {
         const float repetition = a.r.penalties[3 * row], frequency = a.r.penalties[3 * row + 1], presence = a.r.penalties[3 * row + 2];
-        // a lane has the bits of 32 logits and gives one at a time; places are packed and mended 32 at a time
+        // a lane has the bits of its logits and gives one at a time; places are packed and mended 64 at a time, two to a lane
         uint16_t* mine = packed[warp];
         int waiting = 0;
         auto mend = [&](int from, int k) {   // k of the packed places
-            if (lane < k) {
-                const uint32_t at = mine[from + lane], generated = times[at];
-                if (allowed(at)) {
-                    float l = y[at];
-                    l = l > 0.0f ? __fdiv_rn(l, repetition) : l * repetition;
-                    if (generated) l = l - frequency * (float)generated - presence;
-                    y[at] = l;
+            uint32_t at[2];
+            float l[2];
+            bool on[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                on[h] = lane + 32 * h < k;
+                at[h] = on[h] ? mine[from + lane + 32 * h] : 0u;
+                if (on[h]) l[h] = x[at[h]];
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (on[h] && allowed(at[h])) {
+                    const uint32_t generated = times[at[h]];
+                    float z = l[h] > 0.0f ? __fdiv_rn(l[h], repetition) : l[h] * repetition;
+                    if (generated) z = z - frequency * (float)generated - presence;
+                    y[at[h]] = z;
                 }
             }
             __syncwarp();
@@ -349,9 +362,9 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
             left &= left - 1u;
             waiting += __popc(giving);
             __syncwarp();
-            if (waiting >= 32) {   // the last 32
-                waiting -= 32;
-                mend(waiting, 32);
+            if (waiting >= 64) {   // the last 64
+                waiting -= 64;
+                mend(waiting, 64);
             }
         }
         mend(0, waiting);
