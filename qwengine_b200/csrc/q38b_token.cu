@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const Head
 // come last, the last entry of each token found in the same shared words.
 // Every CTA of a row reads the whole text, so a CTA takes as many logits as leaves three to an SM (two are there at a time), and an id costs
 // six instructions (difference, comparison, address, bit, predicated atomics).  128 rows of 248320: nothing but the counting of one token each
-// 43.5 us = 5.8 TB/s, 16000 tokens of prompt 61, 4000 generated ones 53, both with masks and 32 biases 77.5 = 3.3 TB/s.  Without the bits, every word of
+// 41.5 us = 6.1 TB/s, 16000 tokens of prompt 60, 4000 generated ones 50, both with masks and 32 biases 73.7 = 3.6 TB/s; where the ends of a row were
+// asked for at every place and texts had lengths instead of ends (registers spilled) 43.5, 61, 53 and 77.5.  Before that, without the bits, every word of
 // the counts looked through, 49, 76, 62 and 90; bits of 32 neighbours to a lane, whose 32 places at a time lie in 32 lines, 44, 76, 63 and 93; 32 places
 // mended at a time instead of 64, read back from where they were written, 44, 63, 53 and 79.5.  What was slower there: clusters that
 // share a text by atomics in each other's memory (101 alone, 111 in twos, 161 in eights, all with 8192 logits a CTA); CTAs that stay and bring
@@ -201,7 +202,7 @@ struct LogitsArgs {
     int n, index_offset;
 };
 
-// Counts those of ids[0, len) that are among the n logits from `first` on: a bit for each that occurs, a count for each generated one.
+// Counts those of [ids, end) that are among the n logits from `first` on: a bit for each that occurs, a count for each generated one.
 // (Unsigned: ids below the first and negative ones fall out with those behind the last.)
 template <bool GENERATED>
 __device__ __forceinline__ void count_id(uint32_t words, uint32_t occurs, int id, uint32_t first, uint32_t n) {
@@ -212,14 +213,14 @@ __device__ __forceinline__ void count_id(uint32_t words, uint32_t occurs, int id
         asm volatile("{\n\t.reg .pred p;\n\tsetp.lt.u32 p, %0, %1;\n\t@p red.shared.or.b32 [%2], %3;\n\t}" ::"r"(at), "r"(n), "r"(word), "r"(bit) : "memory");
 }
 template <bool GENERATED>
-__device__ __forceinline__ void count_ids(uint32_t words, uint32_t occurs, const int* ids, long long len, uint32_t first, uint32_t n, int tid) {
-    if (len <= 0) return;
+__device__ __forceinline__ void count_ids(uint32_t words, uint32_t occurs, const int* ids, const int* end, uint32_t first, uint32_t n, int tid) {
+    if (end <= ids) return;
     // four ids a load, two loads of a thread ahead of their atomics; the ends that are no whole 16 bytes by themselves
-    const int head = (int)min(len, (long long)((16 - ((uintptr_t)ids & 15)) & 15) / 4);
-    const long long quads = (len - head) / 4;
+    const int head = (int)min((long long)(end - ids), (long long)((16 - ((uintptr_t)ids & 15)) & 15) / 4);
+    if (tid < head) count_id<GENERATED>(words, occurs, ids[tid], first, n);
     const int4* q = (const int4*)(ids + head) + tid;
-    long long k = tid;
-    for (; k + LG_THREADS < quads; k += 2 * LG_THREADS, q += 2 * LG_THREADS) {
+    const int4* q_end = (const int4*)((uintptr_t)end & ~(uintptr_t)15);   // (behind a head that reaches the end: before q)
+    for (; q + LG_THREADS < q_end; q += 2 * LG_THREADS) {
         const int4 a = __ldg(q), b = __ldg(q + LG_THREADS);
         count_id<GENERATED>(words, occurs, a.x, first, n);
         count_id<GENERATED>(words, occurs, a.y, first, n);
@@ -230,15 +231,16 @@ __device__ __forceinline__ void count_ids(uint32_t words, uint32_t occurs, const
         count_id<GENERATED>(words, occurs, b.z, first, n);
         count_id<GENERATED>(words, occurs, b.w, first, n);
     }
-    if (k < quads) {
+    if (q < q_end) {
         const int4 a = __ldg(q);
         count_id<GENERATED>(words, occurs, a.x, first, n);
         count_id<GENERATED>(words, occurs, a.y, first, n);
         count_id<GENERATED>(words, occurs, a.z, first, n);
         count_id<GENERATED>(words, occurs, a.w, first, n);
     }
-    if (tid < head) count_id<GENERATED>(words, occurs, ids[tid], first, n);
-    if (tid < 4 && head + 4 * quads + tid < len) count_id<GENERATED>(words, occurs, ids[head + 4 * quads + tid], first, n);
+    // (a head that reaches the end leaves no tail)
+    const int* tail = (const int*)q_end + tid;
+    if (tid < 4 && tail >= ids + head && tail < end) count_id<GENERATED>(words, occurs, *tail, first, n);
 }
 
 // VEC: rows of x and y are aligned to 16 bytes, a lane has four neighbours at a time.
@@ -255,16 +257,18 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
     const float* x = a.x + row * a.x_ld + c0;
     float* y = a.y + row * a.y_ld + c0;
     // what the later parts need, on its way before the logits
-    long long text = 0, text_len = 0, bias0 = 0, n_bias = 0;
-    int prompt = 0;
+    const int *text = nullptr, *generated_text = nullptr, *text_end = nullptr;
+    long long bias0 = 0;
+    int n_bias = 0;
     if (counts) {
-        text = a.r.history_begin[row];
-        text_len = a.r.history_begin[row + 1] - text;
-        if (a.r.prompt_len) prompt = (int)max(0LL, min((long long)a.r.prompt_len[row], text_len));
+        const long long begin = a.r.history_begin[row], end = a.r.history_begin[row + 1];
+        text = a.r.history + begin;
+        text_end = a.r.history + end;
+        generated_text = text + (a.r.prompt_len ? max(0LL, min((long long)a.r.prompt_len[row], end - begin)) : 0LL);
     }
     if (a.r.bias_ids) {
         bias0 = a.r.bias_begin[row];
-        n_bias = a.r.bias_begin[row + 1] - bias0;
+        n_bias = (int)(a.r.bias_begin[row + 1] - bias0);
     }
     const int m = !a.r.masks ? -1 : a.r.mask_of_row ? a.r.mask_of_row[row] : row;
     const uint32_t* mask = a.r.masks + (m >= 0 ? m * a.r.mask_ld : 0);
@@ -272,7 +276,16 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
     auto allowed = [&](uint32_t at) { return m < 0 || (mask[(first + at) >> 5] >> ((first + at) & 31u) & 1u); };
     // the logits on their way
     float v[UN][E];
-    if (!in_place) {
+    const bool whole = VEC && n == CHUNK && !in_place;   // nothing to ask of a place
+    if (whole) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int u = 0; u < UN; u++) {
+                const float4 q = *(const float4*)(x + STEP * u + E * tid);
+                v[u][0] = q.x; v[u][1] = q.y; v[u][2] = q.z; v[u][3] = q.w;
+            }
+        }
+    } else if (!in_place) {
 #pragma unroll
         for (int u = 0; u < UN; u++) {
             const int i = STEP * u + E * tid;
@@ -295,18 +308,26 @@ __global__ void __launch_bounds__(LG_THREADS, CHUNK <= 4096 ? 3 : 2) logits_kern
     // biases among the block's logits; a thread keeps its first one's place
     const uint32_t bias_at = tid < n_bias ? (uint32_t)a.r.bias_ids[bias0 + tid] - first : 0xFFFFFFFFu;
     bool any = bias_at < (uint32_t)n;
-    for (long long j = tid + LG_THREADS; j < n_bias; j += LG_THREADS) any |= (uint32_t)a.r.bias_ids[bias0 + j] - first < (uint32_t)n;
+    for (int j = tid + LG_THREADS; j < n_bias; j += LG_THREADS) any |= (uint32_t)a.r.bias_ids[bias0 + j] - first < (uint32_t)n;
     if (counts)
         for (int i = 4 * tid; i < CHUNK; i += 4 * LG_THREADS) *(uint4*)(times + i) = make_uint4(0, 0, 0, 0);
     if (counts) {
         occurs[tid] = 0u;
         __syncthreads();
-        count_ids<false>(smem_u32(times), smem_u32(occurs), a.r.history + text, prompt, first, (uint32_t)n, tid);
-        count_ids<true>(smem_u32(times), smem_u32(occurs), a.r.history + text + prompt, text_len - prompt, first, (uint32_t)n, tid);
+        count_ids<false>(smem_u32(times), smem_u32(occurs), text, generated_text, first, (uint32_t)n, tid);
+        count_ids<true>(smem_u32(times), smem_u32(occurs), generated_text, text_end, first, (uint32_t)n, tid);
     }
     // ... and through
-    if (!in_place || m >= 0) {
-        const float minus_inf = __int_as_float(0xFF800000);
+    const float minus_inf = __int_as_float(0xFF800000);
+    if (whole) {
+        if constexpr (VEC) {
+#pragma unroll
+            for (int u = 0; u < UN; u++) {
+                const uint32_t keep = __shfl_sync(0xffffffffu, bits, E * u + E * lane / 32) >> (E * lane % 32);
+                *(float4*)(y + STEP * u + E * tid) = make_float4(keep & 1u ? v[u][0] : minus_inf, keep & 2u ? v[u][1] : minus_inf, keep & 4u ? v[u][2] : minus_inf, keep & 8u ? v[u][3] : minus_inf);
+            }
+        }
+    } else if (!in_place || m >= 0) {
 #pragma unroll
         for (int u = 0; u < UN; u++) {
             const int i = STEP * u + E * tid;
