@@ -330,11 +330,11 @@ __device__ __forceinline__ void load_x8(const void* x, int kind, long long at, b
 }
 
 // FUSED (one token): warps 2..9 quantize the activations of this CTA's K into operand B and its scales while the first weights are on
-// their way; one launch instead of two: 17408 x 5120 12.2 us against 13.4, 5120 x 17408 14.6 against 15.2.  (With two tokens 13.6 and 13.4,
+// their way; one launch instead of two: 17408 x 5120 12.2 us against 13.4, 5120 x 17408 14.6 against 15.2, both a CTA to an SM.  (With two tokens 13.6 and 13.4,
 // with eight 18.5 and 13.5: every CTA quantizes what one kernel does once, and the weights' ring stands full meanwhile.)
 // The weights of the first stages are asked for before anything else, also before the quantizer's kernel in front has ended.
 template <typename T, int GROUPS, bool FUSED>
-__global__ void __launch_bounds__(MX_THREADS, 1) mx4_gemm_kernel(const MxArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
+__global__ void __launch_bounds__(MX_THREADS, GROUPS == 1 ? 2 : 1) mx4_gemm_kernel(const MxArgs a, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* full = (uint64_t*)smem;
     uint64_t* empty = full + MX_MAX_STAGES;
@@ -733,38 +733,64 @@ mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, co
 }
 
 // How a product is cut: tokens in tiles of n_tile (one tile, or several of 128 or 256: a tile starts on a scale tile's border), K in
-// `splits` parts.
-struct MxCut { int n_tile, stages, splits, box; };   // box: bytes of shared memory for the others' sums (0: over the ring)
+// `splits` parts, few tokens with two CTAs to an SM, each with half of its shared memory.
+struct MxCut { int n_tile, stages, splits, box, per_sm; };   // box: bytes of shared memory for the others' sums (0: over the ring)
 
 int exchange_bytes(const MxCut& c) {
     const int chunks = c.n_tile / 16;
     return (c.splits - 1) * ((chunks + c.splits - 1) / c.splits) * 16 * MX_ROWS * 4;
 }
+// what a CTA has for its ring and what stands behind it
+int mx_ring_bytes(int smem_optin, const MxCut& c) { return (c.per_sm == 2 ? (smem_optin + 1024) / 2 - 1024 : smem_optin) - 1024 - c.box; }
+// stages of weights beside one token's codes
+int mx_fused_stages(int smem_optin, const MxCut& c, int x_steps) { return std::min(MX_MAX_STAGES, (mx_ring_bytes(smem_optin, c) - mx_fused_x_bytes(x_steps)) / MX_FUSED_STAGE); }
 
-// ... by their time in SM clocks: rounds of CTAs, each stage 600 clocks and 5 a token (2048 x 17408 x 5120 174 us in tiles of 256), what starts
-// and drains a CTA, and the exchange of split sums.  (Clusters of three and more leave some SMs unused.)
+// ... by their time in SM clocks, of one wave of CTAs after the other: what starts and drains a CTA, the exchange of split sums, and stages, each as
+// long as a CTA takes alone (two of an SM: twice) or, if that is longer, as its bytes take out of L2 (6400 a clock for all SMs) and its weights out of
+// DRAM (3300).  Fitted to 1024, 5120 and 17408 rows, 16 to 768 tokens, in every number of parts and tiles: the taken cut is within 4 % of the best
+// there, but for one token in six parts (below).  1024 x 5120: 256 tokens 11.1 -> 8.2 us, 512 tokens 20.5 -> 9.0; 5120 x 17408, 256 tokens 24.1 -> 20.8 (before,
+// a stage counted 600 clocks and 5 a token, whoever else ran).
+// Two CTAs of an SM overlap their ends, and parts fill all SMs: 7 x 5120 x 17408 in six parts 13.7 us, in three of whole SMs 14.8; 7 x 12288 x 5120 in two
+// 11.5 and 12.5; one token x 248320 x 5120 112 and 130.  One token's codes take shared memory too, and six parts of 5120 x 17408 leave rings of
+// four stages: 14.2 us against 13.7 in three.  Two such CTAs hold at most 256 columns of tensor memory each, and no other kernel here that allocates
+// columns fits beside one (registers, shared memory): no cluster waits for columns that another waiting one holds.
+// Clusters of three to six leave an eighth of the SMs unused, larger ones three tenths (45, 33, 26, 22, 15 and 15 clusters were there at a time).
 MxCut mx_cut(int sm_count, int smem_optin, int K, int M, int B, double* cost_of) {
     MxCut best = {};
     double best_cost = 0.0;
-    const int steps = (K + MX_K - 1) / MX_K;
-    MxCut c;
-    c.n_tile = B <= MX_MAX_N ? (B + 15) / 16 * 16 : MX_MAX_N;
-    const long long tiles = (long long)((M + MX_ROWS - 1) / MX_ROWS) * ((B + c.n_tile - 1) / c.n_tile);
-    for (c.splits = 1; c.splits <= std::min(MX_MAX_SPLITS, steps); c.splits++) {
-        c.box = c.splits > 1 && c.n_tile <= 32 ? exchange_bytes(c) : 0;
-        c.stages = std::min(std::min(MX_MAX_STAGES, (smem_optin - 1024 - c.box) / mx_stage_bytes(c.n_tile)), (512 - mx_acc_cols(c.n_tile)) / mx_scale_cols(c.n_tile));
-        if (c.splits > 1 && !c.box && exchange_bytes(c) > c.stages * mx_stage_bytes(c.n_tile)) break;
-        const long long slots = c.splits <= 2 ? sm_count : sm_count * 9 / 10 / c.splits * c.splits, ctas = tiles * c.splits;
-        const double cost = (double)((ctas + slots - 1) / slots) * ((steps + c.splits - 1) / c.splits * (600.0 + 5.0 * c.n_tile) + 4000.0 + (c.splits > 1 ? 1500.0 + 10.0 * c.n_tile : 0.0));
-        if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
-    }
+    const int steps = (K + MX_K - 1) / MX_K, whole = B <= MX_MAX_N ? (B + 15) / 16 * 16 : MX_MAX_N;
+    const auto rate = [&](int n, int per_sm) {
+        MxCut c = {};
+        c.n_tile = n;
+        c.per_sm = per_sm;
+        const long long tok_tiles = (B + n - 1) / n, tiles = (long long)((M + MX_ROWS - 1) / MX_ROWS) * tok_tiles;
+        for (c.splits = 1; c.splits <= std::min(MX_MAX_SPLITS, steps); c.splits++) {
+            const int own_steps = (steps + c.splits - 1) / c.splits;
+            c.box = c.splits > 1 && n <= 32 ? exchange_bytes(c) : 0;
+            c.stages = std::min(std::min(MX_MAX_STAGES, mx_ring_bytes(smem_optin, c) / mx_stage_bytes(n)), (512 / per_sm - mx_acc_cols(n)) / mx_scale_cols(n));
+            if (c.splits > 1 && !c.box && exchange_bytes(c) > c.stages * mx_stage_bytes(n)) break;
+            const int sms = c.splits <= 2 ? sm_count : c.splits <= 6 ? sm_count * 7 / 8 : sm_count * 7 / 10;
+            const long long ctas = tiles * c.splits, once = std::max(1, sms / c.splits) * (long long)c.splits, slots = per_sm * once, waves = (ctas + slots - 1) / slots;
+            if (per_sm == 2) {
+                if (ctas <= once || c.stages < 3 || own_steps < 4) continue;   // (shorter ones are all ends: 16 x 2048 x 2048 in eight parts 6.5 us, 5.6 otherwise)
+                if (B == 1 && own_steps * MX_K <= MX_FUSE_MAX_K && (c.splits > 2 || mx_fused_stages(smem_optin, c, own_steps) < 3)) continue;
+            }
+            const double active = (double)std::min(ctas, slots);
+            const double stage = std::max({per_sm * (590.0 + 0.45 * n), active * mx_stage_bytes(n) / 6400.0, active / (double)tok_tiles * (MX_A_BYTES + MX_SFA_BYTES) / 3300.0});
+            const double cost = 3600.0 + (double)waves * (own_steps * stage + (per_sm == 2 ? 0.0 : 3000.0) + 37.0 * n + (c.splits > 1 ? 1900.0 : 0.0));
+            if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
+        }
+    };
+    rate(whole, 1);
+    if (whole > 128) rate(128, 1);
+    if (whole <= 32) rate(whole, 2);
     if (cost_of) *cost_of = best_cost;
     return best;
 }
 
-// Tiles of a product in pairs: 64, 128, 192 or 256 tokens (a tile starts on half a scale tile), by their time in SM clocks: rounds of
-// tiles over the pairs, each stage 350 clocks and 2 a token (measured at 128, 192 and 256 tokens of 2048 x 17408 x 5120: 93, 78 and 74 us;
-// 333 x 16384 x 5120: 22, 21 and 26 us), and what starts and drains a tile, less where two accumulators take turns.
+// Tiles of a product in pairs: 64, 128, 192 or 256 tokens (a tile starts on half a scale tile), by their time in SM clocks as above: rounds of
+// tiles over the pairs (2048 x 17408 x 5120 in tiles of 128, 192 and 256 tokens: 93, 78 and 74 us; 333 x 16384 x 5120: 22, 21 and 26), what starts and
+// drains a pair, and what a tile costs beside its stages, less where two accumulators take turns.
 struct MxPairCut { int n_tile, stages, n_acc, tok_tiles, n_tiles; };
 MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int forced, double* cost_of) {
     MxPairCut best = {};
@@ -785,10 +811,12 @@ MxPairCut mx_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int for
             c.stages = std::min(c.stages, two);
         }
         const int pairs = sm_count / 2;
-        const double cost = (double)((c.n_tiles + pairs - 1) / pairs) * (steps * (350.0 + 2.0 * n) + (c.n_acc == 2 ? 1700.0 : 2700.0));
+        const double active = (double)std::min(c.n_tiles, pairs);
+        const double stage = std::max(400.0 + 0.87 * n, active * 2.0 * mxp_stage_bytes(n) / 6200.0), weights = active / c.tok_tiles * 2.0 * (MX_A_BYTES + MX_SFA_BYTES) / 3300.0;
+        const double cost = 7800.0 + 24.0 * n + (double)((c.n_tiles + pairs - 1) / pairs) * std::max(steps * stage + (c.n_acc == 2 ? 1700.0 : 2700.0), steps * weights);
         if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
     }
-    if (cost_of) *cost_of = best_cost + 4000.0;
+    if (cost_of) *cost_of = best_cost;
     return best;
 }
 
@@ -989,7 +1017,7 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
     const MxCut one = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B, &cost);
     const MxPairCut cut = mx_pair_cut(ctx->sm_count, ctx->smem_optin, K, M, B, ctx->mx4_pairs > 0 ? ctx->mx4_pairs : 0, &pair_cost);
     const bool too_many = (B + one.n_tile - 1) / one.n_tile > 65535;   // token tiles, for a grid's second dimension
-    if (ctx->mx4_pairs > 0 || (ctx->mx4_pairs == 0 && (too_many || (B > 32 && M > MX_ROWS && pair_cost < cost)))) {
+    if (ctx->mx4_pairs > 0 || (ctx->mx4_pairs == 0 && (too_many || (B > 1 && M > MX_ROWS && pair_cost < cost)))) {
         if (!cut.n_tile) return Q38B_ERR_UNSUPPORTED;
         CUtensorMap wmap, xmap, wsmap, xsmap, ymap;
         memset(&ymap, 0, sizeof(ymap));
@@ -1037,7 +1065,7 @@ int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_
         const int steps = (K + MX_K - 1) / MX_K, x_steps = (steps + cut.splits - 1) / cut.splits;
         if (x_steps * MX_K <= MX_FUSE_MAX_K) {
             DeviceGuard on(ctx);
-            cut.stages = std::min(MX_MAX_STAGES, (ctx->smem_optin - 1024 - cut.box - mx_fused_x_bytes(x_steps)) / MX_FUSED_STAGE);
+            cut.stages = mx_fused_stages(ctx->smem_optin, cut, x_steps);
             CUtensorMap wmap, none;
             memset(&none, 0, sizeof(none));
             if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS)) return Q38B_ERR_ARG;

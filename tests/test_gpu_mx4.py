@@ -241,6 +241,47 @@ def test_few_tokens_are_quantized_by_the_product(ctx, B, M, K, dtype, pad):
     assert torch.equal(one.nan_to_num(), ctx.gemm_mx4(W, ctx.quantize_mx4(x)).nan_to_num())
 
 
+@pytest.mark.parametrize("B,M,K", [
+    (1, 19100, 1280), (1, 30000, 96), (2, 19100, 1280), (16, 25000, 1056), (32, 19100, 2080),   # two CTAs to an SM, one part
+    (1, 9700, 2560), (9, 9700, 2304), (7, 5120, 6144), (32, 5000, 6176),                        # ... two and six parts
+    (129, 1024, 5120), (300, 1000, 5152), (513, 1024, 2304), (256, 640, 4000),                  # tiles of 128 tokens in parts
+    (3, 70000, 512), (32, 70001, 288)])                                                         # many rows
+def test_whole_number_products_in_every_cut(ctx, B, M, K):
+    """Sums of whole numbers below 2^24: exact whatever the parts, tiles and kernels; the quantizer inside gives the same, and what lies around stays."""
+    gen = torch.Generator("cuda").manual_seed(B + M + K)
+    x, w = (torch.randint(-4, 5, (n, K), generator=gen, device="cuda").float() for n in (B, M))
+    x[:, ::32], w[:, ::32] = 4, -4                # every block scaled by one: whole numbers up to 4 are E2M1 values
+    whole = torch.full((B + 2, M + 6), 3.0, device="cuda")
+    y = whole[1:B + 1, 3:M + 3]
+    W = ctx.quantize_mx4(w)
+    ctx.gemm_mx4(W, ctx.quantize_mx4(x), out=y)
+    ctx.check()
+    assert torch.equal(y, (x.double() @ w.double().t()).float())
+    assert torch.equal(y, ctx.gemm_mx4(W, x))
+    ctx.check()
+    y.fill_(3.0)
+    assert (whole == 3.0).all()
+
+
+def test_products_on_two_streams_at_once(ctx):
+    """CTAs that share SMs, of one stream's few tokens and the other's many."""
+    w, v = rand(5120, 6144, 1, "bf16").cuda(), rand(19100, 1280, 2, "bf16").cuda()
+    W, V = ctx.quantize_mx4(w), ctx.quantize_mx4(v)
+    a, b, c = rand(7, 6144, 3).cuda(), rand(1, 1280, 4).cuda(), rand(400, 1280, 5).cuda()
+    want = [ctx.gemm_mx4(W, a), ctx.gemm_mx4(V, b), ctx.gemm_mx4(V, c)]
+    torch.cuda.synchronize()
+    sides, got = [torch.cuda.Stream() for _ in range(3)], [[], [], []]
+    for _ in range(10):
+        for i, (m, t) in enumerate(((W, a), (V, b), (V, c))):
+            with torch.cuda.stream(sides[i]):
+                got[i].append(ctx.gemm_mx4(m, t))
+    torch.cuda.synchronize()
+    ctx.check()
+    for i in range(3):
+        for y in got[i]:
+            assert torch.equal(y, want[i])
+
+
 def test_nan_block_reaches_its_row_and_column_only(ctx):
     B, M, K = 20, 140, 256
     x, w = rand(B, K, 1), rand(M, K, 2)
