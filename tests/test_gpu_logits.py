@@ -250,3 +250,15 @@ def test_refusals(ctx):
     with pytest.raises(ValueError):
         ctx.adjust_logits(x.half())
     ctx.check()
+
+
+def test_short_texts_at_every_alignment(ctx):
+    """Texts of 0 to 10 tokens one behind the other, prompts of every length: their 16-byte pieces begin and end anywhere."""
+    g = np.random.default_rng(8)
+    rows, n = 600, 37
+    history = [g.integers(-2, n + 2, int(g.integers(0, 11))).tolist() for _ in range(rows)]
+    prompt = [int(g.integers(0, len(h) + 1)) for h in history]
+    x = (3 * g.standard_normal((rows, n))).astype(np.float32)
+    rules = dict(penalties=np.stack([g.uniform(1, 2, rows), g.uniform(-1, 1, rows), g.uniform(-1, 1, rows)], 1).astype(np.float32).tolist(), history=history, prompt=prompt)
+    check(run(ctx, x, **rules), *definition(x, **rules))
+    check(run(ctx, np.ascontiguousarray(x[:, :36]), **rules), *definition(x[:, :36], **rules))   # four at a time
