@@ -97,7 +97,9 @@ template <typename T> __device__ __forceinline__ void store4(T* p, float4 v) {
     }
 }
 
-// L lanes a head (two heads a warp where 16 do), NV vectors of four elements a lane.  A CTA has heads of one tensor: its pointers and weights
+// L lanes a head (two heads a warp where 16 do, four where 8), NV vectors of four elements a lane: two, so that what a head costs beside its
+// elements is paid half as often (4096 rows of 32 + 8 heads of 128, 16 bits, all rotated, 24.8 us, with one vector 30; four vectors, whose
+// loads no longer fit the registers, 37).  A CTA has heads of one tensor: its pointers and weights
 // are the same for all of them (with heads of both in a CTA 68 us, bound by the issue of instructions: 232 a head, 74 % of the slots).
 template <typename Tin, typename Tout, int L, int NV>
 __global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const HeadsArgs a, int heads_per_cta, int q_ctas, int ctas_per_row) {
@@ -429,15 +431,15 @@ int heads_as(q38b_ctx* ctx, const HeadsArgs& a, cudaStream_t st) {
     const int n_heads = a.t[0].n_heads + a.t[1].n_heads;
     if (heads_by_four(a, sizeof(Tin), sizeof(Tout))) {
         // as many heads a CTA as its warps take at once, fewer where rows alone leave SMs idle
-        const int once = HEADS_WARPS * (a.D <= 64 ? 2 : 1);
+        const int once = HEADS_WARPS * (a.D <= 64 ? 4 : a.D <= 128 ? 2 : 1);
         int per = once * HEADS_BATCH;
         const auto ctas = [&](int n, int of) { return (n + of - 1) / of; };
         while (per > once && (long long)a.rows * (ctas(a.t[0].n_heads, per) + ctas(a.t[1].n_heads, per)) < 2 * ctx->sm_count) per -= once;
         const int q = ctas(a.t[0].n_heads, per), all = q + ctas(a.t[1].n_heads, per);
         const long long grid = (long long)a.rows * all;
         if (grid > 0x7FFFFFFF) return Q38B_ERR_UNSUPPORTED;
-        if (a.D <= 64) heads4_kernel<Tin, Tout, 16, 1><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, q, all);
-        else if (a.D <= 128) heads4_kernel<Tin, Tout, 32, 1><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, q, all);
+        if (a.D <= 64) heads4_kernel<Tin, Tout, 8, 2><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, q, all);
+        else if (a.D <= 128) heads4_kernel<Tin, Tout, 16, 2><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, q, all);
         else heads4_kernel<Tin, Tout, 32, 2><<<(unsigned)grid, 32 * HEADS_WARPS, 0, st>>>(a, per, q, all);
         return launch_status(ctx, cudaSuccess);
     }
