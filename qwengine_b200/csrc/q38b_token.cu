@@ -97,9 +97,25 @@ template <typename T> __device__ __forceinline__ void store4(T* p, float4 v) {
     }
 }
 
+// Two 32-bit products or sums of products an instruction (8192 rows of 32 + 8 heads of 128 in 16 bits 47.3 us, 48.7 one by one)
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\tfma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;\n\t}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 lo2(float4 v) { return make_float2(v.x, v.y); }
+__device__ __forceinline__ float2 hi2(float4 v) { return make_float2(v.z, v.w); }
+__device__ __forceinline__ float4 both(float2 a, float2 b) { return make_float4(a.x, a.y, b.x, b.y); }
+__device__ __forceinline__ float4 mul4(float4 a, float4 b) { return both(mul2(lo2(a), lo2(b)), mul2(hi2(a), hi2(b))); }
+__device__ __forceinline__ float4 fma4(float4 a, float4 b, float4 c) { return both(fma2(lo2(a), lo2(b), lo2(c)), fma2(hi2(a), hi2(b), hi2(c))); }
 // L lanes a head (two heads a warp where 16 do, four where 8), NV vectors of four elements a lane: two, so that what a head costs beside its
-// elements is paid half as often (4096 rows of 32 + 8 heads of 128, 16 bits, all rotated, 24.8 us, with one vector 30; four vectors, whose
-// loads no longer fit the registers, 37).  A CTA has heads of one tensor: its pointers and weights
+// elements is paid half as often (4096 rows of 32 + 8 heads of 128, 16 bits, all rotated, 24.8 us, with one vector 30; four vectors
+// 37; more heads a CTA, one batch after the other, 28).  A CTA has heads of one tensor: its pointers and weights
 // are the same for all of them (with heads of both in a CTA 68 us, bound by the issue of instructions: 232 a head, 74 % of the slots).
 template <typename Tin, typename Tout, int L, int NV>
 __global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const HeadsArgs a, int heads_per_cta, int q_ctas, int ctas_per_row) {
@@ -126,24 +142,28 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const Head
 #pragma unroll
     for (int b = 0; b < HEADS_BATCH; b++) {
         if (h0 + warp * SUB + b * STEP >= h_end) break;   // (the whole warp)
-        float ss = 0.0f;
+        float2 s2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int i = 0; i < NV; i++) ss += x[b][i].x * x[b][i].x + x[b][i].y * x[b][i].y + x[b][i].z * x[b][i].z + x[b][i].w * x[b][i].w;
+        for (int i = 0; i < NV; i++) s2 = fma2(hi2(x[b][i]), hi2(x[b][i]), fma2(lo2(x[b][i]), lo2(x[b][i]), s2));
+        float ss = s2.x + s2.y;
 #pragma unroll
         for (int s = L / 2; s; s >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, s);
         const float r = rsqrtf(ss * a.inv_d + a.eps);
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             float4& z = x[b][i];
-            z = make_float4(z.x * r * w[i].x, z.y * r * w[i].y, z.z * r * w[i].z, z.w * r * w[i].w);
+            z = mul4(mul4(z, make_float4(r, r, r, r)), w[i]);
         }
         if (a.adjacent) {
 #pragma unroll
             for (int i = 0; i < NV; i++) {
                 const int j = 2 * (l + L * i);   // pairs j and j + 1
                 float4& z = x[b][i];
-                if (j < half) z = make_float4(z.x * cs[j] - z.y * sn[j], z.y * cs[j] + z.x * sn[j], z.z, z.w);
-                if (j + 1 < half) z = make_float4(z.x, z.y, z.z * cs[j + 1] - z.w * sn[j + 1], z.w * cs[j + 1] + z.z * sn[j + 1]);
+                if (j < half) {
+                    const float2 c2 = *(const float2*)(cs + j), n2 = *(const float2*)(sn + j);   // (behind the last pair: whatever is there)
+                    const float2 p = make_float2(z.x, z.z), o = make_float2(z.y, z.w), u = fma2(o, make_float2(-n2.x, -n2.y), mul2(p, c2)), q = fma2(p, n2, mul2(o, c2));
+                    z = j + 1 < half ? make_float4(u.x, q.x, u.y, q.y) : make_float4(u.x, q.x, z.z, z.w);
+                }
             }
         } else if (half) {
             float4* mine = swap[warp] + lane / L * L * NV;
@@ -161,7 +181,7 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const Head
                     float4 n = *(const float4*)(sn + j);
                     if (!second) n = make_float4(-n.x, -n.y, -n.z, -n.w);
                     float4& z = x[b][i];
-                    z = make_float4(z.x * cj.x + o.x * n.x, z.y * cj.y + o.y * n.y, z.z * cj.z + o.z * n.z, z.w * cj.w + o.w * n.w);
+                    z = fma4(o, n, mul4(z, cj));
                 }
             }
             __syncwarp();
