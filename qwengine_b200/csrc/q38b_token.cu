@@ -4,6 +4,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstring>
 
 #include "../../include/q38b200.h"
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(32 * HEADS_WARPS, 10) heads4_kernel(const Head
 // each generated one.  Then the logits pass through the mask, and those that occur, few, are mended from where they were read: a lane has the bits of
 // the logits 512 apart, so that a warp's share of a bit is 32 neighbours, and places are packed so that no warp computes for one lane.  Biases
 // come last, the last entry of each token found in the same shared words.
-// Every CTA of a row reads the whole text, so a CTA takes as many logits as leaves three to an SM (two are there at a time), and an id costs
+// Every CTA of a row reads the whole text, so a CTA takes many logits where there are many rows (logits_in), and an id costs
 // six instructions (difference, comparison, address, bit, predicated atomics).  128 rows of 248320: nothing but the counting of one token each
 // 41.5 us = 6.1 TB/s, 16000 tokens of prompt 60, 4000 generated ones 50, both with masks and 32 biases 73.7 = 3.6 TB/s; where the ends of a row were
 // asked for at every place and texts had lengths instead of ends (registers spilled) 43.5, 61, 53 and 77.5.  Before that, without the bits, every word of
@@ -483,10 +485,21 @@ int logits_as(q38b_ctx* ctx, const LogitsArgs& a, int n_rows, cudaStream_t st) {
 }
 template <bool VEC>
 int logits_in(q38b_ctx* ctx, const LogitsArgs& a, int n_rows, cudaStream_t st) {
-    // as many logits a CTA as still leaves three CTAs to every SM, or the fewest
-    const auto fills = [&](int chunk) { return (long long)n_rows * ((a.n + chunk - 1) / chunk) >= 3 * ctx->sm_count; };
-    return fills(16384) ? logits_as<16384, VEC>(ctx, a, n_rows, st) : fills(8192) ? logits_as<8192, VEC>(ctx, a, n_rows, st)
-         : fills(4096)  ? logits_as<4096, VEC>(ctx, a, n_rows, st) : logits_as<2048, VEC>(ctx, a, n_rows, st);
+    // The least time by waves of CTAs, three to an SM (two of 8192 and 16384 logits): what a wave takes beside what every call takes, in parts
+    // of some 0.3 us, more where each CTA reads a text; a last wave that is not full counts half, but for the largest.  (Before, the most logits that
+    // left three CTAs to every SM: 4 rows of 248320 then were 488 CTAs for 444 places and took 5.1 us, 11.6 with 20000 tokens, biases and masks; so
+    // 4.3 and 10.6, 16 rows 8.1 -> 7.4 and 17.6 -> 15.2.)
+    const int chunks[] = {16384, 8192, 4096, 2048}, per_sm[] = {2, 2, 3, 3}, wave[] = {30, 20, 18, 12}, wave_of_texts[] = {30, 21, 22, 18};
+    int best = 0;
+    double least = 0.0;
+    for (int i = 0; i < 4; i++) {
+        if (i < 3 && a.n <= chunks[i] / 2) continue;   // (half of its threads would have nothing)
+        const double waves = (double)n_rows * ((a.n + chunks[i] - 1) / chunks[i]) / (per_sm[i] * ctx->sm_count), whole = std::ceil(waves);
+        const double time = (i == 0 ? whole : std::max(1.0, (whole + waves) / 2.0)) * (a.r.history ? wave_of_texts[i] : wave[i]);
+        if (!best || time < least) { best = chunks[i]; least = time; }
+    }
+    return best == 16384 ? logits_as<16384, VEC>(ctx, a, n_rows, st) : best == 8192 ? logits_as<8192, VEC>(ctx, a, n_rows, st)
+         : best == 4096  ? logits_as<4096, VEC>(ctx, a, n_rows, st) : logits_as<2048, VEC>(ctx, a, n_rows, st);
 }
 
 }  // namespace

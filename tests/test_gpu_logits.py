@@ -262,3 +262,16 @@ def test_short_texts_at_every_alignment(ctx):
     rules = dict(penalties=np.stack([g.uniform(1, 2, rows), g.uniform(-1, 1, rows), g.uniform(-1, 1, rows)], 1).astype(np.float32).tolist(), history=history, prompt=prompt)
     check(run(ctx, x, **rules), *definition(x, **rules))
     check(run(ctx, np.ascontiguousarray(x[:, :36]), **rules), *definition(x[:, :36], **rules))   # four at a time
+
+
+@pytest.mark.parametrize("rows,n,hist,nbias,n_masks,off", [(300, 4000, 200, 9, 4, 0), (3, 70000, 4000, 50, 2, 5), (5, 248320, 0, 4, 2, 0), (9, 248320, 2000, 0, 0, 3), (64, 60001, 300, 3, 0, 0),
+                                                           (100, 32768, 900, 40, 6, 0)])
+def test_pieces_of_every_size(ctx, rows, n, hist, nbias, n_masks, off):
+    """Whole and broken pieces of 2048, 4096, 8192 and 16384 logits, one wave of them and several."""
+    test_four_at_a_time_give_the_bits_of_one(ctx, rows, n, hist, nbias, n_masks, off)
+
+
+def test_pieces_against_the_formula(ctx):
+    for rows, n, hist in ((300, 4000, 20), (40, 16400, 30), (2, 20000, 300)):
+        x, rules = case(rows, n, hist, 6, n, n_masks=3)
+        check(run(ctx, x, **rules), *definition(x, **rules))
