@@ -351,6 +351,9 @@ int q38b_pass_op_qk_norm_rope(q38b_pass* pass, const q38b_pass_heads* q, const q
  * same place).  The rules' device arrays (of max_nb rows) belong to the caller and are read at every run: a host gives each row room for its
  * text, filled with -1, which is passed over, and appends a token by writing it over the first of them. */
 int q38b_pass_op_adjust_logits(q38b_pass* pass, int src_f32, int off, int n, const q38b_logit_rules* rules, int dst_f32, int dst_off);
+/* The same on a shard of the head: the first of the n logits is that of token index_offset. */
+int q38b_pass_op_adjust_logits_at(q38b_pass* pass, int src_f32, int off, int n, int index_offset, const q38b_logit_rules* rules, int dst_f32,
+                                  int dst_off);
 /* After q38b_peer_connect the fp32 buffers of a pass live in the arena and matvec steps push their outputs to every
  * peer; q38b_pass_op_barrier then makes them usable on all ranks.  One barrier may cover several matvecs. */
 int q38b_pass_op_barrier(q38b_pass* pass);

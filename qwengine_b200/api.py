@@ -113,6 +113,7 @@ def load_library():
     lib.q38b_adjust_logits.argtypes = [vp, vp, ll, i32, i32, i32, vp, vp, ll, vp]
     lib.q38b_pass_op_qk_norm_rope.argtypes = [vp, vp, vp, i32, i32, i32, C.c_float, C.c_float, vp, vp]
     lib.q38b_pass_op_adjust_logits.argtypes = [vp, i32, i32, i32, vp, i32, i32]
+    lib.q38b_pass_op_adjust_logits_at.argtypes = [vp, i32, i32, i32, i32, vp, i32, i32]
     lib.q38b_mx4_scale_bytes.argtypes = [i32, i32]
     lib.q38b_mx4_scale_bytes.restype = sz
     lib.q38b_quantize_mx4.argtypes = [vp, vp, i32, ll, i32, i32, vp, ll, vp, vp]
@@ -685,13 +686,13 @@ class Pass:
                                                         positions.data_ptr() if rot else None, inv_freq.data_ptr() if rot else None), "q38b_pass_op_qk_norm_rope")
         self._keep += [positions, inv_freq, q_weight, k_weight]
 
-    def adjust_logits(self, src, off, n, dst=None, dst_off=None, **rules):
-        """The rules of Context.logit_rules on n logits of buffer src (in place where dst is not given); the rules' tensors have max_nb rows, are
-        kept by the pass and read at every run."""
+    def adjust_logits(self, src, off, n, dst=None, dst_off=None, index_offset=0, **rules):
+        """The rules of Context.logit_rules on n logits of buffer src (in place where dst is not given), of which the first is token index_offset's; the
+        rules' tensors have max_nb rows, are kept by the pass and read at every run."""
         dst = src if dst is None else dst
         dst_off = (off if dst == src else 0) if dst_off is None else dst_off
-        packed = self.ctx.logit_rules(self.max_nb, n, **rules)
-        self.ctx._rc(self.lib.q38b_pass_op_adjust_logits(self.h, src, off, n, packed, dst, dst_off), "q38b_pass_op_adjust_logits")
+        packed = self.ctx.logit_rules(self.max_nb, n, index_offset=index_offset, **rules)
+        self.ctx._rc(self.lib.q38b_pass_op_adjust_logits_at(self.h, src, off, n, index_offset, packed, dst, dst_off), "q38b_pass_op_adjust_logits_at")
         self._keep += [t for t in rules.values() if isinstance(t, torch.Tensor)]
 
     def barrier(self):

@@ -56,7 +56,7 @@ struct Op { int kind, a, b, c, d, n, off; };
 struct Buf { void* ptr; int n; bool q8k; void* peer[8]; int n_peer_ranks; bool in_arena; };
 // q38b_pass_op_qk_norm_rope, q38b_pass_op_adjust_logits: what an Op has no room for (Op::a is their number)
 struct HeadsStep { q38b_pass_heads t[2]; int n_tensors, D, rot, adjacent; float eps, scale; const int* positions; const double* inv_freq; };
-struct LogitsStep { q38b_logit_rules rules; };
+struct LogitsStep { q38b_logit_rules rules; int index_offset; };
 struct Mat { uint32_t type; const void* W; size_t row_bytes; int K, M; bool owned; };
 
 struct PeerPtrs { uint32_t* p[8]; };
@@ -393,7 +393,8 @@ int enqueue_ops(q38b_pass* p, int nb, cudaStream_t st) {
             }
             case OP_LOGITS: {   // a: which rules, b: source, off: first logit, n: how many, c: destination, d: its first logit
                 const Buf &from = p->bufs[o.b], &to = p->bufs[o.c];
-                rc = q38b_adjust_logits(ctx, (const float*)from.ptr + o.off, from.n, o.n, nb, 0, &p->logits[o.a].rules, (float*)to.ptr + o.d, to.n, st);
+                const LogitsStep& s = p->logits[o.a];
+                rc = q38b_adjust_logits(ctx, (const float*)from.ptr + o.off, from.n, o.n, nb, s.index_offset, &s.rules, (float*)to.ptr + o.d, to.n, st);
                 break;
             }
             case OP_BARRIER: {
@@ -669,19 +670,24 @@ int q38b_pass_op_qk_norm_rope(q38b_pass* p, const q38b_pass_heads* q, const q38b
     return Q38B_OK;
 }
 
-int q38b_pass_op_adjust_logits(q38b_pass* p, int src, int off, int n, const q38b_logit_rules* rules, int dst, int dst_off) {
+int q38b_pass_op_adjust_logits_at(q38b_pass* p, int src, int off, int n, int index_offset, const q38b_logit_rules* rules, int dst, int dst_off) {
     if (!p || !rules || !is_f32(p, src) || !is_f32(p, dst) || off < 0 || dst_off < 0 || n < 1 || off + (long long)n > p->bufs[src].n || dst_off + (long long)n > p->bufs[dst].n)
         return Q38B_ERR_ARG;
     if (src == dst && off != dst_off && off < dst_off + (long long)n && dst_off < off + (long long)n) return Q38B_ERR_ARG;
-    const int rc = q38b_logit_rules_check(rules, n, 0);
+    if (index_offset < 0 || index_offset > 0x7FFFFFFF - n) return Q38B_ERR_ARG;
+    const int rc = q38b_logit_rules_check(rules, n, index_offset);
     if (rc != Q38B_OK) return rc;
     try {
-        p->logits.push_back({*rules});
+        p->logits.push_back({*rules, index_offset});
         p->ops.push_back({OP_LOGITS, (int)p->logits.size() - 1, src, dst, dst_off, n, off});
     } catch (...) {
         return Q38B_ERR_NOMEM;
     }
     return Q38B_OK;
+}
+
+int q38b_pass_op_adjust_logits(q38b_pass* p, int src, int off, int n, const q38b_logit_rules* rules, int dst, int dst_off) {
+    return q38b_pass_op_adjust_logits_at(p, src, off, n, 0, rules, dst, dst_off);
 }
 
 int q38b_pass_op_swiglu(q38b_pass* p, int g, int g_off, int u, int u_off, int n, int dst) {
