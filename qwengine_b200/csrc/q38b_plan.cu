@@ -648,7 +648,7 @@ int q38b_pass_op_qk_norm_rope(q38b_pass* p, const q38b_pass_heads* q, const q38b
     int n_spans = 0;
     for (int i = 0; i < s.n_tensors; i++) {
         const q38b_pass_heads& t = s.t[i];
-        if (!is_f32(p, t.src) || !is_f32(p, t.dst) || t.n_heads < 1 || t.src_off < 0 || t.dst_off < 0 || t.src_head < 0) return Q38B_ERR_ARG;
+        if (!is_f32(p, t.src) || !is_f32(p, t.dst) || t.n_heads < 1 || t.src_off < 0 || t.dst_off < 0 || t.src_head < 0 || t.dst_head < 0) return Q38B_ERR_ARG;
         if (t.n_heads > 1 && t.dst_head < D) return Q38B_ERR_ARG;
         if ((uintptr_t)t.weight & 3) return Q38B_ERR_ALIGN;
         const long long src_end = t.src_off + (long long)(t.n_heads - 1) * t.src_head + D, dst_end = t.dst_off + (long long)(t.n_heads - 1) * t.dst_head + D;

@@ -532,8 +532,8 @@ int q38b_qk_norm_rope(q38b_ctx* ctx, const q38b_heads* q, const q38b_heads* k, i
         if ((t.n_heads > 1 && t.dst_head < D) || (rows > 1 && t.dst_row < D)) return Q38B_ERR_ARG;
         if (t.n_heads > 1 && rows > 1 && t.dst_row < in_row && t.dst_head < in_head) return Q38B_ERR_ARG;
         if ((uintptr_t)t.src % kind_size(in_kind) || (uintptr_t)t.dst % kind_size(out_kind) || ((uintptr_t)t.weight & 3)) return Q38B_ERR_ALIGN;
-        // in place only element over element
-        if (t.src == t.dst && (in_kind != out_kind || t.src_head != t.dst_head || t.src_row != t.dst_row)) return Q38B_ERR_ARG;
+        // in place only element over element (the strides of one head, of one row say nothing)
+        if (t.src == t.dst && (in_kind != out_kind || (t.n_heads > 1 && t.src_head != t.dst_head) || (rows > 1 && t.src_row != t.dst_row))) return Q38B_ERR_ARG;
     }
     if (((uintptr_t)positions & 3) || ((uintptr_t)inv_freq & 7)) return Q38B_ERR_ALIGN;
     a.D = D;
