@@ -226,9 +226,10 @@ typedef struct q38b_heads {
  *   y_a = scale (z_a cos - z_b sin), y_b = scale (z_b cos + z_a sin) for the pairs (a, b) = (j, j + rot / 2), or (2j, 2j + 1) if
  *   adjacent, j < rot / 2, angle = positions[t] * inv_freq[j]; elements from `rot` on are z.
  * k may be NULL.  positions: int32 [rows], any sign; inv_freq: float64 [rot / 2], finite, radians per position (both may be NULL with
- * rot = 0); the angle is exact to about |position| 2^-52 turns.  in_kind, out_kind: q38b_out_kind of src and dst.  D <= 1024, rot even and
- * at most D.  dst may be src itself (same kind, same strides, but for those of one head or row); otherwise the two must not overlap, nor may the query heads'
- * elements be among the key heads'.  In dst rows lie outside heads (dst_row at least a row's extent) or heads outside rows.  Sums in fp32, outputs rounded once. */
+ * rot = 0); the angle is off by about 2^-28 turns at most, and by |position| 2^-52 max(1, |inv_freq| / 2 pi) turns far out.  in_kind, out_kind:
+ * q38b_out_kind of src and dst.  D <= 1024, rot even and at most D.  dst may be src itself (same kind, same strides, but for those of one
+ * head or row); otherwise the two must not overlap, nor may the query heads' elements be among the key heads'.  In dst rows lie outside
+ * heads (dst_row at least a row's extent) or heads outside rows.  Sums in fp32, outputs rounded once. */
 int q38b_qk_norm_rope(q38b_ctx* ctx, const q38b_heads* q, const q38b_heads* k, int D, int rot, int adjacent, float eps, float scale,
                       const int* positions_dev, const double* inv_freq_dev, int in_kind, int out_kind, int rows, void* stream);
 
