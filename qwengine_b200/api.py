@@ -484,7 +484,8 @@ class Context:
 
     def gemm_mx4(self, W, X, kind=OUT_F32, out=None, accumulate=False):
         """Y [B, W.rows] = X W^T for W an Mx4 and X an Mx4 or activations [B, K] (fp32, fp16 or bf16), which are quantized first.  kind: OUT_* of Y
-        where `out` is not given."""
+        where `out` is not given; accumulate adds to `out`."""
+        _need(out is not None or not accumulate, "gemm_mx4: accumulate needs an out to add to")
         K, M, dev, mx = W.K, W.rows, self._index, isinstance(X, Mx4)
         B = X.rows if mx else X.shape[0]
         if W.codes.get_device() != dev or (X.codes if mx else X).get_device() != dev:
