@@ -273,6 +273,7 @@ class Context:
     # ---- matvec ------------------------------------------------------------------------------
     def gemv(self, fmt, W, xq, K, out=None, accumulate=False, M=None):
         """W uint8 [M, row_bytes]; xq uint8 [nb, K/256*292]; returns y float32 [nb, M] (y[c, r])."""
+        _need(out is not None or not accumulate, "gemv: accumulate needs an out to add to")
         f = F.get(fmt)
         assert W.is_cuda and W.dtype == torch.uint8 and W.dim() == 2 and W.stride(1) == 1
         M = W.shape[0] if M is None else M
@@ -298,6 +299,7 @@ class Context:
 
     def gemv_act_q8(self, fmt, W, q, d, K, out=None, accumulate=False):
         """W uint8 [M, row_bytes]; q int8 [nb, K], d float32 [nb, K/32] (contiguous); returns y float32 [nb, M]."""
+        _need(out is not None or not accumulate, "gemv_act_q8: accumulate needs an out to add to")
         f = F.get(fmt)
         M, nb = W.shape[0], q.shape[0]
         if out is None:
@@ -549,6 +551,7 @@ class Context:
 
     def gemv_f32(self, fmt, W, x, K, scratch=None, out=None, accumulate=False):
         """Matvec from fp32 activations x [nb, K]; `scratch` is a uint8 device tensor for the Q8_K blocks."""
+        _need(out is not None or not accumulate, "gemv_f32: accumulate needs an out to add to")
         f = F.get(fmt)
         nb, M = x.shape[0], W.shape[0]
         if scratch is None:
@@ -578,6 +581,7 @@ class Context:
     def gemm_prefill(self, fmt, W, X, K, out=None, accumulate=False):
         """W uint8 [M, row_bytes]; X bfloat16 or float16 [B, K] (the operand type of the tensor-core product follows X);
         returns Y float32 [B, M] = X @ dequant(W)^T."""
+        _need(out is not None or not accumulate, "gemm_prefill: accumulate needs an out to add to")
         f = F.get(fmt)
         assert X.dtype in (torch.bfloat16, torch.float16) and X.stride(1) == 1
         M, B = W.shape[0], X.shape[0]

@@ -21,3 +21,11 @@ def refused(call):
 def test_gemm_mx4(x):
     W = q.Mx4(torch.zeros(5, 32, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8))
     refused(lambda: context().gemm_mx4(W, W if isinstance(x, str) else x, accumulate=True))
+
+
+def test_products_of_gguf_blocks():
+    c, w = context(), torch.zeros(5, 144, dtype=torch.uint8)
+    refused(lambda: c.gemv("Q4_K", w, torch.zeros(1, 292, dtype=torch.uint8), 256, accumulate=True))
+    refused(lambda: c.gemv_act_q8("Q4_K", w, torch.zeros(1, 256, dtype=torch.int8), torch.zeros(1, 8), 256, accumulate=True))
+    refused(lambda: c.gemv_f32("Q4_K", w, torch.zeros(1, 256), 256, accumulate=True))
+    refused(lambda: c.gemm_prefill("Q4_K", w, torch.zeros(1, 256, dtype=torch.bfloat16), 256, accumulate=True))
