@@ -60,9 +60,9 @@ const char* q38b_status_string(int status);
 int q38b_ctx_set_wait_budget_cycles(q38b_ctx* ctx, long long cycles);
 
 /* Programmatic dependent launch lets a matvec start (and prefetch) while the previous KERNEL of the stream drains.  It
- * is always used between the kernels of a recorded pass.  For direct calls it is off by default, because a direct call
- * may follow a memcpy that fills its operands, which a programmatic launch does not wait for; 1 turns it on for
- * direct calls too (only when every matvec follows a kernel), 0 turns it off everywhere. */
+ * is always used between the kernels of a recorded pass, and between the two of q38b_gemm_mx4_x.  For direct calls it is
+ * off by default, because a direct call may follow a memcpy that fills its operands, which a programmatic launch does not
+ * wait for; 1 turns it on for direct calls too (only when every matvec follows a kernel), 0 turns it off everywhere. */
 int q38b_ctx_set_pdl(q38b_ctx* ctx, int enabled);
 /* With programmatic dependent launch a matvec may start while the previous kernel of the stream is still running.  Its
  * activations always wait for that kernel; its weight stream waits too unless this option is 1, which promises that

@@ -9,7 +9,7 @@ struct q38b_ctx {
     int smem_optin = 0;
     int last_cuda = 0;
     int pdl = 0;               // programmatic dependent launch for direct calls (passes use pass_pdl)
-    int pass_pdl = 1;          // programmatic dependent launch between the kernels of a recorded pass
+    int pass_pdl = 1;          // programmatic dependent launch between the kernels of a recorded pass (and of q38b_gemm_mx4_x)
     int static_weights = 0;    // 1: matvec producers start streaming W before the previous kernel of the stream has finished
     int rowgroup = 1;          // 0: the row-group mapping of the one-column kernel is not used (test hook q38b_debug_set_rowgroup)
     int one_cta = 1;           // one-column kernel with one CTA per SM where such a plan fits; 0: never (test hook q38b_debug_set_one_cta)

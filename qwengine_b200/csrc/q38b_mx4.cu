@@ -961,7 +961,7 @@ int check_operand(const void* codes, long long ld, const void* scales, int K, in
     return ((uintptr_t)codes & 15) || (ld & 15) || ((uintptr_t)scales & 15) ? Q38B_ERR_ALIGN : Q38B_OK;
 }
 
-// the product of two such matrices; behind_quantizer: launched while the kernel that makes X still runs
+// the product of two such matrices; behind_quantizer: launched while the kernel that makes X still runs, where the context allows it
 int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales, int K, int M, const void* X, long long X_ld, const void* X_scales, int B,
              void* Y, int y_kind, long long ldy, int accumulate, void* stream, bool behind_quantizer) {
     if (!ctx || !Y || !known_kind(y_kind) || ldy < M) return Q38B_ERR_ARG;
@@ -971,6 +971,7 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
     if ((uintptr_t)Y % kind_size(y_kind)) return Q38B_ERR_ALIGN;
     DeviceGuard on(ctx);
     cudaStream_t st = (cudaStream_t)stream;
+    const int pdl = behind_quantizer && ctx->pass_pdl ? 1 : 0;
     double cost = 0.0, pair_cost = 0.0;
     const MxCut one = mx_cut(ctx->sm_count, ctx->smem_optin, K, M, B, &cost);
     const MxPairCut cut = mx_pair_cut(ctx->sm_count, ctx->smem_optin, K, M, B, ctx->mx4_pairs > 0 ? ctx->mx4_pairs : 0, &pair_cost);
@@ -983,7 +984,7 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
         if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS) || !encode_codes(&xmap, X, X_ld, K, B, cut.n_tile / 2) || !encode_scales(&wsmap, W_scales, K, M, 1) ||
             !encode_scales(&xsmap, X_scales, K, B, mx_groups(cut.n_tile)))
             return Q38B_ERR_ARG;
-        const MxPairArgs a = {Y, ldy, ctx->d_status, K, M, B, accumulate ? 1 : 0, cut.n_tile, cut.stages, cut.n_acc, cut.tok_tiles, cut.n_tiles, behind_quantizer ? 1 : 0, tma_out};
+        const MxPairArgs a = {Y, ldy, ctx->d_status, K, M, B, accumulate ? 1 : 0, cut.n_tile, cut.stages, cut.n_acc, cut.tok_tiles, cut.n_tiles, pdl, tma_out};
         return y_kind == Q38B_OUT_F32 ? pair_as<float>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st)
              : y_kind == Q38B_OUT_F16 ? pair_as<__half>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st)
                                       : pair_as<__nv_bfloat16>(ctx, a, wmap, xmap, wsmap, xsmap, ymap, st);
@@ -993,7 +994,7 @@ int gemm_mx4(q38b_ctx* ctx, const void* W, long long W_ld, const void* W_scales,
     if (!encode_codes(&wmap, W, W_ld, K, M, MX_ROWS) || !encode_codes(&xmap, X, X_ld, K, B, one.n_tile)) return Q38B_ERR_ARG;
     MxArgs a = mx_args(ctx, one, W_scales, K, M, B, Y, ldy, accumulate);
     a.x_scales = (const uint8_t*)X_scales;
-    a.pdl = behind_quantizer ? 1 : 0;
+    a.pdl = pdl;
     return mx_groups(a.n_tile) == 1 ? gemm_kind<1, false>(ctx, a, one.box, wmap, xmap, y_kind, st) : gemm_kind<2, false>(ctx, a, one.box, wmap, xmap, y_kind, st);
 }
 
