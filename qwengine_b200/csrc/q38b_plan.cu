@@ -260,6 +260,17 @@ void merge_plan(const q38b_pass* p, int nb, std::vector<Merged>& out, std::vecto
     }
 }
 
+// Whether barrier `oi` goes into the prologue of the launch behind it: a merged matvec launch (opened by its folded quantize step or its first
+// matvec) or a SwiGLU kernel, with nothing (not even a gather) in between.  The multi-column kernel has no barrier in its prologue, nor has any
+// other kernel (heads, logit rules, top-k): in front of them the barrier is a kernel of its own.
+bool barrier_joins_launch(const q38b_pass* p, const std::vector<Merged>& merged, const std::vector<char>& skip, size_t oi, int nb) {
+    const size_t j = oi + 1;
+    if (j >= p->ops.size()) return false;
+    bool next_is_merged = false;
+    for (const Merged& mg : merged) next_is_merged |= (mg.quant >= 0 ? mg.quant : mg.first_op) == (int)j;
+    return (next_is_merged && nb == 1) || (!skip[j] && p->ops[j].kind == OP_SWIGLU);
+}
+
 bool merging(const q38b_pass* p, int nb) { return p->merge_steps && (nb > 1 || !p->ctx->uniform_columns); }
 
 int enqueue_ops(q38b_pass* p, int nb, cudaStream_t st) {
@@ -404,14 +415,7 @@ int enqueue_ops(q38b_pass* p, int nb, cudaStream_t st) {
                     ctx->pending_sync_seq = -1;
                     if (rc != Q38B_OK) return rc;
                 }
-                size_t j = oi + 1;
-                while (j < p->ops.size() && (p->ops[j].kind == OP_GATHER || p->ops[j].kind == OP_BARRIER)) j++;
-                bool next_is_merged = false;   // op j opens a merged launch: its folded quantize step or its first matvec
-                for (const Merged& mg : merged) next_is_merged |= (mg.quant >= 0 ? mg.quant : mg.first_op) == (int)j;
-                const bool next_is_swiglu = j < p->ops.size() && !skip[j] && p->ops[j].kind == OP_SWIGLU;
-                const bool adjacent = j == oi + 1;   // nothing (not even a gather) between the barrier and that launch
-                // (the multi-column kernel has no barrier in its prologue: in front of it the barrier is a kernel of its own)
-                if (adjacent && ((next_is_merged && nb == 1) || next_is_swiglu)) ctx->pending_sync_seq = barrier_seq++;
+                if (barrier_joins_launch(p, merged, skip, oi, nb)) ctx->pending_sync_seq = barrier_seq++;
                 else rc = launch_barrier(ctx, 0, 1, barrier_seq++, st);
                 break;
             }
@@ -774,17 +778,12 @@ int q38b_pass_set_merge(q38b_pass* p, int enabled) {
     return Q38B_OK;
 }
 
-// Test hook (not in the public header): runs the launch planner on a list of steps without touching a device.
-// steps[3 i ..] = {kind (0 quantize, 1 matvec, 2 SwiGLU, 3 all-gather, 4 barrier), column buffer, output offset}; every
-// matvec is a 512 x 1024 Q4_K matrix writing 512 floats at its offset.  launch_of[i] receives the position in the step
-// list at which step i is launched (its own index unless it joined an earlier launch), -1 for folded quantize steps.
-int q38b_debug_merge_plan(int n_ranks, int nb, int n_steps, const int* steps, int* launch_of) {
-    if (n_ranks < 1 || nb < 1 || n_steps < 0 || !steps || !launch_of) return Q38B_ERR_ARG;
-    q38b_ctx ctx;
+// The steps of the test hooks below, on a pass without a device: steps[3 i ..] = {kind (0 quantize, 1 matvec, 2 SwiGLU, 3 all-gather, 4 barrier, 5 heads,
+// 6 logit rules, 7 top-k), column buffer, output offset}; every matvec is a 512 x 1024 Q4_K matrix writing 512 floats at its offset.
+static bool debug_steps(q38b_ctx& ctx, q38b_pass& p, int n_ranks, int n_steps, const int* steps) {
     ctx.sm_count = 148;
     ctx.smem_optin = 232448;
     ctx.n_ranks = n_ranks;
-    q38b_pass p;
     p.ctx = &ctx;
     p.mats.push_back({(uint32_t)T_Q4_K, nullptr, 576, 1024, 512, false});
     for (int b = 0; b < 8; b++) p.bufs.push_back({nullptr, 1 << 20, b >= 4, {}, 0, false});   // 0..3 fp32, 4..7 Q8_K columns
@@ -796,9 +795,23 @@ int q38b_debug_merge_plan(int n_ranks, int nb, int n_steps, const int* steps, in
             case 2: p.ops.push_back({OP_SWIGLU, 1, 1, col, 0, 1024, off}); break;
             case 3: p.ops.push_back({OP_GATHER, 1, 0, 0, 0, 512, off}); break;
             case 4: p.ops.push_back({OP_BARRIER, 0, 0, 0, 0, 0, 0}); break;
-            default: return Q38B_ERR_ARG;
+            case 5: p.ops.push_back({OP_HEADS, 0, 0, 0, 0, 0, 0}); break;
+            case 6: p.ops.push_back({OP_LOGITS, 0, 1, 1, off, 512, off}); break;
+            case 7: p.ops.push_back({OP_TOPK, 1, 2, 0, 32, 512, off}); break;
+            default: return false;
         }
     }
+    return true;
+}
+
+// Test hook (not in the public header): runs the launch planner on a list of steps without touching a device.
+// launch_of[i] receives the position in the step list at which step i is launched (its own index unless it joined an earlier launch),
+// -1 for folded quantize steps.
+int q38b_debug_merge_plan(int n_ranks, int nb, int n_steps, const int* steps, int* launch_of) {
+    if (n_ranks < 1 || nb < 1 || n_steps < 0 || !steps || !launch_of) return Q38B_ERR_ARG;
+    q38b_ctx ctx;
+    q38b_pass p;
+    if (!debug_steps(ctx, p, n_ranks, n_steps, steps)) return Q38B_ERR_ARG;
     std::vector<Merged> merged;
     std::vector<char> skip;
     merge_plan(&p, nb, merged, skip);
@@ -808,6 +821,20 @@ int q38b_debug_merge_plan(int n_ranks, int nb, int n_steps, const int* steps, in
         for (int t = 0; t < mg.n; t++) launch_of[mg.ops[t]] = mg.first_op;
     }
     return (int)merged.size();
+}
+
+// Test hook (not in the public header): where the barriers of a list of steps run, for the same planner.  own[i] = 1 for a barrier that is a kernel of its own,
+// 0 for one that the launch behind it begins with, -1 for any other step.
+int q38b_debug_barriers(int n_ranks, int nb, int n_steps, const int* steps, int* own) {
+    if (n_ranks < 1 || nb < 1 || n_steps < 0 || !steps || !own) return Q38B_ERR_ARG;
+    q38b_ctx ctx;
+    q38b_pass p;
+    if (!debug_steps(ctx, p, n_ranks, n_steps, steps)) return Q38B_ERR_ARG;
+    std::vector<Merged> merged;
+    std::vector<char> skip;
+    merge_plan(&p, nb, merged, skip);
+    for (int i = 0; i < n_steps; i++) own[i] = p.ops[i].kind != OP_BARRIER ? -1 : barrier_joins_launch(&p, merged, skip, (size_t)i, nb) ? 0 : 1;
+    return Q38B_OK;
 }
 
 // Test hook (not in the public header): whether a replay with nb columns folds a quantize step of K values at float
