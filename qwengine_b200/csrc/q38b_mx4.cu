@@ -536,6 +536,7 @@ __global__ void __launch_bounds__(MX_THREADS, GROUPS == 1 ? 2 : 1) mx4_gemm_kern
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 1) {
+        if (__builtin_expect(*abort_flag, 0)) settle_after_abort();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(tmem_cols) : "memory");
     }
@@ -726,6 +727,7 @@ mx4_pair_kernel(const MxPairArgs a, const __grid_constant__ CUtensorMap wmap, co
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     cluster_sync_all();   // both CTAs have read their accumulators, and nothing is on its way to the other's barriers
     if (warp == 1) {
+        if (__builtin_expect(*abort_flag, 0)) settle_after_abort();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
     }

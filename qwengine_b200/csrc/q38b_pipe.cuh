@@ -58,6 +58,12 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
     return false;
 }
 
+// A kernel that gave up a wait may still have copies on their way into its shared memory and products into its tensor memory.  Called before it
+// gives either back: they take microseconds, and it stays for 2^21 clocks (a millisecond).
+__device__ __forceinline__ void settle_after_abort() {
+    for (const long long t0 = clock64(); clock64() - t0 < (1LL << 21);) {}
+}
+
 // A counter in shared memory that one thread advances (release) and others poll (acquire) until it exceeds `than`.
 __device__ __forceinline__ void st_release_shared(uint32_t addr, int v) {
     asm volatile("st.release.cta.shared::cta.s32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
