@@ -273,7 +273,8 @@ int q38b_quantize_mx4(q38b_ctx* ctx, const void* x_dev, int x_kind, long long x_
                       void* scales_dev, void* stream);
 /* Scale bytes of another producer, [rows][src_ld] with K / 32 of them in a row, into the tiles above. */
 int q38b_mx4_tile_scales(q38b_ctx* ctx, const void* src_dev, long long src_ld, int K, int rows, void* scales_dev, void* stream);
-/* The values that codes and scales stand for, exact in fp32, rounded once to fp16 / bf16. */
+/* The values that codes and scales stand for, exact in fp32, rounded once to fp16 / bf16 (infinite where they pass the type: in fp32 elements of 4 or 6
+ * with another producer's scale byte of 253, of 2 and more with 254). */
 int q38b_dequant_mx4(q38b_ctx* ctx, const void* codes_dev, long long codes_ld, const void* scales_dev, int K, int rows, void* out_dev,
                      int out_kind, long long out_ld, void* stream);
 /* Y[t * ldy + r] (+)= sum_k X[t][k] W[r][k] for t < B, r < M over those values, on the block-scaled tensor-core instructions; fp32 sums

@@ -424,7 +424,7 @@ class Context:
         return _pack_rules(p, h, hb, pl, bi, bv, bb, mk, ld, mr)
 
     def adjust_logits(self, logits, out=None, index_offset=0, **rules):
-        """logits fp32 [rows, n] (any row stride) -> penalised, biased, masked logits (`out`, which may be `logits`); the rules are those of
+        """logits fp32 [rows, n] (rows any distance of n and more apart) -> penalised, biased, masked logits (`out`, which may be `logits`); the rules are those of
         logit_rules.  Token v is column v - index_offset."""
         rows, n = logits.shape
         ld, one = logits.stride()
@@ -445,7 +445,7 @@ class Context:
 
     # ---- microscaled 4-bit floating point -----------------------------------------------------
     def quantize_mx4(self, x):
-        """x [rows, K] (fp32, fp16 or bf16, any row stride) -> Mx4."""
+        """x [rows, K] (fp32, fp16 or bf16, rows any distance of K and more apart) -> Mx4."""
         rows, K = x.shape
         ld, one = x.stride()
         kind = _OUT_KINDS.get(x.dtype)

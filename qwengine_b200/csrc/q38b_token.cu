@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(256, 6) heads_kernel(const HeadsArgs a) {
 // Heads of up to 256 elements whose rows allow it move four elements a lane at a time.  A CTA has one row (its sines and cosines are computed
 // once, into shared memory) and up to HEADS_BATCH heads a warp, whose loads are all issued first; a head's L lanes add its squares by
 // shuffles and swap partners of the rotation through shared memory.  Bound by memory: 8192 rows of 24 + 4 heads of 256, fp32 to bf16, 62 us =
-// 5.7 TB/s (four heads a warp, eight warps a CTA, three CTAs an SM 77) against 114 us element by element, where every head's warp computed its own angles.
+// 5.7 TB/s (four heads a warp, eight warps a CTA, three CTAs an SM 77) against 104 us element by element, where every head's warp computes its own angles.
 constexpr int HEADS_BATCH = 2, HEADS_WARPS = 4, HEADS_MAX_D = 256;
 
 template <typename T> __device__ __forceinline__ float4 load4(const T* p) {
