@@ -750,14 +750,15 @@ int mx_fused_stages(int smem_optin, const MxCut& c, int x_steps) { return std::m
 // ... by their time in SM clocks, of one wave of CTAs after the other: what starts and drains a CTA, the exchange of split sums, and stages, each as
 // long as a CTA takes alone (two of an SM: twice) or, if that is longer, as its bytes take out of L2 (6400 a clock for all SMs) and its weights out of
 // DRAM (3300).  Fitted to 1024, 5120 and 17408 rows, 16 to 768 tokens, in every number of parts and tiles: the taken cut is within 4 % of the best
-// there, but for one token in six parts (below).  1024 x 5120: 256 tokens 11.1 -> 8.2 us, 512 tokens 20.5 -> 9.0; 5120 x 17408, 256 tokens 24.1 -> 20.8 (before,
+// there, but for one token (below).  1024 x 5120: 256 tokens 11.1 -> 8.2 us, 512 tokens 20.5 -> 9.0; 5120 x 17408, 256 tokens 24.1 -> 20.8 (before,
 // a stage counted 600 clocks and 5 a token, whoever else ran).
 // Two CTAs of an SM overlap their ends, and parts fill all SMs: 7 x 5120 x 17408 in six parts 13.7 us, in three of whole SMs 14.8; 7 x 12288 x 5120 in two
 // 11.5 and 12.5; one token x 248320 x 5120 112 and 130.  One token's codes take shared memory too, of which a ring of three stages has to remain.  And
-// where not all CTAs run at once each wave quantizes its part anew: more than two parts pay in one wave (1 x 6144 x 10240 in five 10.8 us, in two of whole
-// SMs 12.7; 10752 x 10240 in three 14.5, undivided 18.1; 32 of 33 sizes gained, 2560 x 6144 in seven lost 0.4 us) and not in several (24576 x 10240 in four
-// 32.7, undivided 26.3; 19 of 24 sizes lost).  Two such CTAs hold at most 256 columns of tensor memory each, and no other kernel here that
-// allocates columns fits beside one (registers, shared memory): no cluster waits for columns that another waiting one holds.
+// where not all CTAs run at once each wave quantizes its part anew: more than two parts, six at most, pay in one wave (1 x 6144 x 10240 in five 10.8 us, in two
+// of whole SMs 12.7; 10752 x 10240 in three 14.5, undivided 18.1; 55 of 59 drawn sizes gained, up to a quarter, 3200 x 5632 in six lost 0.5 us; in seven 21 of
+// 25 lost) and not in several (24576 x 10240 in four 32.7, undivided 26.3; 19 of 24 lost).  Two such CTAs hold at most 256 columns of tensor memory
+// each, and no other kernel here that allocates columns fits beside one (registers, shared memory): no cluster waits for columns that another waiting
+// one holds.
 // Clusters of three to six leave an eighth of the SMs unused, larger ones three tenths (45, 33, 26, 22, 15 and 15 clusters were there at a time).
 MxCut mx_cut(int sm_count, int smem_optin, int K, int M, int B, double* cost_of) {
     MxCut best = {};
@@ -777,7 +778,7 @@ MxCut mx_cut(int sm_count, int smem_optin, int K, int M, int B, double* cost_of)
             const long long ctas = tiles * c.splits, once = std::max(1, sms / c.splits) * (long long)c.splits, slots = per_sm * once, waves = (ctas + slots - 1) / slots;
             if (per_sm == 2) {
                 if (ctas <= once || c.stages < 3 || own_steps < 4) continue;   // (shorter ones are all ends: 16 x 2048 x 2048 in eight parts 6.5 us, 5.6 otherwise)
-                if (B == 1 && own_steps * MX_K <= MX_FUSE_MAX_K && ((c.splits > 2 && waves > 1) || mx_fused_stages(smem_optin, c, own_steps) < 3)) continue;
+                if (B == 1 && own_steps * MX_K <= MX_FUSE_MAX_K && ((c.splits > 2 && (waves > 1 || c.splits > 6)) || mx_fused_stages(smem_optin, c, own_steps) < 3)) continue;
             }
             const double active = (double)std::min(ctas, slots);
             const double stage = std::max({per_sm * (590.0 + 0.45 * n), active * mx_stage_bytes(n) / 6400.0, active / (double)tok_tiles * (MX_A_BYTES + MX_SFA_BYTES) / 3300.0});

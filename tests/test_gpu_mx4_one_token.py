@@ -1,4 +1,4 @@
-"""One token's product in every number of parts with two CTAs to an SM: sums of whole numbers, exact whatever the cut, in one launch and in two."""
+"""One token's product in every number of parts that two CTAs of an SM take: sums of whole numbers, exact whatever the cut, in one launch and in two."""
 import pytest
 import torch
 
@@ -7,7 +7,7 @@ import qwengine_b200 as q   # noqa: F401
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("M,K", [(10700, 10240), (9216, 5120), (7680, 4096), (8100, 6144), (6144, 10240), (4608, 10240), (2560, 6144),    # 3, 3, 4, 4, 5, 6 and 7 parts in one wave
+@pytest.mark.parametrize("M,K", [(10700, 10240), (9216, 5120), (7680, 4096), (8100, 6144), (6144, 10240), (4608, 10240), (2560, 6144),    # 3, 3, 4, 4, 5 and 6 parts in one wave, 6 of whole SMs
                                  (24576, 10240), (20480, 7168), (12288, 10240)])                                                            # more CTAs than places
 def test_whole_number_products(ctx, M, K):
     gen = torch.Generator("cuda").manual_seed(M + K)
