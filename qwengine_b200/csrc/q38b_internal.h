@@ -46,7 +46,7 @@ const uint32_t* q38b_grid_source(const q38b_ctx* ctx, uint32_t type);
 // Opt-in shared-memory size of a kernel, set once per context (= per device) and kernel
 int q38b_ensure_kernel_smem(q38b_ctx* ctx, const void* kern, int dyn_smem_bytes, bool max_carveout);
 
-// whether the rules of q38b_adjust_logits (q38b_token.cu) are whole and aligned: a q38b_status
+// whether the rules of q38b_adjust_logits (q38b_token.cu) are whole and aligned, for as many logits as it takes: a q38b_status
 struct q38b_logit_rules;
 int q38b_logit_rules_check(const q38b_logit_rules* rules, int n, int index_offset);
 

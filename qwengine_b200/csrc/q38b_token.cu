@@ -518,6 +518,7 @@ int logits_in(q38b_ctx* ctx, const LogitsArgs& a, int n_rows, cudaStream_t st) {
 }  // namespace
 
 int q38b_logit_rules_check(const q38b_logit_rules* rules, int n, int index_offset) {
+    if (n > LG_MAX_N) return Q38B_ERR_UNSUPPORTED;
     if (!rules->penalties != !rules->history || !rules->history != !rules->history_begin || (rules->prompt_len && !rules->history)) return Q38B_ERR_ARG;
     if (!rules->bias_ids != !rules->bias_values || !rules->bias_ids != !rules->bias_begin) return Q38B_ERR_ARG;
     if ((rules->mask_of_row && !rules->masks) || (rules->masks && rules->mask_ld < ((long long)index_offset + n + 31) / 32)) return Q38B_ERR_ARG;

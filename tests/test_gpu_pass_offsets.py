@@ -76,3 +76,13 @@ def test_without_an_offset_logits_begin_at_token_zero(ctx):
     ctx.check()
     assert torch.equal(ps.buffer_tensor(a), ctx.adjust_logits(x, **r))
     ps.close()
+
+
+def test_more_logits_than_a_call_takes_are_not_recorded(ctx):
+    ps = q.Pass(ctx, max_nb=1)
+    a = ps.buffer_f32((1 << 30) + 1)
+    with pytest.raises(api.Q38BError) as e:
+        ps.adjust_logits(a, 0, (1 << 30) + 1)
+    assert e.value.status == -2
+    ps.adjust_logits(a, 1, 1 << 30)
+    ps.close()
