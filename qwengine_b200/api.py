@@ -687,6 +687,7 @@ class Pass:
             here = dst == h["buf"]
             return _pack_pass_heads(h["buf"], off, head, dst, h.get("dst_off", off if here else 0), h.get("dst_head", head if here else D), h["n_heads"], 0 if w is None else w.data_ptr())
         rot = 0 if inv_freq is None else 2 * inv_freq.numel()
+        _need(rot == 0 or positions is not None, "qk_norm_rope: positions int32 [max_nb]")
         self.ctx._rc(self.lib.q38b_pass_op_qk_norm_rope(self.h, pack(q, q_weight), None if k is None else pack(k, k_weight), D, rot, int(bool(adjacent)), eps, scale,
                                                         positions.data_ptr() if rot else None, inv_freq.data_ptr() if rot else None), "q38b_pass_op_qk_norm_rope")
         self._keep += [positions, inv_freq, q_weight, k_weight]
