@@ -291,6 +291,73 @@ int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W_codes, long long W_ld, const vo
                     void* stream);
 
 /* ------------------------------------------------------------------------------------------------------------
+ * A paged cache of keys and values, and the attention that reads it.  No counterpart among the reference interfaces above: the reference keeps
+ * both inside its attention layers.  As for the token's own steps: any current device, the caller's stream, nothing allocated, no work area of
+ * the context's.
+ * ------------------------------------------------------------------------------------------------------------ */
+
+/* The cache: element i of head h of slot s of page p at k + (p * k_page + s * k_slot + h * k_head + i), strides in elements, likewise v; 16-bit
+ * elements (kind: Q38B_OUT_F16 or _BF16); base addresses multiples of 16 bytes, strides positive multiples of 8 elements that keep elements apart
+ * (v's may differ from k's).  D: a multiple of 8, at most 256.  page_size: a power of two, at least 8.  n_pages * page_size at most 2^31 - 1.
+ * The batch: n_seqs (1..65535) sequences.  Token j of sequence s lies in slot j % page_size of page table[s * table_ld + j / page_size] (table_ld >=
+ * table_n, the entries of a sequence that may be read); lengths[s]: its tokens in the cache, the chunk's new ones included; begin[s] .. begin[s + 1] - 1:
+ * the chunk's rows that are its new tokens, which are its last ones (int32, n_seqs + 1 of them, ascending from 0 or more).  table, lengths and begin
+ * are device arrays, read when the kernels run.  Lengths past table_n * page_size count as that many; an entry that is no page's number reads as
+ * zeros and is not written to; rows from begin[n_seqs] on are nobody's and left as they are. */
+typedef struct q38b_paged_kv {
+    void* k;
+    void* v;
+    long long k_page, k_slot, k_head, v_page, v_slot, v_head;
+    int kind, n_pages, page_size, n_heads, D, n_seqs;
+    const int* table;
+    long long table_ld;
+    int table_n;
+    const int* lengths;
+    const int* begin;
+} q38b_paged_kv;
+
+/* New keys and values into their places: row begin[s] + i of k and v (in_kind, element e of head h at row * row_stride + h * head_stride + e) to token
+ * lengths[s] - (begin[s + 1] - begin[s]) + i of sequence s, rounded once to the cache's type.  rows: those of k and v (1 and more); a row whose token
+ * would lie before the sequence's first, or behind its last entry, goes nowhere.  Two rows must not go to one place; k and v must not overlap the
+ * cache. */
+int q38b_cache_append(q38b_ctx* ctx, const q38b_paged_kv* cache, const void* k_dev, const void* v_dev, int in_kind, long long k_row, long long k_head,
+                      long long v_row, long long v_head, int rows, void* stream);
+
+/* Attention of the chunk's rows over their sequences: for new token i of sequence s and query head h, which reads key head h / (n_heads / cache->n_heads),
+ *   out = sum_j softmax_j(scale q . k_j) v_j    over the sequence's tokens j <= lengths[s] - new + i
+ * q: q_kind, element e of head h of a row at row * q_row + h * q_head + e; out likewise in out_kind.  n_heads: a multiple of the cache's.  scale > 0,
+ * finite.  fp32 queries are rounded to the cache's type; products and sums in fp32, weights rounded to the cache's type before they multiply values
+ * (2^-8 of each at most in bf16, 2^-11 in fp16), outputs rounded once.  A row that sees no token gives zeros.  A key or value that a row does not
+ * see has no influence on it, whatever it holds.  lse_dev (or NULL): fp32 [rows][n_heads], the natural logarithm of sum_j exp(scale q . k_j),
+ * -infinity where no token is seen.  rows: those of q and out (1 and more).  work: q38b_attention_work_bytes bytes, 16-byte aligned, the caller's, not
+ * shared with a call that may run at the same time.  out must not overlap q or the cache.  The order of the sums depends on the batch and the
+ * device's SM count: the same call gives the same bits on the same device. */
+size_t q38b_attention_work_bytes(const q38b_ctx* ctx, int n_heads, int n_kv_heads, int D, int rows);
+int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* cache, const void* q_dev, int q_kind, long long q_row, long long q_head, int n_heads, float scale,
+                   void* out_dev, int out_kind, long long out_row, long long out_head, float* lse_dev, int rows, void* work_dev, size_t work_bytes,
+                   void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
+ * 8-bit integers with one scale a row: weights with a scale for each output channel, activations with one for each token.  A matrix of `rows` rows of
+ * K values (1..131071, so that no sum of K products passes 32 bits): codes int8 [rows][ld] (ld >= K a multiple of 16, 16-byte aligned), scales
+ * fp32 [rows].
+ * ------------------------------------------------------------------------------------------------------------ */
+/* x (x_kind, x_ld elements between rows) -> codes and scales: scale = the row's largest magnitude / 127 rounded to fp32, at least 2^-126; code = x / scale
+ * rounded half to even, exactly.  A row with a NaN or an infinity gets the scale NaN and codes of zero.  Bytes between K and ld are left as they are.
+ * x, codes and scales must not overlap; rows at most 2^30. */
+int q38b_quantize_i8(q38b_ctx* ctx, const void* x_dev, int x_kind, long long x_ld, int K, int rows, void* codes_dev, long long codes_ld, float* scales_dev,
+                     void* stream);
+/* Y[t * ldy + r] (+)= X_scales[t] W_scales[r] sum_k X[t][k] W[r][k] for t < B, r < M: exact 32-bit integer sums of any int8 codes, scaled in fp32, rounded
+ * once to y_kind (accumulate: added to Y in fp32 first).  Y must not overlap the operands. */
+int q38b_gemm_i8(q38b_ctx* ctx, const void* W_codes, long long W_ld, const float* W_scales, int K, int M, const void* X_codes, long long X_ld,
+                 const float* X_scales, int B, void* Y_dev, int y_kind, long long ldy, int accumulate, void* stream);
+/* The same from activations as they are: x is quantized into `scratch_dev` (16-byte aligned, the caller's, at least q38b_gemm_i8_scratch_bytes(K, B)
+ * bytes) and multiplied; results equal the two calls' bit for bit. */
+size_t q38b_gemm_i8_scratch_bytes(int K, int B);
+int q38b_gemm_i8_x(q38b_ctx* ctx, const void* W_codes, long long W_ld, const float* W_scales, int K, int M, const void* x_dev, int x_kind, long long x_ld,
+                   int B, void* Y_dev, int y_kind, long long ldy, int accumulate, void* scratch_dev, size_t scratch_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------------------
  * All-HBM planner.  Replaces the reference's residency planner and split upload (plan_residency,
  * src/runtime/planner.cpp:91-163; SplitMat / upload_split, src/runtime/engine.h:55-85, engine.cpp:594-629): every
  * matrix is resident in HBM, row-sharded over the ranks (one process per GPU): rank g of G owns rows

@@ -125,6 +125,15 @@ def load_library():
     lib.q38b_debug_set_mx4_pairs.argtypes = [vp, i32]
     lib.q38b_debug_set_mx4_two_launches.argtypes = [vp, i32]
     lib.q38b_gemm_mx4_x.argtypes = [vp, vp, ll, vp, i32, i32, vp, i32, ll, i32, vp, i32, ll, i32, vp, sz, vp]
+    lib.q38b_cache_append.argtypes = [vp, vp, vp, vp, i32, ll, ll, ll, ll, i32, vp]
+    lib.q38b_attention_work_bytes.argtypes = [vp, i32, i32, i32, i32]
+    lib.q38b_attention_work_bytes.restype = sz
+    lib.q38b_attention.argtypes = [vp, vp, vp, i32, ll, ll, i32, C.c_float, vp, i32, ll, ll, vp, i32, vp, sz, vp]
+    lib.q38b_quantize_i8.argtypes = [vp, vp, i32, ll, i32, i32, vp, ll, vp, vp]
+    lib.q38b_gemm_i8.argtypes = [vp, vp, ll, vp, i32, i32, vp, ll, vp, i32, vp, i32, ll, i32, vp]
+    lib.q38b_gemm_i8_scratch_bytes.argtypes = [i32, i32]
+    lib.q38b_gemm_i8_scratch_bytes.restype = sz
+    lib.q38b_gemm_i8_x.argtypes = [vp, vp, ll, vp, i32, i32, vp, i32, ll, i32, vp, i32, ll, i32, vp, sz, vp]
     _LIB = lib
     return lib
 
@@ -142,6 +151,7 @@ def _stream():
 _pack_heads = struct.Struct("@PPqqqqPi4x").pack      # src, dst, src_row, src_head, dst_row, dst_head, weight, n_heads
 _pack_rules = struct.Struct("@PPPPPPPPqP").pack      # penalties .. bias_begin, masks, mask_ld, mask_of_row
 _pack_pass_heads = struct.Struct("@7i4xP").pack      # q38b_pass_heads: src, src_off, src_head, dst, dst_off, dst_head, n_heads, weight
+_pack_paged = struct.Struct("@PPqqqqqqiiiiiiPqi4xPP").pack   # q38b_paged_kv: k, v, strides, kind .. n_seqs, table, table_ld, table_n, lengths, begin
 _empty = torch.empty_strided
 _F32, _F64, _I32, _I64, _U8 = torch.float32, torch.float64, torch.int32, torch.int64, torch.uint8
 _current_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
@@ -170,6 +180,52 @@ class Mx4:
             raise ValueError("Mx4: codes and scales on one device")
         self.codes, self.scales, self.rows, self.K = codes, scales, rows, 2 * half
         self.ld = ld if rows > 1 else half   # (the stride of a single row says nothing)
+
+
+class I8:
+    """A matrix of 8-bit integers with one scale a row: codes int8 [rows, K] (rows a multiple of 16 bytes apart), scales fp32 [rows]
+    (Context.quantize_i8 makes both; another producer's are taken as they are)."""
+    __slots__ = ("codes", "scales", "rows", "K", "ld")
+
+    def __init__(self, codes, scales):
+        rows, K = codes.shape
+        ld, one = codes.stride()
+        if codes.dtype != torch.int8 or (one != 1 and K != 1) or scales.dtype != _F32 or scales.shape != (rows,) or not scales.is_contiguous():
+            raise ValueError("I8: int8 codes [rows, K], elements side by side, and fp32 scales [rows]")
+        if rows < 1 or K < 1 or (rows > 1 and ld % 16):
+            raise ValueError("I8: at least one row and one value, rows a multiple of 16 bytes apart")
+        if codes.get_device() != scales.get_device():
+            raise ValueError("I8: codes and scales on one device")
+        self.codes, self.scales, self.rows, self.K = codes, scales, rows, K
+        self.ld = ld if rows > 1 else (K + 15) // 16 * 16   # (the stride of a single row says nothing)
+
+
+class PagedCache:
+    """Pages of keys and of values, fp16 or bf16 [pages, page_size, heads, D] each (any strides that are multiples of 8 elements, elements of a head side
+    by side): Context.cache_append writes them, Context.attention reads them."""
+    __slots__ = ("k", "v", "n_pages", "page_size", "n_heads", "D", "kind", "_head")
+
+    def __init__(self, k, v):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in (torch.float16, torch.bfloat16) or k.get_device() != v.get_device():
+            raise ValueError("PagedCache: fp16 or bf16 keys and values [pages, page_size, heads, D] of one shape and type, on one device")
+        self.n_pages, self.page_size, self.n_heads, self.D = k.shape
+        if k.stride(3) != 1 or v.stride(3) != 1:
+            raise ValueError("PagedCache: elements of a head side by side")
+        self.k, self.v, self.kind = k, v, _OUT_KINDS[k.dtype]
+        self._head = (k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], self.kind, self.n_pages, self.page_size, self.n_heads, self.D)
+
+    def batch(self, table, lengths, begin):
+        """The bytes of a q38b_paged_kv of these pages and a checked batch: table int32 [sequences, entries], lengths int32 [sequences], begin int32
+        [sequences + 1]."""
+        n, entries = table.shape
+        ld, one = table.stride()
+        dev = self.k.get_device()
+        if (table.dtype != _I32 or lengths.dtype != _I32 or begin.dtype != _I32 or lengths.shape != (n,) or begin.shape != (n + 1,) or (one != 1 and entries != 1) or
+                not lengths.is_contiguous() or not begin.is_contiguous()):
+            raise ValueError("PagedCache: int32 table [sequences, entries], lengths [sequences], begin [sequences + 1]")
+        if table.get_device() != dev or lengths.get_device() != dev or begin.get_device() != dev:
+            raise ValueError("PagedCache: table, lengths and begin on the cache's device")
+        return _pack_paged(*self._head, n, table.data_ptr(), ld if n > 1 else entries, entries, lengths.data_ptr(), begin.data_ptr())
 
 
 class Context:
@@ -519,6 +575,109 @@ class Context:
                                       1 if accumulate else 0, None if scratch is None else scratch.data_ptr(), need, self._stream())
         if rc:
             self._rc(rc, "q38b_gemm_mx4_x")
+        return out
+
+    # ---- a paged cache of keys and values, and the attention over it ----------------------------------
+    def cache_append(self, cache, k, v, table, lengths, begin):
+        """New keys and values [rows, heads, D] (fp32, or the cache's type; any row and head strides) into their places: row begin[s] + i is token
+        lengths[s] - new + i of sequence s, new = begin[s + 1] - begin[s] (lengths count the new tokens)."""
+        rows, heads, D = k.shape
+        dev, kind = self._index, _OUT_KINDS.get(k.dtype)
+        if kind is None or v.dtype != k.dtype or v.shape != k.shape or heads != cache.n_heads or D != cache.D:
+            raise ValueError("cache_append: keys and values [rows, heads, D] of the cache, in fp32 or its type")
+        k_row, k_head, one = k.stride()
+        v_row, v_head, v_one = v.stride()
+        if one != 1 or v_one != 1 or k.get_device() != dev or v.get_device() != dev or cache.k.get_device() != dev:
+            raise ValueError("cache_append: elements side by side, on the context's device")
+        if rows == 0:
+            return
+        rc = self.lib.q38b_cache_append(self.h, cache.batch(table, lengths, begin), k.data_ptr(), v.data_ptr(), kind, k_row, k_head, v_row, v_head, rows, _current_stream(dev))
+        if rc:
+            self._rc(rc, "q38b_cache_append")
+
+    def attention(self, cache, q, table, lengths, begin, scale=None, kind=None, out=None, lse=None):
+        """q [rows, heads, D] (the cache's type, or fp32, which is rounded to it; any row and head strides): softmax(scale q k) v of each row over its
+        sequence's tokens up to its own; scale: D ** -0.5 by default.  kind: OUT_* of the result (q's type by default); lse: fp32 [rows, heads] for the
+        logarithms of the sums.  Rows of no sequence are left as they are in `out` and `lse`."""
+        rows, heads, D = q.shape
+        dev, q_kind = self._index, _OUT_KINDS.get(q.dtype)
+        q_row, q_head, one = q.stride()
+        if q_kind is None or D != cache.D or one != 1 or q.get_device() != dev or cache.k.get_device() != dev:
+            raise ValueError("attention: fp32, fp16 or bf16 queries [rows, heads, D] on the context's device, elements side by side")
+        if out is None:
+            kind = q_kind if kind is None else kind
+            out_row, out_head = heads * D, D
+            out = _empty((rows, heads, D), (out_row, D, 1), dtype=_OUT_DTYPES[kind], device=self.device)
+        else:
+            kind = _OUT_KINDS.get(out.dtype)
+            out_row, out_head, one = out.stride()
+            if kind is None or out.shape != q.shape or one != 1 or out.get_device() != dev:
+                raise ValueError("attention: out shaped like q, elements side by side, on the context's device")
+        if lse is not None and (lse.dtype != _F32 or lse.shape != (rows, heads) or not lse.is_contiguous() or lse.get_device() != dev):
+            raise ValueError("attention: lse fp32 [rows, heads] on the context's device")
+        if rows == 0:
+            return out
+        need = self.lib.q38b_attention_work_bytes(self.h, heads, cache.n_heads, D, rows)
+        work = _empty((need,), (1,), dtype=_U8, device=self.device)
+        rc = self.lib.q38b_attention(self.h, cache.batch(table, lengths, begin), q.data_ptr(), q_kind, q_row, q_head, heads, D ** -0.5 if scale is None else scale, out.data_ptr(),
+                                     kind, out_row, out_head, None if lse is None else lse.data_ptr(), rows, work.data_ptr(), need, _current_stream(dev))
+        if rc:
+            self._rc(rc, "q38b_attention")
+        return out
+
+    # ---- 8-bit integers with one scale a row -----------------------------------------------------------
+    def quantize_i8(self, x):
+        """x [rows, K] (fp32, fp16 or bf16, rows any distance of K and more apart) -> I8."""
+        rows, K = x.shape
+        ld, one = x.stride()
+        kind = _OUT_KINDS.get(x.dtype)
+        if kind is None or (one != 1 and K != 1) or x.get_device() != self._index:
+            raise ValueError("quantize_i8: fp32, fp16 or bf16 [rows, K] on the context's device")
+        if K == 0 or rows == 0:
+            raise Q38BError(-1, "q38b_quantize_i8")
+        pad = (K + 15) // 16 * 16
+        codes = _empty((rows, K), (pad, 1), dtype=torch.int8, device=self.device)
+        scales = _empty((rows,), (1,), dtype=_F32, device=self.device)
+        rc = self.lib.q38b_quantize_i8(self.h, x.data_ptr(), kind, ld if rows > 1 else K, K, rows, codes.data_ptr(), pad, scales.data_ptr(), _current_stream(self._index))
+        if rc:
+            self._rc(rc, "q38b_quantize_i8")
+        m = I8.__new__(I8)   # (made here: nothing to check)
+        m.codes, m.scales, m.rows, m.K, m.ld = codes, scales, rows, K, pad
+        return m
+
+    def gemm_i8(self, W, X, kind=OUT_F32, out=None, accumulate=False):
+        """Y [B, W.rows] = X W^T for W an I8 and X an I8 or activations [B, K] (fp32, fp16 or bf16), which are quantized first.  kind: OUT_* of Y where
+        `out` is not given; accumulate adds to `out`."""
+        _need(out is not None or not accumulate, "gemm_i8: accumulate needs an out to add to")
+        K, M, dev, i8 = W.K, W.rows, self._index, isinstance(X, I8)
+        B = X.rows if i8 else X.shape[0]
+        if W.codes.get_device() != dev or (X.codes if i8 else X).get_device() != dev:
+            raise ValueError("gemm_i8: operands on the context's device")
+        if out is None:
+            ldy = M
+            out = _empty((B, M), (M, 1), dtype=_OUT_DTYPES[kind], device=self.device)
+        else:
+            kind = _OUT_KINDS.get(out.dtype)
+            _need(kind is not None and out.shape == (B, M) and (M == 1 or out.stride(1) == 1) and out.get_device() == dev, "gemm_i8: out [B, W.rows]")
+            ldy = out.stride(0) if B > 1 else M
+        if i8:
+            _need(X.K == K, "gemm_i8: operands of one K")
+            rc = self.lib.q38b_gemm_i8(self.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), K, M, X.codes.data_ptr(), X.ld, X.scales.data_ptr(), B, out.data_ptr(), kind,
+                                       ldy, 1 if accumulate else 0, _current_stream(dev))
+            if rc:
+                self._rc(rc, "q38b_gemm_i8")
+            return out
+        x_kind = _OUT_KINDS.get(X.dtype)
+        B, k = X.shape
+        ld, one = X.stride()
+        if x_kind is None or (one != 1 and K != 1) or k != K or B == 0:
+            raise ValueError("gemm_i8: activations [B, K] of the weights' K")
+        need = B * ((K + 15) // 16 * 16) + (B * 4 + 15) // 16 * 16   # q38b_gemm_i8_scratch_bytes
+        scratch = _empty((need,), (1,), dtype=_U8, device=self.device)
+        rc = self.lib.q38b_gemm_i8_x(self.h, W.codes.data_ptr(), W.ld, W.scales.data_ptr(), K, M, X.data_ptr(), x_kind, ld if B > 1 else K, B, out.data_ptr(), kind, ldy,
+                                     1 if accumulate else 0, scratch.data_ptr(), need, _current_stream(dev))
+        if rc:
+            self._rc(rc, "q38b_gemm_i8_x")
         return out
 
     def topk(self, logits, k, index_offset=0):
