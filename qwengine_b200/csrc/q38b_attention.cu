@@ -2,119 +2,768 @@
 //
 //   out[i][h] = sum_j softmax_j(scale q[i][h] . k[j][h / G]) v[j][h / G],  j <= length - new + i
 //
-// One pass over the keys with the running maximum m and sum l of a softmax: a new maximum scales what was summed before by exp(m_old - m_new).
+// One pass over the keys with the running maximum m and sum l of a softmax.  The (token, head) pairs that read one key head of one sequence are the rows
+// of a tile (128, or 256 in two), so that a group's heads and a chunk's tokens share what is read of the cache; 128 keys at a time:
+//   S = Q K^T       tcgen05.mma, both operands in shared memory, 128 fp32 columns of tensor memory; two such places in turn
+//   P = 2^(S c - m) by a warpgroup, a thread a row, rounded to the cache's type and written over S; c = scale log2(e)
+//   O += P V        tcgen05.mma with P from tensor memory and V as it lies (its keys are the rows of an MN-major operand)
+// The maximum that is taken off lags behind the true one by up to 2^8: O is rescaled in tensor memory only where a row's maximum has grown by
+// more, which after the first tiles of a text is rare.  fp16 weights carry a factor of 2^7 (they end at 2^15), so that what is 2^-31 of the largest
+// still counts.
+//
+// The work is cut for all SMs whatever the batch is: tiles in the order (sequence, key head, rows), each of as many units as it sees tiles of keys, lie one behind the
+// other and every CTA takes an equal range of the units, worked out on the device from the lengths, begins and table as they are when the kernel runs.  A tile of rows that
+// two or more CTAs share leaves its sums in the work area, and a second kernel joins them, in the order of the keys.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <type_traits>
 
 #include "q38b_cache.cuh"
 #include "q38b_internal.h"
 #include "q38b_pipe.cuh"
 #include "q38b_types.cuh"
+#include "q38b_umma.cuh"
 
 using namespace q38b;
 
 namespace {
 
+constexpr int KEYS = 128;                // keys of a tile
+constexpr int BLOCK_BYTES = KEYS * 128;  // 64 elements of 128 rows, 128-byte swizzle
+constexpr float GROWTH = 8.0f;           // how far, in powers of two, a row's maximum may grow before O is rescaled
+
+// A tile of rows that several CTAs share, as the one that begins it leaves it for the joining kernel
+struct Job { int n_parts, first, n_new, len, kv, row0, rows, pad; };
+
 struct AttnArgs {
     Batch batch;
-    const void *q, *k, *v;
+    const void *q, *v;
     void* out;
     float* lse;
-    long long q_row, q_head, out_row, out_head, k_page, k_slot, k_head, v_page, v_slot, v_head;
-    int q_kind, out_kind, n_heads, n_kv, group, D;
-    float scale;
+    float* slots;
+    Job* jobs;
+    int* status;
+    long long q_row, q_head, out_row, out_head, v_page, v_slot, v_head;
+    const void* k;
+    long long k_page, k_slot, k_head;
+    int q_kind, out_kind, n_heads, n_kv, group, D, box_rows, slot_rows, q_vec, out_vec, pdl;
+    float c;       // scale log2(e)
 };
 
-__device__ __forceinline__ float load_kind(const void* p, int kind, long long at) {
-    return kind == Q38B_OUT_F32 ? ((const float*)p)[at] : kind == Q38B_OUT_F16 ? __half2float(((const __half*)p)[at]) : __bfloat162float(((const __nv_bfloat16*)p)[at]);
-}
-__device__ __forceinline__ void store_kind(void* p, int kind, long long at, float v) {
-    if (kind == Q38B_OUT_F32) ((float*)p)[at] = v;
-    else if (kind == Q38B_OUT_F16) ((__half*)p)[at] = __float2half_rn(v);
-    else ((__nv_bfloat16*)p)[at] = __float2bfloat16_rn(v);
-}
+// Shapes of a variant: heads padded to DP elements, QT tiles of 128 rows
+template <int DP, int QT>
+struct Shape {
+    static constexpr int CW = DP % 128 == 0 ? 128 : 64;        // elements of a stage: 128 keys x CW
+    static constexpr int NCH = DP / CW;                        // stages of a tile of keys (or of values)
+    static constexpr int STAGE = KEYS * CW * 2;
+    static constexpr int Q_BYTES = QT * 128 * DP * 2;
+    static constexpr int ROOM = (232448 - 2048 - Q_BYTES) / STAGE;
+    static constexpr int STAGES = ROOM < 12 ? ROOM : 12;
+    static constexpr int SMEM = 1024 + Q_BYTES + STAGES * STAGE;
+    static constexpr int ROWS = QT * 128;
+    static constexpr int THREADS = 64 + 128 * QT;
+    static_assert(256 + QT * DP <= 512, "tensor memory");
+};
 
-// A block: 64 (token, head) pairs of one key head of one sequence, 32 keys at a time through shared memory; four threads a pair.
-constexpr int SR = 64, SK = 32;
-template <typename C>
-__global__ void __launch_bounds__(256) attention_simple_kernel(const AttnArgs a) {
-    extern __shared__ float sm[];
-    const int W = a.D + 1;
-    float *qs = sm, *ks = qs + SR * W, *vs = ks + SK * W, *ps = vs + SK * W;
-    const int s = (int)blockIdx.z, kvh = (int)blockIdx.y;
-    const int first = a.batch.first(s), n_new = max(a.batch.first(s + 1) - first, 0);
-    const int r0 = (int)blockIdx.x * SR, n_rows = n_new * a.group;
-    if (r0 >= n_rows) return;
-    const int len = a.batch.length(s), r = threadIdx.x / 4, c = threadIdx.x % 4;
-    const int mine = r0 + r, tok = mine / a.group, head = kvh * a.group + mine % a.group;
-    const int seen = mine < n_rows ? max(0, len - n_new + tok + 1) : 0;
-    const int last = min(r0 + SR, n_rows) - 1, most = max(0, len - n_new + last / a.group + 1);
-    for (int i = threadIdx.x; i < SR * a.D; i += 256) {
-        const int rr = r0 + i / a.D, e = i % a.D;
-        float x = 0.0f;
-        if (rr < n_rows) x = load_kind(a.q, a.q_kind, (first + rr / a.group) * a.q_row + (kvh * a.group + rr % a.group) * a.q_head + e);
-        qs[i / a.D * W + e] = to_f32(from_f32<C>(x));
-    }
-    float m = -INFINITY, l = 0.0f, acc[64] = {};
-    for (int j0 = 0; j0 < most; j0 += SK) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < SK * a.D; i += 256) {
-            const int j = j0 + i / a.D, e = i % a.D, page = j < most ? a.batch.page(s, j) : a.batch.n_pages;
-            const long long slot = j & ((1 << a.batch.page_shift) - 1);
-            const bool there = page < a.batch.n_pages;
-            ks[i / a.D * W + e] = there ? to_f32(((const C*)a.k)[page * a.k_page + slot * a.k_slot + kvh * a.k_head + e]) : 0.0f;
-            vs[i / a.D * W + e] = there ? to_f32(((const C*)a.v)[page * a.v_page + slot * a.v_slot + kvh * a.v_head + e]) : 0.0f;
-        }
-        __syncthreads();
-        float p[SK / 4], top = m;
-        for (int n = 0; n < SK / 4; n++) {
-            const int j = c * (SK / 4) + n;
-            float dot = 0.0f;
-            for (int e = 0; e < a.D; e++) dot = fmaf(qs[r * W + e], ks[j * W + e], dot);
-            p[n] = j0 + j < seen ? dot * a.scale : -INFINITY;
-            top = fmaxf(top, p[n]);
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const float at = top == -INFINITY ? 0.0f : top, by = __expf(m - at);
-        float sum = 0.0f;
-        for (int n = 0; n < SK / 4; n++) {
-            p[n] = __expf(p[n] - at);
-            sum += p[n];
-            ps[r * SK + c * (SK / 4) + n] = p[n];
-        }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        l = l * by + sum;
-        m = top;
-        __syncwarp();
-        for (int n = 0; n < 64; n++) {
-            const int e = c + 4 * n;
-            if (e >= a.D) break;
-            float x = acc[n] * by;
-            for (int j = 0; j < SK; j++)
-                if (j0 + j < seen) x = fmaf(ps[r * SK + j], vs[j * W + e], x);
-            acc[n] = x;
+// positions of a tile's stages in the ring, in stages behind the item's first: in the order in which the tensor core takes them
+template <int QT, int NCH> __device__ __forceinline__ uint32_t at_keys(int j) { return (uint32_t)((QT == 2 || j == 0 ? 2 * j : 2 * j - 1) * NCH); }
+template <int QT, int NCH> __device__ __forceinline__ uint32_t at_values(int j, int n) { return (uint32_t)((QT == 2 || j == n - 1 ? 2 * j + 1 : 2 * j + 2) * NCH); }
+
+// The walk of a CTA through its range of units.
+struct Walk {
+    int s, first, n_new, len, kv, tile, n_tiles;   // where it is
+    int row0, rows, seen, units;                   // of the tile of rows: first of the sequence's (token, head) rows, how many, keys the last of them sees, tiles of keys
+    int from, to;                                  // of those, this CTA's
+};
+template <int ROWS>
+__device__ __forceinline__ void walk_sequence(const AttnArgs& a, Walk& w) {
+    w.first = a.batch.first(w.s);
+    w.n_new = max(a.batch.first(w.s + 1) - w.first, 0);
+    w.len = a.batch.length(w.s);
+    w.n_tiles = (w.n_new * a.group + ROWS - 1) / ROWS;
+}
+template <int ROWS>
+__device__ __forceinline__ int tile_seen(const Walk& w, int group, int tile) {
+    const int last = (min((tile + 1) * ROWS, w.n_new * group) - 1) / group;   // token
+    return max(0, w.len - w.n_new + last + 1);
+}
+__device__ __forceinline__ int tile_units(int seen) { return max(1, (seen + KEYS - 1) / KEYS); }   // (a tile that sees nothing is one, too: its zeros are written)
+template <int ROWS>
+__device__ __forceinline__ void walk_tile(const AttnArgs& a, Walk& w) {
+    w.row0 = w.tile * ROWS;
+    w.rows = min(ROWS, w.n_new * a.group - w.row0);
+    w.seen = tile_seen<ROWS>(w, a.group, w.tile);
+    w.units = tile_units(w.seen);
+}
+// on to the next tile of rows; `left`: units of the CTA's range that remain.  false: none
+template <int ROWS>
+__device__ __forceinline__ bool walk_next(const AttnArgs& a, Walk& w, long long& left) {
+    left -= w.to - w.from;
+    if (left <= 0) return false;
+    if (++w.tile == w.n_tiles) {
+        w.tile = 0;
+        if (++w.kv == a.n_kv) {
+            w.kv = 0;
+            do {   // (units remain: so does a sequence that has them)
+                if (++w.s >= a.batch.n_seqs) return false;
+                walk_sequence<ROWS>(a, w);
+            } while (w.n_tiles == 0);
         }
     }
-    if (mine >= n_rows) return;
-    const float inv = seen > 0 ? 1.0f / l : 0.0f;
-    for (int n = 0; n < 64; n++)
-        if (c + 4 * n < a.D) store_kind(a.out, a.out_kind, (first + tok) * a.out_row + head * a.out_head + c + 4 * n, seen > 0 ? acc[n] * inv : 0.0f);
-    if (a.lse && c == 0) a.lse[(long long)(first + tok) * a.n_heads + head] = seen > 0 ? m + logf(l) : -INFINITY;
+    walk_tile<ROWS>(a, w);
+    w.from = 0;
+    w.to = (int)min((long long)w.units, left);
+    return true;
 }
 
+// Units of one key head of a sequence, by one thread or by the lanes of a warp together
+template <int ROWS>
+__device__ __forceinline__ long long sequence_units(const AttnArgs& a, const Walk& w, int lane, int lanes) {
+    long long n = 0;
+    for (int t = lane; t < w.n_tiles; t += lanes) n += tile_units(tile_seen<ROWS>(w, a.group, t));
+    return n;
+}
+
+struct Plan {             // in shared memory
+    long long sums[16];
+    long long total, left;
+    Walk walk;
+    int active;           // CTAs with work
+};
+
+// All threads: the batch's units, this CTA's range of them, and the tile of rows it begins in.
+template <int ROWS, int THREADS>
+__device__ __forceinline__ void plan_work(const AttnArgs& a, Plan* p) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int WARPS = THREADS / 32;
+    // few sequences: a warp each, its lanes along the tiles; many: a thread each
+    const bool wide = a.batch.n_seqs <= WARPS;
+    const int per_round = wide ? WARPS : THREADS, rounds = (a.batch.n_seqs + per_round - 1) / per_round;
+    const auto units_of = [&](int s) {
+        Walk w;
+        w.s = s;
+        w.n_tiles = 0;
+        if (s < a.batch.n_seqs) walk_sequence<ROWS>(a, w);
+        if (!wide) return a.n_kv * sequence_units<ROWS>(a, w, 0, 1);
+        long long n = sequence_units<ROWS>(a, w, lane, 32);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
+        return lane == 0 ? a.n_kv * n : 0LL;
+    };
+    long long mine = 0, units = 0;   // units: of the last round
+    for (int r = 0; r < rounds; r++) {
+        units = units_of(r * per_round + (wide ? warp : (int)threadIdx.x));
+        mine += units;
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    if (lane == 0) p->sums[warp] = mine;
+    __syncthreads();
+    long long total = 0;
+    for (int w = 0; w < WARPS; w++) total += p->sums[w];
+    const int active = (int)min((long long)gridDim.x, total), cta = (int)blockIdx.x;
+    if (threadIdx.x == 0) {
+        p->total = total;
+        p->active = active;
+        p->left = 0;
+    }
+    __syncthreads();
+    if (cta >= active) return;
+    const long long begin = total * cta / active, end = total * (cta + 1) / active;
+    long long before = 0;            // units of the rounds before
+    for (int r = 0; r < rounds; r++) {
+        if (rounds > 1) units = units_of(r * per_round + (wide ? warp : (int)threadIdx.x));
+        long long upto = units;      // inclusive sums
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const long long o = __shfl_up_sync(0xffffffffu, upto, d);
+            if (lane >= d) upto += o;
+        }
+        if (lane == 31) p->sums[warp] = upto;
+        __syncthreads();
+        long long base = before;
+        for (int w = 0; w < WARPS; w++) {
+            if (w < warp) base += p->sums[w];
+            before += p->sums[w];
+        }
+        const long long at = base + upto - units;
+        if (units > 0 && begin >= at && begin < at + units) {   // one thread of the block
+            Walk w;
+            w.s = r * per_round + (wide ? warp : (int)threadIdx.x);
+            walk_sequence<ROWS>(a, w);
+            const long long per_head = units / a.n_kv;
+            long long in = begin - at;
+            w.kv = (int)(in / per_head);
+            in -= w.kv * per_head;
+            for (w.tile = 0;; w.tile++) {
+                walk_tile<ROWS>(a, w);
+                if (in < w.units) break;
+                in -= w.units;
+            }
+            w.from = (int)in;
+            w.to = (int)min((long long)w.units, in + (end - begin));
+            p->walk = w;
+            p->left = end - begin;
+        }
+        __syncthreads();
+    }
+}
+
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr) {
+    // MN-major, 128-byte swizzle: a row of 128 bytes is 64 of the operand's N, eight of them (K) a group, groups 1024 bytes apart (SBO); the next 64 of N a
+    // block further (LBO)
+    return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(BLOCK_BYTES >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z),
+                 "r"(w), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+// 16 columns of this warp's 32 rows, on their way until tmem_st_wait
+__device__ __forceinline__ void tmem_st16_start(uint32_t taddr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+        "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+template <typename C> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if constexpr (std::is_same<C, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+template <typename C> constexpr float WEIGHT_BIAS = std::is_same<C, __half>::value ? 7.0f : 0.0f;
+// whether either 16-bit number of a word is an infinity or a NaN
+template <typename C> __device__ __forceinline__ uint32_t no_number(uint32_t w) {
+    constexpr uint32_t E = std::is_same<C, __half>::value ? 0x7C00u : 0x7F80u;
+    return ((w & E) == E ? 0xFFFFu : 0u) | ((w >> 16 & E) == E ? 0xFFFF0000u : 0u);
+}
+template <typename T> __device__ __forceinline__ float load_as(const void* p, long long at) { return to_f32(((const T*)p)[at]); }
+
+// Eight elements of a query as they go to shared memory: rounded to the cache's type
 template <typename C>
-int attention_as(q38b_ctx* ctx, const AttnArgs& a, int rows, cudaStream_t st) {
-    auto kern = attention_simple_kernel<C>;
-    const int smem = ((SR + 2 * SK) * (a.D + 1) + SR * SK) * 4;
+__device__ __forceinline__ uint4 query_eight(const AttnArgs& a, long long at) {
+    uint4 r;
+    if (a.q_kind == Q38B_OUT_F32) {
+        float v[8];
+        const float* p = (const float*)a.q + at;
+        if (a.q_vec) {
+            *(float4*)v = *(const float4*)p;
+            *(float4*)(v + 4) = *(const float4*)(p + 4);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = p[i];
+        }
+        r.x = pack2<C>(v[0], v[1]); r.y = pack2<C>(v[2], v[3]); r.z = pack2<C>(v[4], v[5]); r.w = pack2<C>(v[6], v[7]);
+        return r;
+    }
+    const uint16_t* p = (const uint16_t*)a.q + at;
+    if (a.q_vec) return *(const uint4*)p;
+    uint32_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) h[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+    return make_uint4(h[0], h[1], h[2], h[3]);
+}
+
+// 16 outputs of a row, of which the first `n` are there
+__device__ __forceinline__ void store16(const AttnArgs& a, long long at, const float (&f)[16], int n) {
+    if (a.out_kind == Q38B_OUT_F32) {
+        float* p = (float*)a.out + at;
+        if (a.out_vec) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                if (i < n) *(float4*)(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (i < n) p[i] = f[i];
+        }
+        return;
+    }
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(f[2 * i], f[2 * i + 1]) : pack2<__nv_bfloat16>(f[2 * i], f[2 * i + 1]);
+    uint16_t* p = (uint16_t*)a.out + at;
+    if (a.out_vec) {
+        if (n > 0) *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
+        if (n > 8) *(uint4*)(p + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (i < n) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
+    }
+}
+
+template <typename C, int DP, int QT>
+__global__ void __launch_bounds__(Shape<DP, QT>::THREADS, 1)
+attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
+    using Sh = Shape<DP, QT>;
+    constexpr int CW = Sh::CW, NCH = Sh::NCH, STAGE = Sh::STAGE, STAGES = Sh::STAGES, ROWS = Sh::ROWS;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t* full = (uint64_t*)smem;
+    uint64_t* empty = full + 12;
+    uint64_t* s_full = empty + 12;   // [2] scores are there
+    uint64_t* p_full = s_full + 2;   // [2] weights are there
+    uint64_t* o_done = p_full + 2;   // [QT] weights times values are added
+    uint64_t* q_full = o_done + 2;
+    uint32_t* tmem_slot = (uint32_t*)(q_full + 1);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    volatile int* spoilt = abort_flag + 1;   // [2]: the item that met values that are no numbers among keys that not all of its rows see
+    Plan* plan = (Plan*)(smem + 512);
+    uint8_t* q_at = smem + 1024;
+    uint8_t* ring = q_at + Sh::Q_BYTES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        spoilt[0] = spoilt[1] = -1;
+        for (int s = 0; s < STAGES; s++) {
+            mbar_init(smem_u32(&full[s]), 1);
+            mbar_init(smem_u32(&empty[s]), 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(smem_u32(&s_full[s]), 1);
+            mbar_init(smem_u32(&p_full[s]), 4);
+            mbar_init(smem_u32(&o_done[s]), 1);
+        }
+        mbar_init(smem_u32(q_full), 4 * QT);
+        mbar_fence_init();
+        fence_proxy_async();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    plan_work<ROWS, Sh::THREADS>(a, plan);   // (ends with a barrier of the block)
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *tmem_slot;
+    long long left = plan->left;
+    const bool any = left > 0;
+    Walk w = plan->walk;
+
+    if (any && warp == 0) {
+        // ---------------- keys and values: a lane a box of at most 128 slots x 64 elements ----------------
+        const int boxes = KEYS / a.box_rows, part = lane % boxes, block = lane / boxes;   // lanes behind the last box do nothing
+        const bool mine = block < CW / 64;
+        const uint32_t to = (uint32_t)(block * BLOCK_BYTES + part * a.box_rows * 128), ring_u = smem_u32(ring), full_u = smem_u32(full), empty_u = smem_u32(empty);
+        const int slots = (1 << a.batch.page_shift) - 1;
+        uint32_t at = 0;   // stages filled so far
+        do {
+            const int n = w.to - w.from;
+            const auto page_of = [&](int j) {   // of this lane's box of tile j; keys nobody sees come as zeros, from a page that is not there
+                const int token = (w.from + j) * KEYS + part * a.box_rows;
+                return token < w.seen ? a.batch.page(w.s, token) : a.batch.n_pages;
+            };
+            const auto ask = [&](const CUtensorMap* map, int j, int page) {
+                const int slot = ((w.from + j) * KEYS + part * a.box_rows) & slots;
+#pragma unroll
+                for (int c = 0; c < NCH; c++, at++) {
+                    const uint32_t st = at % STAGES, use = at / STAGES;
+                    mbar_wait_bounded(empty_u + 8u * st, (use & 1u) ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
+                    if (lane == 0) mbar_arrive_expect_tx(full_u + 8u * st, STAGE);
+                    __syncwarp();
+                    if (mine) tma_load_4d(ring_u + st * STAGE + to, map, c * CW + block * 64, slot, w.kv, page, full_u + 8u * st);
+                }
+            };
+            int page_k = page_of(0), page_v = page_k;
+            ask(&kmap, 0, page_k);
+            for (int j = 0; j < n; j++) {
+                if (QT == 2) {
+                    const int next = j + 1 < n ? page_of(j + 1) : 0;
+                    ask(&vmap, j, page_v);
+                    if (j + 1 < n) ask(&kmap, j + 1, next);
+                    page_v = next;
+                } else {
+                    const int next = j + 1 < n ? page_of(j + 1) : 0;
+                    if (j + 1 < n) ask(&kmap, j + 1, next);
+                    ask(&vmap, j, page_v);
+                    page_v = next;
+                }
+            }
+        } while (walk_next<ROWS>(a, w, left));
+    } else if (any && warp == 1) {
+        // ---------------- products ----------------
+        constexpr uint32_t TYPE = std::is_same<C, __half>::value ? 0u : 1u;
+        constexpr uint32_t idesc_s = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        constexpr uint32_t idesc_o = (1u << 4) | (TYPE << 7) | (TYPE << 10) | (1u << 16) | ((uint32_t)(CW >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        const uint64_t kdesc0 = umma_desc_sw128(0), vdesc0 = umma_desc_mn_sw128(0);
+        const uint32_t q_u = smem_u32(q_at), ring_u = smem_u32(ring), full_u = smem_u32(full), empty_u = smem_u32(empty);
+        uint32_t ring0 = 0, p_phase = 0, item = 0;
+        do {
+            const int tiles = w.to - w.from, n = QT * tiles;
+            mbar_wait_bounded(smem_u32(q_full), item & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+            const auto scores = [&](int i) {
+                const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
+                const uint32_t d = tmem + (uint32_t)((i & 1) * KEYS);
+#pragma unroll
+                for (int c = 0; c < NCH; c++) {
+                    const uint32_t at = ring0 + at_keys<QT, NCH>(tile) + c, st = at % STAGES;
+                    mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t qd = kdesc0 + ((q_u + (uint32_t)(t * 128 * DP * 2 + c * CW / 64 * BLOCK_BYTES)) >> 4), kd = kdesc0 + ((ring_u + st * STAGE) >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < CW / 16; k++) {
+                            const uint64_t off = (uint64_t)((k / 4 * BLOCK_BYTES + k % 4 * 32) >> 4);
+                            mma_ss(d, qd + off, kd + off, idesc_s, c > 0 || k > 0 ? 1u : 0u);
+                        }
+                        if (QT == 1 || t == 1) umma_commit<false>(empty_u + 8u * st);
+                        if (c == NCH - 1) umma_commit<false>(smem_u32(&s_full[i & 1]));
+                    }
+                    __syncwarp();
+                }
+            };
+            scores(0);
+            if (n > 1) scores(1);
+            for (int i = 0; i < n; i++) {
+                const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
+                mbar_wait_bounded(smem_u32(&p_full[i & 1]), p_phase >> (i & 1) & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                p_phase ^= 1u << (i & 1);
+#pragma unroll
+                for (int c = 0; c < NCH; c++) {
+                    const uint32_t at = ring0 + at_values<QT, NCH>(tile, tiles) + c, st = at % STAGES;
+                    mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t d = tmem + (uint32_t)(256 + t * DP + c * CW), p = tmem + (uint32_t)((i & 1) * KEYS);
+                    const uint64_t vd = vdesc0 + ((ring_u + st * STAGE) >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < KEYS / 16; k++) mma_ts(d, p + (uint32_t)(8 * k), vd + (uint64_t)(k * 2048 >> 4), idesc_o, k > 0 || tile > 0 ? 1u : 0u);
+                        if (QT == 1 || t == 1) umma_commit<false>(empty_u + 8u * st);
+                        if (c == NCH - 1) umma_commit<false>(smem_u32(&o_done[t]));
+                    }
+                    __syncwarp();
+                }
+                if (i + 2 < n) scores(i + 2);
+            }
+            ring0 += (uint32_t)(2 * tiles * NCH);
+            item++;
+        } while (walk_next<ROWS>(a, w, left));
+    } else if (any) {
+        // ---------------- weights: warpgroup t has the rows of tile t, a thread a row ----------------
+        const int t = QT == 2 ? (warp - 2) >> 2 : 0, quad = warp & 3, row = 128 * t + 32 * quad + lane;   // of the tile of rows
+        const uint32_t lanes = (uint32_t)(32 * quad) << 16;
+        const uint32_t o_tm = tmem + lanes + (uint32_t)(256 + t * DP);
+        const auto load_queries = [&](const Walk& v) {
+            constexpr int UNITS = DP / 8;    // 16-byte pieces of a row
+            uint8_t* to = q_at + t * 128 * DP * 2;
+#pragma unroll 4
+            for (int u = lane; u < 32 * UNITS; u += 32) {
+                const int r = 32 * quad + u / UNITS, e = u % UNITS * 8, flat = v.row0 + 128 * t + r;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (128 * t + r < v.rows && e < a.D) x = query_eight<C>(a, (long long)(v.first + flat / a.group) * a.q_row + (long long)(v.kv * a.group + flat % a.group) * a.q_head + e);
+                *(uint4*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16) = x;
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(q_full));
+        };
+        uint32_t ring0 = 0, s_phase = 0, done = 0;   // done: products P V of this warpgroup's rows so far
+        int item = 0;
+        load_queries(w);
+        bool more = true;
+        while (more) {
+            const int tiles = w.to - w.from;
+            const int tok = (w.row0 + row) / a.group;
+            const int limit = row < w.rows ? max(0, w.len - w.n_new + tok + 1) : w.seen;                          // keys this row sees
+            const int least = max(0, w.len - w.n_new + (w.row0 + min(128 * t + 32 * quad, w.rows - 1)) / a.group + 1);   // ... the warp's first row
+            const int least_item = max(0, w.len - w.n_new + w.row0 / a.group + 1);                                    // ... the item's first row
+            float m = -INFINITY, l = 0.0f;   // m: what is taken off, times c
+            for (int i = 0; i < tiles; i++) {
+                const int slot = QT == 2 ? t : i & 1, j0 = (w.from + i) * KEYS;
+                const uint32_t s_tm = tmem + lanes + (uint32_t)(slot * KEYS);
+                mbar_wait_bounded(smem_u32(&s_full[slot]), s_phase >> slot & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+                s_phase ^= 1u << slot;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t v[KEYS];
+#pragma unroll
+                for (int k = 0; k < KEYS; k += 16) tmem_ld16_start(s_tm + (uint32_t)k, v + k);
+                tmem_ld_wait();
+#pragma unroll
+                for (int k = 0; k < KEYS; k += 16) tmem_ld_arrived(v + k);
+                if (j0 + KEYS > least) {
+                    const int n = limit - j0;
+#pragma unroll
+                    for (int k = 0; k < KEYS; k++) v[k] = k < n ? v[k] : 0xFF800000u;
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int k = 0; k < KEYS; k++) top = fmaxf(top, __uint_as_float(v[k]));
+                top *= a.c;
+                if (i == 0) {
+                    m = top;
+                } else if (__any_sync(0xffffffffu, top > m + GROWTH)) {
+                    const float now = fmaxf(m, top), by = now == -INFINITY ? 1.0f : exp2_fast(m - now);
+                    mbar_wait_bounded(smem_u32(&o_done[t]), (done - 1) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                    for (int k = 0; k < DP; k += 16) {
+                        uint32_t o[16];
+                        tmem_ld16(o_tm + (uint32_t)k, o);
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+                        tmem_st16_start(o_tm + (uint32_t)k, o);
+                    }
+                    l *= by;
+                    m = now;
+                }
+                const float off = (m == -INFINITY ? 0.0f : -m) + WEIGHT_BIAS<C>;
+                float sum[4] = {};
+#pragma unroll
+                for (int k = 0; k < KEYS; k += 2) {
+                    const float p = exp2_fast(fmaf(__uint_as_float(v[k]), a.c, off)), r = exp2_fast(fmaf(__uint_as_float(v[k + 1]), a.c, off));
+                    sum[k / 2 % 2 * 2] += p;
+                    sum[k / 2 % 2 * 2 + 1] += r;
+                    v[k / 2] = pack2<C>(p, r);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+                for (int k = 0; k < KEYS / 2; k += 16) tmem_st16_start(s_tm + (uint32_t)k, v + k);
+                // Values of slots behind the last key that is seen may be anything, and so may values that some of the rows do not see: no product with
+                // a weight of zero takes them away if they are no numbers.
+                if (j0 + KEYS > least_item) {
+                    const int seen = w.seen - j0, rest = min(KEYS, (seen + a.box_rows - 1) / a.box_rows * a.box_rows);   // slots from `seen` to `rest` came with a page
+                    const bool some = least_item < w.seen;
+#pragma unroll 1
+                    for (int c = 0; c < NCH; c++) {
+                        const uint32_t at = ring0 + at_values<QT, NCH>(i, tiles) + c, st = at % STAGES;
+                        mbar_wait_bounded(smem_u32(&full[st]), at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                        uint8_t* p = ring + st * STAGE;
+                        for (int u = 32 * quad + lane; u < CW / 8 * KEYS; u += 128) {
+                            const int j = u % (8 * KEYS) / 8;   // 16-byte pieces lie in rows of eight
+                            if (j >= rest || (j < seen && !some)) continue;
+                            uint4* x = (uint4*)p + u;
+                            if (j >= seen) {
+                                *x = make_uint4(0, 0, 0, 0);
+                                continue;
+                            }
+                            uint4 y = *x;
+                            const uint4 bad = make_uint4(no_number<C>(y.x), no_number<C>(y.y), no_number<C>(y.z), no_number<C>(y.w));
+                            if (bad.x | bad.y | bad.z | bad.w) {
+                                spoilt[item & 1] = item;
+                                __threadfence_block();   // (whoever finds these zeros finds the mark too)
+                                *x = make_uint4(y.x & ~bad.x, y.y & ~bad.y, y.z & ~bad.z, y.w & ~bad.w);
+                            }
+                        }
+                    }
+                    fence_proxy_async();
+                }
+                tmem_st_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&p_full[slot]));
+                done++;
+            }
+            ring0 += (uint32_t)(2 * tiles * NCH);
+            // the next item's queries go in place before this one's outputs leave (its scores are all done)
+            const Walk now = w;
+            const bool was_spoilt_item = least_item < now.seen;
+            mbar_wait_bounded(smem_u32(&o_done[t]), (done - 1) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (was_spoilt_item && spoilt[item & 1] == item) {
+                // Rare: what was taken out of the products goes to the rows that see it, a value at a time.
+                const int lo = max(least_item / KEYS * KEYS, now.from * KEYS), hi = min(now.seen, now.to * KEYS);
+                const uint8_t* q_row = q_at + t * 128 * DP * 2;
+                const int r = row - 128 * t;
+                for (int j = lo; j < hi; j++) {
+                    const int page = a.batch.page(now.s, j);
+                    if (page >= a.batch.n_pages) continue;
+                    const long long in = j & ((1 << a.batch.page_shift) - 1);
+                    const long long v_at = page * a.v_page + in * a.v_slot + now.kv * a.v_head, k_at = page * a.k_page + in * a.k_slot + now.kv * a.k_head;
+                    float weight = 0.0f;
+                    bool known = false;
+                    for (int e = 0; e < a.D; e++) {
+                        const float x = load_as<C>(a.v, v_at + e);
+                        if (fabsf(x) < INFINITY) continue;
+                        if (!known) {
+                            float dot = 0.0f;
+                            for (int d = 0; d < a.D; d++)
+                                dot = fmaf(to_f32(*(const C*)(q_row + d / 64 * BLOCK_BYTES + r * 128 + ((d % 64 / 8) ^ (r & 7)) * 16 + d % 8 * 2)), load_as<C>(a.k, k_at + d), dot);
+                            weight = exp2_fast(fmaf(dot, a.c, (m == -INFINITY ? 0.0f : -m) + WEIGHT_BIAS<C>));
+                            known = true;
+                        }
+                        uint32_t o;
+                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(o_tm + (uint32_t)e) : "memory");
+                        tmem_ld_wait();
+                        asm volatile("" : "+r"(o));
+                        if (j < limit) o = __float_as_uint(fmaf(weight, x, __uint_as_float(o)));
+                        asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(o_tm + (uint32_t)e), "r"(o) : "memory");
+                        tmem_st_wait();
+                    }
+                }
+                __syncwarp();
+            }
+            more = walk_next<ROWS>(a, w, left);
+            if (more) load_queries(w);
+            const bool whole = now.from == 0 && now.to == now.units;
+            const int flat = now.row0 + row, head = now.kv * a.group + flat % a.group;
+            const long long out_row = now.first + flat / a.group;
+            if (whole) {
+                const float by = limit > 0 ? 1.0f / l : 0.0f;
+#pragma unroll 1
+                for (int k = 0; k < DP; k += 16) {
+                    uint32_t o[16];
+                    float f[16];
+                    tmem_ld16(o_tm + (uint32_t)k, o);
+#pragma unroll
+                    for (int e = 0; e < 16; e++) f[e] = limit > 0 ? __uint_as_float(o[e]) * by : 0.0f;
+                    if (row < now.rows && k < a.D) store16(a, out_row * a.out_row + (long long)head * a.out_head + k, f, a.D - k);
+                }
+                if (a.lse && row < now.rows) a.lse[out_row * a.n_heads + head] = limit > 0 ? 0.6931471805599453f * (m + log2f(l) - WEIGHT_BIAS<C>) : -INFINITY;
+            } else {
+                // a place in the work area: [4 columns][row] and each row's m and l behind
+                float* to = a.slots + (long long)(2 * blockIdx.x + (now.from == 0 ? 1 : 0)) * a.slot_rows * (DP + 4);
+#pragma unroll 1
+                for (int k = 0; k < DP; k += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(o_tm + (uint32_t)k, o);
+                    if (row < now.rows)
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) *(uint4*)(to + (long long)((k + e) / 4 * a.slot_rows + row) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                }
+                if (row < now.rows) *(float2*)(to + (long long)a.slot_rows * DP + 2 * row) = make_float2(m, l);
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            item++;
+        }
+    }
+    // The last tile of rows, if others go on with it, is this CTA's to announce: its parts are this CTA's and those of the CTAs up to the one with its last unit.
+    if (threadIdx.x == 64) {
+        Job job = {};
+        if (any) {
+            const long long total = plan->total, end = total * (blockIdx.x + 1) / plan->active;
+            if (w.from == 0 && w.to < w.units) {
+                const long long last = end + (w.units - w.to) - 1;   // its last unit
+                job.n_parts = (int)(((last + 1) * plan->active - 1) / total) - (int)blockIdx.x + 1;
+                job.first = w.first;
+                job.n_new = w.n_new;
+                job.len = w.len;
+                job.kv = w.kv;
+                job.row0 = w.row0;
+                job.rows = w.rows;
+            }
+        }
+        a.jobs[blockIdx.x] = job;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (a.pdl) pdl_launch_dependents();
+    if (warp == 1) {
+        if (__builtin_expect(*abort_flag, 0)) settle_after_abort();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// Joins the parts of a tile of rows: a thread four elements of a row.
+template <int DP>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, float bias) {
+    if (a.pdl) pdl_wait_prior();
+    const Job job = a.jobs[blockIdx.x];
+    const int at = (int)(blockIdx.y * 256 + threadIdx.x), row = at / (DP / 4), e = at % (DP / 4) * 4;
+    if (job.n_parts == 0 || row >= job.rows) return;
+    const long long slot = (long long)a.slot_rows * (DP + 4);
+    const auto place = [&](int p) { return a.slots + (p == 0 ? 2 * (long long)blockIdx.x + 1 : 2 * ((long long)blockIdx.x + p)) * slot; };
+    float top = -INFINITY;
+    for (int p = 0; p < job.n_parts; p++) top = fmaxf(top, place(p)[(long long)a.slot_rows * DP + 2 * row]);
+    const float off = top == -INFINITY ? 0.0f : top;
+    float l = 0.0f, o[4] = {};
+#pragma unroll 4
+    for (int p = 0; p < job.n_parts; p++) {
+        const float* s = place(p);
+        const float2 ml = *(const float2*)(s + (long long)a.slot_rows * DP + 2 * row);
+        const float4 x = *(const float4*)(s + (long long)(e / 4 * a.slot_rows + row) * 4);
+        const float by = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - off);
+        l = fmaf(by, ml.y, l);
+        o[0] = fmaf(by, x.x, o[0]);
+        o[1] = fmaf(by, x.y, o[1]);
+        o[2] = fmaf(by, x.z, o[2]);
+        o[3] = fmaf(by, x.w, o[3]);
+    }
+    const int flat = job.row0 + row, head = job.kv * a.group + flat % a.group;
+    const long long out_row = job.first + flat / a.group;
+    const bool sees = job.len - job.n_new + flat / a.group + 1 > 0;
+    const float by = 1.0f / l;
+    if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (off + log2f(l) - bias) : -INFINITY;
+    if (e >= a.D) return;
+#pragma unroll
+    for (int i = 0; i < 4; i++) o[i] = sees ? o[i] * by : 0.0f;
+    const long long to = out_row * a.out_row + (long long)head * a.out_head + e;
+    if (a.out_kind == Q38B_OUT_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) ((float*)a.out)[to + i] = o[i];
+    } else {
+        const uint32_t lo = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(o[0], o[1]) : pack2<__nv_bfloat16>(o[0], o[1]);
+        const uint32_t hi = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(o[2], o[3]) : pack2<__nv_bfloat16>(o[2], o[3]);
+        uint16_t* p = (uint16_t*)a.out + to;
+        if (a.out_vec) {
+            *(uint2*)p = make_uint2(lo, hi);
+        } else {
+            p[0] = (uint16_t)lo; p[1] = (uint16_t)(lo >> 16); p[2] = (uint16_t)hi; p[3] = (uint16_t)(hi >> 16);
+        }
+    }
+}
+
+bool encode_pages(CUtensorMap* map, const q38b_paged_kv* c, const void* base, long long page, long long slot, long long head, int box_rows) {
+    const cuuint64_t dims[4] = {(cuuint64_t)c->D, (cuuint64_t)c->page_size, (cuuint64_t)c->n_heads, (cuuint64_t)c->n_pages};
+    // (the stride of one head or one page is never used: any that is allowed)
+    const cuuint64_t strides[3] = {(cuuint64_t)slot * 2, (cuuint64_t)(c->n_heads > 1 ? head : slot) * 2, (cuuint64_t)(c->n_pages > 1 ? page : slot) * 2};
+    const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
+    EncodeTiledFn enc = encode_fn();
+    return enc && enc(map, c->kind == Q38B_OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int padded(int D) { return (D + 63) / 64 * 64; }
+// rows of a place in the work area
+int slot_rows(int group, int D, int rows) { return (int)std::min((long long)(padded(D) <= 128 ? 256 : 128), (long long)rows * group); }
+
+template <typename C, int DP, int QT>
+int attention_as(q38b_ctx* ctx, const AttnArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t st) {
+    auto kern = attention_kernel<C, DP, QT>;
     const int rc = q38b_ensure_kernel_smem(ctx, (const void*)kern, ctx->smem_optin, false);
     if (rc != Q38B_OK) return rc;
-    kern<<<dim3((unsigned)(((long long)rows * a.group + SR - 1) / SR), (unsigned)a.n_kv, (unsigned)a.batch.n_seqs), 256, smem, st>>>(a);
-    return launch_status(ctx, cudaSuccess);
+    kern<<<(unsigned)ctx->sm_count, Shape<DP, QT>::THREADS, Shape<DP, QT>::SMEM, st>>>(a, kmap, vmap);
+    const int done = launch_status(ctx, cudaSuccess);
+    if (done != Q38B_OK) return done;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)ctx->sm_count, (unsigned)((std::min(a.slot_rows, Shape<DP, QT>::ROWS) * (DP / 4) + 255) / 256));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.pdl ? 1 : 0;
+    return launch_status(ctx, cudaLaunchKernelEx(&cfg, attention_join_kernel<DP>, a, WEIGHT_BIAS<C>));
+}
+template <typename C>
+int attention_for(q38b_ctx* ctx, const AttnArgs& a, bool two, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t st) {
+    switch (padded(a.D)) {
+        case 64: return two ? attention_as<C, 64, 2>(ctx, a, kmap, vmap, st) : attention_as<C, 64, 1>(ctx, a, kmap, vmap, st);
+        case 128: return two ? attention_as<C, 128, 2>(ctx, a, kmap, vmap, st) : attention_as<C, 128, 1>(ctx, a, kmap, vmap, st);
+        case 192: return attention_as<C, 192, 1>(ctx, a, kmap, vmap, st);
+        default: return attention_as<C, 256, 1>(ctx, a, kmap, vmap, st);
+    }
 }
 
 bool known_kind(int kind) { return kind == Q38B_OUT_F32 || kind == Q38B_OUT_F16 || kind == Q38B_OUT_BF16; }
@@ -124,7 +773,10 @@ int kind_size(int kind) { return kind == Q38B_OUT_F32 ? 4 : 2; }
 
 extern "C" {
 
-size_t q38b_attention_work_bytes(const q38b_ctx* ctx, int n_heads, int n_kv_heads, int D, int rows) { return 16; }
+size_t q38b_attention_work_bytes(const q38b_ctx* ctx, int n_heads, int n_kv_heads, int D, int rows) {
+    if (!ctx || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads || D < 8 || D > 256 || D % 8 || rows < 1) return 0;
+    return (size_t)ctx->sm_count * (sizeof(Job) + 2 * (size_t)slot_rows(n_heads / n_kv_heads, D, rows) * (padded(D) + 4) * 4);
+}
 
 int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_kind, long long q_row, long long q_head, int n_heads, float scale, void* out,
                    int out_kind, long long out_row, long long out_head, float* lse, int rows, void* work, size_t work_bytes, void* stream) {
@@ -134,12 +786,31 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     if (n_heads < 1 || n_heads % c->n_heads || q_row < 0 || q_head < 0 || out_row < 0 || out_head < 0) return Q38B_ERR_ARG;
     if ((n_heads > 1 && out_head < c->D) || (rows > 1 && out_row < c->D)) return Q38B_ERR_ARG;
     if (q_kind != Q38B_OUT_F32 && q_kind != c->kind) return Q38B_ERR_UNSUPPORTED;
+    if ((long long)rows * n_heads > 0x3FFFFFFF) return Q38B_ERR_UNSUPPORTED;
     if ((uintptr_t)q % kind_size(q_kind) || (uintptr_t)out % kind_size(out_kind) || ((uintptr_t)lse & 3) || ((uintptr_t)work & 15)) return Q38B_ERR_ALIGN;
-    if (work_bytes < q38b_attention_work_bytes(ctx, n_heads, c->n_heads, c->D, rows)) return Q38B_ERR_NOMEM;
+    if (work_bytes < 16 || work_bytes < q38b_attention_work_bytes(ctx, n_heads, c->n_heads, c->D, rows)) return Q38B_ERR_NOMEM;
     DeviceGuard on(ctx);
-    const AttnArgs a = {batch_of(c, rows), q, c->k, c->v, out, lse, q_row, q_head, out_row, out_head, c->k_page, c->k_slot, c->k_head, c->v_page, c->v_slot, c->v_head,
-                        q_kind, out_kind, n_heads, c->n_heads, n_heads / c->n_heads, c->D, scale};
-    return c->kind == Q38B_OUT_F16 ? attention_as<__half>(ctx, a, rows, (cudaStream_t)stream) : attention_as<__nv_bfloat16>(ctx, a, rows, (cudaStream_t)stream);
+    AttnArgs a;
+    memset(&a, 0, sizeof(a));
+    a.batch = batch_of(c, rows);
+    a.q = q; a.k = c->k; a.v = c->v; a.out = out; a.lse = lse;
+    a.q_row = q_row; a.q_head = q_head; a.out_row = out_row; a.out_head = out_head;
+    a.k_page = c->k_page; a.k_slot = c->k_slot; a.k_head = c->k_head; a.v_page = c->v_page; a.v_slot = c->v_slot; a.v_head = c->v_head;
+    a.q_kind = q_kind; a.out_kind = out_kind; a.n_heads = n_heads; a.n_kv = c->n_heads; a.group = n_heads / c->n_heads; a.D = c->D;
+    a.box_rows = std::min(c->page_size, KEYS);
+    a.slot_rows = slot_rows(a.group, c->D, rows);
+    a.jobs = (Job*)work;
+    a.slots = (float*)((uint8_t*)work + (size_t)ctx->sm_count * sizeof(Job));
+    a.status = ctx->d_status;
+    a.q_vec = (((uintptr_t)q | (uintptr_t)(q_row * kind_size(q_kind)) | (uintptr_t)(q_head * kind_size(q_kind))) & 15) == 0;
+    a.out_vec = (((uintptr_t)out | (uintptr_t)(out_row * kind_size(out_kind)) | (uintptr_t)(out_head * kind_size(out_kind))) & 15) == 0;
+    a.pdl = ctx->pass_pdl ? 1 : 0;
+    a.c = (float)((double)scale * 1.4426950408889634);
+    CUtensorMap kmap, vmap;
+    if (!encode_pages(&kmap, c, c->k, c->k_page, c->k_slot, c->k_head, a.box_rows) || !encode_pages(&vmap, c, c->v, c->v_page, c->v_slot, c->v_head, a.box_rows)) return Q38B_ERR_ARG;
+    // two tiles of rows share the keys' way into shared memory where sequences fill more than one on average
+    const bool two = (long long)rows * a.group > 128LL * c->n_seqs;
+    return c->kind == Q38B_OUT_F16 ? attention_for<__half>(ctx, a, two, kmap, vmap, (cudaStream_t)stream) : attention_for<__nv_bfloat16>(ctx, a, two, kmap, vmap, (cudaStream_t)stream);
 }
 
 }  // extern "C"
