@@ -5,7 +5,7 @@
 // One pass over the keys with the running maximum m and sum l of a softmax.  The (token, head) pairs that read one key head of one sequence are the rows
 // of a tile (128, or 256 in two), so that a group's heads and a chunk's tokens share what is read of the cache; 128 keys at a time:
 //   S = Q K^T       tcgen05.mma, both operands in shared memory, 128 fp32 columns of tensor memory; two such places in turn
-//   P = 2^(S c - m) by a warpgroup, a thread a row, rounded to the cache's type and written over S; c = scale log2(e)
+//   P = 2^(S c - m) by a warpgroup, a thread a row, rounded to the cache's type and written over S; c = scale log2(e).  Two warpgroups take turns: S has two places
 //   O += P V        tcgen05.mma with P from tensor memory and V as it lies (its keys are the rows of an MN-major operand)
 // The maximum that is taken off lags behind the true one by up to 2^8: O is rescaled in tensor memory only where a row's maximum has grown by
 // more, which after the first tiles of a text is rare.  fp16 weights carry a factor of 2^7 (they end at 2^15), so that what is 2^-31 of the largest
@@ -35,6 +35,7 @@ namespace {
 
 constexpr int KEYS = 128;                // keys of a tile
 constexpr int BLOCK_BYTES = KEYS * 128;  // 64 elements of 128 rows, 128-byte swizzle
+constexpr int HEAD = 7168;               // shared memory in front of the queries: barriers, the plan, maxima and sums of rows
 constexpr float GROWTH = 8.0f;           // how far, in powers of two, a row's maximum may grow before O is rescaled
 
 // A tile of rows that several CTAs share, as the one that begins it leaves it for the joining kernel
@@ -62,11 +63,11 @@ struct Shape {
     static constexpr int NCH = DP / CW;                        // stages of a tile of keys (or of values)
     static constexpr int STAGE = KEYS * CW * 2;
     static constexpr int Q_BYTES = QT * 128 * DP * 2;
-    static constexpr int ROOM = (232448 - 2048 - Q_BYTES) / STAGE;
+    static constexpr int ROOM = (232448 - HEAD - Q_BYTES) / STAGE;
     static constexpr int STAGES = ROOM < 12 ? ROOM : 12;
-    static constexpr int SMEM = 1024 + Q_BYTES + STAGES * STAGE;
+    static constexpr int SMEM = HEAD + Q_BYTES + STAGES * STAGE;
     static constexpr int ROWS = QT * 128;
-    static constexpr int THREADS = 64 + 128 * QT;
+    static constexpr int THREADS = 64 + 256;                  // a warp loads, a warp multiplies, two warpgroups make weights
     static_assert(256 + QT * DP <= 512, "tensor memory");
 };
 
@@ -243,6 +244,27 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// two floats in 64 bits, and operations on both
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 template <typename C> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
     if constexpr (std::is_same<C, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -321,13 +343,16 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     uint64_t* empty = full + 12;
     uint64_t* s_full = empty + 12;   // [2] scores are there
     uint64_t* p_full = s_full + 2;   // [2] weights are there
-    uint64_t* o_done = p_full + 2;   // [QT] weights times values are added
-    uint64_t* q_full = o_done + 2;
+    uint64_t* o_done = p_full + 2;   // [2] ... have been multiplied with values
+    uint64_t* m_full = o_done + 2;   // [2][4] QT = 1: the maxima that a warp of either warpgroup took off are known to the other
+    uint64_t* q_full = m_full + 8;
     uint32_t* tmem_slot = (uint32_t*)(q_full + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     volatile int* spoilt = abort_flag + 1;   // [2]: the item that met values that are no numbers among keys that not all of its rows see
     Plan* plan = (Plan*)(smem + 512);
-    uint8_t* q_at = smem + 1024;
+    float* m_rows = (float*)(smem + 1024);       // [2][128]
+    float2* ml_rows = (float2*)(smem + 2048);    // [2][2][128]
+    uint8_t* q_at = smem + HEAD;
     uint8_t* ring = q_at + Sh::Q_BYTES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -343,7 +368,8 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             mbar_init(smem_u32(&p_full[s]), 4);
             mbar_init(smem_u32(&o_done[s]), 1);
         }
-        mbar_init(smem_u32(q_full), 4 * QT);
+        for (int s = 0; s < 8; s++) mbar_init(smem_u32(&m_full[s]), 1);
+        mbar_init(smem_u32(q_full), 8);
         mbar_fence_init();
         fence_proxy_async();
     }
@@ -448,7 +474,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
 #pragma unroll
                         for (int k = 0; k < KEYS / 16; k++) mma_ts(d, p + (uint32_t)(8 * k), vd + (uint64_t)(k * 2048 >> 4), idesc_o, k > 0 || tile > 0 ? 1u : 0u);
                         if (QT == 1 || t == 1) umma_commit<false>(empty_u + 8u * st);
-                        if (c == NCH - 1) umma_commit<false>(smem_u32(&o_done[t]));
+                        if (c == NCH - 1) umma_commit<false>(smem_u32(&o_done[i & 1]));
                     }
                     __syncwarp();
                 }
@@ -458,15 +484,19 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             item++;
         } while (walk_next<ROWS>(a, w, left));
     } else if (any) {
-        // ---------------- weights: warpgroup t has the rows of tile t, a thread a row ----------------
-        const int t = QT == 2 ? (warp - 2) >> 2 : 0, quad = warp & 3, row = 128 * t + 32 * quad + lane;   // of the tile of rows
-        const uint32_t lanes = (uint32_t)(32 * quad) << 16;
-        const uint32_t o_tm = tmem + lanes + (uint32_t)(256 + t * DP);
+        // ---------------- weights: warpgroup g takes the scores that lie in place g, a thread a row ----------------
+        // QT = 2: those of its own 128 rows.  QT = 1: those of every other tile of keys; the maxima go from one warpgroup to the other, and each has a sum of its own.
+        const int g = (warp - 2) >> 2, quad = warp & 3, t = QT == 2 ? g : 0, row = 128 * t + 32 * quad + lane;   // row: of the tile of rows
+        const uint32_t lanes = (uint32_t)(32 * quad) << 16, o_tm = tmem + lanes + (uint32_t)(256 + t * DP), s_tm = tmem + lanes + (uint32_t)(g * KEYS);
+        const uint32_t s_bar = smem_u32(&s_full[g]), p_bar = smem_u32(&p_full[g]), done_u = smem_u32(o_done);
+        constexpr int COLS = QT == 2 ? DP : DP / 2;     // of the outputs this warpgroup stores
+        const int col0 = QT == 2 ? 0 : g * COLS;
         const auto load_queries = [&](const Walk& v) {
-            constexpr int UNITS = DP / 8;    // 16-byte pieces of a row
+            constexpr int UNITS = DP / 8, ALL = 32 * UNITS, SHARE = QT == 2 ? ALL : ALL / 2;    // 16-byte pieces of a row, of the warp's rows, of those its own
             uint8_t* to = q_at + t * 128 * DP * 2;
+            const int first = QT == 2 ? 0 : g * SHARE;
 #pragma unroll 4
-            for (int u = lane; u < 32 * UNITS; u += 32) {
+            for (int u = first + lane; u < first + SHARE; u += 32) {
                 const int r = 32 * quad + u / UNITS, e = u % UNITS * 8, flat = v.row0 + 128 * t + r;
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (128 * t + r < v.rows && e < a.D) x = query_eight<C>(a, (long long)(v.first + flat / a.group) * a.q_row + (long long)(v.kv * a.group + flat % a.group) * a.q_head + e);
@@ -476,67 +506,101 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(q_full));
         };
-        uint32_t ring0 = 0, s_phase = 0, done = 0;   // done: products P V of this warpgroup's rows so far
+        uint32_t ring0 = 0, s_use = 0, m_use = 0, done[2] = {0, 0};   // done: products P V from either place up to this item
         int item = 0;
         load_queries(w);
         bool more = true;
         while (more) {
-            const int tiles = w.to - w.from;
+            const int tiles = w.to - w.from, n = QT * tiles;
             const int tok = (w.row0 + row) / a.group;
             const int limit = row < w.rows ? max(0, w.len - w.n_new + tok + 1) : w.seen;                          // keys this row sees
             const int least = max(0, w.len - w.n_new + (w.row0 + min(128 * t + 32 * quad, w.rows - 1)) / a.group + 1);   // ... the warp's first row
             const int least_item = max(0, w.len - w.n_new + w.row0 / a.group + 1);                                    // ... the item's first row
+            const bool idle = 128 * t + 32 * quad >= w.rows;   // no row of this warp's is there
             float m = -INFINITY, l = 0.0f;   // m: what is taken off, times c
-            for (int i = 0; i < tiles; i++) {
-                const int slot = QT == 2 ? t : i & 1, j0 = (w.from + i) * KEYS;
-                const uint32_t s_tm = tmem + lanes + (uint32_t)(slot * KEYS);
-                mbar_wait_bounded(smem_u32(&s_full[slot]), s_phase >> slot & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
-                s_phase ^= 1u << slot;
+            for (int i = g; i < n; i += 2) {
+                const int tile = QT == 2 ? i >> 1 : i, j0 = (w.from + tile) * KEYS;
+                mbar_wait_bounded(s_bar, s_use & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+                s_use++;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t v[KEYS];
+                if (!idle) {
+                    // a half of the scores at a time (all of a row's in registers spilled a fifth of them); the first stays for the weights
+                    constexpr int HALF = KEYS / 2;
+                    uint32_t v[HALF];
+                    const int seen = limit - j0;
+                    const bool masked = j0 + KEYS > least;
+                    const auto load_half = [&](int h) {
 #pragma unroll
-                for (int k = 0; k < KEYS; k += 16) tmem_ld16_start(s_tm + (uint32_t)k, v + k);
-                tmem_ld_wait();
+                        for (int k = 0; k < HALF; k += 16) tmem_ld16_start(s_tm + (uint32_t)(h * HALF + k), v + k);
+                        tmem_ld_wait();
 #pragma unroll
-                for (int k = 0; k < KEYS; k += 16) tmem_ld_arrived(v + k);
-                if (j0 + KEYS > least) {
-                    const int n = limit - j0;
+                        for (int k = 0; k < HALF; k += 16) tmem_ld_arrived(v + k);
+                        if (masked)
 #pragma unroll
-                    for (int k = 0; k < KEYS; k++) v[k] = k < n ? v[k] : 0xFF800000u;
-                }
-                float top = -INFINITY;
+                            for (int k = 0; k < HALF; k++) v[k] = h * HALF + k < seen ? v[k] : 0xFF800000u;
+                    };
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < KEYS; k++) top = fmaxf(top, __uint_as_float(v[k]));
-                top *= a.c;
-                if (i == 0) {
-                    m = top;
-                } else if (__any_sync(0xffffffffu, top > m + GROWTH)) {
-                    const float now = fmaxf(m, top), by = now == -INFINITY ? 1.0f : exp2_fast(m - now);
-                    mbar_wait_bounded(smem_u32(&o_done[t]), (done - 1) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-                    for (int k = 0; k < DP; k += 16) {
-                        uint32_t o[16];
-                        tmem_ld16(o_tm + (uint32_t)k, o);
+                    for (int h = 1; h >= 0; h--) {
+                        load_half(h);
 #pragma unroll
-                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
-                        tmem_st16_start(o_tm + (uint32_t)k, o);
+                        for (int k = 0; k < HALF; k += 8)
+#pragma unroll
+                            for (int x = 0; x < 4; x++) top[x] = fmaxf(fmaxf(top[x], __uint_as_float(v[k + 2 * x])), __uint_as_float(v[k + 2 * x + 1]));
                     }
-                    l *= by;
+                    const float here = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.c;
+                    float before = m;        // what the tile before took off
+                    if (QT == 1 && i > 0) {
+                        mbar_wait_bounded(smem_u32(&m_full[4 * (g ^ 1) + quad]), m_use & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+                        m_use++;
+                        before = m_rows[(g ^ 1) * 128 + 32 * quad + lane];
+                    }
+                    float now = before;
+                    if (tile == 0) {
+                        now = here;
+                    } else if (__any_sync(0xffffffffu, here > before + GROWTH)) {
+                        now = fmaxf(before, here);
+                        const float by = now == -INFINITY ? 1.0f : exp2_fast(before - now);
+                        const int last = i - (QT == 2 ? 2 : 1);   // the product that has to be there
+                        mbar_wait_bounded(done_u + 8u * (uint32_t)(last & 1), (done[last & 1] + (uint32_t)(last >> 1)) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                        for (int k = 0; k < DP; k += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_tm + (uint32_t)k, o);
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * by);
+                            tmem_st16_start(o_tm + (uint32_t)k, o);
+                        }
+                        tmem_st_wait();
+                    }
+                    if (QT == 1 && i + 1 < n) {
+                        m_rows[g * 128 + 32 * quad + lane] = now;
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(smem_u32(&m_full[4 * g + quad]));
+                    }
+                    if (now != m) l *= m == -INFINITY ? 0.0f : exp2_fast(m - now);
                     m = now;
-                }
-                const float off = (m == -INFINITY ? 0.0f : -m) + WEIGHT_BIAS<C>;
-                float sum[4] = {};
+                    const float off = (m == -INFINITY ? 0.0f : -m) + WEIGHT_BIAS<C>;
+                    const uint64_t c2 = pack_f32x2(a.c, a.c), off2 = pack_f32x2(off, off);
+                    uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int k = 0; k < KEYS; k += 2) {
-                    const float p = exp2_fast(fmaf(__uint_as_float(v[k]), a.c, off)), r = exp2_fast(fmaf(__uint_as_float(v[k + 1]), a.c, off));
-                    sum[k / 2 % 2 * 2] += p;
-                    sum[k / 2 % 2 * 2 + 1] += r;
-                    v[k / 2] = pack2<C>(p, r);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    for (int h = 0; h < 2; h++) {
+                        if (h) load_half(1);
 #pragma unroll
-                for (int k = 0; k < KEYS / 2; k += 16) tmem_st16_start(s_tm + (uint32_t)k, v + k);
+                        for (int k = 0; k < HALF; k += 2) {
+                            const float2 x = unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), c2, off2));
+                            const float p = exp2_fast(x.x), r = exp2_fast(x.y);
+                            sum[k / 2 % 2] = add_f32x2(sum[k / 2 % 2], pack_f32x2(p, r));
+                            v[k / 2] = pack2<C>(p, r);
+                        }
+                        // (over scores that are in registers already)
+#pragma unroll
+                        for (int k = 0; k < HALF / 2; k += 16) tmem_st16_start(s_tm + (uint32_t)(h * HALF / 2 + k), v + k);
+                    }
+                    const float2 sums = unpack_f32x2(add_f32x2(sum[0], sum[1]));
+                    l += sums.x + sums.y;
+                }
                 // Values of slots behind the last key that is seen may be anything, and so may values that some of the rows do not see: no product with
                 // a weight of zero takes them away if they are no numbers.
                 if (j0 + KEYS > least_item) {
@@ -544,7 +608,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     const bool some = least_item < w.seen;
 #pragma unroll 1
                     for (int c = 0; c < NCH; c++) {
-                        const uint32_t at = ring0 + at_values<QT, NCH>(i, tiles) + c, st = at % STAGES;
+                        const uint32_t at = ring0 + at_values<QT, NCH>(tile, tiles) + c, st = at % STAGES;
                         mbar_wait_bounded(smem_u32(&full[st]), at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
                         uint8_t* p = ring + st * STAGE;
                         for (int u = 32 * quad + lane; u < CW / 8 * KEYS; u += 128) {
@@ -569,16 +633,27 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 tmem_st_wait();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&p_full[slot]));
-                done++;
+                if (lane == 0) mbar_arrive(p_bar);
             }
             ring0 += (uint32_t)(2 * tiles * NCH);
-            // the next item's queries go in place before this one's outputs leave (its scores are all done)
+            if (QT == 1) {   // both warpgroups' maxima and sums: the later of the maxima is the larger
+                float2* mine = ml_rows + (item & 1) * 256 + 32 * quad + lane;
+                mine[128 * g] = make_float2(m, l);
+                named_bar_sync(1 + quad, 64);   // (the other warp of these rows; all scores of the item are there)
+                const float2 other = mine[128 * (g ^ 1)];
+                const float top = fmaxf(m, other.x);
+                l = (m == -INFINITY ? 0.0f : l * exp2_fast(m - top)) + (other.x == -INFINITY ? 0.0f : other.y * exp2_fast(other.x - top));
+                m = top;
+            }
             const Walk now = w;
-            const bool was_spoilt_item = least_item < now.seen;
-            mbar_wait_bounded(smem_u32(&o_done[t]), (done - 1) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (was_spoilt_item && spoilt[item & 1] == item) {
+            {
+                const int last = QT == 2 ? n - 2 + g : n - 1;
+                mbar_wait_bounded(done_u + 8u * (uint32_t)(last & 1), (done[last & 1] + (uint32_t)(last >> 1)) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
+            done[0] += (uint32_t)((n + 1) >> 1);
+            done[1] += (uint32_t)(n >> 1);
+            if (least_item < now.seen && spoilt[item & 1] == item) {
                 // Rare: what was taken out of the products goes to the rows that see it, a value at a time.
                 const int lo = max(least_item / KEYS * KEYS, now.from * KEYS), hi = min(now.seen, now.to * KEYS);
                 const uint8_t* q_row = q_at + t * 128 * DP * 2;
@@ -590,7 +665,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     const long long v_at = page * a.v_page + in * a.v_slot + now.kv * a.v_head, k_at = page * a.k_page + in * a.k_slot + now.kv * a.k_head;
                     float weight = 0.0f;
                     bool known = false;
-                    for (int e = 0; e < a.D; e++) {
+                    for (int e = col0; e < min(a.D, col0 + COLS); e++) {
                         const float x = load_as<C>(a.v, v_at + e);
                         if (fabsf(x) < INFINITY) continue;
                         if (!known) {
@@ -609,17 +684,19 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                         tmem_st_wait();
                     }
                 }
-                __syncwarp();
+                if (QT == 1) named_bar_sync(1 + quad, 64);   // (the other warp reads the same queries)
             }
+            // the next item's queries go in place before this one's outputs leave
             more = walk_next<ROWS>(a, w, left);
             if (more) load_queries(w);
             const bool whole = now.from == 0 && now.to == now.units;
             const int flat = now.row0 + row, head = now.kv * a.group + flat % a.group;
             const long long out_row = now.first + flat / a.group;
-            if (whole) {
+            if (idle) {
+            } else if (whole) {
                 const float by = limit > 0 ? 1.0f / l : 0.0f;
 #pragma unroll 1
-                for (int k = 0; k < DP; k += 16) {
+                for (int k = col0; k < col0 + COLS; k += 16) {
                     uint32_t o[16];
                     float f[16];
                     tmem_ld16(o_tm + (uint32_t)k, o);
@@ -627,19 +704,19 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     for (int e = 0; e < 16; e++) f[e] = limit > 0 ? __uint_as_float(o[e]) * by : 0.0f;
                     if (row < now.rows && k < a.D) store16(a, out_row * a.out_row + (long long)head * a.out_head + k, f, a.D - k);
                 }
-                if (a.lse && row < now.rows) a.lse[out_row * a.n_heads + head] = limit > 0 ? 0.6931471805599453f * (m + log2f(l) - WEIGHT_BIAS<C>) : -INFINITY;
+                if (a.lse && row < now.rows && col0 == 0) a.lse[out_row * a.n_heads + head] = limit > 0 ? 0.6931471805599453f * (m + log2f(l) - WEIGHT_BIAS<C>) : -INFINITY;
             } else {
                 // a place in the work area: [4 columns][row] and each row's m and l behind
                 float* to = a.slots + (long long)(2 * blockIdx.x + (now.from == 0 ? 1 : 0)) * a.slot_rows * (DP + 4);
 #pragma unroll 1
-                for (int k = 0; k < DP; k += 16) {
+                for (int k = col0; k < col0 + COLS; k += 16) {
                     uint32_t o[16];
                     tmem_ld16(o_tm + (uint32_t)k, o);
                     if (row < now.rows)
 #pragma unroll
                         for (int e = 0; e < 16; e += 4) *(uint4*)(to + (long long)((k + e) / 4 * a.slot_rows + row) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
                 }
-                if (row < now.rows) *(float2*)(to + (long long)a.slot_rows * DP + 2 * row) = make_float2(m, l);
+                if (row < now.rows && col0 == 0) *(float2*)(to + (long long)a.slot_rows * DP + 2 * row) = make_float2(m, l);
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             item++;
