@@ -604,22 +604,21 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 // Values of slots behind the last key that is seen may be anything, and so may values that some of the rows do not see: no product with
                 // a weight of zero takes them away if they are no numbers.
                 if (j0 + KEYS > least_item) {
-                    const int seen = w.seen - j0, rest = min(KEYS, (seen + a.box_rows - 1) / a.box_rows * a.box_rows);   // slots from `seen` to `rest` came with a page
-                    const bool some = least_item < w.seen;
+                    // rows of this stage's values: from `lo` on some of the item's rows do not see them, from `seen` on none does; up to `rest` they came with a page
+                    const int lo = max(0, least_item - j0), seen = w.seen - j0, rest = min(KEYS, (seen + a.box_rows - 1) / a.box_rows * a.box_rows);
 #pragma unroll 1
                     for (int c = 0; c < NCH; c++) {
                         const uint32_t at = ring0 + at_values<QT, NCH>(tile, tiles) + c, st = at % STAGES;
                         mbar_wait_bounded(smem_u32(&full[st]), at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
-                        uint8_t* p = ring + st * STAGE;
-                        for (int u = 32 * quad + lane; u < CW / 8 * KEYS; u += 128) {
-                            const int j = u % (8 * KEYS) / 8;   // 16-byte pieces lie in rows of eight
-                            if (j >= rest || (j < seen && !some)) continue;
-                            uint4* x = (uint4*)p + u;
+                        // 16-byte pieces: eight to a row of a block of 64 elements, whose order in the row does not matter here
+                        for (int u = 32 * quad + lane; u < (rest - lo) * (CW / 8); u += 128) {
+                            const int j = lo + u / (CW / 8);
+                            uint4* x = (uint4*)(ring + st * STAGE + u % (CW / 8) / 8 * BLOCK_BYTES + j * 128) + u % 8;
                             if (j >= seen) {
                                 *x = make_uint4(0, 0, 0, 0);
                                 continue;
                             }
-                            uint4 y = *x;
+                            const uint4 y = *x;
                             const uint4 bad = make_uint4(no_number<C>(y.x), no_number<C>(y.y), no_number<C>(y.z), no_number<C>(y.w));
                             if (bad.x | bad.y | bad.z | bad.w) {
                                 spoilt[item & 1] = item;
@@ -655,7 +654,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             done[1] += (uint32_t)(n >> 1);
             if (least_item < now.seen && spoilt[item & 1] == item) {
                 // Rare: what was taken out of the products goes to the rows that see it, a value at a time.
-                const int lo = max(least_item / KEYS * KEYS, now.from * KEYS), hi = min(now.seen, now.to * KEYS);
+                const int lo = max(least_item, now.from * KEYS), hi = min(now.seen, now.to * KEYS);
                 const uint8_t* q_row = q_at + t * 128 * DP * 2;
                 const int r = row - 128 * t;
                 for (int j = lo; j < hi; j++) {

@@ -211,3 +211,29 @@ def test_wrapper_refusals(ctx):
     for bad in (lambda: ctx.quantize_i8(torch.empty((0, 64), device="cuda")), lambda: ctx.quantize_i8(torch.empty((1, 131072), device="cuda"))):
         with pytest.raises(api.Q38BError):
             bad()
+
+
+@pytest.mark.parametrize("mode", [64, 128, 192, 256, -10, -20, -1, -2, -3, -4, -5, -6, -7, -8, -12, -22, -23, -25, -28])
+def test_every_cut_gives_the_same_sums(ctx, mode):
+    """Pairs of CTAs with every tile, single CTAs with K in every number of parts: exact sums, so the same bits."""
+    for B, M, K in ((1, 700, 2000), (20, 300, 1300), (60, 130, 4096), (200, 513, 1111), (520, 256, 640)):
+        if mode // 10 == -2 or -mode // 10 == 2:
+            if B > 64:
+                continue
+        (xc, xs), (wc, ws) = codes(B, K, B), codes(M, K, M)
+        X = ctx.quantize_i8(torch.zeros((B, K), device="cuda"))
+        W = ctx.quantize_i8(torch.zeros((M, K), device="cuda"))
+        X.codes.copy_(xc.cuda()), X.scales.copy_(xs.cuda()), W.codes.copy_(wc.cuda()), W.scales.copy_(ws.cuda())
+        for kind in (0, 2):
+            want = ctx.gemm_i8(W, X, kind=kind)
+            room = torch.full((B, M + 3), 7.0, device="cuda", dtype=want.dtype)
+            ctx.debug_set_i8_cut(mode)
+            try:
+                got = ctx.gemm_i8(W, X, kind=kind)
+                ctx.gemm_i8(W, X, out=room[:, 1:M + 1])
+            finally:
+                ctx.debug_set_i8_cut(0)
+            ctx.check()
+            assert torch.equal(got, want) and torch.equal(room[:, 1:M + 1], want) and bool((room[:, 0] == 7).all()) and bool((room[:, M + 1:] == 7).all())
+            if kind == 0:
+                check_product(want, xc.numpy().astype(np.int64), xs.numpy(), wc.numpy().astype(np.int64), ws.numpy(), "f32")
