@@ -101,16 +101,14 @@ __device__ __forceinline__ void walk_tile(const AttnArgs& a, Walk& w) {
     w.seen = tile_seen<ROWS>(w, a.group, w.tile);
     w.units = tile_units(w.seen);
 }
-// on to the next tile of rows; `left`: units of the CTA's range that remain.  false: none
+// the tile of rows behind this one; false: there is none
 template <int ROWS>
-__device__ __forceinline__ bool walk_next(const AttnArgs& a, Walk& w, long long& left) {
-    left -= w.to - w.from;
-    if (left <= 0) return false;
+__device__ __forceinline__ bool walk_on(const AttnArgs& a, Walk& w) {
     if (++w.tile == w.n_tiles) {
         w.tile = 0;
         if (++w.kv == a.n_kv) {
             w.kv = 0;
-            do {   // (units remain: so does a sequence that has them)
+            do {
                 if (++w.s >= a.batch.n_seqs) return false;
                 walk_sequence<ROWS>(a, w);
             } while (w.n_tiles == 0);
@@ -118,8 +116,23 @@ __device__ __forceinline__ bool walk_next(const AttnArgs& a, Walk& w, long long&
     }
     walk_tile<ROWS>(a, w);
     w.from = 0;
+    return true;
+}
+// on to the next tile of rows; `left`: units of the CTA's range that remain.  false: none
+template <int ROWS>
+__device__ __forceinline__ bool walk_next(const AttnArgs& a, Walk& w, long long& left) {
+    left -= w.to - w.from;
+    if (left <= 0 || !walk_on<ROWS>(a, w)) return false;
     w.to = (int)min((long long)w.units, left);
     return true;
+}
+
+// A part of a tile of rows that others finish costs about as much as a tile of keys for every 32 of its rows (its sums go out to memory and come back).  So a range that
+// would begin or end within that of a tile's ends begins or ends there instead (5 sequences of 77 to 333 new tokens, 15 + 5 heads of 96: 62 us cut exactly, MEASURED_RAGGED so).
+__device__ __forceinline__ int dear(const Walk& w) { return w.rows / 32; }
+__device__ __forceinline__ int moved_cut(const Walk& w, int in) {   // a cut `in` units behind the first of a tile's
+    if (in > dear(w) && w.units - in > dear(w)) return in;
+    return 2 * in <= w.units ? 0 : w.units;
 }
 
 // Units of one key head of a sequence, by one thread or by the lanes of a warp together
@@ -132,14 +145,22 @@ __device__ __forceinline__ long long sequence_units(const AttnArgs& a, const Wal
 
 struct Plan {             // in shared memory
     long long sums[16];
-    long long total, left;
-    Walk walk;
-    int active;           // CTAs with work
+    long long total, cut[2];   // units of all; this CTA's first and the one behind its last
+    Walk walk;                 // the tile of rows it begins in
+    int active;                // CTAs among which the units are divided
 };
+// where CTA c of `active` would begin if units were divided exactly
+__device__ __forceinline__ long long exact_cut(long long total, int active, int c) {
+    if (total < 1LL << 31) {
+        const int each = (int)total / active, rest = (int)total % active;
+        return (long long)each * c + rest * c / active;
+    }
+    return total / active * c + total % active * c / active;
+}
 
-// All threads: the batch's units, this CTA's range of them, and the tile of rows it begins in.
+// All threads: the batch's units, this CTA's range of them, and the tile of rows it begins in.  false: nothing to do
 template <int ROWS, int THREADS>
-__device__ __forceinline__ void plan_work(const AttnArgs& a, Plan* p) {
+__device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int WARPS = THREADS / 32;
     // few sequences: a warp each, its lanes along the tiles; many: a thread each
@@ -157,6 +178,7 @@ __device__ __forceinline__ void plan_work(const AttnArgs& a, Plan* p) {
         return lane == 0 ? a.n_kv * n : 0LL;
     };
     long long mine = 0, units = 0;   // units: of the last round
+#pragma unroll 1
     for (int r = 0; r < rounds; r++) {
         units = units_of(r * per_round + (wide ? warp : (int)threadIdx.x));
         mine += units;
@@ -166,17 +188,18 @@ __device__ __forceinline__ void plan_work(const AttnArgs& a, Plan* p) {
     if (lane == 0) p->sums[warp] = mine;
     __syncthreads();
     long long total = 0;
+#pragma unroll
     for (int w = 0; w < WARPS; w++) total += p->sums[w];
     const int active = (int)min((long long)gridDim.x, total), cta = (int)blockIdx.x;
+    if (cta >= active) return false;
+    const long long begin = exact_cut(total, active, cta), end = cta + 1 == active ? total : exact_cut(total, active, cta + 1);
     if (threadIdx.x == 0) {
         p->total = total;
         p->active = active;
-        p->left = 0;
+        if (end == total) p->cut[1] = total;
     }
-    __syncthreads();
-    if (cta >= active) return;
-    const long long begin = total * cta / active, end = total * (cta + 1) / active;
     long long before = 0;            // units of the rounds before
+#pragma unroll 1
     for (int r = 0; r < rounds; r++) {
         if (rounds > 1) units = units_of(r * per_round + (wide ? warp : (int)threadIdx.x));
         long long upto = units;      // inclusive sums
@@ -185,34 +208,46 @@ __device__ __forceinline__ void plan_work(const AttnArgs& a, Plan* p) {
             const long long o = __shfl_up_sync(0xffffffffu, upto, d);
             if (lane >= d) upto += o;
         }
+        __syncthreads();             // (the sums before have been read)
         if (lane == 31) p->sums[warp] = upto;
         __syncthreads();
         long long base = before;
+#pragma unroll
         for (int w = 0; w < WARPS; w++) {
             if (w < warp) base += p->sums[w];
             before += p->sums[w];
         }
         const long long at = base + upto - units;
-        if (units > 0 && begin >= at && begin < at + units) {   // one thread of the block
+#pragma unroll 1
+        for (int i = 0; i < 2; i++) {
+            const long long cut = i ? end : begin;
+            if (!(units > 0 && cut >= at && cut < at + units)) continue;   // one thread of the block goes on, for each of the two
             Walk w;
             w.s = r * per_round + (wide ? warp : (int)threadIdx.x);
             walk_sequence<ROWS>(a, w);
             const long long per_head = units / a.n_kv;
-            long long in = begin - at;
-            w.kv = (int)(in / per_head);
-            in -= w.kv * per_head;
+            long long in = cut - at;
+            w.kv = 0;
+            if (in >= per_head) {
+                w.kv = (int)(in / per_head);
+                in -= w.kv * per_head;
+            }
             for (w.tile = 0;; w.tile++) {
                 walk_tile<ROWS>(a, w);
                 if (in < w.units) break;
                 in -= w.units;
             }
-            w.from = (int)in;
-            w.to = (int)min((long long)w.units, in + (end - begin));
-            p->walk = w;
-            p->left = end - begin;
+            const int to = moved_cut(w, (int)in);
+            p->cut[i] = cut - in + to;
+            if (i == 0) {
+                w.from = to;
+                if (to == w.units && !walk_on<ROWS>(a, w)) w.from = 0;   // (the last tile's end: nothing to do)
+                p->walk = w;
+            }
         }
-        __syncthreads();
     }
+    __syncthreads();
+    return p->cut[1] > p->cut[0];
 }
 
 __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr) {
@@ -242,27 +277,6 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-// two floats in 64 bits, and operations on both
-__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 template <typename C> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -356,6 +370,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     uint8_t* ring = q_at + Sh::Q_BYTES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    if (threadIdx.x == 32) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
+    }
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         spoilt[0] = spoilt[1] = -1;
@@ -378,12 +396,12 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    plan_work<ROWS, Sh::THREADS>(a, plan);   // (ends with a barrier of the block)
+    const bool any = plan_work<ROWS, Sh::THREADS>(a, plan);   // (with barriers of the block)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
-    long long left = plan->left;
-    const bool any = left > 0;
+    long long left = any ? plan->cut[1] - plan->cut[0] : 0;
     Walk w = plan->walk;
+    w.to = (int)min((long long)w.units, w.from + left);
 
     if (any && warp == 0) {
         // ---------------- keys and values: a lane a box of at most 128 slots x 64 elements ----------------
@@ -457,26 +475,28 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     __syncwarp();
                 }
             };
-            scores(0);
-            if (n > 1) scores(1);
-            for (int i = 0; i < n; i++) {
-                const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
-                mbar_wait_bounded(smem_u32(&p_full[i & 1]), p_phase >> (i & 1) & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
-                p_phase ^= 1u << (i & 1);
+            // two scores ahead of the products with values; one copy of either's code (a CTA of few tiles waits for its instructions)
+#pragma unroll 1
+            for (int i = -2; i < n; i++) {
+                if (i >= 0) {
+                    const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
+                    mbar_wait_bounded(smem_u32(&p_full[i & 1]), p_phase >> (i & 1) & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                    p_phase ^= 1u << (i & 1);
 #pragma unroll
-                for (int c = 0; c < NCH; c++) {
-                    const uint32_t at = ring0 + at_values<QT, NCH>(tile, tiles) + c, st = at % STAGES;
-                    mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t d = tmem + (uint32_t)(256 + t * DP + c * CW), p = tmem + (uint32_t)((i & 1) * KEYS);
-                    const uint64_t vd = vdesc0 + ((ring_u + st * STAGE) >> 4);
-                    if (elect_one()) {
+                    for (int c = 0; c < NCH; c++) {
+                        const uint32_t at = ring0 + at_values<QT, NCH>(tile, tiles) + c, st = at % STAGES;
+                        mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        const uint32_t d = tmem + (uint32_t)(256 + t * DP + c * CW), p = tmem + (uint32_t)((i & 1) * KEYS);
+                        const uint64_t vd = vdesc0 + ((ring_u + st * STAGE) >> 4);
+                        if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < KEYS / 16; k++) mma_ts(d, p + (uint32_t)(8 * k), vd + (uint64_t)(k * 2048 >> 4), idesc_o, k > 0 || tile > 0 ? 1u : 0u);
-                        if (QT == 1 || t == 1) umma_commit<false>(empty_u + 8u * st);
-                        if (c == NCH - 1) umma_commit<false>(smem_u32(&o_done[i & 1]));
+                            for (int k = 0; k < KEYS / 16; k++) mma_ts(d, p + (uint32_t)(8 * k), vd + (uint64_t)(k * 2048 >> 4), idesc_o, k > 0 || tile > 0 ? 1u : 0u);
+                            if (QT == 1 || t == 1) umma_commit<false>(empty_u + 8u * st);
+                            if (c == NCH - 1) umma_commit<false>(smem_u32(&o_done[i & 1]));
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
                 if (i + 2 < n) scores(i + 2);
             }
@@ -492,15 +512,26 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         constexpr int COLS = QT == 2 ? DP : DP / 2;     // of the outputs this warpgroup stores
         const int col0 = QT == 2 ? 0 : g * COLS;
         const auto load_queries = [&](const Walk& v) {
-            constexpr int UNITS = DP / 8, ALL = 32 * UNITS, SHARE = QT == 2 ? ALL : ALL / 2;    // 16-byte pieces of a row, of the warp's rows, of those its own
-            uint8_t* to = q_at + t * 128 * DP * 2;
-            const int first = QT == 2 ? 0 : g * SHARE;
-#pragma unroll 4
-            for (int u = first + lane; u < first + SHARE; u += 32) {
-                const int r = 32 * quad + u / UNITS, e = u % UNITS * 8, flat = v.row0 + 128 * t + r;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (128 * t + r < v.rows && e < a.D) x = query_eight<C>(a, (long long)(v.first + flat / a.group) * a.q_row + (long long)(v.kv * a.group + flat % a.group) * a.q_head + e);
-                *(uint4*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16) = x;
+            constexpr int UNITS = DP / 8, SHARE = (QT == 2 ? 32 : 16) * UNITS, AHEAD = SHARE / 32 % 8 == 0 ? 8 : 4;    // 16-byte pieces of a row; of this warp's share; of a lane on their way
+            const int flat = v.row0 + row, there = row < v.rows, first = QT == 2 ? 0 : 16 * g;                      // (QT = 1: rows 16 g to 16 g + 15 of the 32)
+            const long long my_row = (long long)(v.first + flat / a.group) * a.q_row + (long long)(v.kv * a.group + flat % a.group) * a.q_head;
+            uint8_t* to = q_at + t * 128 * DP * 2 + 32 * quad * 128;
+#pragma unroll 1
+            for (int u0 = 0; u0 < SHARE; u0 += 32 * AHEAD) {
+                uint4 x[AHEAD];
+#pragma unroll
+                for (int n = 0; n < AHEAD; n++) {
+                    const int u = u0 + 32 * n + lane, r = first + u / UNITS, e = u % UNITS * 8;
+                    const long long at = __shfl_sync(0xffffffffu, my_row, r);
+                    const bool here = __shfl_sync(0xffffffffu, there, r) && e < a.D;
+                    x[n] = make_uint4(0, 0, 0, 0);
+                    if (here) x[n] = query_eight<C>(a, at + e);
+                }
+#pragma unroll
+                for (int n = 0; n < AHEAD; n++) {
+                    const int u = u0 + 32 * n + lane, r = first + u / UNITS, e = u % UNITS * 8;
+                    *(uint4*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16) = x[n];
+                }
             }
             fence_proxy_async();
             __syncwarp();
@@ -559,7 +590,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     if (tile == 0) {
                         now = here;
                     } else if (__any_sync(0xffffffffu, here > before + GROWTH)) {
-                        now = fmaxf(before, here);
+                        if (here > before + GROWTH) now = here;   // (a row by itself: what its neighbours see changes no bit of it)
                         const float by = now == -INFINITY ? 1.0f : exp2_fast(before - now);
                         const int last = i - (QT == 2 ? 2 : 1);   // the product that has to be there
                         mbar_wait_bounded(done_u + 8u * (uint32_t)(last & 1), (done[last & 1] + (uint32_t)(last >> 1)) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
@@ -725,10 +756,9 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     if (threadIdx.x == 64) {
         Job job = {};
         if (any) {
-            const long long total = plan->total, end = total * (blockIdx.x + 1) / plan->active;
             if (w.from == 0 && w.to < w.units) {
-                const long long last = end + (w.units - w.to) - 1;   // its last unit
-                job.n_parts = (int)(((last + 1) * plan->active - 1) / total) - (int)blockIdx.x + 1;
+                const long long last = plan->cut[1] + (w.units - w.to) - dear(w) - 1;   // the last unit in which one of its other parts may begin
+                job.n_parts = (int)(((last + 1) * plan->active - 1) / plan->total) - (int)blockIdx.x + 1;
                 job.first = w.first;
                 job.n_new = w.n_new;
                 job.len = w.len;
@@ -884,8 +914,8 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     a.c = (float)((double)scale * 1.4426950408889634);
     CUtensorMap kmap, vmap;
     if (!encode_pages(&kmap, c, c->k, c->k_page, c->k_slot, c->k_head, a.box_rows) || !encode_pages(&vmap, c, c->v, c->v_page, c->v_slot, c->v_head, a.box_rows)) return Q38B_ERR_ARG;
-    // two tiles of rows share the keys' way into shared memory where sequences fill more than one on average
-    const bool two = (long long)rows * a.group > 128LL * c->n_seqs;
+    // two tiles of rows share the keys' way into shared memory where sequences fill more than one on average and there are enough of them for all SMs
+    const bool two = (long long)rows * a.group > 128LL * c->n_seqs && (long long)rows * n_heads >= 256LL * ctx->sm_count;
     return c->kind == Q38B_OUT_F16 ? attention_for<__half>(ctx, a, two, kmap, vmap, (cudaStream_t)stream) : attention_for<__nv_bfloat16>(ctx, a, two, kmap, vmap, (cudaStream_t)stream);
 }
 

@@ -7,11 +7,19 @@
 #include <cuda.h>
 #include <cuda.h>
 #include <cuda.h>
+#include <cuda.h>
+#include <cuda.h>
+#include <cuda.h>
+#include <cuda.h>
+#include <cuda.h>
+#include <cuda.h>
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <type_traits>
 
 #include "../../include/q38b200.h"
 #include "q38b_host.h"
@@ -39,17 +47,28 @@ __device__ __forceinline__ RowScale row_scale(uint32_t top) {   // bit pattern o
     r.keep = bad ? 0u : ~0u;
     return r;
 }
-// the code in the low byte (rounding by an addition: conversions run at a quarter of the rate)
-__device__ __forceinline__ uint32_t code_of(float x, const RowScale& r) {
-    constexpr float MAGIC = 12582912.0f;   // 1.5 * 2^23: whole numbers lie one apart
-    float t = fmaf(x, r.inv, MAGIC);
-    const float n = t - MAGIC, rest = fmaf(-n, r.scale, x);
-    if (fabsf(rest) >= r.half) {
-        const bool odd = (__float_as_uint(t) & 1u) != 0u;
-        if (rest > r.half || (rest == r.half && odd)) t += 1.0f;
-        else if (rest < -r.half || (rest == -r.half && odd)) t -= 1.0f;
+// Eight codes, each in the low byte of a word (rounding by an addition: conversions run at a quarter of the rate).  The remainders are looked at together: whether any of the
+// eight may have to move is one branch (one for each made the kernel three times as long, and it waited for instructions).
+constexpr float MAGIC = 12582912.0f;   // 1.5 * 2^23: whole numbers lie one apart
+__device__ __forceinline__ void codes_of(const float (&x)[8], const RowScale& r, float (&t)[8]) {
+    float worst = 0.0f;
+    const uint64_t inv = pack_f32x2(r.inv, r.inv), scale = pack_f32x2(r.scale, r.scale), magic = pack_f32x2(MAGIC, MAGIC), minus = pack_f32x2(-1.0f, -1.0f);
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) {
+        const uint64_t v = pack_f32x2(x[i], x[i + 1]), u = fma_f32x2(v, inv, magic);
+        const float2 rest = unpack_f32x2(fma_f32x2(fma_f32x2(u, minus, magic), scale, v)), c = unpack_f32x2(u);
+        t[i] = c.x;
+        t[i + 1] = c.y;
+        worst = fmaxf(fmaxf(worst, fabsf(rest.x)), fabsf(rest.y));
     }
-    return __float_as_uint(t);
+    if (worst >= r.half) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float rest = fmaf(MAGIC - t[i], r.scale, x[i]);
+            const bool odd = (__float_as_uint(t[i]) & 1u) != 0u;
+            t[i] += rest > r.half || (rest == r.half && odd) ? 1.0f : rest < -r.half || (rest == -r.half && odd) ? -1.0f : 0.0f;
+        }
+    }
 }
 
 // Eight neighbours of a row as they lie in memory
@@ -59,12 +78,24 @@ template <typename T> __device__ __forceinline__ void raw8_values(const Raw8<T>&
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = to_f32(e[i]);
 }
+// the larger ones of two times two numbers, a NaN where either is one
+template <typename T> __device__ __forceinline__ uint32_t max_nan2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <typename T> __device__ __forceinline__ uint32_t raw8_top2(const Raw8<T>& r) {   // 16-bit types: the largest magnitudes of the even and of the odd four
+    return max_nan2<T>(max_nan2<T>(r.q[0].x & 0x7FFF7FFFu, r.q[0].y & 0x7FFF7FFFu), max_nan2<T>(r.q[0].z & 0x7FFF7FFFu, r.q[0].w & 0x7FFF7FFFu));
+}
+template <typename T> __device__ __forceinline__ uint32_t top_of2(uint32_t m) {
+    const unsigned short top = (unsigned short)max(m & 0x7FFFu, m >> 16 & 0x7FFFu);
+    return __float_as_uint(to_f32(*(const T*)&top));
+}
 // the bit pattern (in fp32) of the largest magnitude: magnitudes compare like their bits, a NaN's exceeds them all
 template <typename T> __device__ __forceinline__ uint32_t raw8_top(const Raw8<T>& r) {
     if constexpr (sizeof(T) == 2) {
-        const uint32_t m = __vmaxu2(__vmaxu2(r.q[0].x & 0x7FFF7FFFu, r.q[0].y & 0x7FFF7FFFu), __vmaxu2(r.q[0].z & 0x7FFF7FFFu, r.q[0].w & 0x7FFF7FFFu));
-        const unsigned short top = (unsigned short)max(m & 0xFFFFu, m >> 16);
-        return __float_as_uint(to_f32(*(const T*)&top));
+        return top_of2<T>(raw8_top2<T>(r));
     } else {
         const float* v = (const float*)r.q;
         uint32_t top = 0u;
@@ -78,40 +109,50 @@ template <typename T> __device__ __forceinline__ uint32_t raw8_top(const Raw8<T>
 // codes: every value is read once.  What is longer than 20480 is read twice.  Bound by memory: 17408 x 5120 from bf16 MEASURED_W, against
 // 110 us with single elements read twice; 77 x 5120 from fp32 MEASURED_F.
 constexpr int PIECES = 4;
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(640) i8_quantize_kernel(const T* x, long long x_ld, int K, int rows, int per_block, int8_t* codes, long long codes_ld, float* scales) {
+// VEC: whole pieces, aligned (the rest of a row's code, unused, took half of the instructions issued).  WARP: eight rows a block.
+template <typename T, bool VEC, bool WARP>
+__global__ void __launch_bounds__(WARP ? 256 : 640, sizeof(T) == 2 && !WARP ? 2 : 1) i8_quantize_kernel(const T* x, long long x_ld, int K, int rows, int8_t* codes, long long codes_ld, float* scales) {
     pdl_launch_dependents();   // (a product behind it brings its first weights meanwhile)
     __shared__ uint32_t tops[32];
-    const int threads = (int)blockDim.x / per_block, t = (int)threadIdx.x % threads;
-    const long long row = (long long)blockIdx.x * per_block + threadIdx.x / threads;
+    const int threads = WARP ? 32 : (int)blockDim.x, t = WARP ? (int)threadIdx.x % 32 : (int)threadIdx.x;
+    const long long row = WARP ? (long long)blockIdx.x * 8 + threadIdx.x / 32 : (long long)blockIdx.x;
     const int pieces = (K + 7) / 8;
     const bool here = row < rows;
     const T* p = x + row * x_ld;
     int8_t* to = codes + row * codes_ld;
     const auto load = [&](int u) {
-        Raw8<T> r = {};
-        if (VEC && 8 * u + 8 <= K) {
-            r = *(const Raw8<T>*)(p + 8 * u);
+        if constexpr (VEC) {
+            return *(const Raw8<T>*)(p + 8 * u);
         } else {
             T e[8] = {};
 #pragma unroll
             for (int i = 0; i < 8; i++)
                 if (8 * u + i < K) e[i] = p[8 * u + i];
+            Raw8<T> r;
             memcpy(&r, e, sizeof(e));
+            return r;
         }
-        return r;
     };
     Raw8<T> raw[PIECES] = {};
     uint32_t top = 0u;
 #pragma unroll
     for (int j = 0; j < PIECES; j++)
         if (here && t + j * threads < pieces) raw[j] = load(t + j * threads);
+    if constexpr (sizeof(T) == 2) {
+        uint32_t m[PIECES];
 #pragma unroll
-    for (int j = 0; j < PIECES; j++) top = max(top, raw8_top<T>(raw[j]));
+        for (int j = 0; j < PIECES; j++) m[j] = raw8_top2<T>(raw[j]);
+#pragma unroll
+        for (int j = 1; j < PIECES; j++) m[0] = max_nan2<T>(m[0], m[j]);
+        top = top_of2<T>(m[0]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) top = max(top, raw8_top<T>(raw[j]));
+    }
     if (here)
         for (int u = t + PIECES * threads; u < pieces; u += threads) top = max(top, raw8_top<T>(load(u)));
     top = __reduce_max_sync(0xffffffffu, top);
-    if (threads > 32) {
+    if constexpr (!WARP) {
         if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
         __syncthreads();
         top = __reduce_max_sync(0xffffffffu, (int)(threadIdx.x % 32) < threads / 32 ? tops[threadIdx.x % 32] : 0u);
@@ -120,16 +161,16 @@ __global__ void __launch_bounds__(640) i8_quantize_kernel(const T* x, long long 
     const RowScale s = row_scale(top);
     if (t == 0) scales[row] = s.scale;
     const auto store = [&](int u, const Raw8<T>& r) {
-        float v[8];
-        uint32_t c[8];
+        float v[8], f[8];
         raw8_values<T>(r, v);
-#pragma unroll
-        for (int i = 0; i < 8; i++) c[i] = code_of(v[i], s);
+        codes_of(v, s, f);
+        const uint32_t* c = (const uint32_t*)f;
         const uint2 w = make_uint2(__byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410) & s.keep,
                                    __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410) & s.keep);
-        if (8 * u + 8 <= K) {
+        if (VEC || 8 * u + 8 <= K) {
             *(uint2*)(to + 8 * u) = w;
         } else {
+#pragma unroll 1
             for (int i = 0; 8 * u + i < K; i++) to[8 * u + i] = (int8_t)((i < 4 ? w.x : w.y) >> (8 * (i % 4)));
         }
     };
@@ -529,7 +570,9 @@ int exchange_bytes(const I8Cut& c) {
 int i8_ring_bytes(int smem_optin, const I8Cut& c) { return (c.per_sm == 2 ? (smem_optin + 1024) / 2 - 1024 : smem_optin) - 1024 - c.box; }
 
 // ... by their time in SM clocks, of one wave of CTAs after the other: what starts and drains a CTA, the exchange of split sums, and stages, each as long as a CTA
-// takes alone (two of an SM: twice) or, if that is longer, as its bytes take out of L2 (6400 a clock for all SMs) and its weights out of DRAM (3300).
+// takes alone (two of an SM: twice) or, if that is longer, as its bytes take out of L2 (8600 a clock for all SMs; pairs 6450) and its weights out of DRAM
+// (3200).  Fitted to 105 sizes (7 matrices, 1 to 2048 tokens) in every cut: the taken one is 1.7 % behind the best on average, 10 % at most (17408 x 5120, 256 tokens 32.4 us in single
+// CTAs, 29.4 in pairs; 4096 x 4096, 1024 tokens 26.3 and 24.1).
 I8Cut i8_cut(int sm_count, int smem_optin, int K, int M, int B, int forced_splits, int forced_per_sm, double* cost_of) {
     I8Cut best = {};
     double best_cost = 0.0;
@@ -550,8 +593,8 @@ I8Cut i8_cut(int sm_count, int smem_optin, int K, int M, int B, int forced_split
             const long long ctas = tiles * c.splits, once = std::max(1, sms / c.splits) * (long long)c.splits, slots = per_sm * once, waves = (ctas + slots - 1) / slots;
             if (per_sm == 2 && !forced_per_sm && (ctas <= once || own_steps < 4)) continue;
             const double active = (double)std::min(ctas, slots);
-            const double stage = std::max({per_sm * (590.0 + 0.45 * n), active * i8_stage_bytes(n) / 6400.0, active / (double)tok_tiles * I8_A_BYTES / 3300.0});
-            const double cost = 3600.0 + (double)waves * (own_steps * stage + (per_sm == 2 ? 0.0 : 3000.0) + 37.0 * n + (c.splits > 1 ? 1900.0 : 0.0));
+            const double stage = std::max({per_sm * (590.0 + 0.5 * n), active * i8_stage_bytes(n) / 8600.0, active / (double)tok_tiles * I8_A_BYTES / 3200.0});
+            const double cost = 3600.0 + (double)waves * (own_steps * stage + (per_sm == 2 ? 0.0 : 2000.0) + 28.0 * n + (c.splits > 1 ? 1900.0 : 0.0));
             if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
         }
     };
@@ -578,8 +621,8 @@ I8PairCut i8_pair_cut(int sm_count, int smem_optin, int K, int M, int B, int for
         c.stages = std::min(I8_MAX_STAGES, (smem_optin - I8P_FIXED_SMEM) / i8p_stage_bytes(n));
         const int pairs = sm_count / 2;
         const double active = (double)std::min(c.n_tiles, pairs);
-        const double stage = std::max(400.0 + 0.87 * n, active * 2.0 * i8p_stage_bytes(n) / 6200.0), weights = active / c.tok_tiles * 2.0 * I8_A_BYTES / 3300.0;
-        const double cost = 7800.0 + 24.0 * n + (double)((c.n_tiles + pairs - 1) / pairs) * std::max(steps * stage + 1700.0, steps * weights);
+        const double stage = std::max(310.0 + 1.2 * n, active * 2.0 * i8p_stage_bytes(n) / 6450.0), weights = active / c.tok_tiles * 2.0 * I8_A_BYTES / 3200.0;
+        const double cost = 7800.0 + 25.0 * n + (double)((c.n_tiles + pairs - 1) / pairs) * std::max(steps * stage + 2200.0, steps * weights);
         if (!best.n_tile || cost < best_cost) { best = c; best_cost = cost; }
     }
     if (cost_of) *cost_of = best_cost;
@@ -599,11 +642,17 @@ int check_operand(const void* codes, long long ld, const float* scales, int K, i
 template <typename T>
 int quantize_as(q38b_ctx* ctx, const void* x, long long x_ld, int K, int rows, int8_t* codes, long long codes_ld, float* scales, cudaStream_t st) {
     // a warp a row and eight rows a block where that is enough, otherwise a block a row
-    const int pieces = (K + 7) / 8, warps = std::min(20, (pieces + 32 * PIECES - 1) / (32 * PIECES)), per_block = warps == 1 ? 8 : 1;
-    const unsigned grid = (unsigned)((rows + (long long)per_block - 1) / per_block), block = (unsigned)(32 * (warps == 1 ? 8 : warps));
-    const bool vec = (((uintptr_t)x | (uintptr_t)(x_ld * (long long)sizeof(T))) & 15) == 0;
-    if (vec) i8_quantize_kernel<T, true><<<grid, block, 0, st>>>((const T*)x, x_ld, K, rows, per_block, codes, codes_ld, scales);
-    else i8_quantize_kernel<T, false><<<grid, block, 0, st>>>((const T*)x, x_ld, K, rows, per_block, codes, codes_ld, scales);
+    const int pieces = (K + 7) / 8, warps = std::min(20, (pieces + 32 * PIECES - 1) / (32 * PIECES));
+    const bool vec = K % 8 == 0 && (((uintptr_t)x | (uintptr_t)(x_ld * (long long)sizeof(T))) & 15) == 0;
+    const T* p = (const T*)x;
+    if (warps == 1) {
+        const unsigned grid = (unsigned)((rows + 7LL) / 8);
+        if (vec) i8_quantize_kernel<T, true, true><<<grid, 256, 0, st>>>(p, x_ld, K, rows, codes, codes_ld, scales);
+        else i8_quantize_kernel<T, false, true><<<grid, 256, 0, st>>>(p, x_ld, K, rows, codes, codes_ld, scales);
+    } else {
+        if (vec) i8_quantize_kernel<T, true, false><<<(unsigned)rows, (unsigned)(32 * warps), 0, st>>>(p, x_ld, K, rows, codes, codes_ld, scales);
+        else i8_quantize_kernel<T, false, false><<<(unsigned)rows, (unsigned)(32 * warps), 0, st>>>(p, x_ld, K, rows, codes, codes_ld, scales);
+    }
     return launch_status(ctx, cudaSuccess);
 }
 

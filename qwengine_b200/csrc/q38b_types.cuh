@@ -1,7 +1,9 @@
-// q38b_types.cuh -- 16- and 32-bit floats to and from fp32: the element types of the activation-side kernels.
+// q38b_types.cuh -- 16- and 32-bit floats to and from fp32: the element types of the activation-side kernels; pairs of floats.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <cstdint>
 
 namespace q38b {
 
@@ -13,5 +15,27 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32(float v) { return v; }
 template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
+
+// two floats in 64 bits, and operations on both
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f32x2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 
 }  // namespace q38b
