@@ -54,7 +54,10 @@ struct AttnArgs {
     long long k_page, k_slot, k_head;
     int q_kind, out_kind, n_heads, n_kv, group, D, box_rows, slot_rows, q_vec, out_vec, pdl;
     float c;       // scale log2(e)
+    uint32_t group_mul;   // x / group = x group_mul >> group_shift for 0 <= x < 2^31
+    int group_shift;
 };
+__device__ __forceinline__ int by_group(const AttnArgs& a, int x) { return (int)((uint64_t)(uint32_t)x * a.group_mul >> a.group_shift); }
 
 // Shapes of a variant: heads padded to DP elements, QT tiles of 128 rows
 template <int DP, int QT>
@@ -67,7 +70,7 @@ struct Shape {
     static constexpr int STAGES = ROOM < 12 ? ROOM : 12;
     static constexpr int SMEM = HEAD + Q_BYTES + STAGES * STAGE;
     static constexpr int ROWS = QT * 128;
-    static constexpr int THREADS = 64 + 256;                  // a warp loads, a warp multiplies, two warpgroups make weights
+    static constexpr int THREADS = 384;                       // warps 0, 2, 3 load, warp 1 multiplies, two warpgroups make weights
     static_assert(256 + QT * DP <= 512, "tensor memory");
 };
 
@@ -89,8 +92,8 @@ __device__ __forceinline__ void walk_sequence(const AttnArgs& a, Walk& w) {
     w.n_tiles = (w.n_new * a.group + ROWS - 1) / ROWS;
 }
 template <int ROWS>
-__device__ __forceinline__ int tile_seen(const Walk& w, int group, int tile) {
-    const int last = (min((tile + 1) * ROWS, w.n_new * group) - 1) / group;   // token
+__device__ __forceinline__ int tile_seen(const AttnArgs& a, const Walk& w, int tile) {
+    const int last = by_group(a, min((tile + 1) * ROWS, w.n_new * a.group) - 1);   // token
     return max(0, w.len - w.n_new + last + 1);
 }
 __device__ __forceinline__ int tile_units(int seen) { return max(1, (seen + KEYS - 1) / KEYS); }   // (a tile that sees nothing is one, too: its zeros are written)
@@ -98,7 +101,7 @@ template <int ROWS>
 __device__ __forceinline__ void walk_tile(const AttnArgs& a, Walk& w) {
     w.row0 = w.tile * ROWS;
     w.rows = min(ROWS, w.n_new * a.group - w.row0);
-    w.seen = tile_seen<ROWS>(w, a.group, w.tile);
+    w.seen = tile_seen<ROWS>(a, w, w.tile);
     w.units = tile_units(w.seen);
 }
 // the tile of rows behind this one; false: there is none
@@ -120,10 +123,10 @@ __device__ __forceinline__ bool walk_on(const AttnArgs& a, Walk& w) {
 }
 // on to the next tile of rows; `left`: units of the CTA's range that remain.  false: none
 template <int ROWS>
-__device__ __forceinline__ bool walk_next(const AttnArgs& a, Walk& w, long long& left) {
+__device__ __forceinline__ bool walk_next(const AttnArgs& a, Walk& w, int& left) {
     left -= w.to - w.from;
     if (left <= 0 || !walk_on<ROWS>(a, w)) return false;
-    w.to = (int)min((long long)w.units, left);
+    w.to = min(w.units, left);
     return true;
 }
 
@@ -137,26 +140,21 @@ __device__ __forceinline__ int moved_cut(const Walk& w, int in) {   // a cut `in
 
 // Units of one key head of a sequence, by one thread or by the lanes of a warp together
 template <int ROWS>
-__device__ __forceinline__ long long sequence_units(const AttnArgs& a, const Walk& w, int lane, int lanes) {
-    long long n = 0;
-    for (int t = lane; t < w.n_tiles; t += lanes) n += tile_units(tile_seen<ROWS>(w, a.group, t));
+__device__ __forceinline__ int sequence_units(const AttnArgs& a, const Walk& w, int lane, int lanes) {
+    int n = 0;
+#pragma unroll 1
+    for (int t = lane; t < w.n_tiles; t += lanes) n += tile_units(tile_seen<ROWS>(a, w, t));
     return n;
 }
 
 struct Plan {             // in shared memory
-    long long sums[16];
-    long long total, cut[2];   // units of all; this CTA's first and the one behind its last
-    Walk walk;                 // the tile of rows it begins in
+    int sums[16];
+    int total, cut[2];         // units of all; this CTA's first and the one behind its last
     int active;                // CTAs among which the units are divided
+    Walk walk;                 // the tile of rows it begins in
 };
-// where CTA c of `active` would begin if units were divided exactly
-__device__ __forceinline__ long long exact_cut(long long total, int active, int c) {
-    if (total < 1LL << 31) {
-        const int each = (int)total / active, rest = (int)total % active;
-        return (long long)each * c + rest * c / active;
-    }
-    return total / active * c + total % active * c / active;
-}
+// where CTA c of `active` would begin if units were divided exactly: total c / active
+__device__ __forceinline__ int exact_cut(int each, int rest, int active, int c) { return each * c + rest * c / active; }
 
 // All threads: the batch's units, this CTA's range of them, and the tile of rows it begins in.  false: nothing to do
 template <int ROWS, int THREADS>
@@ -171,73 +169,65 @@ __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p) {
         w.s = s;
         w.n_tiles = 0;
         if (s < a.batch.n_seqs) walk_sequence<ROWS>(a, w);
-        if (!wide) return a.n_kv * sequence_units<ROWS>(a, w, 0, 1);
-        long long n = sequence_units<ROWS>(a, w, lane, 32);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) n += __shfl_xor_sync(0xffffffffu, n, d);
-        return lane == 0 ? a.n_kv * n : 0LL;
+        int n = sequence_units<ROWS>(a, w, wide ? lane : 0, wide ? 32 : 1);
+        if (wide) {
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (lane > 0) n = 0;
+        }
+        return a.n_kv * n;
     };
-    long long mine = 0, units = 0;   // units: of the last round
+    int mine = 0, units = 0;   // units: of the last round
 #pragma unroll 1
     for (int r = 0; r < rounds; r++) {
         units = units_of(r * per_round + (wide ? warp : (int)threadIdx.x));
         mine += units;
     }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, d);
+    mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) p->sums[warp] = mine;
     __syncthreads();
-    long long total = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) total += p->sums[w];
-    const int active = (int)min((long long)gridDim.x, total), cta = (int)blockIdx.x;
+    const int total = __reduce_add_sync(0xffffffffu, lane < WARPS ? p->sums[lane] : 0);
+    const int active = min((int)gridDim.x, total), cta = (int)blockIdx.x;
     if (cta >= active) return false;
-    const long long begin = exact_cut(total, active, cta), end = cta + 1 == active ? total : exact_cut(total, active, cta + 1);
+    const int each = total / active, rest = total - each * active, begin = exact_cut(each, rest, active, cta), end = exact_cut(each, rest, active, cta + 1);
     if (threadIdx.x == 0) {
         p->total = total;
         p->active = active;
         if (end == total) p->cut[1] = total;
     }
-    long long before = 0;            // units of the rounds before
+    int before = 0;            // units of the rounds before
 #pragma unroll 1
     for (int r = 0; r < rounds; r++) {
         if (rounds > 1) units = units_of(r * per_round + (wide ? warp : (int)threadIdx.x));
-        long long upto = units;      // inclusive sums
+        int upto = units;      // inclusive sums
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const long long o = __shfl_up_sync(0xffffffffu, upto, d);
+            const int o = __shfl_up_sync(0xffffffffu, upto, d);
             if (lane >= d) upto += o;
         }
-        __syncthreads();             // (the sums before have been read)
+        __syncthreads();       // (the sums before have been read)
         if (lane == 31) p->sums[warp] = upto;
         __syncthreads();
-        long long base = before;
-#pragma unroll
-        for (int w = 0; w < WARPS; w++) {
-            if (w < warp) base += p->sums[w];
-            before += p->sums[w];
-        }
-        const long long at = base + upto - units;
+        const int sum = lane < WARPS ? p->sums[lane] : 0;
+        const int at = before + __reduce_add_sync(0xffffffffu, lane < warp ? sum : 0) + upto - units;
+        before += __reduce_add_sync(0xffffffffu, sum);
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
-            const long long cut = i ? end : begin;
+            const int cut = i ? end : begin;
             if (!(units > 0 && cut >= at && cut < at + units)) continue;   // one thread of the block goes on, for each of the two
             Walk w;
             w.s = r * per_round + (wide ? warp : (int)threadIdx.x);
             walk_sequence<ROWS>(a, w);
-            const long long per_head = units / a.n_kv;
-            long long in = cut - at;
-            w.kv = 0;
-            if (in >= per_head) {
-                w.kv = (int)(in / per_head);
-                in -= w.kv * per_head;
-            }
+            const int per_head = units / a.n_kv;
+            w.kv = min((cut - at) / per_head, a.n_kv - 1);
+            int in = cut - at - w.kv * per_head;
+#pragma unroll 1
             for (w.tile = 0;; w.tile++) {
                 walk_tile<ROWS>(a, w);
-                if (in < w.units) break;
+                if (in < w.units || w.tile + 1 == w.n_tiles) break;
                 in -= w.units;
             }
-            const int to = moved_cut(w, (int)in);
+            in = max(0, min(in, w.units - 1));   // (begins that do not ascend may pass what 32 bits count; whatever comes of them stays inside)
+            const int to = moved_cut(w, in);
             p->cut[i] = cut - in + to;
             if (i == 0) {
                 w.from = to;
@@ -399,14 +389,15 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     const bool any = plan_work<ROWS, Sh::THREADS>(a, plan);   // (with barriers of the block)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
-    long long left = any ? plan->cut[1] - plan->cut[0] : 0;
+    int left = any ? plan->cut[1] - plan->cut[0] : 0;
     Walk w = plan->walk;
-    w.to = (int)min((long long)w.units, w.from + left);
+    w.to = min(w.units, w.from + left);
 
-    if (any && warp == 0) {
-        // ---------------- keys and values: a lane a box of at most 128 slots x 64 elements ----------------
-        const int boxes = KEYS / a.box_rows, part = lane % boxes, block = lane / boxes;   // lanes behind the last box do nothing
-        const bool mine = block < CW / 64;
+    if (any && (warp == 0 || warp == 2 || warp == 3)) {
+        // ---------------- keys and values: a lane of one of three warps a box of at most 128 slots x 64 elements ----------------
+        // (A warp issues its lanes' copies one by one, some 80 clocks each: the 64 of 128 keys and values in pages of 16 took it as long as the memory does.)
+        const int boxes = KEYS / a.box_rows, loader = warp == 0 ? 0 : warp - 1, box = 3 * lane + loader, part = box & (boxes - 1), block = box / boxes;
+        const bool mine = block < CW / 64;   // lanes behind the last box do nothing
         const uint32_t to = (uint32_t)(block * BLOCK_BYTES + part * a.box_rows * 128), ring_u = smem_u32(ring), full_u = smem_u32(full), empty_u = smem_u32(empty);
         const int slots = (1 << a.batch.page_shift) - 1;
         uint32_t at = 0;   // stages filled so far
@@ -422,7 +413,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 for (int c = 0; c < NCH; c++, at++) {
                     const uint32_t st = at % STAGES, use = at / STAGES;
                     mbar_wait_bounded(empty_u + 8u * st, (use & 1u) ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
-                    if (lane == 0) mbar_arrive_expect_tx(full_u + 8u * st, STAGE);
+                    if (threadIdx.x == 0) mbar_arrive_expect_tx(full_u + 8u * st, STAGE);
                     __syncwarp();
                     if (mine) tma_load_4d(ring_u + st * STAGE + to, map, c * CW + block * 64, slot, w.kv, page, full_u + 8u * st);
                 }
@@ -506,31 +497,33 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     } else if (any) {
         // ---------------- weights: warpgroup g takes the scores that lie in place g, a thread a row ----------------
         // QT = 2: those of its own 128 rows.  QT = 1: those of every other tile of keys; the maxima go from one warpgroup to the other, and each has a sum of its own.
-        const int g = (warp - 2) >> 2, quad = warp & 3, t = QT == 2 ? g : 0, row = 128 * t + 32 * quad + lane;   // row: of the tile of rows
+        const int g = (warp >> 2) - 1, quad = warp & 3, t = QT == 2 ? g : 0, row = 128 * t + 32 * quad + lane;   // row: of the tile of rows
         const uint32_t lanes = (uint32_t)(32 * quad) << 16, o_tm = tmem + lanes + (uint32_t)(256 + t * DP), s_tm = tmem + lanes + (uint32_t)(g * KEYS);
         const uint32_t s_bar = smem_u32(&s_full[g]), p_bar = smem_u32(&p_full[g]), done_u = smem_u32(o_done);
         constexpr int COLS = QT == 2 ? DP : DP / 2;     // of the outputs this warpgroup stores
         const int col0 = QT == 2 ? 0 : g * COLS;
         const auto load_queries = [&](const Walk& v) {
-            constexpr int UNITS = DP / 8, SHARE = (QT == 2 ? 32 : 16) * UNITS, AHEAD = SHARE / 32 % 8 == 0 ? 8 : 4;    // 16-byte pieces of a row; of this warp's share; of a lane on their way
-            const int flat = v.row0 + row, there = row < v.rows, first = QT == 2 ? 0 : 16 * g;                      // (QT = 1: rows 16 g to 16 g + 15 of the 32)
-            const long long my_row = (long long)(v.first + flat / a.group) * a.q_row + (long long)(v.kv * a.group + flat % a.group) * a.q_head;
+            constexpr int UNITS = DP / 8, AHEAD = 8, STEP = QT == 2 ? 32 : 64;    // 16-byte pieces of a row; of a lane on their way; (QT = 1: the two warps of these rows take turns)
+            const int here = min(32, v.rows - (128 * t + 32 * quad)), pieces = here * UNITS;   // rows that are not there keep whatever they hold: it meets no other row
             uint8_t* to = q_at + t * 128 * DP * 2 + 32 * quad * 128;
+            if (here > 0) {
+                const int flat = v.row0 + row, in = by_group(a, flat);
+                const long long my_row = (long long)(v.first + in) * a.q_row + (long long)(v.kv * a.group + flat - in * a.group) * a.q_head;
 #pragma unroll 1
-            for (int u0 = 0; u0 < SHARE; u0 += 32 * AHEAD) {
-                uint4 x[AHEAD];
+                for (int u0 = (QT == 2 ? 0 : 32 * g) + lane; u0 - lane < pieces; u0 += STEP * AHEAD) {
+                    uint4 x[AHEAD];
 #pragma unroll
-                for (int n = 0; n < AHEAD; n++) {
-                    const int u = u0 + 32 * n + lane, r = first + u / UNITS, e = u % UNITS * 8;
-                    const long long at = __shfl_sync(0xffffffffu, my_row, r);
-                    const bool here = __shfl_sync(0xffffffffu, there, r) && e < a.D;
-                    x[n] = make_uint4(0, 0, 0, 0);
-                    if (here) x[n] = query_eight<C>(a, at + e);
-                }
+                    for (int n = 0; n < AHEAD; n++) {
+                        const int u = u0 + STEP * n, r = u / UNITS, e = u % UNITS * 8;
+                        const long long at = __shfl_sync(0xffffffffu, my_row, r & 31);
+                        x[n] = make_uint4(0, 0, 0, 0);
+                        if (u < pieces && e < a.D) x[n] = query_eight<C>(a, at + e);
+                    }
 #pragma unroll
-                for (int n = 0; n < AHEAD; n++) {
-                    const int u = u0 + 32 * n + lane, r = first + u / UNITS, e = u % UNITS * 8;
-                    *(uint4*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16) = x[n];
+                    for (int n = 0; n < AHEAD; n++) {
+                        const int u = u0 + STEP * n, r = u / UNITS, e = u % UNITS * 8;
+                        if (u < pieces) *(uint4*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16) = x[n];
+                    }
                 }
             }
             fence_proxy_async();
@@ -543,10 +536,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         bool more = true;
         while (more) {
             const int tiles = w.to - w.from, n = QT * tiles;
-            const int tok = (w.row0 + row) / a.group;
+            const int tok = by_group(a, w.row0 + row);
             const int limit = row < w.rows ? max(0, w.len - w.n_new + tok + 1) : w.seen;                          // keys this row sees
-            const int least = max(0, w.len - w.n_new + (w.row0 + min(128 * t + 32 * quad, w.rows - 1)) / a.group + 1);   // ... the warp's first row
-            const int least_item = max(0, w.len - w.n_new + w.row0 / a.group + 1);                                    // ... the item's first row
+            const int least = max(0, w.len - w.n_new + by_group(a, w.row0 + min(128 * t + 32 * quad, w.rows - 1)) + 1);   // ... the warp's first row
+            const int least_item = max(0, w.len - w.n_new + by_group(a, w.row0) + 1);                                    // ... the item's first row
             const bool idle = 128 * t + 32 * quad >= w.rows;   // no row of this warp's is there
             float m = -INFINITY, l = 0.0f;   // m: what is taken off, times c
             for (int i = g; i < n; i += 2) {
@@ -571,7 +564,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                             for (int k = 0; k < HALF; k++) v[k] = h * HALF + k < seen ? v[k] : 0xFF800000u;
                     };
                     float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
+#pragma unroll 1
                     for (int h = 1; h >= 0; h--) {
                         load_half(h);
 #pragma unroll
@@ -615,7 +608,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     const float off = (m == -INFINITY ? 0.0f : -m) + WEIGHT_BIAS<C>;
                     const uint64_t c2 = pack_f32x2(a.c, a.c), off2 = pack_f32x2(off, off);
                     uint64_t sum[2] = {0, 0};
-#pragma unroll
+#pragma unroll 1
                     for (int h = 0; h < 2; h++) {
                         if (h) load_half(1);
 #pragma unroll
@@ -720,8 +713,8 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             more = walk_next<ROWS>(a, w, left);
             if (more) load_queries(w);
             const bool whole = now.from == 0 && now.to == now.units;
-            const int flat = now.row0 + row, head = now.kv * a.group + flat % a.group;
-            const long long out_row = now.first + flat / a.group;
+            const int head = now.kv * a.group + now.row0 + row - tok * a.group;
+            const long long out_row = now.first + tok;
             if (idle) {
             } else if (whole) {
                 const float by = limit > 0 ? 1.0f / l : 0.0f;
@@ -753,12 +746,15 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         }
     }
     // The last tile of rows, if others go on with it, is this CTA's to announce: its parts are this CTA's and those of the CTAs up to the one with its last unit.
-    if (threadIdx.x == 64) {
+    if (threadIdx.x == 128) {
         Job job = {};
         if (any) {
             if (w.from == 0 && w.to < w.units) {
-                const long long last = plan->cut[1] + (w.units - w.to) - dear(w) - 1;   // the last unit in which one of its other parts may begin
-                job.n_parts = (int)(((last + 1) * plan->active - 1) / plan->total) - (int)blockIdx.x + 1;
+                // its parts: up to the last CTA that begins in it, no nearer to its end than a cut may lie
+                const int last = plan->cut[1] + (w.units - w.to) - dear(w) - 1, each = plan->total / plan->active, rest = plan->total - each * plan->active;
+                int c = min(plan->active - 1, (int)((float)last * (float)plan->active / (float)plan->total) + 1);   // (within one of it)
+                while (c > (int)blockIdx.x && exact_cut(each, rest, plan->active, c) > last) c--;
+                job.n_parts = c - (int)blockIdx.x + 1;
                 job.first = w.first;
                 job.n_new = w.n_new;
                 job.len = w.len;
@@ -893,6 +889,8 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     if ((n_heads > 1 && out_head < c->D) || (rows > 1 && out_row < c->D)) return Q38B_ERR_ARG;
     if (q_kind != Q38B_OUT_F32 && q_kind != c->kind) return Q38B_ERR_UNSUPPORTED;
     if ((long long)rows * n_heads > 0x3FFFFFFF) return Q38B_ERR_UNSUPPORTED;
+    // (units are counted in 32 bits)
+    if (((long long)rows * n_heads / 128 + (long long)c->n_seqs * c->n_heads) * ((long long)c->table_n * c->page_size / KEYS + 1) > 0x7FFFFFFF) return Q38B_ERR_UNSUPPORTED;
     if ((uintptr_t)q % kind_size(q_kind) || (uintptr_t)out % kind_size(out_kind) || ((uintptr_t)lse & 3) || ((uintptr_t)work & 15)) return Q38B_ERR_ALIGN;
     if (work_bytes < 16 || work_bytes < q38b_attention_work_bytes(ctx, n_heads, c->n_heads, c->D, rows)) return Q38B_ERR_NOMEM;
     DeviceGuard on(ctx);
@@ -912,6 +910,10 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     a.out_vec = (((uintptr_t)out | (uintptr_t)(out_row * kind_size(out_kind)) | (uintptr_t)(out_head * kind_size(out_kind))) & 15) == 0;
     a.pdl = ctx->pass_pdl ? 1 : 0;
     a.c = (float)((double)scale * 1.4426950408889634);
+    int log = 0;
+    while (1LL << log < a.group) log++;
+    a.group_shift = 31 + log;
+    a.group_mul = (uint32_t)(((1ULL << a.group_shift) + a.group - 1) / a.group);
     CUtensorMap kmap, vmap;
     if (!encode_pages(&kmap, c, c->k, c->k_page, c->k_slot, c->k_head, a.box_rows) || !encode_pages(&vmap, c, c->v, c->v_page, c->v_slot, c->v_head, a.box_rows)) return Q38B_ERR_ARG;
     // two tiles of rows share the keys' way into shared memory where sequences fill more than one on average and there are enough of them for all SMs
