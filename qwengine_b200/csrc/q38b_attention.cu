@@ -55,7 +55,7 @@ struct AttnArgs {
     int q_kind, out_kind, n_heads, n_kv, group, D, box_rows, slot_rows, q_vec, out_vec, pdl;
     float c;       // scale log2(e)
     uint32_t group_mul;   // x / group = x group_mul >> group_shift for 0 <= x < 2^31
-    int group_shift;
+    int group_shift, ctas;
 };
 __device__ __forceinline__ int by_group(const AttnArgs& a, int x) { return (int)((uint64_t)(uint32_t)x * a.group_mul >> a.group_shift); }
 
@@ -130,11 +130,16 @@ __device__ __forceinline__ bool walk_next(const AttnArgs& a, Walk& w, int& left)
     return true;
 }
 
+#ifndef DEARV
+#define DEARV 8192
+#endif
+constexpr int DEAR = DEARV;
 // A part of a tile of rows that others finish costs about as much as a tile of keys for every 32 of its rows (its sums go out to memory and come back).  So a range that
 // would begin or end within that of a tile's ends begins or ends there instead (5 sequences of 77 to 333 new tokens, 15 + 5 heads of 96: 62 us cut exactly, MEASURED_RAGGED so).
-__device__ __forceinline__ int dear(const Walk& w) { return w.rows / 32; }
+template <int DP> __device__ __forceinline__ int dear(const Walk& w) { return w.rows * DP / DEAR; }
+template <int DP>
 __device__ __forceinline__ int moved_cut(const Walk& w, int in) {   // a cut `in` units behind the first of a tile's
-    if (in > dear(w) && w.units - in > dear(w)) return in;
+    if (in > dear<DP>(w) && w.units - in > dear<DP>(w)) return in;
     return 2 * in <= w.units ? 0 : w.units;
 }
 
@@ -157,7 +162,7 @@ struct Plan {             // in shared memory
 __device__ __forceinline__ int exact_cut(int each, int rest, int active, int c) { return each * c + rest * c / active; }
 
 // All threads: the batch's units, this CTA's range of them, and the tile of rows it begins in.  false: nothing to do
-template <int ROWS, int THREADS>
+template <int DP, int ROWS, int THREADS>
 __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int WARPS = THREADS / 32;
@@ -227,7 +232,7 @@ __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p) {
                 in -= w.units;
             }
             in = max(0, min(in, w.units - 1));   // (begins that do not ascend may pass what 32 bits count; whatever comes of them stays inside)
-            const int to = moved_cut(w, in);
+            const int to = moved_cut<DP>(w, in);
             p->cut[i] = cut - in + to;
             if (i == 0) {
                 w.from = to;
@@ -360,6 +365,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     uint8_t* ring = q_at + Sh::Q_BYTES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    if (a.pdl) pdl_launch_dependents();   // (the joining kernel's blocks wait on SMs that have no work)
     if (threadIdx.x == 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
@@ -386,7 +392,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    const bool any = plan_work<ROWS, Sh::THREADS>(a, plan);   // (with barriers of the block)
+    const bool any = plan_work<DP, ROWS, Sh::THREADS>(a, plan);   // (with barriers of the block)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
     int left = any ? plan->cut[1] - plan->cut[0] : 0;
@@ -751,7 +757,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         if (any) {
             if (w.from == 0 && w.to < w.units) {
                 // its parts: up to the last CTA that begins in it, no nearer to its end than a cut may lie
-                const int last = plan->cut[1] + (w.units - w.to) - dear(w) - 1, each = plan->total / plan->active, rest = plan->total - each * plan->active;
+                const int last = plan->cut[1] + (w.units - w.to) - dear<DP>(w) - 1, each = plan->total / plan->active, rest = plan->total - each * plan->active;
                 int c = min(plan->active - 1, (int)((float)last * (float)plan->active / (float)plan->total) + 1);   // (within one of it)
                 while (c > (int)blockIdx.x && exact_cut(each, rest, plan->active, c) > last) c--;
                 job.n_parts = c - (int)blockIdx.x + 1;
@@ -767,7 +773,6 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (a.pdl) pdl_launch_dependents();
     if (warp == 1) {
         if (__builtin_expect(*abort_flag, 0)) settle_after_abort();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -775,51 +780,105 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     }
 }
 
-// Joins the parts of a tile of rows: a thread four elements of a row.
+// Joins the parts of tiles of rows.  A piece of work is 32 rows (the lanes: what a part left lies so) of two groups of four elements where there are many
+// parts, to each of which four warps go with every fourth part, of eight groups where there are few.  The blocks share out the pieces of all tiles that were cut.
 template <int DP>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, float bias) {
+    __shared__ int upto[256], sums[8];
+    __shared__ float4 o_of[8][32];
+    __shared__ float2 ml_of[8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_jobs = a.ctas;
     if (a.pdl) pdl_wait_prior();
-    const Job job = a.jobs[blockIdx.x];
-    const int at = (int)(blockIdx.y * 256 + threadIdx.x), row = at / (DP / 4), e = at % (DP / 4) * 4;
-    if (job.n_parts == 0 || row >= job.rows) return;
-    const long long slot = (long long)a.slot_rows * (DP + 4);
-    const auto place = [&](int p) { return a.slots + (p == 0 ? 2 * (long long)blockIdx.x + 1 : 2 * ((long long)blockIdx.x + p)) * slot; };
-    float top = -INFINITY;
-    for (int p = 0; p < job.n_parts; p++) top = fmaxf(top, place(p)[(long long)a.slot_rows * DP + 2 * row]);
-    const float off = top == -INFINITY ? 0.0f : top;
-    float l = 0.0f, o[4] = {};
-#pragma unroll 4
-    for (int p = 0; p < job.n_parts; p++) {
-        const float* s = place(p);
-        const float2 ml = *(const float2*)(s + (long long)a.slot_rows * DP + 2 * row);
-        const float4 x = *(const float4*)(s + (long long)(e / 4 * a.slot_rows + row) * 4);
-        const float by = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - off);
-        l = fmaf(by, ml.y, l);
-        o[0] = fmaf(by, x.x, o[0]);
-        o[1] = fmaf(by, x.y, o[1]);
-        o[2] = fmaf(by, x.z, o[2]);
-        o[3] = fmaf(by, x.w, o[3]);
+    // pieces of the jobs before and of each itself
+    const auto warps_a_group = [](int n_parts) { return n_parts >= 8 ? 4 : 1; };
+    int n = 0;
+    if ((int)threadIdx.x < n_jobs) {
+        const Job j = a.jobs[threadIdx.x];
+        if (j.n_parts > 0) n = (j.rows + 31) / 32 * (DP / 4 * warps_a_group(j.n_parts) / 8);
     }
-    const int flat = job.row0 + row, head = job.kv * a.group + flat % a.group;
-    const long long out_row = job.first + flat / a.group;
-    const bool sees = job.len - job.n_new + flat / a.group + 1 > 0;
-    const float by = 1.0f / l;
-    if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (off + log2f(l) - bias) : -INFINITY;
-    if (e >= a.D) return;
 #pragma unroll
-    for (int i = 0; i < 4; i++) o[i] = sees ? o[i] * by : 0.0f;
-    const long long to = out_row * a.out_row + (long long)head * a.out_head + e;
-    if (a.out_kind == Q38B_OUT_F32) {
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, n, d);
+        if (lane >= d) n += o;
+    }
+    if (lane == 31) sums[warp] = n;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) n += sums[w];
+    upto[threadIdx.x] = n;
+    __syncthreads();
+    const int total = upto[255];
+    const long long slot = (long long)a.slot_rows * (DP + 4);
+    for (int piece = (int)blockIdx.x; piece < total; piece += (int)gridDim.x) {
+        int lo = 0;   // the first job whose pieces end behind this one
 #pragma unroll
-        for (int i = 0; i < 4; i++) ((float*)a.out)[to + i] = o[i];
-    } else {
-        const uint32_t lo = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(o[0], o[1]) : pack2<__nv_bfloat16>(o[0], o[1]);
-        const uint32_t hi = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(o[2], o[3]) : pack2<__nv_bfloat16>(o[2], o[3]);
-        uint16_t* p = (uint16_t*)a.out + to;
-        if (a.out_vec) {
-            *(uint2*)p = make_uint2(lo, hi);
+        for (int d = 128; d; d >>= 1)
+            if (upto[lo + d - 1] <= piece) lo += d;
+        const Job job = a.jobs[lo];
+        const int in = piece - (lo ? upto[lo - 1] : 0), wpg = warps_a_group(job.n_parts), groups = 8 / wpg, chunks = DP / 4 / groups;
+        const int row = in / chunks * 32 + lane, col = in % chunks * groups + warp / wpg, part = warp % wpg;
+        const bool here = row < job.rows;
+        float m = -INFINITY, l = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const auto add = [&](float m2, float l2, const float4& o2) {
+            const float top = fmaxf(m, m2), by = m == -INFINITY ? 0.0f : exp2_fast(m - top), by2 = m2 == -INFINITY ? 0.0f : exp2_fast(m2 - top);
+            l = l * by + l2 * by2;
+            o.x = o.x * by + o2.x * by2;
+            o.y = o.y * by + o2.y * by2;
+            o.z = o.z * by + o2.z * by2;
+            o.w = o.w * by + o2.w * by2;
+            m = top;
+        };
+        if (here) {
+            constexpr int AHEAD = 4;
+#pragma unroll 1
+            for (int p0 = part; p0 < job.n_parts; p0 += wpg * AHEAD) {
+                float2 ml[AHEAD];
+                float4 x[AHEAD];
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) {
+                    const int p = p0 + wpg * i;
+                    ml[i] = make_float2(-INFINITY, 0.0f);
+                    x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (p < job.n_parts) {
+                        const float* s = a.slots + (p == 0 ? 2 * (long long)lo + 1 : 2 * ((long long)lo + p)) * slot;
+                        ml[i] = *(const float2*)(s + (long long)a.slot_rows * DP + 2 * row);
+                        x[i] = *(const float4*)(s + (long long)(col * a.slot_rows + row) * 4);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++)
+                    if (p0 + wpg * i < job.n_parts) add(ml[i].x, ml[i].y, x[i]);
+            }
+        }
+        if (wpg > 1) {   // (the same for the whole block)
+            o_of[warp][lane] = o;
+            ml_of[warp][lane] = make_float2(m, l);
+            __syncthreads();
+            if (part == 0)
+                for (int i = 1; i < wpg; i++) add(ml_of[warp + i][lane].x, ml_of[warp + i][lane].y, o_of[warp + i][lane]);
+            __syncthreads();
+        }
+        if (part != 0 || !here) continue;
+        const int tok = by_group(a, job.row0 + row), head = job.kv * a.group + job.row0 + row - tok * a.group, e = 4 * col;
+        const long long out_row = job.first + tok;
+        const bool sees = job.len - job.n_new + tok + 1 > 0;
+        const float by = 1.0f / l;
+        if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (m + log2f(l) - bias) : -INFINITY;
+        if (e >= a.D) continue;
+        const float f[4] = {sees ? o.x * by : 0.0f, sees ? o.y * by : 0.0f, sees ? o.z * by : 0.0f, sees ? o.w * by : 0.0f};
+        const long long to = out_row * a.out_row + (long long)head * a.out_head + e;
+        if (a.out_kind == Q38B_OUT_F32) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) ((float*)a.out)[to + i] = f[i];
         } else {
-            p[0] = (uint16_t)lo; p[1] = (uint16_t)(lo >> 16); p[2] = (uint16_t)hi; p[3] = (uint16_t)(hi >> 16);
+            const uint32_t w0 = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(f[0], f[1]) : pack2<__nv_bfloat16>(f[0], f[1]);
+            const uint32_t w1 = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(f[2], f[3]) : pack2<__nv_bfloat16>(f[2], f[3]);
+            uint16_t* p = (uint16_t*)a.out + to;
+            if (a.out_vec) {
+                *(uint2*)p = make_uint2(w0, w1);
+            } else {
+                p[0] = (uint16_t)w0; p[1] = (uint16_t)(w0 >> 16); p[2] = (uint16_t)w1; p[3] = (uint16_t)(w1 >> 16);
+            }
         }
     }
 }
@@ -834,6 +893,7 @@ bool encode_pages(CUtensorMap* map, const q38b_paged_kv* c, const void* base, lo
                       CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+int ctas(const q38b_ctx* ctx) { return std::min(ctx->sm_count, 256); }   // (the joining kernel counts their work with a thread each)
 int padded(int D) { return (D + 63) / 64 * 64; }
 // rows of a place in the work area
 int slot_rows(int group, int D, int rows) { return (int)std::min((long long)(padded(D) <= 128 ? 256 : 128), (long long)rows * group); }
@@ -843,12 +903,12 @@ int attention_as(q38b_ctx* ctx, const AttnArgs& a, const CUtensorMap& kmap, cons
     auto kern = attention_kernel<C, DP, QT>;
     const int rc = q38b_ensure_kernel_smem(ctx, (const void*)kern, ctx->smem_optin, false);
     if (rc != Q38B_OK) return rc;
-    kern<<<(unsigned)ctx->sm_count, Shape<DP, QT>::THREADS, Shape<DP, QT>::SMEM, st>>>(a, kmap, vmap);
+    kern<<<(unsigned)ctas(ctx), Shape<DP, QT>::THREADS, Shape<DP, QT>::SMEM, st>>>(a, kmap, vmap);
     const int done = launch_status(ctx, cudaSuccess);
     if (done != Q38B_OK) return done;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3((unsigned)ctx->sm_count, (unsigned)((std::min(a.slot_rows, Shape<DP, QT>::ROWS) * (DP / 4) + 255) / 256));
+    cfg.gridDim = dim3(4u * (unsigned)ctx->sm_count);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -877,7 +937,7 @@ extern "C" {
 
 size_t q38b_attention_work_bytes(const q38b_ctx* ctx, int n_heads, int n_kv_heads, int D, int rows) {
     if (!ctx || n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads || D < 8 || D > 256 || D % 8 || rows < 1) return 0;
-    return (size_t)ctx->sm_count * (sizeof(Job) + 2 * (size_t)slot_rows(n_heads / n_kv_heads, D, rows) * (padded(D) + 4) * 4);
+    return (size_t)ctas(ctx) * (sizeof(Job) + 2 * (size_t)slot_rows(n_heads / n_kv_heads, D, rows) * (padded(D) + 4) * 4);
 }
 
 int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_kind, long long q_row, long long q_head, int n_heads, float scale, void* out,
@@ -903,8 +963,9 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     a.q_kind = q_kind; a.out_kind = out_kind; a.n_heads = n_heads; a.n_kv = c->n_heads; a.group = n_heads / c->n_heads; a.D = c->D;
     a.box_rows = std::min(c->page_size, KEYS);
     a.slot_rows = slot_rows(a.group, c->D, rows);
+    a.ctas = ctas(ctx);
     a.jobs = (Job*)work;
-    a.slots = (float*)((uint8_t*)work + (size_t)ctx->sm_count * sizeof(Job));
+    a.slots = (float*)((uint8_t*)work + (size_t)ctas(ctx) * sizeof(Job));
     a.status = ctx->d_status;
     a.q_vec = (((uintptr_t)q | (uintptr_t)(q_row * kind_size(q_kind)) | (uintptr_t)(q_head * kind_size(q_kind))) & 15) == 0;
     a.out_vec = (((uintptr_t)out | (uintptr_t)(out_row * kind_size(out_kind)) | (uintptr_t)(out_head * kind_size(out_kind))) & 15) == 0;
