@@ -55,7 +55,7 @@ struct AttnArgs {
     int q_kind, out_kind, n_heads, n_kv, group, D, box_rows, slot_rows, q_vec, out_vec, pdl;
     float c;       // scale log2(e)
     uint32_t group_mul;   // x / group = x group_mul >> group_shift for 0 <= x < 2^31
-    int group_shift, ctas;
+    int group_shift, ctas, q_shift;   // q_shift: log2 of the bytes of a query's element
 };
 __device__ __forceinline__ int by_group(const AttnArgs& a, int x) { return (int)((uint64_t)(uint32_t)x * a.group_mul >> a.group_shift); }
 
@@ -288,58 +288,15 @@ template <typename C> __device__ __forceinline__ uint32_t no_number(uint32_t w) 
 }
 template <typename T> __device__ __forceinline__ float load_as(const void* p, long long at) { return to_f32(((const T*)p)[at]); }
 
-// Eight elements of a query as they go to shared memory: rounded to the cache's type
 template <typename C>
-__device__ __forceinline__ uint4 query_eight(const AttnArgs& a, long long at) {
-    uint4 r;
-    if (a.q_kind == Q38B_OUT_F32) {
-        float v[8];
-        const float* p = (const float*)a.q + at;
-        if (a.q_vec) {
-            *(float4*)v = *(const float4*)p;
-            *(float4*)(v + 4) = *(const float4*)(p + 4);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = p[i];
-        }
-        r.x = pack2<C>(v[0], v[1]); r.y = pack2<C>(v[2], v[3]); r.z = pack2<C>(v[4], v[5]); r.w = pack2<C>(v[6], v[7]);
-        return r;
-    }
-    const uint16_t* p = (const uint16_t*)a.q + at;
-    if (a.q_vec) return *(const uint4*)p;
-    uint32_t h[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) h[i] = (uint32_t)p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
-    return make_uint4(h[0], h[1], h[2], h[3]);
+__device__ __forceinline__ float query_one(const AttnArgs& a, long long at) {
+    return a.q_kind == Q38B_OUT_F32 ? to_f32(from_f32<C>(((const float*)a.q)[at])) : to_f32(((const C*)a.q)[at]);
 }
 
-// 16 outputs of a row, of which the first `n` are there
-__device__ __forceinline__ void store16(const AttnArgs& a, long long at, const float (&f)[16], int n) {
-    if (a.out_kind == Q38B_OUT_F32) {
-        float* p = (float*)a.out + at;
-        if (a.out_vec) {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                if (i < n) *(float4*)(p + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (i < n) p[i] = f[i];
-        }
-        return;
-    }
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) w[i] = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(f[2 * i], f[2 * i + 1]) : pack2<__nv_bfloat16>(f[2 * i], f[2 * i + 1]);
-    uint16_t* p = (uint16_t*)a.out + at;
-    if (a.out_vec) {
-        if (n > 0) *(uint4*)p = make_uint4(w[0], w[1], w[2], w[3]);
-        if (n > 8) *(uint4*)(p + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-            if (i < n) p[i] = (uint16_t)(w[i / 2] >> (16 * (i & 1)));
-    }
+__device__ __forceinline__ void store_one(const AttnArgs& a, long long at, float f) {
+    if (a.out_kind == Q38B_OUT_F32) ((float*)a.out)[at] = f;
+    else if (a.out_kind == Q38B_OUT_F16) ((__half*)a.out)[at] = __float2half_rn(f);
+    else ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(f);
 }
 
 template <typename C, int DP, int QT>
@@ -355,10 +312,12 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     uint64_t* o_done = p_full + 2;   // [2] ... have been multiplied with values
     uint64_t* m_full = o_done + 2;   // [2][4] QT = 1: the maxima that a warp of either warpgroup took off are known to the other
     uint64_t* q_full = m_full + 8;
-    uint32_t* tmem_slot = (uint32_t*)(q_full + 1);
+    uint64_t* w_full = q_full + 1;   // [8] a tile of rows is known
+    uint32_t* tmem_slot = (uint32_t*)(w_full + 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     volatile int* spoilt = abort_flag + 1;   // [2]: the item that met values that are no numbers among keys that not all of its rows see
     Plan* plan = (Plan*)(smem + 512);
+    Walk* walks = (Walk*)(smem + 6144);          // [8] the CTA's tiles of rows, as the first loading warp goes through them (it is at most half a ring ahead)
     float* m_rows = (float*)(smem + 1024);       // [2][128]
     float2* ml_rows = (float2*)(smem + 2048);    // [2][2][128]
     uint8_t* q_at = smem + HEAD;
@@ -384,6 +343,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         }
         for (int s = 0; s < 8; s++) mbar_init(smem_u32(&m_full[s]), 1);
         mbar_init(smem_u32(q_full), 8);
+        for (int s = 0; s < 8; s++) mbar_init(smem_u32(&w_full[s]), 1);
         mbar_fence_init();
         fence_proxy_async();
     }
@@ -407,15 +367,34 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         const uint32_t to = (uint32_t)(block * BLOCK_BYTES + part * a.box_rows * 128), ring_u = smem_u32(ring), full_u = smem_u32(full), empty_u = smem_u32(empty);
         const int slots = (1 << a.batch.page_shift) - 1;
         uint32_t at = 0;   // stages filled so far
+        int item = 0;
+        const auto publish = [&](const Walk& v) {
+            if (threadIdx.x == 0) {
+                walks[item & 7] = v;
+                mbar_arrive(smem_u32(&w_full[item & 7]));
+            }
+            item++;
+        };
         do {
+            publish(w);
             const int n = w.to - w.from;
-            const auto page_of = [&](int j) {   // of this lane's box of tile j; keys nobody sees come as zeros, from a page that is not there
-                const int token = (w.from + j) * KEYS + part * a.box_rows;
-                return token < w.seen ? a.batch.page(w.s, token) : a.batch.n_pages;
+            // the steps in the order in which the tensor core takes them: keys K0 K1 V0 K2 V1 .. (QT = 1), K0 V0 K1 V1 .. (QT = 2); a step's page is looked up during the one before
+            const auto tile_of = [&](int i, bool& values) {
+                values = QT == 2 ? i & 1 : i == 2 * n - 1 || (i > 0 && !(i & 1));
+                return QT == 2 ? i >> 1 : i == 2 * n - 1 ? n - 1 : values ? i / 2 - 1 : (i + 1) / 2;
             };
-            const auto ask = [&](const CUtensorMap* map, int j, int page) {
-                const int slot = ((w.from + j) * KEYS + part * a.box_rows) & slots;
-#pragma unroll
+            const auto page_of = [&](int i) {   // of this lane's box; keys nobody sees come as zeros, from a page that is not there
+                bool values;
+                const int token = (w.from + tile_of(i, values)) * KEYS + part * a.box_rows;
+                return i < 2 * n && token < w.seen ? a.batch.page(w.s, token) : a.batch.n_pages;
+            };
+            int page = page_of(0);
+#pragma unroll 1
+            for (int i = 0; i < 2 * n; i++) {
+                bool values;
+                const int slot = ((w.from + tile_of(i, values)) * KEYS + part * a.box_rows) & slots, next = page_of(i + 1);
+                const CUtensorMap* map = values ? &vmap : &kmap;
+#pragma unroll 1
                 for (int c = 0; c < NCH; c++, at++) {
                     const uint32_t st = at % STAGES, use = at / STAGES;
                     mbar_wait_bounded(empty_u + 8u * st, (use & 1u) ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
@@ -423,23 +402,11 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     __syncwarp();
                     if (mine) tma_load_4d(ring_u + st * STAGE + to, map, c * CW + block * 64, slot, w.kv, page, full_u + 8u * st);
                 }
-            };
-            int page_k = page_of(0), page_v = page_k;
-            ask(&kmap, 0, page_k);
-            for (int j = 0; j < n; j++) {
-                if (QT == 2) {
-                    const int next = j + 1 < n ? page_of(j + 1) : 0;
-                    ask(&vmap, j, page_v);
-                    if (j + 1 < n) ask(&kmap, j + 1, next);
-                    page_v = next;
-                } else {
-                    const int next = j + 1 < n ? page_of(j + 1) : 0;
-                    if (j + 1 < n) ask(&kmap, j + 1, next);
-                    ask(&vmap, j, page_v);
-                    page_v = next;
-                }
+                page = next;
             }
         } while (walk_next<ROWS>(a, w, left));
+        w.to = w.from;   // no more
+        publish(w);
     } else if (any && warp == 1) {
         // ---------------- products ----------------
         constexpr uint32_t TYPE = std::is_same<C, __half>::value ? 0u : 1u;
@@ -448,13 +415,15 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         const uint64_t kdesc0 = umma_desc_sw128(0), vdesc0 = umma_desc_mn_sw128(0);
         const uint32_t q_u = smem_u32(q_at), ring_u = smem_u32(ring), full_u = smem_u32(full), empty_u = smem_u32(empty);
         uint32_t ring0 = 0, p_phase = 0, item = 0;
-        do {
-            const int tiles = w.to - w.from, n = QT * tiles;
+        for (;;) {
+            mbar_wait_bounded(smem_u32(&w_full[item & 7]), item >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+            const int tiles = walks[item & 7].to - walks[item & 7].from, n = QT * tiles;
+            if (tiles <= 0) break;
             mbar_wait_bounded(smem_u32(q_full), item & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
             const auto scores = [&](int i) {
                 const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
                 const uint32_t d = tmem + (uint32_t)((i & 1) * KEYS);
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < NCH; c++) {
                     const uint32_t at = ring0 + at_keys<QT, NCH>(tile) + c, st = at % STAGES;
                     mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
@@ -479,7 +448,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
                     mbar_wait_bounded(smem_u32(&p_full[i & 1]), p_phase >> (i & 1) & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
                     p_phase ^= 1u << (i & 1);
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < NCH; c++) {
                         const uint32_t at = ring0 + at_values<QT, NCH>(tile, tiles) + c, st = at % STAGES;
                         mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
@@ -499,7 +468,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             }
             ring0 += (uint32_t)(2 * tiles * NCH);
             item++;
-        } while (walk_next<ROWS>(a, w, left));
+        }
     } else if (any) {
         // ---------------- weights: warpgroup g takes the scores that lie in place g, a thread a row ----------------
         // QT = 2: those of its own 128 rows.  QT = 1: those of every other tile of keys; the maxima go from one warpgroup to the other, and each has a sum of its own.
@@ -509,7 +478,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         constexpr int COLS = QT == 2 ? DP : DP / 2;     // of the outputs this warpgroup stores
         const int col0 = QT == 2 ? 0 : g * COLS;
         const auto load_queries = [&](const Walk& v) {
-            constexpr int UNITS = DP / 8, AHEAD = 8, STEP = QT == 2 ? 32 : 64;    // 16-byte pieces of a row; of a lane on their way; (QT = 1: the two warps of these rows take turns)
+            constexpr int UNITS = DP / 8, AHEAD = 4, STEP = QT == 2 ? 32 : 64;    // 16-byte pieces of a row; of a lane on their way; (QT = 1: the two warps of these rows take turns)
             const int here = min(32, v.rows - (128 * t + 32 * quad)), pieces = here * UNITS;   // rows that are not there keep whatever they hold: it meets no other row
             uint8_t* to = q_at + t * 128 * DP * 2 + 32 * quad * 128;
             if (here > 0) {
@@ -517,18 +486,38 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 const long long my_row = (long long)(v.first + in) * a.q_row + (long long)(v.kv * a.group + flat - in * a.group) * a.q_head;
 #pragma unroll 1
                 for (int u0 = (QT == 2 ? 0 : 32 * g) + lane; u0 - lane < pieces; u0 += STEP * AHEAD) {
-                    uint4 x[AHEAD];
+                    long long at[AHEAD];
+                    uint4 x[AHEAD], y[AHEAD];
+                    // 16 bytes of the cache's type, or 32 of fp32, of each piece; what is not aligned goes an element at a time below
 #pragma unroll
                     for (int n = 0; n < AHEAD; n++) {
-                        const int u = u0 + STEP * n, r = u / UNITS, e = u % UNITS * 8;
-                        const long long at = __shfl_sync(0xffffffffu, my_row, r & 31);
-                        x[n] = make_uint4(0, 0, 0, 0);
-                        if (u < pieces && e < a.D) x[n] = query_eight<C>(a, at + e);
+                        const int u = u0 + STEP * n;
+                        at[n] = __shfl_sync(0xffffffffu, my_row, u / UNITS & 31) + u % UNITS * 8;
+                        x[n] = y[n] = make_uint4(0, 0, 0, 0);
+                        if (a.q_vec && u < pieces && u % UNITS * 8 < a.D) {
+                            const uint4* p = (const uint4*)((const uint8_t*)a.q + (at[n] << a.q_shift));
+                            x[n] = p[0];
+                            if (a.q_shift == 2) y[n] = p[1];
+                        }
                     }
 #pragma unroll
                     for (int n = 0; n < AHEAD; n++) {
                         const int u = u0 + STEP * n, r = u / UNITS, e = u % UNITS * 8;
+                        if (a.q_shift == 2)
+                            x[n] = make_uint4(pack2<C>(__uint_as_float(x[n].x), __uint_as_float(x[n].y)), pack2<C>(__uint_as_float(x[n].z), __uint_as_float(x[n].w)),
+                                              pack2<C>(__uint_as_float(y[n].x), __uint_as_float(y[n].y)), pack2<C>(__uint_as_float(y[n].z), __uint_as_float(y[n].w)));
                         if (u < pieces) *(uint4*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16) = x[n];
+                    }
+                }
+                if (!a.q_vec) {
+                    __syncwarp();
+#pragma unroll 1
+                    for (int u = (QT == 2 ? 0 : 32 * g) + lane; u - lane < pieces; u += STEP) {
+                        const int r = u / UNITS, e = u % UNITS * 8;
+                        const long long at = __shfl_sync(0xffffffffu, my_row, r & 31) + e;
+                        if (u < pieces && e < a.D)
+#pragma unroll 1
+                            for (int i = 0; i < 8; i++) *(C*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16 + 2 * i) = from_f32<C>(query_one<C>(a, at + i));
                     }
                 }
             }
@@ -537,17 +526,131 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             if (lane == 0) mbar_arrive(smem_u32(q_full));
         };
         uint32_t ring0 = 0, s_use = 0, m_use = 0, done[2] = {0, 0};   // done: products P V from either place up to this item
-        int item = 0;
-        load_queries(w);
-        bool more = true;
-        while (more) {
-            const int tiles = w.to - w.from, n = QT * tiles;
-            const int tok = by_group(a, w.row0 + row);
-            const int limit = row < w.rows ? max(0, w.len - w.n_new + tok + 1) : w.seen;                          // keys this row sees
+        int item;   // the tile of rows in front of the one that is worked on
+        const auto walk_of = [&](int i) {
+            mbar_wait_bounded(smem_u32(&w_full[i & 7]), (uint32_t)i >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+            return walks[i & 7];
+        };
+        // A round ends a tile of rows: the next one's queries go in place while its last products run, its outputs leave, the next one's scores become weights.
+        Walk next = walk_of(0);
+        float m = -INFINITY, l = 0.0f;   // m: what is taken off, times c
+        int tiles = 0, n = 0, tok = 0, limit = 0, least_item = 0;
+        bool idle = true;
+        for (item = -1;; item++) {
+            const bool more = next.to > next.from;
+            if (more) load_queries(next);
+            if (item >= 0) {
+                {
+                    const int last = QT == 2 ? n - 2 + g : n - 1;
+                    mbar_wait_bounded(done_u + 8u * (uint32_t)(last & 1), (done[last & 1] + (uint32_t)(last >> 1)) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                }
+                done[0] += (uint32_t)((n + 1) >> 1);
+                done[1] += (uint32_t)(n >> 1);
+                if (least_item < w.seen && spoilt[item & 1] == item) {
+                    // Rare: what was taken out of the products goes to the rows that see it, a value at a time.
+                    const int lo = max(least_item, w.from * KEYS), hi = min(w.seen, w.to * KEYS);
+                    const long long q_row = (long long)(w.first + tok) * a.q_row + (long long)(w.kv * a.group + w.row0 + row - tok * a.group) * a.q_head;
+                    for (int j = lo; j < hi; j++) {
+                        const int page = a.batch.page(w.s, j);
+                        if (page >= a.batch.n_pages) continue;
+                        const long long in = j & ((1 << a.batch.page_shift) - 1);
+                        const long long v_at = page * a.v_page + in * a.v_slot + w.kv * a.v_head, k_at = page * a.k_page + in * a.k_slot + w.kv * a.k_head;
+                        float weight = 0.0f;
+                        bool known = false;
+                        for (int e = col0; e < min(a.D, col0 + COLS); e++) {
+                            const float x = load_as<C>(a.v, v_at + e);
+                            if (fabsf(x) < INFINITY) continue;
+                            if (!known) {
+                                float dot = 0.0f;
+                                if (row < w.rows)
+                                    for (int d = 0; d < a.D; d++) dot = fmaf(query_one<C>(a, q_row + d), load_as<C>(a.k, k_at + d), dot);
+                                weight = exp2_fast(fmaf(dot, a.c, (m == -INFINITY ? 0.0f : -m) + WEIGHT_BIAS<C>));
+                                known = true;
+                            }
+                            uint32_t o;
+                            __syncwarp();
+                            asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(o_tm + (uint32_t)e) : "memory");
+                            tmem_ld_wait();
+                            asm volatile("" : "+r"(o));
+                            if (j < limit) o = __float_as_uint(fmaf(weight, x, __uint_as_float(o)));
+                            asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(o_tm + (uint32_t)e), "r"(o) : "memory");
+                            tmem_st_wait();
+                        }
+                    }
+                }
+                const bool whole = w.from == 0 && w.to == w.units;
+                const int head = w.kv * a.group + w.row0 + row - tok * a.group;
+                const long long out_row = w.first + tok;
+                if (idle) {
+                } else if (whole) {
+                    const float by = limit > 0 ? 1.0f / l : 0.0f;
+                    const long long out_at = out_row * a.out_row + (long long)head * a.out_head;
+                    if (a.out_vec && (a.out_kind == Q38B_OUT_F32 || a.out_kind == (std::is_same<C, __half>::value ? Q38B_OUT_F16 : Q38B_OUT_BF16))) {
+#pragma unroll 1
+                        for (int k0 = col0; k0 < col0 + COLS; k0 += 32) {
+                            uint32_t o[32];
+                            tmem_ld16_start(o_tm + (uint32_t)k0, o);
+                            tmem_ld16_start(o_tm + (uint32_t)k0 + 16, o + 16);
+                            tmem_ld_wait();
+                            tmem_ld_arrived(o);
+                            tmem_ld_arrived(o + 16);
+                            if (row >= w.rows) continue;
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] = limit > 0 ? __float_as_uint(__uint_as_float(o[e]) * by) : 0u;
+                            if (a.out_kind == Q38B_OUT_F32) {
+#pragma unroll
+                                for (int e = 0; e < 32; e += 4)
+                                    if (k0 + e < a.D) *(uint4*)((float*)a.out + out_at + k0 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 32; e += 2) o[e / 2] = pack2<C>(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+#pragma unroll
+                                for (int e = 0; e < 32; e += 8)
+                                    if (k0 + e < a.D) *(uint4*)((uint16_t*)a.out + out_at + k0 + e) = make_uint4(o[e / 2], o[e / 2 + 1], o[e / 2 + 2], o[e / 2 + 3]);
+                            }
+                        }
+                    } else {   // another type or alignment: a column at a time
+#pragma unroll 1
+                        for (int k = col0; k < min(a.D, col0 + COLS); k++) {
+                            uint32_t o;
+                            asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(o_tm + (uint32_t)k) : "memory");
+                            tmem_ld_wait();
+                            asm volatile("" : "+r"(o));
+                            if (row < w.rows) store_one(a, out_at + k, limit > 0 ? __uint_as_float(o) * by : 0.0f);
+                        }
+                    }
+                    if (a.lse && row < w.rows && col0 == 0) a.lse[out_row * a.n_heads + head] = limit > 0 ? 0.6931471805599453f * (m + log2f(l) - WEIGHT_BIAS<C>) : -INFINITY;
+                } else {
+                    // a place in the work area: [4 columns][row] and each row's m and l behind
+                    float* to = a.slots + (long long)(2 * blockIdx.x + (w.from == 0 ? 1 : 0)) * a.slot_rows * (DP + 4);
+#pragma unroll 1
+                    for (int k = col0; k < col0 + COLS; k += 32) {
+                        uint32_t o[32];
+                        tmem_ld16_start(o_tm + (uint32_t)k, o);
+                        tmem_ld16_start(o_tm + (uint32_t)k + 16, o + 16);
+                        tmem_ld_wait();
+                        tmem_ld_arrived(o);
+                        tmem_ld_arrived(o + 16);
+                        if (row < w.rows)
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4) *(uint4*)(to + (long long)((k + e) / 4 * a.slot_rows + row) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                    }
+                    if (row < w.rows && col0 == 0) *(float2*)(to + (long long)a.slot_rows * DP + 2 * row) = make_float2(m, l);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            }
+            if (!more) break;
+            w = next;
+            tiles = w.to - w.from;
+            n = QT * tiles;
+            tok = by_group(a, w.row0 + row);
+            limit = row < w.rows ? max(0, w.len - w.n_new + tok + 1) : w.seen;                          // keys this row sees
             const int least = max(0, w.len - w.n_new + by_group(a, w.row0 + min(128 * t + 32 * quad, w.rows - 1)) + 1);   // ... the warp's first row
-            const int least_item = max(0, w.len - w.n_new + by_group(a, w.row0) + 1);                                    // ... the item's first row
-            const bool idle = 128 * t + 32 * quad >= w.rows;   // no row of this warp's is there
-            float m = -INFINITY, l = 0.0f;   // m: what is taken off, times c
+            least_item = max(0, w.len - w.n_new + by_group(a, w.row0) + 1);                                    // ... the item's first row
+            idle = 128 * t + 32 * quad >= w.rows;   // no row of this warp's is there
+            m = -INFINITY;
+            l = 0.0f;
             for (int i = g; i < n; i += 2) {
                 const int tile = QT == 2 ? i >> 1 : i, j0 = (w.from + tile) * KEYS;
                 mbar_wait_bounded(s_bar, s_use & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
@@ -651,7 +754,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                             const uint4 y = *x;
                             const uint4 bad = make_uint4(no_number<C>(y.x), no_number<C>(y.y), no_number<C>(y.z), no_number<C>(y.w));
                             if (bad.x | bad.y | bad.z | bad.w) {
-                                spoilt[item & 1] = item;
+                                spoilt[(item + 1) & 1] = item + 1;
                                 __threadfence_block();   // (whoever finds these zeros finds the mark too)
                                 *x = make_uint4(y.x & ~bad.x, y.y & ~bad.y, y.z & ~bad.z, y.w & ~bad.w);
                             }
@@ -666,7 +769,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             }
             ring0 += (uint32_t)(2 * tiles * NCH);
             if (QT == 1) {   // both warpgroups' maxima and sums: the later of the maxima is the larger
-                float2* mine = ml_rows + (item & 1) * 256 + 32 * quad + lane;
+                float2* mine = ml_rows + ((item + 1) & 1) * 256 + 32 * quad + lane;
                 mine[128 * g] = make_float2(m, l);
                 named_bar_sync(1 + quad, 64);   // (the other warp of these rows; all scores of the item are there)
                 const float2 other = mine[128 * (g ^ 1)];
@@ -674,81 +777,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 l = (m == -INFINITY ? 0.0f : l * exp2_fast(m - top)) + (other.x == -INFINITY ? 0.0f : other.y * exp2_fast(other.x - top));
                 m = top;
             }
-            const Walk now = w;
-            {
-                const int last = QT == 2 ? n - 2 + g : n - 1;
-                mbar_wait_bounded(done_u + 8u * (uint32_t)(last & 1), (done[last & 1] + (uint32_t)(last >> 1)) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            }
-            done[0] += (uint32_t)((n + 1) >> 1);
-            done[1] += (uint32_t)(n >> 1);
-            if (least_item < now.seen && spoilt[item & 1] == item) {
-                // Rare: what was taken out of the products goes to the rows that see it, a value at a time.
-                const int lo = max(least_item, now.from * KEYS), hi = min(now.seen, now.to * KEYS);
-                const uint8_t* q_row = q_at + t * 128 * DP * 2;
-                const int r = row - 128 * t;
-                for (int j = lo; j < hi; j++) {
-                    const int page = a.batch.page(now.s, j);
-                    if (page >= a.batch.n_pages) continue;
-                    const long long in = j & ((1 << a.batch.page_shift) - 1);
-                    const long long v_at = page * a.v_page + in * a.v_slot + now.kv * a.v_head, k_at = page * a.k_page + in * a.k_slot + now.kv * a.k_head;
-                    float weight = 0.0f;
-                    bool known = false;
-                    for (int e = col0; e < min(a.D, col0 + COLS); e++) {
-                        const float x = load_as<C>(a.v, v_at + e);
-                        if (fabsf(x) < INFINITY) continue;
-                        if (!known) {
-                            float dot = 0.0f;
-                            for (int d = 0; d < a.D; d++)
-                                dot = fmaf(to_f32(*(const C*)(q_row + d / 64 * BLOCK_BYTES + r * 128 + ((d % 64 / 8) ^ (r & 7)) * 16 + d % 8 * 2)), load_as<C>(a.k, k_at + d), dot);
-                            weight = exp2_fast(fmaf(dot, a.c, (m == -INFINITY ? 0.0f : -m) + WEIGHT_BIAS<C>));
-                            known = true;
-                        }
-                        uint32_t o;
-                        asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(o) : "r"(o_tm + (uint32_t)e) : "memory");
-                        tmem_ld_wait();
-                        asm volatile("" : "+r"(o));
-                        if (j < limit) o = __float_as_uint(fmaf(weight, x, __uint_as_float(o)));
-                        asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(o_tm + (uint32_t)e), "r"(o) : "memory");
-                        tmem_st_wait();
-                    }
-                }
-                if (QT == 1) named_bar_sync(1 + quad, 64);   // (the other warp reads the same queries)
-            }
-            // the next item's queries go in place before this one's outputs leave
-            more = walk_next<ROWS>(a, w, left);
-            if (more) load_queries(w);
-            const bool whole = now.from == 0 && now.to == now.units;
-            const int head = now.kv * a.group + now.row0 + row - tok * a.group;
-            const long long out_row = now.first + tok;
-            if (idle) {
-            } else if (whole) {
-                const float by = limit > 0 ? 1.0f / l : 0.0f;
-#pragma unroll 1
-                for (int k = col0; k < col0 + COLS; k += 16) {
-                    uint32_t o[16];
-                    float f[16];
-                    tmem_ld16(o_tm + (uint32_t)k, o);
-#pragma unroll
-                    for (int e = 0; e < 16; e++) f[e] = limit > 0 ? __uint_as_float(o[e]) * by : 0.0f;
-                    if (row < now.rows && k < a.D) store16(a, out_row * a.out_row + (long long)head * a.out_head + k, f, a.D - k);
-                }
-                if (a.lse && row < now.rows && col0 == 0) a.lse[out_row * a.n_heads + head] = limit > 0 ? 0.6931471805599453f * (m + log2f(l) - WEIGHT_BIAS<C>) : -INFINITY;
-            } else {
-                // a place in the work area: [4 columns][row] and each row's m and l behind
-                float* to = a.slots + (long long)(2 * blockIdx.x + (now.from == 0 ? 1 : 0)) * a.slot_rows * (DP + 4);
-#pragma unroll 1
-                for (int k = col0; k < col0 + COLS; k += 16) {
-                    uint32_t o[16];
-                    tmem_ld16(o_tm + (uint32_t)k, o);
-                    if (row < now.rows)
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4) *(uint4*)(to + (long long)((k + e) / 4 * a.slot_rows + row) * 4) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                }
-                if (row < now.rows && col0 == 0) *(float2*)(to + (long long)a.slot_rows * DP + 2 * row) = make_float2(m, l);
-            }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            item++;
+            next = walk_of(item + 2);
         }
     }
     // The last tile of rows, if others go on with it, is this CTA's to announce: its parts are this CTA's and those of the CTAs up to the one with its last unit.
@@ -967,6 +996,7 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     a.jobs = (Job*)work;
     a.slots = (float*)((uint8_t*)work + (size_t)ctas(ctx) * sizeof(Job));
     a.status = ctx->d_status;
+    a.q_shift = q_kind == Q38B_OUT_F32 ? 2 : 1;
     a.q_vec = (((uintptr_t)q | (uintptr_t)(q_row * kind_size(q_kind)) | (uintptr_t)(q_head * kind_size(q_kind))) & 15) == 0;
     a.out_vec = (((uintptr_t)out | (uintptr_t)(out_row * kind_size(out_kind)) | (uintptr_t)(out_head * kind_size(out_kind))) & 15) == 0;
     a.pdl = ctx->pass_pdl ? 1 : 0;
