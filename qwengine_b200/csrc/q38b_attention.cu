@@ -35,7 +35,7 @@ namespace {
 
 constexpr int KEYS = 128;                // keys of a tile
 constexpr int BLOCK_BYTES = KEYS * 128;  // 64 elements of 128 rows, 128-byte swizzle
-constexpr int HEAD = 7168;               // shared memory in front of the queries: barriers, the plan, maxima and sums of rows
+constexpr int HEAD = 3072;               // shared memory in front of the queries: barriers, the plan, maxima and sums of rows (no more, or D = 256 has a stage less)
 constexpr float GROWTH = 8.0f;           // how far, in powers of two, a row's maximum may grow before O is rescaled
 
 // A tile of rows that several CTAs share, as the one that begins it leaves it for the joining kernel
@@ -316,10 +316,11 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     uint32_t* tmem_slot = (uint32_t*)(w_full + 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     volatile int* spoilt = abort_flag + 1;   // [2]: the item that met values that are no numbers among keys that not all of its rows see
-    Plan* plan = (Plan*)(smem + 512);
-    Walk* walks = (Walk*)(smem + 6144);          // [8] the CTA's tiles of rows, as the first loading warp goes through them (it is at most half a ring ahead)
+    Plan* plan = (Plan*)(smem + 400);
+    Walk* walks = (Walk*)(smem + 560);             // [8] the CTA's tiles of rows, as the first loading warp goes through them (it is at most half a ring ahead)
     float* m_rows = (float*)(smem + 1024);       // [2][128]
-    float2* ml_rows = (float2*)(smem + 2048);    // [2][2][128]
+    float* l_rows = (float*)(smem + 2048);       // [2][128]
+    static_assert(sizeof(Plan) <= 160 && 560 + 8 * sizeof(Walk) <= 1024, "shared memory");
     uint8_t* q_at = smem + HEAD;
     uint8_t* ring = q_at + Sh::Q_BYTES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -769,12 +770,12 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             }
             ring0 += (uint32_t)(2 * tiles * NCH);
             if (QT == 1) {   // both warpgroups' maxima and sums: the later of the maxima is the larger
-                float2* mine = ml_rows + ((item + 1) & 1) * 256 + 32 * quad + lane;
-                mine[128 * g] = make_float2(m, l);
+                m_rows[g * 128 + 32 * quad + lane] = m;
+                l_rows[g * 128 + 32 * quad + lane] = l;
                 named_bar_sync(1 + quad, 64);   // (the other warp of these rows; all scores of the item are there)
-                const float2 other = mine[128 * (g ^ 1)];
-                const float top = fmaxf(m, other.x);
-                l = (m == -INFINITY ? 0.0f : l * exp2_fast(m - top)) + (other.x == -INFINITY ? 0.0f : other.y * exp2_fast(other.x - top));
+                const float m2 = m_rows[(g ^ 1) * 128 + 32 * quad + lane], l2 = l_rows[(g ^ 1) * 128 + 32 * quad + lane], top = fmaxf(m, m2);
+                named_bar_sync(1 + quad, 64);   // (both have read)
+                l = (m == -INFINITY ? 0.0f : l * exp2_fast(m - top)) + (m2 == -INFINITY ? 0.0f : l2 * exp2_fast(m2 - top));
                 m = top;
             }
             next = walk_of(item + 2);
