@@ -325,7 +325,6 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     uint8_t* ring = q_at + Sh::Q_BYTES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    if (a.pdl) pdl_launch_dependents();   // (the joining kernel's blocks wait on SMs that have no work)
     if (threadIdx.x == 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
@@ -424,7 +423,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             const auto scores = [&](int i) {
                 const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
                 const uint32_t d = tmem + (uint32_t)((i & 1) * KEYS);
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < NCH; c++) {
                     const uint32_t at = ring0 + at_keys<QT, NCH>(tile) + c, st = at % STAGES;
                     mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
@@ -449,7 +448,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
                     mbar_wait_bounded(smem_u32(&p_full[i & 1]), p_phase >> (i & 1) & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
                     p_phase ^= 1u << (i & 1);
-#pragma unroll 1
+#pragma unroll
                     for (int c = 0; c < NCH; c++) {
                         const uint32_t at = ring0 + at_values<QT, NCH>(tile, tiles) + c, st = at % STAGES;
                         mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
@@ -803,6 +802,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if (a.pdl) pdl_launch_dependents();
     if (warp == 1) {
         if (__builtin_expect(*abort_flag, 0)) settle_after_abort();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
