@@ -132,6 +132,7 @@ def load_library():
     lib.q38b_quantize_i8.argtypes = [vp, vp, i32, ll, i32, i32, vp, ll, vp, vp]
     lib.q38b_gemm_i8.argtypes = [vp, vp, ll, vp, i32, i32, vp, ll, vp, i32, vp, i32, ll, i32, vp]
     lib.q38b_debug_set_i8_cut.argtypes = [vp, i32]
+    lib.q38b_debug_set_attention_two.argtypes = [vp, i32]
     lib.q38b_gemm_i8_scratch_bytes.argtypes = [i32, i32]
     lib.q38b_gemm_i8_scratch_bytes.restype = sz
     lib.q38b_gemm_i8_x.argtypes = [vp, vp, ll, vp, i32, i32, vp, i32, ll, i32, vp, i32, ll, i32, vp, sz, vp]
@@ -294,6 +295,10 @@ class Context:
     def debug_set_mx4_pairs(self, mode):
         """Test hook: 4-bit products in pairs of CTAs never (-1), with tiles of `mode` tokens, by the rule (0)."""
         self._rc(self.lib.q38b_debug_set_mx4_pairs(self.h, int(mode)), "q38b_debug_set_mx4_pairs")
+
+    def debug_set_attention_two(self, mode):
+        """Test hook: 1 two tiles of rows together wherever there is such a variant, -1 never, 0 by the rule."""
+        self._rc(self.lib.q38b_debug_set_attention_two(self.h, int(mode)), "q38b_debug_set_attention_two")
 
     def debug_set_i8_cut(self, mode):
         """Test hook: 64, 128, 192, 256 8-bit products in pairs of CTAs with tiles of so many tokens; -(10 p + s) in single CTAs, p to an SM, K in s parts; 0 by the rule."""

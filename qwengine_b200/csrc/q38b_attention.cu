@@ -59,19 +59,20 @@ struct AttnArgs {
 };
 __device__ __forceinline__ int by_group(const AttnArgs& a, int x) { return (int)((uint64_t)(uint32_t)x * a.group_mul >> a.group_shift); }
 
-// Shapes of a variant: heads padded to DP elements, QT tiles of 128 rows
-template <int DP, int QT>
+// Shapes of a variant: heads padded to DP elements, QT tiles of 128 rows, or PAIR: two CTAs that multiply as one, each with 128 of 256 rows, half of the keys of
+// a tile and half of the values' columns
+template <int DP, int QT, bool PAIR>
 struct Shape {
-    static constexpr int CW = DP % 128 == 0 ? 128 : 64;        // elements of a stage: 128 keys x CW
-    static constexpr int NCH = DP / CW;                        // stages of a tile of keys (or of values)
+    static constexpr int CW = DP % 128 == 0 ? 128 : 64;        // elements of a stage: 128 keys x CW (PAIR: 64 keys x DP, 128 values x DP / 2)
+    static constexpr int NCH = PAIR ? 1 : DP / CW;             // stages of a tile of keys (or of values)
     static constexpr int STAGE = KEYS * CW * 2;
     static constexpr int Q_BYTES = QT * 128 * DP * 2;
     static constexpr int ROOM = (232448 - HEAD - Q_BYTES) / STAGE;
     static constexpr int STAGES = ROOM < 12 ? ROOM : 12;
     static constexpr int SMEM = HEAD + Q_BYTES + STAGES * STAGE;
-    static constexpr int ROWS = QT * 128;
+    static constexpr int ROWS = (PAIR ? 2 : QT) * 128;
     static constexpr int THREADS = 384;                       // warps 0, 2, 3 load, warp 1 multiplies, two warpgroups make weights
-    static_assert(256 + QT * DP <= 512, "tensor memory");
+    static_assert(256 + QT * DP <= 512 && (!PAIR || (QT == 1 && DP == 256)), "tensor memory; halves of whole blocks");
 };
 
 // positions of a tile's stages in the ring, in stages behind the item's first: in the order in which the tensor core takes them
@@ -143,6 +144,9 @@ __device__ __forceinline__ int moved_cut(const Walk& w, int in) {   // a cut `in
     return 2 * in <= w.units ? 0 : w.units;
 }
 
+// keys that all of a tile's rows see
+__device__ __forceinline__ int least_seen(const AttnArgs& a, const Walk& w) { return max(0, w.len - w.n_new + by_group(a, w.row0) + 1); }
+
 // Units of one key head of a sequence, by one thread or by the lanes of a warp together
 template <int ROWS>
 __device__ __forceinline__ int sequence_units(const AttnArgs& a, const Walk& w, int lane, int lanes) {
@@ -163,7 +167,7 @@ __device__ __forceinline__ int exact_cut(int each, int rest, int active, int c) 
 
 // All threads: the batch's units, this CTA's range of them, and the tile of rows it begins in.  false: nothing to do
 template <int DP, int ROWS, int THREADS>
-__device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p) {
+__device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p, int cta, int n_ctas) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int WARPS = THREADS / 32;
     // few sequences: a warp each, its lanes along the tiles; many: a thread each
@@ -191,7 +195,7 @@ __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p) {
     if (lane == 0) p->sums[warp] = mine;
     __syncthreads();
     const int total = __reduce_add_sync(0xffffffffu, lane < WARPS ? p->sums[lane] : 0);
-    const int active = min((int)gridDim.x, total), cta = (int)blockIdx.x;
+    const int active = min(n_ctas, total);
     if (cta >= active) return false;
     const int each = total / active, rest = total - each * active, begin = exact_cut(each, rest, active, cta), end = exact_cut(each, rest, active, cta + 1);
     if (threadIdx.x == 0) {
@@ -255,11 +259,25 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
                  "r"(w), "r"(bar)
                  : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+// counted on a barrier of either CTA of a pair
+__device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(y),
+                 "r"(z), "r"(w), "r"(bar)
+                 : "memory");
 }
+template <bool PAIR>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+template <bool PAIR>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+    if constexpr (PAIR)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
 // 16 columns of this warp's 32 rows, on their way until tmem_st_wait
 __device__ __forceinline__ void tmem_st16_start(uint32_t taddr, const uint32_t* v) {
@@ -299,10 +317,10 @@ __device__ __forceinline__ void store_one(const AttnArgs& a, long long at, float
     else ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(f);
 }
 
-template <typename C, int DP, int QT>
-__global__ void __launch_bounds__(Shape<DP, QT>::THREADS, 1)
+template <typename C, int DP, int QT, bool PAIR>
+__global__ void __launch_bounds__(Shape<DP, QT, PAIR>::THREADS, 1)
 attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
-    using Sh = Shape<DP, QT>;
+    using Sh = Shape<DP, QT, PAIR>;
     constexpr int CW = Sh::CW, NCH = Sh::NCH, STAGE = Sh::STAGE, STAGES = Sh::STAGES, ROWS = Sh::ROWS;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t* full = (uint64_t*)smem;
@@ -313,17 +331,19 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     uint64_t* m_full = o_done + 2;   // [2][4] QT = 1: the maxima that a warp of either warpgroup took off are known to the other
     uint64_t* q_full = m_full + 8;
     uint64_t* w_full = q_full + 1;   // [8] a tile of rows is known
-    uint32_t* tmem_slot = (uint32_t*)(w_full + 8);
+    uint64_t* v_here = w_full + 8;   // [STAGES] PAIR: this CTA's values of a tile that some rows do not see all of
+    uint32_t* tmem_slot = (uint32_t*)(v_here + 8);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     volatile int* spoilt = abort_flag + 1;   // [2]: the item that met values that are no numbers among keys that not all of its rows see
-    Plan* plan = (Plan*)(smem + 400);
-    Walk* walks = (Walk*)(smem + 560);             // [8] the CTA's tiles of rows, as the first loading warp goes through them (it is at most half a ring ahead)
+    Plan* plan = (Plan*)(smem + 464);
+    Walk* walks = (Walk*)(smem + 600);             // [8] the CTA's tiles of rows, as the first loading warp goes through them (it is at most half a ring ahead)
     float* m_rows = (float*)(smem + 1024);       // [2][128]
     float* l_rows = (float*)(smem + 2048);       // [2][128]
-    static_assert(sizeof(Plan) <= 160 && 560 + 8 * sizeof(Walk) <= 1024, "shared memory");
+    static_assert(sizeof(Plan) <= 136 && 600 + 8 * sizeof(Walk) <= 1024 && (!PAIR || STAGES <= 8), "shared memory");
     uint8_t* q_at = smem + HEAD;
     uint8_t* ring = q_at + Sh::Q_BYTES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? (int)cluster_rank() : 0, cta = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;   // (a pair counts as one)
 
     if (threadIdx.x == 32) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
@@ -338,21 +358,30 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         }
         for (int s = 0; s < 2; s++) {
             mbar_init(smem_u32(&s_full[s]), 1);
-            mbar_init(smem_u32(&p_full[s]), 4);
+            mbar_init(smem_u32(&p_full[s]), PAIR ? 8 : 4);
             mbar_init(smem_u32(&o_done[s]), 1);
         }
         for (int s = 0; s < 8; s++) mbar_init(smem_u32(&m_full[s]), 1);
-        mbar_init(smem_u32(q_full), 8);
-        for (int s = 0; s < 8; s++) mbar_init(smem_u32(&w_full[s]), 1);
+        mbar_init(smem_u32(q_full), PAIR ? 16 : 8);
+        for (int s = 0; s < 8; s++) {
+            mbar_init(smem_u32(&w_full[s]), 1);
+            mbar_init(smem_u32(&v_here[s]), 1);
+        }
         mbar_fence_init();
         fence_proxy_async();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    const bool any = plan_work<DP, ROWS, Sh::THREADS>(a, plan);   // (with barriers of the block)
+    const bool any = plan_work<DP, ROWS, Sh::THREADS>(a, plan, cta, PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x);   // (with barriers of the block)
+    if constexpr (PAIR) cluster_sync_all();   // the other CTA's barriers are initialised
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
     int left = any ? plan->cut[1] - plan->cut[0] : 0;
@@ -362,9 +391,13 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     if (any && (warp == 0 || warp == 2 || warp == 3)) {
         // ---------------- keys and values: a lane of one of three warps a box of at most 128 slots x 64 elements ----------------
         // (A warp issues its lanes' copies one by one, some 80 clocks each: the 64 of 128 keys and values in pages of 16 took it as long as the memory does.)
-        const int boxes = KEYS / a.box_rows, loader = warp == 0 ? 0 : warp - 1, box = 3 * lane + loader, part = box & (boxes - 1), block = box / boxes;
-        const bool mine = block < CW / 64;   // lanes behind the last box do nothing
-        const uint32_t to = (uint32_t)(block * BLOCK_BYTES + part * a.box_rows * 128), ring_u = smem_u32(ring), full_u = smem_u32(full), empty_u = smem_u32(empty);
+        // A box of keys: block `block[0]` of 64 elements, slots `in[0]` and on of the tile; of values: [1].
+        const int loader = warp == 0 ? 0 : warp - 1, box = 3 * lane + loader, k_boxes = (PAIR ? KEYS / 2 : KEYS) / a.box_rows, v_boxes = KEYS / a.box_rows;
+        const bool mine = box < v_boxes * (CW / 64);   // lanes behind the last box do nothing
+        const int k_block = box / k_boxes, k_part = box % k_boxes * a.box_rows, v_block = box / v_boxes, v_part = box % v_boxes * a.box_rows;
+        const int in[2] = {k_part + (PAIR ? rank * (KEYS / 2) : 0), v_part}, x0[2] = {k_block * 64, v_block * 64 + (PAIR ? rank * 128 : 0)};
+        const uint32_t to[2] = {(uint32_t)(k_block * (PAIR ? BLOCK_BYTES / 2 : BLOCK_BYTES) + k_part * 128), (uint32_t)(v_block * BLOCK_BYTES + v_part * 128)};
+        const uint32_t ring_u = smem_u32(ring), full_u = PAIR ? peer_smem(smem_u32(full), 0u) : smem_u32(full), empty_u = smem_u32(empty);
         const int slots = (1 << a.batch.page_shift) - 1;
         uint32_t at = 0;   // stages filled so far
         int item = 0;
@@ -385,22 +418,35 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             };
             const auto page_of = [&](int i) {   // of this lane's box; keys nobody sees come as zeros, from a page that is not there
                 bool values;
-                const int token = (w.from + tile_of(i, values)) * KEYS + part * a.box_rows;
+                const int tile = tile_of(i, values), token = (w.from + tile) * KEYS + in[values];
                 return i < 2 * n && token < w.seen ? a.batch.page(w.s, token) : a.batch.n_pages;
             };
             int page = page_of(0);
 #pragma unroll 1
             for (int i = 0; i < 2 * n; i++) {
                 bool values;
-                const int slot = ((w.from + tile_of(i, values)) * KEYS + part * a.box_rows) & slots, next = page_of(i + 1);
+                const int j0 = (w.from + tile_of(i, values)) * KEYS, slot = (j0 + in[values]) & slots, next = page_of(i + 1);
                 const CUtensorMap* map = values ? &vmap : &kmap;
+                const bool looked_at = PAIR && values && j0 + KEYS > least_seen(a, w);   // these the other warps of this CTA wait for themselves
 #pragma unroll 1
                 for (int c = 0; c < NCH; c++, at++) {
                     const uint32_t st = at % STAGES, use = at / STAGES;
                     mbar_wait_bounded(empty_u + 8u * st, (use & 1u) ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
-                    if (threadIdx.x == 0) mbar_arrive_expect_tx(full_u + 8u * st, STAGE);
-                    __syncwarp();
-                    if (mine) tma_load_4d(ring_u + st * STAGE + to, map, c * CW + block * 64, slot, w.kv, page, full_u + 8u * st);
+                    if constexpr (PAIR) {
+                        const uint32_t here = smem_u32(&v_here[st]);
+                        if (threadIdx.x == 0) {
+                            if (looked_at) mbar_arrive_expect_tx(here, STAGE);
+                            if (rank == 0 && looked_at) mbar_arrive(smem_u32(&full[st]));
+                            if (rank == 0 && !looked_at) mbar_arrive_expect_tx(smem_u32(&full[st]), 2 * STAGE);
+                        }
+                        __syncwarp();
+                        if (mine && looked_at) tma_load_4d(ring_u + st * STAGE + to[values], map, x0[values], slot, w.kv, page, here);
+                        if (mine && !looked_at) tma_load_4d_pair(ring_u + st * STAGE + to[values], map, x0[values], slot, w.kv, page, full_u + 8u * st);
+                    } else {
+                        if (threadIdx.x == 0) mbar_arrive_expect_tx(full_u + 8u * st, STAGE);
+                        __syncwarp();
+                        if (mine) tma_load_4d(ring_u + st * STAGE + to[values], map, c * CW + x0[values], slot, w.kv, page, full_u + 8u * st);
+                    }
                 }
                 page = next;
             }
@@ -408,10 +454,12 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         w.to = w.from;   // no more
         publish(w);
     } else if (any && warp == 1) {
+        if (PAIR && rank) {   // (the other CTA issues for both)
+        } else {
         // ---------------- products ----------------
         constexpr uint32_t TYPE = std::is_same<C, __half>::value ? 0u : 1u;
-        constexpr uint32_t idesc_s = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-        constexpr uint32_t idesc_o = (1u << 4) | (TYPE << 7) | (TYPE << 10) | (1u << 16) | ((uint32_t)(CW >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        constexpr uint32_t idesc_s = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
+        constexpr uint32_t idesc_o = (1u << 4) | (TYPE << 7) | (TYPE << 10) | (1u << 16) | ((uint32_t)((PAIR ? DP : CW) >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
         const uint64_t kdesc0 = umma_desc_sw128(0), vdesc0 = umma_desc_mn_sw128(0);
         const uint32_t q_u = smem_u32(q_at), ring_u = smem_u32(ring), full_u = smem_u32(full), empty_u = smem_u32(empty);
         uint32_t ring0 = 0, p_phase = 0, item = 0;
@@ -431,12 +479,11 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     const uint64_t qd = kdesc0 + ((q_u + (uint32_t)(t * 128 * DP * 2 + c * CW / 64 * BLOCK_BYTES)) >> 4), kd = kdesc0 + ((ring_u + st * STAGE) >> 4);
                     if (elect_one()) {
 #pragma unroll
-                        for (int k = 0; k < CW / 16; k++) {
-                            const uint64_t off = (uint64_t)((k / 4 * BLOCK_BYTES + k % 4 * 32) >> 4);
-                            mma_ss(d, qd + off, kd + off, idesc_s, c > 0 || k > 0 ? 1u : 0u);
-                        }
-                        if (QT == 1 || t == 1) umma_commit<false>(empty_u + 8u * st);
-                        if (c == NCH - 1) umma_commit<false>(smem_u32(&s_full[i & 1]));
+                        for (int k = 0; k < (PAIR ? DP : CW) / 16; k++)
+                            mma_ss<PAIR>(d, qd + (uint64_t)((k / 4 * BLOCK_BYTES + k % 4 * 32) >> 4), kd + (uint64_t)((k / 4 * (PAIR ? BLOCK_BYTES / 2 : BLOCK_BYTES) + k % 4 * 32) >> 4), idesc_s,
+                                         c > 0 || k > 0 ? 1u : 0u);
+                        if (QT == 1 || t == 1) umma_commit<PAIR>(empty_u + 8u * st);
+                        if (c == NCH - 1) umma_commit<PAIR>(smem_u32(&s_full[i & 1]));
                     }
                     __syncwarp();
                 }
@@ -457,9 +504,9 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                         const uint64_t vd = vdesc0 + ((ring_u + st * STAGE) >> 4);
                         if (elect_one()) {
 #pragma unroll
-                            for (int k = 0; k < KEYS / 16; k++) mma_ts(d, p + (uint32_t)(8 * k), vd + (uint64_t)(k * 2048 >> 4), idesc_o, k > 0 || tile > 0 ? 1u : 0u);
-                            if (QT == 1 || t == 1) umma_commit<false>(empty_u + 8u * st);
-                            if (c == NCH - 1) umma_commit<false>(smem_u32(&o_done[i & 1]));
+                            for (int k = 0; k < KEYS / 16; k++) mma_ts<PAIR>(d, p + (uint32_t)(8 * k), vd + (uint64_t)(k * 2048 >> 4), idesc_o, k > 0 || tile > 0 ? 1u : 0u);
+                            if (QT == 1 || t == 1) umma_commit<PAIR>(empty_u + 8u * st);
+                            if (c == NCH - 1) umma_commit<PAIR>(smem_u32(&o_done[i & 1]));
                         }
                         __syncwarp();
                     }
@@ -469,18 +516,23 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             ring0 += (uint32_t)(2 * tiles * NCH);
             item++;
         }
+        }
     } else if (any) {
         // ---------------- weights: warpgroup g takes the scores that lie in place g, a thread a row ----------------
         // QT = 2: those of its own 128 rows.  QT = 1: those of every other tile of keys; the maxima go from one warpgroup to the other, and each has a sum of its own.
-        const int g = (warp >> 2) - 1, quad = warp & 3, t = QT == 2 ? g : 0, row = 128 * t + 32 * quad + lane;   // row: of the tile of rows
-        const uint32_t lanes = (uint32_t)(32 * quad) << 16, o_tm = tmem + lanes + (uint32_t)(256 + t * DP), s_tm = tmem + lanes + (uint32_t)(g * KEYS);
-        const uint32_t s_bar = smem_u32(&s_full[g]), p_bar = smem_u32(&p_full[g]), done_u = smem_u32(o_done);
+        const int g = (warp >> 2) - 1, quad = warp & 3, qt = QT == 2 ? g : 0, t = PAIR ? rank : qt, row = 128 * t + 32 * quad + lane;   // row: of the tile of rows
+        const uint32_t lanes = (uint32_t)(32 * quad) << 16, o_tm = tmem + lanes + (uint32_t)(256 + qt * DP), s_tm = tmem + lanes + (uint32_t)(g * KEYS);
+        const uint32_t s_bar = smem_u32(&s_full[g]), p_bar = PAIR ? peer_smem(smem_u32(&p_full[g]), 0u) : smem_u32(&p_full[g]), done_u = smem_u32(o_done);
         constexpr int COLS = QT == 2 ? DP : DP / 2;     // of the outputs this warpgroup stores
         const int col0 = QT == 2 ? 0 : g * COLS;
+        const auto arrive = [](uint32_t bar) {   // PAIR: at the CTA that issues
+            if constexpr (PAIR) mbar_arrive_peer(bar);
+            else mbar_arrive(bar);
+        };
         const auto load_queries = [&](const Walk& v) {
             constexpr int UNITS = DP / 8, AHEAD = 4, STEP = QT == 2 ? 32 : 64;    // 16-byte pieces of a row; of a lane on their way; (QT = 1: the two warps of these rows take turns)
             const int here = min(32, v.rows - (128 * t + 32 * quad)), pieces = here * UNITS;   // rows that are not there keep whatever they hold: it meets no other row
-            uint8_t* to = q_at + t * 128 * DP * 2 + 32 * quad * 128;
+            uint8_t* to = q_at + qt * 128 * DP * 2 + 32 * quad * 128;
             if (here > 0) {
                 const int flat = v.row0 + row, in = by_group(a, flat);
                 const long long my_row = (long long)(v.first + in) * a.q_row + (long long)(v.kv * a.group + flat - in * a.group) * a.q_head;
@@ -523,9 +575,9 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             }
             fence_proxy_async();
             __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(q_full));
+            if (lane == 0) arrive(PAIR ? peer_smem(smem_u32(q_full), 0u) : smem_u32(q_full));
         };
-        uint32_t ring0 = 0, s_use = 0, m_use = 0, done[2] = {0, 0};   // done: products P V from either place up to this item
+        uint32_t ring0 = 0, s_use = 0, m_use = 0, looked = 0, done[2] = {0, 0};   // done: products P V from either place up to this item
         int item;   // the tile of rows in front of the one that is worked on
         const auto walk_of = [&](int i) {
             mbar_wait_bounded(smem_u32(&w_full[i & 7]), (uint32_t)i >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
@@ -623,7 +675,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     if (a.lse && row < w.rows && col0 == 0) a.lse[out_row * a.n_heads + head] = limit > 0 ? 0.6931471805599453f * (m + log2f(l) - WEIGHT_BIAS<C>) : -INFINITY;
                 } else {
                     // a place in the work area: [4 columns][row] and each row's m and l behind
-                    float* to = a.slots + (long long)(2 * blockIdx.x + (w.from == 0 ? 1 : 0)) * a.slot_rows * (DP + 4);
+                    float* to = a.slots + (long long)(2 * cta + (w.from == 0 ? 1 : 0)) * a.slot_rows * (DP + 4);
 #pragma unroll 1
                     for (int k = col0; k < col0 + COLS; k += 32) {
                         uint32_t o[32];
@@ -647,7 +699,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             tok = by_group(a, w.row0 + row);
             limit = row < w.rows ? max(0, w.len - w.n_new + tok + 1) : w.seen;                          // keys this row sees
             const int least = max(0, w.len - w.n_new + by_group(a, w.row0 + min(128 * t + 32 * quad, w.rows - 1)) + 1);   // ... the warp's first row
-            least_item = max(0, w.len - w.n_new + by_group(a, w.row0) + 1);                                    // ... the item's first row
+            least_item = least_seen(a, w);                                                                    // ... the item's first row
             idle = 128 * t + 32 * quad >= w.rows;   // no row of this warp's is there
             m = -INFINITY;
             l = 0.0f;
@@ -742,7 +794,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
 #pragma unroll 1
                     for (int c = 0; c < NCH; c++) {
                         const uint32_t at = ring0 + at_values<QT, NCH>(tile, tiles) + c, st = at % STAGES;
-                        mbar_wait_bounded(smem_u32(&full[st]), at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                        mbar_wait_bounded(PAIR ? smem_u32(&v_here[st]) : smem_u32(&full[st]), (PAIR ? looked >> st : at / STAGES) & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
                         // 16-byte pieces: eight to a row of a block of 64 elements, whose order in the row does not matter here
                         for (int u = 32 * quad + lane; u < (rest - lo) * (CW / 8); u += 128) {
                             const int j = lo + u / (CW / 8);
@@ -755,6 +807,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                             const uint4 bad = make_uint4(no_number<C>(y.x), no_number<C>(y.y), no_number<C>(y.z), no_number<C>(y.w));
                             if (bad.x | bad.y | bad.z | bad.w) {
                                 spoilt[(item + 1) & 1] = item + 1;
+                                if constexpr (PAIR) {    // (the other CTA's rows multiply these columns too)
+                                    st_peer_f32(peer_smem(smem_u32((const void*)&spoilt[(item + 1) & 1]), (uint32_t)(rank ^ 1)), (uint32_t)(item + 1));
+                                    asm volatile("fence.acq_rel.cluster;" ::: "memory");
+                                }
                                 __threadfence_block();   // (whoever finds these zeros finds the mark too)
                                 *x = make_uint4(y.x & ~bad.x, y.y & ~bad.y, y.z & ~bad.z, y.w & ~bad.w);
                             }
@@ -765,8 +821,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 tmem_st_wait();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_bar);
+                if (lane == 0) arrive(p_bar);
             }
+            if constexpr (PAIR)   // the stages whose values were waited for here, by either warpgroup
+                for (int i = max(0, least_item / KEYS - w.from); i < tiles; i++) looked ^= 1u << ((ring0 + at_values<QT, NCH>(i, tiles)) % STAGES);
             ring0 += (uint32_t)(2 * tiles * NCH);
             if (QT == 1) {   // both warpgroups' maxima and sums: the later of the maxima is the larger
                 m_rows[g * 128 + 32 * quad + lane] = m;
@@ -781,15 +839,15 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         }
     }
     // The last tile of rows, if others go on with it, is this CTA's to announce: its parts are this CTA's and those of the CTAs up to the one with its last unit.
-    if (threadIdx.x == 128) {
+    if (threadIdx.x == 128 && rank == 0) {
         Job job = {};
         if (any) {
             if (w.from == 0 && w.to < w.units) {
                 // its parts: up to the last CTA that begins in it, no nearer to its end than a cut may lie
                 const int last = plan->cut[1] + (w.units - w.to) - dear<DP>(w) - 1, each = plan->total / plan->active, rest = plan->total - each * plan->active;
                 int c = min(plan->active - 1, (int)((float)last * (float)plan->active / (float)plan->total) + 1);   // (within one of it)
-                while (c > (int)blockIdx.x && exact_cut(each, rest, plan->active, c) > last) c--;
-                job.n_parts = c - (int)blockIdx.x + 1;
+                while (c > cta && exact_cut(each, rest, plan->active, c) > last) c--;
+                job.n_parts = c - cta + 1;
                 job.first = w.first;
                 job.n_new = w.n_new;
                 job.len = w.len;
@@ -798,16 +856,19 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 job.rows = w.rows;
             }
         }
-        a.jobs[blockIdx.x] = job;
+        a.jobs[cta] = job;
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (a.pdl) pdl_launch_dependents();
+    if constexpr (PAIR) cluster_sync_all();   // both CTAs have read their sums, and nothing is on its way to the other's barriers
     if (warp == 1) {
         if (__builtin_expect(*abort_flag, 0)) settle_after_abort();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
+    if constexpr (PAIR) cluster_sync_all();   // neither CTA leaves before both have given it back
 }
 
 // Joins the parts of tiles of rows.  A piece of work is 32 rows (the lanes: what a part left lies so) of two groups of four elements where there are many
@@ -928,20 +989,30 @@ int padded(int D) { return (D + 63) / 64 * 64; }
 // rows of a place in the work area
 int slot_rows(int group, int D, int rows) { return (int)std::min((long long)(padded(D) <= 128 ? 256 : 128), (long long)rows * group); }
 
-template <typename C, int DP, int QT>
+template <typename C, int DP, int QT, bool PAIR = false>
 int attention_as(q38b_ctx* ctx, const AttnArgs& a, const CUtensorMap& kmap, const CUtensorMap& vmap, cudaStream_t st) {
-    auto kern = attention_kernel<C, DP, QT>;
+    using Sh = Shape<DP, QT, PAIR>;
+    auto kern = attention_kernel<C, DP, QT, PAIR>;
     const int rc = q38b_ensure_kernel_smem(ctx, (const void*)kern, ctx->smem_optin, false);
     if (rc != Q38B_OK) return rc;
-    kern<<<(unsigned)ctas(ctx), Shape<DP, QT>::THREADS, Shape<DP, QT>::SMEM, st>>>(a, kmap, vmap);
-    const int done = launch_status(ctx, cudaSuccess);
-    if (done != Q38B_OK) return done;
     cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)(PAIR ? 2 * a.ctas : a.ctas));
+    cfg.blockDim = dim3(Sh::THREADS);
+    cfg.dynamicSmemBytes = Sh::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = PAIR ? 1 : 0;
+    const int done = launch_status(ctx, cudaLaunchKernelEx(&cfg, kern, a, kmap, vmap));
+    if (done != Q38B_OK) return done;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(4u * (unsigned)ctx->sm_count);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
@@ -954,7 +1025,7 @@ int attention_for(q38b_ctx* ctx, const AttnArgs& a, bool two, const CUtensorMap&
         case 64: return two ? attention_as<C, 64, 2>(ctx, a, kmap, vmap, st) : attention_as<C, 64, 1>(ctx, a, kmap, vmap, st);
         case 128: return two ? attention_as<C, 128, 2>(ctx, a, kmap, vmap, st) : attention_as<C, 128, 1>(ctx, a, kmap, vmap, st);
         case 192: return attention_as<C, 192, 1>(ctx, a, kmap, vmap, st);
-        default: return attention_as<C, 256, 1>(ctx, a, kmap, vmap, st);
+        default: return two ? attention_as<C, 256, 1, true>(ctx, a, kmap, vmap, st) : attention_as<C, 256, 1>(ctx, a, kmap, vmap, st);
     }
 }
 
@@ -991,9 +1062,14 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     a.q_row = q_row; a.q_head = q_head; a.out_row = out_row; a.out_head = out_head;
     a.k_page = c->k_page; a.k_slot = c->k_slot; a.k_head = c->k_head; a.v_page = c->v_page; a.v_slot = c->v_slot; a.v_head = c->v_head;
     a.q_kind = q_kind; a.out_kind = out_kind; a.n_heads = n_heads; a.n_kv = c->n_heads; a.group = n_heads / c->n_heads; a.D = c->D;
-    a.box_rows = std::min(c->page_size, KEYS);
-    a.slot_rows = slot_rows(a.group, c->D, rows);
-    a.ctas = ctas(ctx);
+    // Two tiles of rows share the keys' and values' way into shared memory, in one CTA (heads of at most 128) or in a pair of them (more than 192), where sequences fill
+    // more than one on average and there are enough of them for all SMs.
+    const bool two = ctx->attention_two ? ctx->attention_two > 0
+                                        : (long long)rows * a.group > 128LL * c->n_seqs && (long long)rows * n_heads >= (padded(c->D) == 256 ? 128LL : 256LL) * ctx->sm_count;
+    const bool pair = two && padded(c->D) == 256;
+    a.box_rows = std::min(c->page_size, pair ? KEYS / 2 : KEYS);
+    a.slot_rows = slot_rows(a.group, pair ? 128 : c->D, rows);
+    a.ctas = pair ? ctas(ctx) / 2 : ctas(ctx);
     a.jobs = (Job*)work;
     a.slots = (float*)((uint8_t*)work + (size_t)ctas(ctx) * sizeof(Job));
     a.status = ctx->d_status;
@@ -1008,9 +1084,14 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     a.group_mul = (uint32_t)(((1ULL << a.group_shift) + a.group - 1) / a.group);
     CUtensorMap kmap, vmap;
     if (!encode_pages(&kmap, c, c->k, c->k_page, c->k_slot, c->k_head, a.box_rows) || !encode_pages(&vmap, c, c->v, c->v_page, c->v_slot, c->v_head, a.box_rows)) return Q38B_ERR_ARG;
-    // two tiles of rows share the keys' way into shared memory where sequences fill more than one on average and there are enough of them for all SMs
-    const bool two = (long long)rows * a.group > 128LL * c->n_seqs && (long long)rows * n_heads >= 256LL * ctx->sm_count;
     return c->kind == Q38B_OUT_F16 ? attention_for<__half>(ctx, a, two, kmap, vmap, (cudaStream_t)stream) : attention_for<__nv_bfloat16>(ctx, a, two, kmap, vmap, (cudaStream_t)stream);
+}
+
+// Test hook (not in the public header): two tiles of rows together never (-1), wherever there is such a variant (1), by the rule (0).
+int q38b_debug_set_attention_two(q38b_ctx* ctx, int mode) {
+    if (!ctx || mode < -1 || mode > 1) return Q38B_ERR_ARG;
+    ctx->attention_two = mode;
+    return Q38B_OK;
 }
 
 }  // extern "C"

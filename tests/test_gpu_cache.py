@@ -20,6 +20,14 @@ DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
 KIND = {"f32": 0, "f16": 1, "bf16": 2}
 
 
+@pytest.fixture(params=["by rule", "two tiles of rows"])
+def tiles(ctx, request):
+    """The variants with two tiles of rows together, which the rule takes for many rows only, at the sizes of these tests too."""
+    ctx.debug_set_attention_two(1 if request.param.startswith("two") else 0)
+    yield
+    ctx.debug_set_attention_two(0)
+
+
 class Text:
     """A batch of sequences in a cache: plan = [(new tokens, tokens in all)], their keys and values in 64 bits beside the pages that hold them.  Slots that no
     token has, and pages that no sequence has, hold NaN."""
@@ -125,55 +133,61 @@ def run(ctx, plan, nq=6, nk=2, D=64, page=16, dtype="bf16", src=None, dst=None, 
 
 @pytest.mark.parametrize("D", [8, 16, 40, 64, 72, 80, 96, 128, 136, 192, 200, 256])
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
-def test_head_sizes(ctx, D, dtype):
+def test_head_sizes(ctx, tiles, D, dtype):
     run(ctx, [(1, 1), (3, 200), (70, 70)], D=D, dtype=dtype)
 
 
 @pytest.mark.parametrize("nq,nk", [(1, 1), (7, 1), (4, 4), (24, 4), (15, 5), (128, 1), (130, 1), (300, 1)])
 @pytest.mark.parametrize("D", [64, 256])
-def test_groups(ctx, nq, nk, D):
+def test_groups(ctx, tiles, nq, nk, D):
     run(ctx, [(1, 300), (5, 140)], nq=nq, nk=nk, D=D)
 
 
 @pytest.mark.parametrize("page", [8, 16, 32, 64, 128, 256, 1024])
 @pytest.mark.parametrize("D", [64, 96, 256])
-def test_page_sizes(ctx, page, D):
+def test_page_sizes(ctx, tiles, page, D):
     run(ctx, [(1, 1), (2, 129), (9, 300), (1, 1025)], page=page, D=D)
 
 
 @pytest.mark.parametrize("total", [1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 255, 256, 257, 700])
 @pytest.mark.parametrize("new", [1, 2, 22, 43])
 @pytest.mark.parametrize("D", [128, 256])
-def test_lengths(ctx, total, new, D):
+def test_lengths(ctx, tiles, total, new, D):
     run(ctx, [(new, total)], D=D, seed=total)     # some chunks are longer than their text: rows that see nothing
 
 
-def test_ragged_batches(ctx):
+def test_many_rows(ctx):
+    """Enough rows for the rule to take two tiles of them together: several sequences, cuts inside tiles."""
+    for D, nq, nk, dtype in ((256, 24, 4, "bf16"), (128, 48, 8, "f16"), (64, 48, 8, "bf16")):
+        run(ctx, [(700, 900), (1, 300), (130, 131)], nq=nq, nk=nk, D=D, dtype=dtype)
+
+
+def test_ragged_batches(ctx, tiles):
     run(ctx, [(0, 50), (1, 700), (0, 0), (33, 33), (5, 0), (1, 1), (2, 1), (64, 500), (0, 3)], D=256)
     run(ctx, [(0, 50), (1, 700), (0, 0), (33, 33), (5, 0), (1, 1), (2, 1), (64, 500), (0, 3)], D=96, dtype="f16", page=32)
     run(ctx, [(1, 1 + 37 * s % 400) for s in range(70)], D=128, nq=4, nk=2)
 
 
 @pytest.mark.parametrize("src,dst", [("f32", "f32"), ("f32", "bf16"), ("bf16", "f32"), ("bf16", "f16")])
-def test_types(ctx, src, dst):
+def test_types(ctx, tiles, src, dst):
     run(ctx, [(1, 90), (40, 150)], D=256, src=src, dst=dst)
     run(ctx, [(1, 90), (40, 150)], D=80, src=src, dst=dst)
 
 
 @pytest.mark.parametrize("layout", ["head", "both"])
 @pytest.mark.parametrize("nk", [1, 3])
-def test_layouts(ctx, layout, nk):
+def test_layouts(ctx, tiles, layout, nk):
     run(ctx, [(1, 90), (40, 150)], nq=2 * nk, nk=nk, D=128, layout=layout)
     run(ctx, [(3, 90)], nq=2 * nk, nk=nk, D=256, layout=layout, page=64)
 
 
 @pytest.mark.parametrize("scale", [1e-3, 1.0, 20.0])
-def test_scales(ctx, scale):
+def test_scales(ctx, tiles, scale):
     run(ctx, [(1, 400), (30, 300)], D=64, scale=scale)
     run(ctx, [(1, 400), (30, 300)], D=256, scale=scale, dtype="f16")
 
 
-def test_growing_scores(ctx):
+def test_growing_scores(ctx, tiles):
     """Keys whose scores rise along the text, by steps small and large: the running maximum moves in every tile, or in some."""
     for rise in (0.01, 0.05, 0.4):
         for D in (64, 256):
@@ -189,12 +203,12 @@ def test_growing_scores(ctx):
             check(text, x, got, D ** -0.5)
 
 
-def test_entries_that_are_no_pages(ctx):
+def test_entries_that_are_no_pages(ctx, tiles):
     for D in (64, 256):
         run(ctx, [(2, 100), (1, 40)], D=D, bad=[(0, 2, -1), (1, 0, 1 << 30), (0, 5, 1000)])
 
 
-def test_lengths_and_rows_past_their_ends(ctx):
+def test_lengths_and_rows_past_their_ends(ctx, tiles):
     """Lengths past the table, rows past q, begins that fall: clamped, nothing outside is touched."""
     text = Text([(2, 64), (3, 64)], 2, 64, 16, spare_entries=0)
     text.k.nan_to_num_(0.5), text.v.nan_to_num_(0.25)
@@ -218,7 +232,7 @@ def test_lengths_and_rows_past_their_ends(ctx):
 
 @pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
-def test_what_a_row_does_not_see_has_no_influence(ctx, D, what):
+def test_what_a_row_does_not_see_has_no_influence(ctx, tiles, D, what):
     """NaN and infinities in keys and values of later tokens of the chunk itself."""
     plan, nq, nk = [(40, 150), (3, 10)], 4, 2
     text, x, got = run(ctx, plan, nq=nq, nk=nk, D=D)
@@ -267,7 +281,7 @@ def test_the_same_bits_and_graphs(ctx):
     ctx.check()
 
 
-def test_strided_queries_and_outputs(ctx):
+def test_strided_queries_and_outputs(ctx, tiles):
     """Queries beside their gates, outputs inside a larger tensor, at any alignment."""
     text = Text([(1, 90), (20, 60)], 2, 128, 16)
     base = torch.randn((21, 8 * 2 * 128 + 3), device="cuda").bfloat16()
@@ -300,7 +314,7 @@ def test_far_pages(ctx):
     check(text, x, got, 0.125)
 
 
-def test_long_text(ctx):
+def test_long_text(ctx, tiles):
     """70001 tokens, whose scores' maxima come late."""
     for D, nk in ((256, 1), (64, 2)):
         text = Text([(2, 70001)], nk, D, 64, seed=2)
