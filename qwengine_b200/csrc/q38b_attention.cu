@@ -55,7 +55,7 @@ struct AttnArgs {
     int q_kind, out_kind, n_heads, n_kv, group, D, box_rows, slot_rows, q_vec, out_vec, pdl;
     float c;       // scale log2(e)
     uint32_t group_mul;   // x / group = x group_mul >> group_shift for 0 <= x < 2^31
-    int group_shift, ctas, q_shift;   // q_shift: log2 of the bytes of a query's element
+    int group_shift, ctas, q_shift, out_shift;   // log2 of the bytes of an element
 };
 __device__ __forceinline__ int by_group(const AttnArgs& a, int x) { return (int)((uint64_t)(uint32_t)x * a.group_mul >> a.group_shift); }
 
@@ -530,35 +530,48 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             else mbar_arrive(bar);
         };
         const auto load_queries = [&](const Walk& v) {
-            constexpr int UNITS = DP / 8, AHEAD = 4, STEP = QT == 2 ? 32 : 64;    // 16-byte pieces of a row; of a lane on their way; (QT = 1: the two warps of these rows take turns)
+            constexpr int UNITS = DP / 8, STEP = QT == 2 ? 32 : 64;    // 16-byte pieces of a row; (QT = 1: the two warps of these rows take turns)
             const int here = min(32, v.rows - (128 * t + 32 * quad)), pieces = here * UNITS;   // rows that are not there keep whatever they hold: it meets no other row
             uint8_t* to = q_at + qt * 128 * DP * 2 + 32 * quad * 128;
             if (here > 0) {
                 const int flat = v.row0 + row, in = by_group(a, flat);
                 const long long my_row = (long long)(v.first + in) * a.q_row + (long long)(v.kv * a.group + flat - in * a.group) * a.q_head;
+                const auto put = [&](int u, const uint4& x) {
+                    const int r = u / UNITS, e = u % UNITS * 8;
+                    if (u < pieces) *(uint4*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16) = x;
+                };
+                const auto ask = [&](int u, int half) {   // 16 bytes of a piece
+                    const long long at = __shfl_sync(0xffffffffu, my_row, u / UNITS & 31) + u % UNITS * 8;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (u < pieces && u % UNITS * 8 < a.D) x = ((const uint4*)((const uint8_t*)a.q + (at << a.q_shift)))[half];
+                    return x;
+                };
+                const int u1 = (QT == 2 ? 0 : 32 * g) + lane;
+                if (a.q_vec && a.q_shift == 1) {   // all of them on their way at once, past the registers
 #pragma unroll 1
-                for (int u0 = (QT == 2 ? 0 : 32 * g) + lane; u0 - lane < pieces; u0 += STEP * AHEAD) {
-                    long long at[AHEAD];
-                    uint4 x[AHEAD], y[AHEAD];
-                    // 16 bytes of the cache's type, or 32 of fp32, of each piece; what is not aligned goes an element at a time below
-#pragma unroll
-                    for (int n = 0; n < AHEAD; n++) {
-                        const int u = u0 + STEP * n;
-                        at[n] = __shfl_sync(0xffffffffu, my_row, u / UNITS & 31) + u % UNITS * 8;
-                        x[n] = y[n] = make_uint4(0, 0, 0, 0);
-                        if (a.q_vec && u < pieces && u % UNITS * 8 < a.D) {
-                            const uint4* p = (const uint4*)((const uint8_t*)a.q + (at[n] << a.q_shift));
-                            x[n] = p[0];
-                            if (a.q_shift == 2) y[n] = p[1];
-                        }
+                    for (int u = u1; u - lane < pieces; u += STEP) {
+                        const int r = u / UNITS, e = u % UNITS * 8;
+                        const long long at = __shfl_sync(0xffffffffu, my_row, r & 31) + e;
+                        if (u < pieces)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to) + (uint32_t)(e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16)),
+                                         "l"((const uint16_t*)a.q + (e < a.D ? at : 0)), "r"(e < a.D ? 16 : 0)
+                                         : "memory");
                     }
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                } else if (a.q_vec) {
+                    constexpr int AHEAD = 4;
+#pragma unroll 1
+                    for (int u0 = u1; u0 - lane < pieces; u0 += STEP * AHEAD) {
+                        uint4 x[AHEAD], y[AHEAD];
 #pragma unroll
-                    for (int n = 0; n < AHEAD; n++) {
-                        const int u = u0 + STEP * n, r = u / UNITS, e = u % UNITS * 8;
-                        if (a.q_shift == 2)
-                            x[n] = make_uint4(pack2<C>(__uint_as_float(x[n].x), __uint_as_float(x[n].y)), pack2<C>(__uint_as_float(x[n].z), __uint_as_float(x[n].w)),
-                                              pack2<C>(__uint_as_float(y[n].x), __uint_as_float(y[n].y)), pack2<C>(__uint_as_float(y[n].z), __uint_as_float(y[n].w)));
-                        if (u < pieces) *(uint4*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16) = x[n];
+                        for (int n = 0; n < AHEAD; n++) {
+                            x[n] = ask(u0 + STEP * n, 0);
+                            y[n] = ask(u0 + STEP * n, 1);
+                        }
+#pragma unroll
+                        for (int n = 0; n < AHEAD; n++)
+                            put(u0 + STEP * n, make_uint4(pack2<C>(__uint_as_float(x[n].x), __uint_as_float(x[n].y)), pack2<C>(__uint_as_float(x[n].z), __uint_as_float(x[n].w)),
+                                                          pack2<C>(__uint_as_float(y[n].x), __uint_as_float(y[n].y)), pack2<C>(__uint_as_float(y[n].z), __uint_as_float(y[n].w))));
                     }
                 }
                 if (!a.q_vec) {
@@ -647,19 +660,26 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                             tmem_ld_wait();
                             tmem_ld_arrived(o);
                             tmem_ld_arrived(o + 16);
-                            if (row >= w.rows) continue;
 #pragma unroll
                             for (int e = 0; e < 32; e++) o[e] = limit > 0 ? __float_as_uint(__uint_as_float(o[e]) * by) : 0u;
-                            if (a.out_kind == Q38B_OUT_F32) {
-#pragma unroll
-                                for (int e = 0; e < 32; e += 4)
-                                    if (k0 + e < a.D) *(uint4*)((float*)a.out + out_at + k0 + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                            } else {
+                            if (a.out_kind != Q38B_OUT_F32)
 #pragma unroll
                                 for (int e = 0; e < 32; e += 2) o[e / 2] = pack2<C>(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+                            if (row >= w.rows) continue;
+                            // whole sectors of 32 bytes where they are aligned: stores of 16 went to 32 lines each as well (128 rows of 256 in 5500 clocks)
+                            uint8_t* to = (uint8_t*)a.out + ((out_at + k0) << a.out_shift);
+                            const int bytes = min(32, a.D - k0) << a.out_shift;
+                            if (a.out_vec == 2) {
 #pragma unroll
-                                for (int e = 0; e < 32; e += 8)
-                                    if (k0 + e < a.D) *(uint4*)((uint16_t*)a.out + out_at + k0 + e) = make_uint4(o[e / 2], o[e / 2 + 1], o[e / 2 + 2], o[e / 2 + 3]);
+                                for (int i = 0; i < 4; i++)
+                                    if (32 * i < bytes)
+                                        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + 32 * i), "r"(o[8 * i]), "r"(o[8 * i + 1]), "r"(o[8 * i + 2]), "r"(o[8 * i + 3]),
+                                                     "r"(o[8 * i + 4]), "r"(o[8 * i + 5]), "r"(o[8 * i + 6]), "r"(o[8 * i + 7])
+                                                     : "memory");
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 8; i++)
+                                    if (16 * i < bytes) *(uint4*)(to + 16 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
                             }
                         }
                     } else {   // another type or alignment: a column at a time
@@ -1063,9 +1083,10 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     a.k_page = c->k_page; a.k_slot = c->k_slot; a.k_head = c->k_head; a.v_page = c->v_page; a.v_slot = c->v_slot; a.v_head = c->v_head;
     a.q_kind = q_kind; a.out_kind = out_kind; a.n_heads = n_heads; a.n_kv = c->n_heads; a.group = n_heads / c->n_heads; a.D = c->D;
     // Two tiles of rows share the keys' and values' way into shared memory, in one CTA (heads of at most 128) or in a pair of them (more than 192), where sequences fill
-    // more than one on average and there are enough of them for all SMs.
+    // more than one on average and there are enough of them: of 12288 (row, head) pairs of 256 elements behind 2000 tokens 60.3 -> 51.8 us, 7512 pairs 40.5 -> 44.4; 32768 of 128
+    // behind nothing 44.5 -> 36.2, 10016 14.0 -> 16.8.
     const bool two = ctx->attention_two ? ctx->attention_two > 0
-                                        : (long long)rows * a.group > 128LL * c->n_seqs && (long long)rows * n_heads >= (padded(c->D) == 256 ? 128LL : 256LL) * ctx->sm_count;
+                                        : (long long)rows * a.group > 128LL * c->n_seqs && (long long)rows * n_heads >= (padded(c->D) == 256 ? 80LL : 128LL) * ctx->sm_count;
     const bool pair = two && padded(c->D) == 256;
     a.box_rows = std::min(c->page_size, pair ? KEYS / 2 : KEYS);
     a.slot_rows = slot_rows(a.group, pair ? 128 : c->D, rows);
@@ -1075,7 +1096,9 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     a.status = ctx->d_status;
     a.q_shift = q_kind == Q38B_OUT_F32 ? 2 : 1;
     a.q_vec = (((uintptr_t)q | (uintptr_t)(q_row * kind_size(q_kind)) | (uintptr_t)(q_head * kind_size(q_kind))) & 15) == 0;
-    a.out_vec = (((uintptr_t)out | (uintptr_t)(out_row * kind_size(out_kind)) | (uintptr_t)(out_head * kind_size(out_kind))) & 15) == 0;
+    a.out_shift = out_kind == Q38B_OUT_F32 ? 2 : 1;
+    const uintptr_t out_at = (uintptr_t)out | (uintptr_t)(out_row * kind_size(out_kind)) | (uintptr_t)(out_head * kind_size(out_kind)) | (uintptr_t)(c->D * kind_size(out_kind));
+    a.out_vec = out_at % 32 == 0 ? 2 : out_at % 16 == 0 ? 1 : 0;
     a.pdl = ctx->pass_pdl ? 1 : 0;
     a.c = (float)((double)scale * 1.4426950408889634);
     int log = 0;
