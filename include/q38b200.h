@@ -326,7 +326,7 @@ int q38b_cache_append(q38b_ctx* ctx, const q38b_paged_kv* cache, const void* k_d
 /* Attention of the chunk's rows over their sequences: for new token i of sequence s and query head h, which reads key head h / (n_heads / cache->n_heads),
  *   out = sum_j softmax_j(scale q . k_j) v_j    over the sequence's tokens j <= lengths[s] - new + i
  * q: q_kind, element e of head h of a row at row * q_row + h * q_head + e; out likewise in out_kind.  n_heads: a multiple of the cache's.  scale > 0,
- * finite.  fp32 queries are rounded to the cache's type; products and sums in fp32, weights rounded to the cache's type before they multiply values
+ * finite; rows * n_heads below 2^30, and (rows * n_heads / 128 + n_seqs * cache->n_heads) * (table_n * page_size / 128 + 1) below 2^31.  fp32 queries are rounded to the cache's type; products and sums in fp32, weights rounded to the cache's type before they multiply values
  * (2^-8 of each at most in bf16, 2^-11 in fp16), outputs rounded once.  A row that sees no token gives zeros.  A key or value that a row does not
  * see has no influence on it, whatever it holds.  lse_dev (or NULL): fp32 [rows][n_heads], the natural logarithm of sum_j exp(scale q . k_j),
  * -infinity where no token is seen.  rows: those of q and out (1 and more).  work: q38b_attention_work_bytes bytes, 16-byte aligned, the caller's, not
@@ -423,6 +423,12 @@ int q38b_pass_op_adjust_logits(q38b_pass* pass, int src_f32, int off, int n, con
 /* The same on a shard of the head: the first of the n logits is that of token index_offset. */
 int q38b_pass_op_adjust_logits_at(q38b_pass* pass, int src_f32, int off, int n, int index_offset, const q38b_logit_rules* rules, int dst_f32,
                                   int dst_off);
+/* q38b_cache_append and q38b_attention between two steps of a pass: a column is a row of the batch (max_nb of them at most; a run for fewer columns ends the
+ * batch there), offsets and strides in floats of a column.  k and v: buffer, first element of head 0, distance of two heads.  q: queries from src, outputs
+ * to dst, which must not overlap; weight NULL.  The cache and its device arrays belong to the caller; table, lengths and begin are read at every run.  The work area is
+ * the pass's. */
+int q38b_pass_op_cache_append(q38b_pass* pass, const q38b_paged_kv* cache, int k_f32, int k_off, int k_head, int v_f32, int v_off, int v_head);
+int q38b_pass_op_attention(q38b_pass* pass, const q38b_paged_kv* cache, const q38b_pass_heads* q, float scale);
 /* After q38b_peer_connect the fp32 buffers of a pass live in the arena and matvec steps push their outputs to every
  * peer; q38b_pass_op_barrier then makes them usable on all ranks.  One barrier may cover several matvecs. */
 int q38b_pass_op_barrier(q38b_pass* pass);

@@ -129,6 +129,8 @@ def load_library():
     lib.q38b_attention_work_bytes.argtypes = [vp, i32, i32, i32, i32]
     lib.q38b_attention_work_bytes.restype = sz
     lib.q38b_attention.argtypes = [vp, vp, vp, i32, ll, ll, i32, C.c_float, vp, i32, ll, ll, vp, i32, vp, sz, vp]
+    lib.q38b_pass_op_cache_append.argtypes = [vp, vp, i32, i32, i32, i32, i32, i32]
+    lib.q38b_pass_op_attention.argtypes = [vp, vp, vp, C.c_float]
     lib.q38b_quantize_i8.argtypes = [vp, vp, i32, ll, i32, i32, vp, ll, vp, vp]
     lib.q38b_gemm_i8.argtypes = [vp, vp, ll, vp, i32, i32, vp, ll, vp, i32, vp, i32, ll, i32, vp]
     lib.q38b_debug_set_i8_cut.argtypes = [vp, i32]
@@ -869,6 +871,22 @@ class Pass:
         packed = self.ctx.logit_rules(self.max_nb, n, index_offset=index_offset, **rules)
         self.ctx._rc(self.lib.q38b_pass_op_adjust_logits_at(self.h, src, off, n, index_offset, packed, dst, dst_off), "q38b_pass_op_adjust_logits_at")
         self._keep += [t for t in rules.values() if isinstance(t, torch.Tensor)]
+
+    def cache_append(self, cache, k, v, table, lengths, begin):
+        """k, v: dicts of buf and, if need be, off (0) and head (D): the columns' new keys and values into a PagedCache, as Context.cache_append does.  The cache and the int32
+        device tensors table, lengths and begin are kept by the pass and read at every run; a column is a row of the batch."""
+        _need(cache.k.device == self.ctx.device, "cache_append: a cache on the context's device")
+        self.ctx._rc(self.lib.q38b_pass_op_cache_append(self.h, cache.batch(table, lengths, begin), k["buf"], k.get("off", 0), k.get("head", cache.D), v["buf"], v.get("off", 0),
+                                                        v.get("head", cache.D)), "q38b_pass_op_cache_append")
+        self._keep += [cache, table, lengths, begin]
+
+    def attention(self, cache, q, out, table, lengths, begin, scale=None):
+        """q: dict of buf, n_heads and, if need be, off (0), head (D); out: dict of buf and, if need be, off (0), head (D): Context.attention of the columns over a PagedCache.
+        What is said of cache_append holds."""
+        _need(cache.k.device == self.ctx.device, "attention: a cache on the context's device")
+        heads = _pack_pass_heads(q["buf"], q.get("off", 0), q.get("head", cache.D), out["buf"], out.get("off", 0), out.get("head", cache.D), q["n_heads"], 0)
+        self.ctx._rc(self.lib.q38b_pass_op_attention(self.h, cache.batch(table, lengths, begin), heads, cache.D ** -0.5 if scale is None else scale), "q38b_pass_op_attention")
+        self._keep += [cache, table, lengths, begin]
 
     def barrier(self):
         self.ctx._rc(self.lib.q38b_pass_op_barrier(self.h), "q38b_pass_op_barrier")

@@ -1069,9 +1069,7 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     if (n_heads < 1 || n_heads % c->n_heads || q_row < 0 || q_head < 0 || out_row < 0 || out_head < 0) return Q38B_ERR_ARG;
     if ((n_heads > 1 && out_head < c->D) || (rows > 1 && out_row < c->D)) return Q38B_ERR_ARG;
     if (q_kind != Q38B_OUT_F32 && q_kind != c->kind) return Q38B_ERR_UNSUPPORTED;
-    if ((long long)rows * n_heads > 0x3FFFFFFF) return Q38B_ERR_UNSUPPORTED;
-    // (units are counted in 32 bits)
-    if (((long long)rows * n_heads / 128 + (long long)c->n_seqs * c->n_heads) * ((long long)c->table_n * c->page_size / KEYS + 1) > 0x7FFFFFFF) return Q38B_ERR_UNSUPPORTED;
+    if (!attention_fits(c, n_heads, rows)) return Q38B_ERR_UNSUPPORTED;
     if ((uintptr_t)q % kind_size(q_kind) || (uintptr_t)out % kind_size(out_kind) || ((uintptr_t)lse & 3) || ((uintptr_t)work & 15)) return Q38B_ERR_ALIGN;
     if (work_bytes < 16 || work_bytes < q38b_attention_work_bytes(ctx, n_heads, c->n_heads, c->D, rows)) return Q38B_ERR_NOMEM;
     DeviceGuard on(ctx);

@@ -4,13 +4,16 @@
 #include <dlfcn.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "../../include/q38b200.h"
 #include "q38b_act.cuh"
 #include "q38b_pipe.cuh"
+#include "q38b_cache.cuh"
 #include "q38b_internal.h"
 
 using namespace q38b;
@@ -51,12 +54,14 @@ Nccl& nccl() {
 }
 constexpr int NCCL_FLOAT = 7;
 
-enum OpKind { OP_QUANT, OP_GEMV, OP_SWIGLU, OP_GATHER, OP_BARRIER, OP_TOPK, OP_HEADS, OP_LOGITS };
+enum OpKind { OP_QUANT, OP_GEMV, OP_SWIGLU, OP_GATHER, OP_BARRIER, OP_TOPK, OP_HEADS, OP_LOGITS, OP_APPEND, OP_ATTENTION };
 struct Op { int kind, a, b, c, d, n, off; };
 struct Buf { void* ptr; int n; bool q8k; void* peer[8]; int n_peer_ranks; bool in_arena; };
 // q38b_pass_op_qk_norm_rope, q38b_pass_op_adjust_logits: what an Op has no room for (Op::a is their number)
 struct HeadsStep { q38b_pass_heads t[2]; int n_tensors, D, rot, adjacent; float eps, scale; const int* positions; const double* inv_freq; };
 struct LogitsStep { q38b_logit_rules rules; int index_offset; };
+// q38b_pass_op_cache_append (keys, values) and q38b_pass_op_attention (queries and outputs, one tensor): their number is Op::a
+struct CacheStep { q38b_paged_kv cache; q38b_pass_heads t[2]; float scale; void* work; size_t work_bytes; };
 struct Mat { uint32_t type; const void* W; size_t row_bytes; int K, M; bool owned; };
 
 struct PeerPtrs { uint32_t* p[8]; };
@@ -86,6 +91,8 @@ struct q38b_pass {
     std::vector<Op> ops;
     std::vector<HeadsStep> heads;
     std::vector<LogitsStep> logits;
+    std::vector<CacheStep> caches;
+    std::vector<std::pair<void*, size_t>> work;   // areas of the attention steps: one behind the other they share the last that is large enough
     cudaGraphExec_t graphs[9] = {};
     size_t arena_mark = (size_t)-1;
     int peer_store = 1;
@@ -408,6 +415,21 @@ int enqueue_ops(q38b_pass* p, int nb, cudaStream_t st) {
                 rc = q38b_adjust_logits(ctx, (const float*)from.ptr + o.off, from.n, o.n, nb, s.index_offset, &s.rules, (float*)to.ptr + o.d, to.n, st);
                 break;
             }
+            case OP_APPEND: {
+                const CacheStep& s = p->caches[o.a];
+                const Buf &k = p->bufs[s.t[0].src], &v = p->bufs[s.t[1].src];
+                rc = q38b_cache_append(ctx, &s.cache, (const float*)k.ptr + s.t[0].src_off, (const float*)v.ptr + s.t[1].src_off, Q38B_OUT_F32, k.n, s.t[0].src_head, v.n, s.t[1].src_head,
+                                       nb, st);
+                break;
+            }
+            case OP_ATTENTION: {
+                const CacheStep& s = p->caches[o.a];
+                const q38b_pass_heads& t = s.t[0];
+                const Buf &from = p->bufs[t.src], &to = p->bufs[t.dst];
+                rc = q38b_attention(ctx, &s.cache, (const float*)from.ptr + t.src_off, Q38B_OUT_F32, from.n, t.src_head, t.n_heads, s.scale, (float*)to.ptr + t.dst_off, Q38B_OUT_F32, to.n,
+                                    t.dst_head, nullptr, nb, s.work, s.work_bytes, st);
+                break;
+            }
             case OP_BARRIER: {
                 if (n_barriers == 0) break;
                 if (ctx->pending_sync_seq >= 0) {   // two barriers in a row: the earlier one runs by itself
@@ -549,6 +571,7 @@ void q38b_pass_destroy(q38b_pass* p) {
     for (auto& b : p->bufs) if (b.ptr && !b.in_arena) cudaFree(b.ptr);
     if (p->arena_mark != (size_t)-1) p->ctx->arena_used = p->arena_mark;   // passes release arena space in LIFO order
     for (auto& m : p->mats) if (m.owned && m.W) cudaFree((void*)m.W);
+    for (auto& w : p->work) cudaFree(w.first);
     if (p->cap_stream) cudaStreamDestroy(p->cap_stream);
     if (p->pin_in) cudaFreeHost(p->pin_in);
     if (p->pin_out) cudaFreeHost(p->pin_out);
@@ -694,6 +717,53 @@ int q38b_pass_op_adjust_logits(q38b_pass* p, int src, int off, int n, const q38b
     return q38b_pass_op_adjust_logits_at(p, src, off, n, 0, rules, dst, dst_off);
 }
 
+int q38b_pass_op_cache_append(q38b_pass* p, const q38b_paged_kv* cache, int k, int k_off, int k_head, int v, int v_off, int v_head) {
+    if (!p || !is_f32(p, k) || !is_f32(p, v) || k_off < 0 || v_off < 0 || k_head < 0 || v_head < 0) return Q38B_ERR_ARG;
+    const int rc = paged_kv_check(cache);
+    if (rc != Q38B_OK) return rc;
+    if (k_off + (long long)(cache->n_heads - 1) * k_head + cache->D > p->bufs[k].n || v_off + (long long)(cache->n_heads - 1) * v_head + cache->D > p->bufs[v].n) return Q38B_ERR_ARG;
+    CacheStep s = {*cache, {}, 0.0f, nullptr, 0};
+    s.t[0].src = k; s.t[0].src_off = k_off; s.t[0].src_head = k_head;
+    s.t[1].src = v; s.t[1].src_off = v_off; s.t[1].src_head = v_head;
+    try {
+        p->caches.push_back(s);
+        p->ops.push_back({OP_APPEND, (int)p->caches.size() - 1, 0, 0, 0, 0, 0});
+    } catch (...) {
+        return Q38B_ERR_NOMEM;
+    }
+    return Q38B_OK;
+}
+
+int q38b_pass_op_attention(q38b_pass* p, const q38b_paged_kv* cache, const q38b_pass_heads* q, float scale) {
+    if (!p || !q || !is_f32(p, q->src) || !is_f32(p, q->dst) || q->weight || q->n_heads < 1 || q->src_off < 0 || q->dst_off < 0 || q->src_head < 0 || q->dst_head < 0) return Q38B_ERR_ARG;
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return Q38B_ERR_ARG;
+    const int rc = paged_kv_check(cache);
+    if (rc != Q38B_OK) return rc;
+    if (q->n_heads % cache->n_heads || (q->n_heads > 1 && q->dst_head < cache->D)) return Q38B_ERR_ARG;
+    const long long src_end = q->src_off + (long long)(q->n_heads - 1) * q->src_head + cache->D, dst_end = q->dst_off + (long long)(q->n_heads - 1) * q->dst_head + cache->D;
+    if (src_end > p->bufs[q->src].n || dst_end > p->bufs[q->dst].n) return Q38B_ERR_ARG;
+    if (q->src == q->dst && q->src_off < dst_end && q->dst_off < src_end) return Q38B_ERR_ARG;
+    if (!attention_fits(cache, q->n_heads, p->max_nb)) return Q38B_ERR_UNSUPPORTED;
+    CacheStep s = {*cache, {*q, {}}, scale, nullptr, q38b_attention_work_bytes(p->ctx, q->n_heads, cache->n_heads, cache->D, p->max_nb)};
+    try {
+        if (p->work.empty() || p->work.back().second < s.work_bytes) {
+            p->work.push_back({nullptr, s.work_bytes});
+            const cudaError_t e = cudaMalloc(&p->work.back().first, s.work_bytes);
+            if (e != cudaSuccess) {
+                p->work.pop_back();
+                p->ctx->last_cuda = (int)e;
+                return Q38B_ERR_CUDA;
+            }
+        }
+        s.work = p->work.back().first;
+        p->caches.push_back(s);
+        p->ops.push_back({OP_ATTENTION, (int)p->caches.size() - 1, 0, 0, 0, 0, 0});
+    } catch (...) {
+        return Q38B_ERR_NOMEM;
+    }
+    return Q38B_OK;
+}
+
 int q38b_pass_op_swiglu(q38b_pass* p, int g, int g_off, int u, int u_off, int n, int dst) {
     if (!p || !is_f32(p, g) || !is_f32(p, u) || !is_q8k(p, dst) || n % 256 || g_off < 0 || u_off < 0) return Q38B_ERR_ARG;
     if (g_off + n > p->bufs[g].n || u_off + n > p->bufs[u].n || p->bufs[dst].n < n || p->bufs[g].n != p->bufs[u].n) return Q38B_ERR_ARG;
@@ -779,7 +849,7 @@ int q38b_pass_set_merge(q38b_pass* p, int enabled) {
 }
 
 // The steps of the test hooks below, on a pass without a device: steps[3 i ..] = {kind (0 quantize, 1 matvec, 2 SwiGLU, 3 all-gather, 4 barrier, 5 heads,
-// 6 logit rules, 7 top-k), column buffer, output offset}; every matvec is a 512 x 1024 Q4_K matrix writing 512 floats at its offset.
+// 6 logit rules, 7 top-k, 8 cache append, 9 attention), column buffer, output offset}; every matvec is a 512 x 1024 Q4_K matrix writing 512 floats at its offset.
 static bool debug_steps(q38b_ctx& ctx, q38b_pass& p, int n_ranks, int n_steps, const int* steps) {
     ctx.sm_count = 148;
     ctx.smem_optin = 232448;
@@ -798,6 +868,8 @@ static bool debug_steps(q38b_ctx& ctx, q38b_pass& p, int n_ranks, int n_steps, c
             case 5: p.ops.push_back({OP_HEADS, 0, 0, 0, 0, 0, 0}); break;
             case 6: p.ops.push_back({OP_LOGITS, 0, 1, 1, off, 512, off}); break;
             case 7: p.ops.push_back({OP_TOPK, 1, 2, 0, 32, 512, off}); break;
+            case 8: p.ops.push_back({OP_APPEND, 0, 0, 0, 0, 0, 0}); break;
+            case 9: p.ops.push_back({OP_ATTENTION, 0, 0, 0, 0, 0, 0}); break;
             default: return false;
         }
     }
@@ -868,7 +940,7 @@ int q38b_pass_kernel_count(const q38b_pass* p) {
     for (size_t i = 0; i < p->ops.size(); i++) {
         const Op& o = p->ops[i];
         n += !skip[i] && (o.kind != OP_GATHER) && (o.kind != OP_BARRIER || p->ctx->n_ranks > 1);
-        n += o.kind == OP_TOPK;   // two kernels
+        n += o.kind == OP_TOPK || o.kind == OP_ATTENTION;   // two kernels
     }
     return n + (int)merged.size();
 }

@@ -64,7 +64,7 @@ def total_weight_bytes(n_layers=N_LAYERS, head=True):
     return sum(m.nbytes for m in all_specs(n_layers, head))
 
 
-def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather="peer", replicate_small=True, heads=None, rules=None):
+def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather="peer", replicate_small=True, heads=None, rules=None, cache=None):
     """Records the pass on `ps` (qwengine_b200.Pass).
 
     make_matrix(spec, rows) -> matrix id for this rank's shard of `rows` rows (rows = spec.M // world);
@@ -81,6 +81,9 @@ def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather
     heads: dict(positions, inv_freq, q_weight, k_weight, eps) of device tensors (Pass.qk_norm_rope): the attention layers then norm and rotate their
     query heads (24 of 256, beside their gates) and key heads (4 of 256) in place, as the reference does before its attention.
     rules: dict of Context.logit_rules' tensors: the head's logits are penalised, biased and masked in place before the top-k.
+    cache: dict(caches, table, lengths, begin): one PagedCache (4 key heads of 256) for each attention layer and the batch's device tensors (Pass.attention).  The
+    attention layers then write their keys and values into it, and their query heads' attention over it, instead of the first projection outputs, goes
+    on to the output projection (the sigmoid gate between the two is the host's).
     Returns dict(in_buf, out_buf, out_len, topk_buf, topk_k).
     """
     x_in = ps.buffer_f32(HIDDEN)           # the token's hidden state: read by layer 0 only, never written, so that
@@ -93,6 +96,7 @@ def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather
     gu = ps.buffer_f32(2 * FF)             # gate | up
     hq = ps.buffer_q8k(FF)
     ffn = ps.buffer_f32(HIDDEN)            # FFN block outputs (see below)
+    mixed = ps.buffer_f32(INNER) if cache is not None else None   # the attention's outputs
     logits = ps.buffer_f32(VOCAB) if head else None
     peer = world > 1 and gather == "peer"   # needs Context.peer_connect before the pass is created
     if hasattr(ps, "set_peer_store"):
@@ -128,7 +132,11 @@ def build(ps, make_matrix, n_layers=N_LAYERS, head=True, rank=0, world=1, gather
         sync(not whole)
         if attn and heads is not None:
             ps.qk_norm_rope(dict(buf=big, n_heads=12288 // (2 * HEAD_DIM), head=2 * HEAD_DIM), dict(buf=kv, n_heads=1024 // HEAD_DIM), HEAD_DIM, **heads)
-        ps.quantize(big, 0, INNER, iq)
+        if attn and cache is not None:
+            batch = (cache["table"], cache["lengths"], cache["begin"])
+            ps.cache_append(cache["caches"][il // 4], dict(buf=kv), dict(buf=kv, off=1024), *batch)
+            ps.attention(cache["caches"][il // 4], dict(buf=big, n_heads=INNER // HEAD_DIM, head=2 * HEAD_DIM), dict(buf=mixed), *batch)
+        ps.quantize(mixed if attn and cache is not None else big, 0, INNER, iq)
         matvec(proj_out, iq, x, 0, shard=not whole)
         sync(not whole)
         ps.quantize(x, 0, HIDDEN, xq)
