@@ -5,6 +5,8 @@
     python -m qwengine_b200.single --op mx4 --M 17408 --K 5120 --tokens 2048          # 4-bit weights and activations, the quantizer included
     python -m qwengine_b200.single --op heads --tokens 8192                           # 24 + 4 heads of 256: norm, rotation
     python -m qwengine_b200.single --op logits --tokens 128 --history 8000            # penalties and a mask on rows of 248320
+    python -m qwengine_b200.single --op i8 --M 17408 --K 5120 --tokens 2048           # 8-bit integer weights and activations, the quantizer included
+    python -m qwengine_b200.single --op attention --tokens 4096 --history 28672       # 24 + 4 heads of 256 over a paged cache; --seqs 32 --tokens 1: decoding
 
 Matvec: `copies` distinct resident matrices (random valid blocks; by default enough to exceed 1.5 GB, far beyond L2)
 are recorded as one pass and replayed as a CUDA graph, so host launch overhead does not count.
@@ -14,18 +16,19 @@ import json
 
 import torch
 
-from . import Context, Pass, formats as F
+from . import Context, PagedCache, Pass, formats as F
 
 
 def main():
     ap = argparse.ArgumentParser()
-    ap.add_argument("--op", default="gemv", choices=["gemv", "prefill", "mx4", "heads", "logits"])
+    ap.add_argument("--op", default="gemv", choices=["gemv", "prefill", "mx4", "heads", "logits", "i8", "attention"])
     ap.add_argument("--fmt", default="IQ3_XXS")
     ap.add_argument("--M", type=int, default=17408)
     ap.add_argument("--K", type=int, default=5120)
     ap.add_argument("--nb", type=int, default=1)
     ap.add_argument("--tokens", type=int, default=1024)
     ap.add_argument("--history", type=int, default=1000)
+    ap.add_argument("--seqs", type=int, default=1)
     ap.add_argument("--copies", type=int, default=0)
     ap.add_argument("--reps", type=int, default=5)
     ap.add_argument("--no-pdl", action="store_true")
@@ -126,7 +129,35 @@ def logits(ctx, a):
     print(json.dumps({"op": "logits", "rows": a.tokens, "history": a.history, "us": round(us, 2), "GBps": round(a.tokens * (n * 8.125 + a.history * 4) / us / 1e3, 1)}))
 
 
-STEPS = {"mx4": mx4, "heads": heads, "logits": logits}
+def i8(ctx, a):
+    copies = a.copies or int(3e8 // (a.M * a.K)) + 1
+    Ws = [ctx.quantize_i8(torch.randn((a.M, a.K), device="cuda", dtype=torch.bfloat16)) for _ in range(copies)]
+    x = torch.randn((a.tokens, a.K), device="cuda", dtype=torch.bfloat16)
+    y = torch.empty((a.tokens, a.M), device="cuda", dtype=torch.bfloat16)
+    us = timed([lambda W=W: ctx.gemm_i8(W, x, out=y) for W in Ws], a.reps)
+    ctx.check()
+    print(json.dumps({"op": "i8", "M": a.M, "K": a.K, "tokens": a.tokens, "copies": copies, "us": round(us, 2), "weight_GBps": round(a.M * a.K / us / 1e3, 1),
+                      "TOPs": round(2.0 * a.tokens * a.M * a.K / us / 1e6, 1)}))
+
+
+def attention(ctx, a):
+    text, page = a.tokens + a.history, 64
+    per = (text + page - 1) // page
+    copies = a.copies or int(3e8 // (a.seqs * text * 4096)) + 1
+    caches = [PagedCache(*(torch.randn((a.seqs * per, page, 4, 256), device="cuda", dtype=torch.bfloat16) for _ in range(2))) for _ in range(min(copies, 40))]
+    table = torch.arange(a.seqs * per, device="cuda", dtype=torch.int32).view(a.seqs, per)
+    lengths = torch.full((a.seqs,), text, device="cuda", dtype=torch.int32)
+    begin = torch.arange(a.seqs + 1, device="cuda", dtype=torch.int32) * a.tokens
+    x = torch.randn((a.seqs * a.tokens, 24, 256), device="cuda", dtype=torch.bfloat16)
+    y = torch.empty_like(x)
+    us = timed([lambda c=c: ctx.attention(c, x, table, lengths, begin, out=y) for c in caches], a.reps)
+    ctx.check()
+    pairs = a.seqs * (a.tokens * a.history + a.tokens * (a.tokens + 1) // 2)
+    print(json.dumps({"op": "attention", "seqs": a.seqs, "tokens": a.tokens, "history": a.history, "copies": len(caches), "us": round(us, 2),
+                      "GBps": round((a.seqs * text * 4096 + x.numel() * 4) / us / 1e3, 1), "TFLOPs": round(4 * pairs * 24 * 256 / us / 1e6, 1)}))
+
+
+STEPS = {"mx4": mx4, "heads": heads, "logits": logits, "i8": i8, "attention": attention}
 
 
 if __name__ == "__main__":

@@ -63,7 +63,7 @@ def test_append(lib, change, status):
 @pytest.mark.parametrize("change,status", [
     (dict(q=None), ARG), (dict(out=None), ARG), (dict(cache=None), ARG), (dict(work=None), ARG), (dict(rows=0), ARG), (dict(n_heads=0), ARG), (dict(n_heads=3), ARG), (dict(q_kind=4), ARG),
     (dict(out_kind=-1), ARG), (dict(q_kind=1), UNSUPPORTED), (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG), (dict(scale=float("nan")), ARG), (dict(scale=float("inf")), ARG),
-    (dict(q_row=-1), ARG), (dict(q_head=-1), ARG), (dict(out_row=63), ARG), (dict(out_head=32), ARG), (dict(q=P + 1), ALIGN), (dict(out=P + 1), ALIGN), (dict(out_kind=0, out=P + 2), ALIGN),
+    (dict(q_row=-1), ARG), (dict(q_head=-1), ARG), (dict(out_row=63), ARG), (dict(out_head=32), ARG), (dict(out_row=255), ARG), (dict(out_row=64), ARG), (dict(out_row=64, out_head=319), ARG), (dict(q=P + 1), ALIGN), (dict(out=P + 1), ALIGN), (dict(out_kind=0, out=P + 2), ALIGN),
     (dict(lse=P + 2), ALIGN), (dict(work=P + 8), ALIGN), (dict(work_bytes=15), NOMEM)])
 def test_attention(lib, change, status):
     a = dict(cache=paged(), q=P, q_kind=2, q_row=256, q_head=64, n_heads=4, scale=0.125, out=P, out_kind=2, out_row=256, out_head=64, lse=None, rows=5, work=P, work_bytes=1 << 40)

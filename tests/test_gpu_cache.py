@@ -156,6 +156,13 @@ def test_lengths(ctx, tiles, total, new, D):
     run(ctx, [(new, total)], D=D, seed=total)     # some chunks are longer than their text: rows that see nothing
 
 
+@pytest.mark.parametrize("n", [383, 384, 385, 1000])
+def test_many_sequences(ctx, tiles, n):
+    rng = np.random.default_rng(n)
+    run(ctx, [(int(k), int(t)) for k, t in zip(rng.integers(0, 3, n), rng.integers(0, 60, n))], nq=2, nk=1, D=64)
+    run(ctx, [(0, 5)] * (n - 1) + [(1, 300)], nq=2, nk=1, D=256)
+
+
 def test_many_rows(ctx):
     """Enough rows for the rule to take two tiles of them together: several sequences, cuts inside tiles."""
     for D, nq, nk, dtype in ((256, 24, 4, "bf16"), (128, 48, 8, "f16"), (64, 48, 8, "bf16")):
