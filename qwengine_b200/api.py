@@ -210,24 +210,27 @@ class PagedCache:
     __slots__ = ("k", "v", "n_pages", "page_size", "n_heads", "D", "kind", "_head")
 
     def __init__(self, k, v):
-        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.dtype not in (torch.float16, torch.bfloat16) or k.get_device() != v.get_device():
+        shape, dtype = k.shape, k.dtype
+        kind = _OUT_KINDS.get(dtype, OUT_F32)
+        if len(shape) != 4 or 0 in shape or shape != v.shape or dtype is not v.dtype or kind == OUT_F32 or k.get_device() != v.get_device():
             raise ValueError("PagedCache: fp16 or bf16 keys and values [pages, page_size, heads, D] of one shape and type, on one device")
-        self.n_pages, self.page_size, self.n_heads, self.D = k.shape
-        if k.stride(3) != 1 or v.stride(3) != 1:
+        k_page, k_slot, k_head, k_one = k.stride()
+        v_page, v_slot, v_head, v_one = v.stride()
+        if k_one != 1 or v_one != 1:
             raise ValueError("PagedCache: elements of a head side by side")
-        self.k, self.v, self.kind = k, v, _OUT_KINDS[k.dtype]
-        self._head = (k.data_ptr(), v.data_ptr(), *k.stride()[:3], *v.stride()[:3], self.kind, self.n_pages, self.page_size, self.n_heads, self.D)
+        self.n_pages, self.page_size, self.n_heads, self.D = pages, size, heads, D = shape
+        self.k, self.v, self.kind = k, v, kind
+        self._head = (k.data_ptr(), v.data_ptr(), k_page, k_slot, k_head, v_page, v_slot, v_head, kind, pages, size, heads, D)
 
     def batch(self, table, lengths, begin):
         """The bytes of a q38b_paged_kv of these pages and a checked batch: table int32 [sequences, entries], lengths int32 [sequences], begin int32
         [sequences + 1]."""
         n, entries = table.shape
         ld, one = table.stride()
-        dev = self.k.get_device()
-        if (table.dtype != _I32 or lengths.dtype != _I32 or begin.dtype != _I32 or lengths.shape != (n,) or begin.shape != (n + 1,) or (one != 1 and entries != 1) or
+        if (table.dtype is not _I32 or lengths.dtype is not _I32 or begin.dtype is not _I32 or lengths.shape != (n,) or begin.shape != (n + 1,) or (one != 1 and entries != 1) or
                 not lengths.is_contiguous() or not begin.is_contiguous()):
             raise ValueError("PagedCache: int32 table [sequences, entries], lengths [sequences], begin [sequences + 1]")
-        if table.get_device() != dev or lengths.get_device() != dev or begin.get_device() != dev:
+        if not self.k.get_device() == table.get_device() == lengths.get_device() == begin.get_device():
             raise ValueError("PagedCache: table, lengths and begin on the cache's device")
         return _pack_paged(*self._head, n, table.data_ptr(), ld if n > 1 else entries, entries, lengths.data_ptr(), begin.data_ptr())
 
@@ -245,6 +248,7 @@ class Context:
         if rc:
             raise Q38BError(rc, "q38b_ctx_create")
         self.h = h
+        self._ctas = min(torch.cuda.get_device_properties(device).multi_processor_count, 256)   # of the attention's kernel
 
     def close(self):
         if getattr(self, "h", None):
@@ -629,7 +633,8 @@ class Context:
             raise ValueError("attention: lse fp32 [rows, heads] on the context's device")
         if rows == 0:
             return out
-        need = self.lib.q38b_attention_work_bytes(self.h, heads, cache.n_heads, D, rows)
+        wide = (D + 63) // 64 * 64
+        need = self._ctas * (32 + 8 * min(256 if wide <= 128 else 128, rows * (heads // cache.n_heads)) * (wide + 4))   # q38b_attention_work_bytes
         work = _empty((need,), (1,), dtype=_U8, device=self.device)
         rc = self.lib.q38b_attention(self.h, cache.batch(table, lengths, begin), q.data_ptr(), q_kind, q_row, q_head, heads, D ** -0.5 if scale is None else scale, out.data_ptr(),
                                      kind, out_row, out_head, None if lse is None else lse.data_ptr(), rows, work.data_ptr(), need, _current_stream(dev))

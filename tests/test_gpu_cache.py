@@ -375,6 +375,20 @@ def test_append_finds_rows_of_many_sequences(ctx):
         assert int((text.k != 0).sum()) == text.rows * 8
 
 
+def test_the_wrappers_work_area_is_the_librarys(ctx):
+    """The wrapper counts its bytes itself: less would be refused, more is not needed."""
+    for D, nq, nk, rows in ((64, 4, 2, 1), (8, 1, 1, 7), (128, 48, 8, 300), (136, 6, 6, 9), (256, 24, 4, 3), (256, 24, 4, 5000)):
+        asked = []
+        text = Text([(0, 5)], nk, D, 16)
+        real, ctx_lib = api._empty, ctx.lib
+        api._empty = lambda shape, *a, **kw: (asked.append(shape), real(shape, *a, **kw))[1]
+        try:
+            ctx.attention(text.cache, torch.zeros((rows, nq, D), dtype=torch.bfloat16, device="cuda"), text.table, text.lengths, text.begin)
+        finally:
+            api._empty = real
+        assert asked[-1] == (ctx_lib.q38b_attention_work_bytes(ctx.h, nq, nk, D, rows),)
+
+
 def test_wrapper_refusals(ctx):
     text = Text([(1, 20)], 2, 64, 16)
     x = torch.randn((1, 4, 64), device="cuda").bfloat16()
