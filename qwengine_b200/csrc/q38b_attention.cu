@@ -98,6 +98,9 @@ __device__ __forceinline__ int tile_seen(const AttnArgs& a, const Walk& w, int t
     return max(0, w.len - w.n_new + last + 1);
 }
 __device__ __forceinline__ int tile_units(int seen) { return max(1, (seen + KEYS - 1) / KEYS); }   // (a tile that sees nothing is one, too: its zeros are written)
+// A tile of rows costs what it sees and a start (queries, first scores, outputs: 5900 to 9900 clocks where a tile of keys takes 2200 to 3600): three tiles of keys more, which
+// lie in front of its first.  Without them 2048 tokens of a fresh text, whose first rows see little, were 103 us (one CTA with ten tiles of rows took 1.7 of the average's time).
+constexpr int START = 3;
 template <int ROWS>
 __device__ __forceinline__ void walk_tile(const AttnArgs& a, Walk& w) {
     w.row0 = w.tile * ROWS;
@@ -122,22 +125,23 @@ __device__ __forceinline__ bool walk_on(const AttnArgs& a, Walk& w) {
     w.from = 0;
     return true;
 }
-// on to the next tile of rows; `left`: units of the CTA's range that remain.  false: none
+// how far the CTA goes in the tile of rows where it is; `left`: units of its range that remain, starts included
+__device__ __forceinline__ void walk_to(Walk& w, int& left) {
+    if (w.from == 0) left -= START;
+    w.to = min(w.units, w.from + left);
+    left -= w.to - w.from;
+}
+// on to the next tile of rows.  false: none
 template <int ROWS>
 __device__ __forceinline__ bool walk_next(const AttnArgs& a, Walk& w, int& left) {
-    left -= w.to - w.from;
     if (left <= 0 || !walk_on<ROWS>(a, w)) return false;
-    w.to = min(w.units, left);
+    walk_to(w, left);
     return true;
 }
 
-#ifndef DEARV
-#define DEARV 8192
-#endif
-constexpr int DEAR = DEARV;
 // A part of a tile of rows that others finish costs about as much as a tile of keys for every 32 of its rows (its sums go out to memory and come back).  So a range that
 // would begin or end within that of a tile's ends begins or ends there instead (5 sequences of 77 to 333 new tokens, 15 + 5 heads of 96: 62 us cut exactly, MEASURED_RAGGED so).
-template <int DP> __device__ __forceinline__ int dear(const Walk& w) { return w.rows * DP / DEAR; }
+template <int DP> __device__ __forceinline__ int dear(const Walk& w) { return w.rows * DP / 8192; }
 template <int DP>
 __device__ __forceinline__ int moved_cut(const Walk& w, int in) {   // a cut `in` units behind the first of a tile's
     if (in > dear<DP>(w) && w.units - in > dear<DP>(w)) return in;
@@ -152,7 +156,7 @@ template <int ROWS>
 __device__ __forceinline__ int sequence_units(const AttnArgs& a, const Walk& w, int lane, int lanes) {
     int n = 0;
 #pragma unroll 1
-    for (int t = lane; t < w.n_tiles; t += lanes) n += tile_units(tile_seen<ROWS>(a, w, t));
+    for (int t = lane; t < w.n_tiles; t += lanes) n += START + tile_units(tile_seen<ROWS>(a, w, t));
     return n;
 }
 
@@ -232,12 +236,12 @@ __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p, int cta, i
 #pragma unroll 1
             for (w.tile = 0;; w.tile++) {
                 walk_tile<ROWS>(a, w);
-                if (in < w.units || w.tile + 1 == w.n_tiles) break;
-                in -= w.units;
+                if (in < START + w.units || w.tile + 1 == w.n_tiles) break;
+                in -= START + w.units;
             }
-            in = max(0, min(in, w.units - 1));   // (begins that do not ascend may pass what 32 bits count; whatever comes of them stays inside)
-            const int to = moved_cut<DP>(w, in);
-            p->cut[i] = cut - in + to;
+            in = max(0, min(in, START + w.units - 1));   // (begins that do not ascend may pass what 32 bits count; whatever comes of them stays inside)
+            const int to = moved_cut<DP>(w, max(0, in - START));
+            p->cut[i] = cut - in + (to ? START + to : 0);
             if (i == 0) {
                 w.from = to;
                 if (to == w.units && !walk_on<ROWS>(a, w)) w.from = 0;   // (the last tile's end: nothing to do)
@@ -386,7 +390,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     const uint32_t tmem = *tmem_slot;
     int left = any ? plan->cut[1] - plan->cut[0] : 0;
     Walk w = plan->walk;
-    w.to = min(w.units, w.from + left);
+    if (any) walk_to(w, left);
 
     if (any && (warp == 0 || warp == 2 || warp == 3)) {
         // ---------------- keys and values: a lane of one of three warps a box of at most 128 slots x 64 elements ----------------
