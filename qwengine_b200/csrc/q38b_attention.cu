@@ -140,7 +140,7 @@ __device__ __forceinline__ bool walk_next(const AttnArgs& a, Walk& w, int& left)
 }
 
 // A part of a tile of rows that others finish costs about as much as a tile of keys for every 32 of its rows (its sums go out to memory and come back).  So a range that
-// would begin or end within that of a tile's ends begins or ends there instead (5 sequences of 77 to 333 new tokens, 15 + 5 heads of 96: 62 us cut exactly, MEASURED_RAGGED so).
+// would begin or end within that of a tile's ends begins or ends there instead (5 sequences of 77 to 333 new tokens, 15 + 5 heads of 96: 56 us cut exactly, 39 so).
 template <int DP> __device__ __forceinline__ int dear(const Walk& w) { return w.rows * DP / 8192; }
 template <int DP>
 __device__ __forceinline__ int moved_cut(const Walk& w, int in) {   // a cut `in` units behind the first of a tile's
