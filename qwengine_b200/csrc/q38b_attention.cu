@@ -4,8 +4,8 @@
 //
 // One pass over the keys with the running maximum m and sum l of a softmax.  The (token, head) pairs that read one key head of one sequence are the rows
 // of a tile (128, or 256 in two), so that a group's heads and a chunk's tokens share what is read of the cache; 128 keys at a time:
-//   S = Q K^T       tcgen05.mma, both operands in shared memory, 128 fp32 columns of tensor memory; two such places in turn
-//   P = 2^(S c - m) by a warpgroup, a thread a row, rounded to the cache's type and written over S; c = scale log2(e).  Two warpgroups take turns: S has two places
+//   S = Q K^T       tcgen05.mma, both operands in shared memory, 128 fp32 columns of tensor memory
+//   P = 2^(S c - m) by a warpgroup, a thread a row, rounded to the cache's type and written over S; c = scale log2(e).  S has two places, for which two warpgroups take turns
 //   O += P V        tcgen05.mma with P from tensor memory and V as it lies (its keys are the rows of an MN-major operand)
 // The maximum that is taken off lags behind the true one by up to 2^8: O is rescaled in tensor memory only where a row's maximum has grown by
 // more, which after the first tiles of a text is rare.  fp16 weights carry a factor of 2^7 (they end at 2^15), so that what is 2^-31 of the largest
@@ -13,7 +13,13 @@
 //
 // The work is cut for all SMs whatever the batch is: tiles in the order (sequence, key head, rows), each of as many units as it sees tiles of keys, lie one behind the
 // other and every CTA takes an equal range of the units, worked out on the device from the lengths, begins and table as they are when the kernel runs.  A tile of rows that
-// two or more CTAs share leaves its sums in the work area, and a second kernel joins them, in the order of the keys.
+// two or more CTAs share leaves its sums in the work area, and a second kernel joins them, always in the same order.
+//
+// Three variants of one kernel.  Few rows: a CTA by itself; keys and values stream (32 sequences of 1600 to 32000 tokens, 24 + 4 heads of 256, a token each: 365 us = 6.6 TB/s).
+// Many rows: two tiles of 128 rows in a CTA (heads of at most 128 elements), whose keys and values then cross shared memory once; for heads of 193 to 256 a pair of CTAs that
+// multiply as one (cta_group::2), each with half of the keys of a tile and half of the values' columns: one CTA by itself moves 128 KB into shared memory for 128 keys and
+// the tensor core reads 192 KB of it, 2560 clocks at 128 bytes where the products need 2048 (measured 2700), the pair moves and reads half as much (4096 tokens behind 28672:
+// 2.61 -> 2.26 ms, 1370 TFLOP/s).
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -457,10 +463,8 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         } while (walk_next<ROWS>(a, w, left));
         w.to = w.from;   // no more
         publish(w);
-    } else if (any && warp == 1) {
-        if (PAIR && rank) {   // (the other CTA issues for both)
-        } else {
-        // ---------------- products ----------------
+    } else if (any && warp == 1 && rank == 0) {
+        // ---------------- products (of a pair: for both) ----------------
         constexpr uint32_t TYPE = std::is_same<C, __half>::value ? 0u : 1u;
         constexpr uint32_t idesc_s = (1u << 4) | (TYPE << 7) | (TYPE << 10) | ((uint32_t)(KEYS >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
         constexpr uint32_t idesc_o = (1u << 4) | (TYPE << 7) | (TYPE << 10) | (1u << 16) | ((uint32_t)((PAIR ? DP : CW) >> 3) << 17) | ((uint32_t)((PAIR ? 256 : 128) >> 4) << 24);
@@ -520,8 +524,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             ring0 += (uint32_t)(2 * tiles * NCH);
             item++;
         }
-        }
-    } else if (any) {
+    } else if (any && warp >= 4) {
         // ---------------- weights: warpgroup g takes the scores that lie in place g, a thread a row ----------------
         // QT = 2: those of its own 128 rows.  QT = 1: those of every other tile of keys; the maxima go from one warpgroup to the other, and each has a sum of its own.
         const int g = (warp >> 2) - 1, quad = warp & 3, qt = QT == 2 ? g : 0, t = PAIR ? rank : qt, row = 128 * t + 32 * quad + lane;   // row: of the tile of rows
@@ -584,9 +587,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     for (int u = (QT == 2 ? 0 : 32 * g) + lane; u - lane < pieces; u += STEP) {
                         const int r = u / UNITS, e = u % UNITS * 8;
                         const long long at = __shfl_sync(0xffffffffu, my_row, r & 31) + e;
-                        if (u < pieces && e < a.D)
+                        if (u >= pieces) continue;
+                        C* x = (C*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16);
 #pragma unroll 1
-                            for (int i = 0; i < 8; i++) *(C*)(to + e / 64 * BLOCK_BYTES + r * 128 + ((e % 64 / 8) ^ (r & 7)) * 16 + 2 * i) = from_f32<C>(query_one<C>(a, at + i));
+                        for (int i = 0; i < 8; i++) x[i] = from_f32<C>(e < a.D ? query_one<C>(a, at + i) : 0.0f);
                     }
                 }
             }

@@ -60,10 +60,10 @@ inline int paged_kv_check(const q38b_paged_kv* c) {
     return Q38B_OK;
 }
 
-// whether the attention counts such a batch's work in 32 bits: (row, head) pairs, and tiles of 128 of them times tiles of 128 keys
+// whether the attention counts such a batch's work in 32 bits: (row, head) pairs, and tiles of 128 of them times tiles of 128 keys (and three more for a start)
 inline bool attention_fits(const q38b_paged_kv* c, int n_heads, int rows) {
     return (long long)rows * n_heads <= 0x3FFFFFFF &&
-           ((long long)rows * n_heads / 128 + (long long)c->n_seqs * c->n_heads) * ((long long)c->table_n * c->page_size / 128 + 1) <= 0x7FFFFFFF;
+           ((long long)rows * n_heads / 128 + (long long)c->n_seqs * c->n_heads) * ((long long)c->table_n * c->page_size / 128 + 4) <= 0x7FFFFFFF;
 }
 
 inline q38b::Batch batch_of(const q38b_paged_kv* c, int rows) {

@@ -72,6 +72,13 @@ def test_attention(lib, change, status):
     assert lib.q38b_attention(CTX, *a.values(), None) == status
 
 
+def test_attention_of_more_work_than_is_counted(lib):
+    call = lambda cache, rows, nq=4: lib.q38b_attention(CTX, C.byref(cache), P, 2, 256, 64, nq, 0.125, P, 2, 64 * nq, 64, None, rows, P, 15, None)   # noqa: E731
+    assert call(paged(), (1 << 30) // 4) == UNSUPPORTED and call(paged(), (1 << 30) // 4 - 1) == NOMEM
+    wide = dict(table_n=1 << 20, table_ld=1 << 20, page_size=1024, n_pages=1 << 20, k_page=1 << 17, v_page=1 << 17)      # 2^30 tokens: 2^23 tiles of keys
+    assert call(paged(**wide), 64 * 32) == NOMEM and call(paged(**wide), 64 * 128) == UNSUPPORTED
+
+
 def test_quantize_i8(lib):
     q = lambda x=P, kind=0, ld=64, K=64, rows=3, c=P, cld=64, s=P: lib.q38b_quantize_i8(CTX, x, kind, ld, K, rows, c, cld, s, None)   # noqa: E731
     assert [q(x=None), q(kind=3), q(ld=63), q(K=0), q(K=131072, ld=1 << 20, cld=1 << 20), q(rows=0), q(rows=(1 << 30) + 1), q(c=None), q(s=None), q(cld=48)] == [ARG] * 10

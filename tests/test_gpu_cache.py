@@ -302,6 +302,20 @@ def test_strided_queries_and_outputs(ctx, tiles):
         assert bool((room[:, :, :off] == 2).all()) and bool((room[:, :, off + 128:] == 2).all())
 
 
+@pytest.mark.parametrize("D", [8, 40, 72, 136, 200])
+def test_queries_of_any_alignment_in_padded_heads(ctx, tiles, D):
+    """What lies behind a head's elements in shared memory (here: whatever a text of NaN left there) must not get into its scores."""
+    spoilt = Text([(64, 64)], 1, 256, 16)
+    spoilt.k.fill_(float("nan")), spoilt.v.fill_(float("nan"))
+    for src in ("bf16", "f32"):
+        ctx.attention(spoilt.cache, torch.full((64, 6, 256), float("nan"), device="cuda", dtype=torch.bfloat16), spoilt.table, spoilt.lengths, spoilt.begin)
+        text = Text([(1, 90), (20, 60)], 2, D, 16)
+        x = torch.randn((21, 8 * (D + 1) + 1), device="cuda").to(DTYPES[src])[:, 1:].unflatten(1, (8, D + 1))[:, :, :D]
+        got = ctx.attention(text.cache, x, text.table, text.lengths, text.begin)
+        ctx.check()
+        check(text, x, got, D ** -0.5)
+
+
 def test_far_pages(ctx):
     """Pages whose elements lie past 2^32 bytes from the first."""
     page_bytes = 5 << 30
