@@ -4,9 +4,9 @@ Shapes follow the reference model (docs/gguf_inventory.md:58-80 of the reference
 Engine::decode_batch, src/runtime/engine.cpp:1770-1849): 64 layers of hidden size 5120, three of every four a
 Gated-DeltaNet layer (in_proj 16384 x 5120, out 5120 x 6144), every fourth a gated-attention layer (q+gate
 12288 x 5120, k and v 1024 x 5120, o 5120 x 6144), each followed by the FFN (gate, up 17408 x 5120, SwiGLU, down
-5120 x 17408), then the 248320 x 5120 output head.  The recurrence / attention between the projections is not
-part of this path: the first 6144 outputs of the input projection stand in for its result, so that every matvec
-still consumes data produced by the step before it.  The FFN output of the last layer feeds the head; the other
+5120 x 17408), then the 248320 x 5120 output head.  The recurrence between the projections is not
+part of this path, the attention only where build is given a cache: the first 6144 outputs of the input projection stand in for their results,
+so that every matvec still consumes data produced by the step before it.  The FFN output of the last layer feeds the head; the other
 layers' FFN outputs end in a buffer of their own (see build).
 
 Sharding (one process per GPU): rank g of G owns rows [g*M/G, (g+1)*M/G) of every matrix and the fp32 output
