@@ -1078,6 +1078,7 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     if ((n_heads > 1 && out_head < c->D) || (rows > 1 && out_row < c->D)) return Q38B_ERR_ARG;
     // rows lie outside heads, or heads outside rows
     if (n_heads > 1 && rows > 1 && out_row < (n_heads - 1) * out_head + c->D && out_head < (rows - 1) * out_row + c->D) return Q38B_ERR_ARG;
+    if (q == out) return Q38B_ERR_ARG;   // (a row's queries may be read when another part of it is written)
     if (q_kind != Q38B_OUT_F32 && q_kind != c->kind) return Q38B_ERR_UNSUPPORTED;
     if (!attention_fits(c, n_heads, rows)) return Q38B_ERR_UNSUPPORTED;
     if ((uintptr_t)q % kind_size(q_kind) || (uintptr_t)out % kind_size(out_kind) || ((uintptr_t)lse & 3) || ((uintptr_t)work & 15)) return Q38B_ERR_ALIGN;

@@ -46,7 +46,7 @@ BAD_CACHES = [
 @pytest.mark.parametrize("change,status", BAD_CACHES)
 def test_caches(lib, change, status):
     assert lib.q38b_cache_append(CTX, C.byref(paged(**change)), P, P, 2, 128, 64, 128, 64, 5, None) == status
-    assert lib.q38b_attention(CTX, C.byref(paged(**change)), P, 2, 256, 64, 4, 0.125, P, 2, 256, 64, None, 5, P, 1 << 40, None) == status
+    assert lib.q38b_attention(CTX, C.byref(paged(**change)), P + 4096, 2, 256, 64, 4, 0.125, P, 2, 256, 64, None, 5, P, 1 << 40, None) == status
 
 
 @pytest.mark.parametrize("change,status", [
@@ -61,19 +61,19 @@ def test_append(lib, change, status):
 
 
 @pytest.mark.parametrize("change,status", [
-    (dict(q=None), ARG), (dict(out=None), ARG), (dict(cache=None), ARG), (dict(work=None), ARG), (dict(rows=0), ARG), (dict(n_heads=0), ARG), (dict(n_heads=3), ARG), (dict(q_kind=4), ARG),
+    (dict(q=None), ARG), (dict(out=None), ARG), (dict(q=P), ARG), (dict(cache=None), ARG), (dict(work=None), ARG), (dict(rows=0), ARG), (dict(n_heads=0), ARG), (dict(n_heads=3), ARG), (dict(q_kind=4), ARG),
     (dict(out_kind=-1), ARG), (dict(q_kind=1), UNSUPPORTED), (dict(scale=0.0), ARG), (dict(scale=-1.0), ARG), (dict(scale=float("nan")), ARG), (dict(scale=float("inf")), ARG),
     (dict(q_row=-1), ARG), (dict(q_head=-1), ARG), (dict(out_row=63), ARG), (dict(out_head=32), ARG), (dict(out_row=255), ARG), (dict(out_row=64), ARG), (dict(out_row=64, out_head=319), ARG), (dict(q=P + 1), ALIGN), (dict(out=P + 1), ALIGN), (dict(out_kind=0, out=P + 2), ALIGN),
     (dict(lse=P + 2), ALIGN), (dict(work=P + 8), ALIGN), (dict(work_bytes=15), NOMEM)])
 def test_attention(lib, change, status):
-    a = dict(cache=paged(), q=P, q_kind=2, q_row=256, q_head=64, n_heads=4, scale=0.125, out=P, out_kind=2, out_row=256, out_head=64, lse=None, rows=5, work=P, work_bytes=1 << 40)
+    a = dict(cache=paged(), q=P + 4096, q_kind=2, q_row=256, q_head=64, n_heads=4, scale=0.125, out=P, out_kind=2, out_row=256, out_head=64, lse=None, rows=5, work=P, work_bytes=1 << 40)
     a.update(change)
     a["cache"] = C.byref(a["cache"]) if a["cache"] else None
     assert lib.q38b_attention(CTX, *a.values(), None) == status
 
 
 def test_attention_of_more_work_than_is_counted(lib):
-    call = lambda cache, rows, nq=4: lib.q38b_attention(CTX, C.byref(cache), P, 2, 256, 64, nq, 0.125, P, 2, 64 * nq, 64, None, rows, P, 15, None)   # noqa: E731
+    call = lambda cache, rows, nq=4: lib.q38b_attention(CTX, C.byref(cache), P + 4096, 2, 256, 64, nq, 0.125, P, 2, 64 * nq, 64, None, rows, P, 15, None)   # noqa: E731
     assert call(paged(), (1 << 30) // 4) == UNSUPPORTED and call(paged(), (1 << 30) // 4 - 1) == NOMEM
     wide = dict(table_n=1 << 20, table_ld=1 << 20, page_size=1024, n_pages=1 << 20, k_page=1 << 17, v_page=1 << 17)      # 2^30 tokens: 2^23 tiles of keys
     assert call(paged(**wide), 64 * 32) == NOMEM and call(paged(**wide), 64 * 128) == UNSUPPORTED
