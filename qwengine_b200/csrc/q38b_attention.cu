@@ -41,7 +41,7 @@ namespace {
 
 constexpr int KEYS = 128;                // keys of a tile
 constexpr int BLOCK_BYTES = KEYS * 128;  // 64 elements of 128 rows, 128-byte swizzle
-constexpr int HEAD = 3072;               // shared memory in front of the queries: barriers, the plan, maxima and sums of rows (no more, or D = 256 has a stage less)
+constexpr int HEAD = 3 * 1024;               // shared memory in front of the queries: barriers, the plan, maxima and sums of rows (no more, or D = 256 has a stage less)
 constexpr float GROWTH = 8.0f;           // how far, in powers of two, a row's maximum may grow before O is rescaled
 
 // A tile of rows that several CTAs share, as the one that begins it leaves it for the joining kernel
