@@ -42,6 +42,7 @@ namespace {
 constexpr int KEYS = 128;                // keys of a tile
 constexpr int BLOCK_BYTES = KEYS * 128;  // 64 elements of 128 rows, 128-byte swizzle
 constexpr int HEAD = 3 * 1024;               // shared memory in front of the queries: barriers, the plan, maxima and sums of rows (no more, or D = 256 has a stage less)
+constexpr int FEW = 8;                  // rows of a sequence and key head up to which few_rows() is taken
 constexpr float GROWTH = 8.0f;           // how far, in powers of two, a row's maximum may grow before O is rescaled
 
 // A tile of rows that several CTAs share, as the one that begins it leaves it for the joining kernel
@@ -177,17 +178,21 @@ __device__ __forceinline__ int exact_cut(int each, int rest, int active, int c) 
 
 // All threads: the batch's units, this CTA's range of them, and the tile of rows it begins in.  false: nothing to do
 template <int DP, int ROWS, int THREADS>
-__device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p, int cta, int n_ctas) {
+__device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p, int cta, int n_ctas, bool& few) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int WARPS = THREADS / 32;
     // few sequences: a warp each, its lanes along the tiles; many: a thread each
     const bool wide = a.batch.n_seqs <= WARPS;
     const int per_round = wide ? WARPS : THREADS, rounds = (a.batch.n_seqs + per_round - 1) / per_round;
+    int most = 0;              // (token, head) rows of a sequence
     const auto units_of = [&](int s) {
         Walk w;
         w.s = s;
         w.n_tiles = 0;
-        if (s < a.batch.n_seqs) walk_sequence<ROWS>(a, w);
+        if (s < a.batch.n_seqs) {
+            walk_sequence<ROWS>(a, w);
+            most = max(most, w.n_new * a.group);
+        }
         int n = sequence_units<ROWS>(a, w, wide ? lane : 0, wide ? 32 : 1);
         if (wide) {
             n = __reduce_add_sync(0xffffffffu, n);
@@ -203,7 +208,7 @@ __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p, int cta, i
     }
     mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) p->sums[warp] = mine;
-    __syncthreads();
+    few = !__syncthreads_or(most > FEW);
     const int total = __reduce_add_sync(0xffffffffu, lane < WARPS ? p->sums[lane] : 0);
     const int active = min(n_ctas, total);
     if (cta >= active) return false;
@@ -314,6 +319,17 @@ template <typename C> __device__ __forceinline__ uint32_t no_number(uint32_t w) 
     constexpr uint32_t E = std::is_same<C, __half>::value ? 0x7C00u : 0x7F80u;
     return ((w & E) == E ? 0xFFFFu : 0u) | ((w >> 16 & E) == E ? 0xFFFF0000u : 0u);
 }
+template <typename C> __device__ __forceinline__ float bits_as(uint32_t bits) {
+    if constexpr (std::is_same<C, __half>::value) return __half2float(__ushort_as_half((uint16_t)bits));
+    else return __uint_as_float(bits << 16);
+}
+// 0 x + sum of either 16-bit number
+template <typename C> __device__ __forceinline__ uint32_t add_zero_times(uint32_t x, uint32_t sum) {
+    uint32_t r;
+    if constexpr (std::is_same<C, __half>::value) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(sum));
+    else asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(x), "r"(0u), "r"(sum));
+    return r;
+}
 template <typename T> __device__ __forceinline__ float load_as(const void* p, long long at) { return to_f32(((const T*)p)[at]); }
 
 template <typename C>
@@ -325,6 +341,315 @@ __device__ __forceinline__ void store_one(const AttnArgs& a, long long at, float
     if (a.out_kind == Q38B_OUT_F32) ((float*)a.out)[at] = f;
     else if (a.out_kind == Q38B_OUT_F16) ((__half*)a.out)[at] = __float2half_rn(f);
     else ((__nv_bfloat16*)a.out)[at] = __float2bfloat16_rn(f);
+}
+
+// Four elements of a head: f by, or nothing for a row that sees nothing
+__device__ __forceinline__ void store_four(const AttnArgs& a, long long head, int e, const float* f, float by, bool sees) {
+    if (e >= a.D) return;
+    const float x[4] = {sees ? f[0] * by : 0.0f, sees ? f[1] * by : 0.0f, sees ? f[2] * by : 0.0f, sees ? f[3] * by : 0.0f};
+    const long long to = head + e;
+    if (a.out_kind == Q38B_OUT_F32) {
+        if (a.out_vec) *(float4*)((float*)a.out + to) = make_float4(x[0], x[1], x[2], x[3]);
+        else
+#pragma unroll
+            for (int i = 0; i < 4; i++) ((float*)a.out)[to + i] = x[i];
+        return;
+    }
+    const uint32_t w0 = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(x[0], x[1]) : pack2<__nv_bfloat16>(x[0], x[1]);
+    const uint32_t w1 = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(x[2], x[3]) : pack2<__nv_bfloat16>(x[2], x[3]);
+    uint16_t* p = (uint16_t*)a.out + to;
+    if (a.out_vec) {
+        *(uint2*)p = make_uint2(w0, w1);
+    } else {
+        p[0] = (uint16_t)w0; p[1] = (uint16_t)(w0 >> 16); p[2] = (uint16_t)w1; p[3] = (uint16_t)(w1 >> 16);
+    }
+}
+
+// ---- few rows: at most 8 (token, head) rows of each key head, a decoding batch ----
+// The tensor core's 128 rows would be nearly empty, and what a tile of keys costs besides its bytes (scores to registers, weights back, three hand-overs) is more than these take to
+// come.  So eight warps work by themselves on warp-wide products with keys, and values' columns, as the 16 rows and the queries as the 8 columns (m16n8k16): warp kg takes
+// keys 16 kg .. 16 kg + 15 of every tile, with a maximum, a sum and outputs of its own in registers.  11 elements of the cache a clock and SM need 90 multiplications, these products have 975
+// (measured).  Nothing is waited for but the memory; at the end of a tile of rows the eight warps' sums meet in shared memory while the ring fills.
+template <typename C>
+__device__ __forceinline__ void mma_16x8x16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<C, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void load_matrices(uint32_t* r, uint32_t at) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+template <typename C, int DP>
+__device__ __forceinline__ void few_rows(const AttnArgs& a, Walk& w, int cta, uint8_t* q_at, uint8_t* ring, uint64_t* full, uint64_t* empty, uint64_t* meet, uint64_t* w_full,
+                                         const Walk* walks, float2* ml, volatile int* abort_flag) {
+    using Sh = Shape<DP, 1, false>;
+    constexpr int CW = Sh::CW, NCH = Sh::NCH, STAGES = Sh::STAGES, STAGE = Sh::STAGE;
+    constexpr int Q_BLOCK = FEW * 128, Q_PLACE = DP / 64 * Q_BLOCK;   // queries: two places, blocks of 8 rows x 64 elements
+    constexpr int ROW = DP + 4;                                       // floats between a row's sums and the next's: those of 8 columns and 4 pairs of rows fall into different banks
+    constexpr int PASS = 6;                                           // rows whose sums meet at once
+    constexpr int MT = DP / 16, CT = CW / 16;                         // 16 columns each: of a head, of a stage
+    static_assert(FEW == 8 && 2 * Q_PLACE + 8 * PASS * ROW * 4 <= Sh::Q_BYTES, "shared memory");
+    const int kg = (int)(threadIdx.x >> 5) - 4, lane = threadIdx.x & 31, tid = threadIdx.x - 128, quad = lane >> 2, pair = lane & 3;
+    float* sums = (float*)(q_at + 2 * Q_PLACE);   // [8 warps][PASS rows][ROW]
+    const uint32_t ring_u = smem_u32(ring), full_u = smem_u32(full), empty_u = smem_u32(empty), meet_u = smem_u32(meet), read_u = meet_u + 8;
+    // a lane's part in loading four times 8 x 8: keys or rows lie 128 bytes apart, 16-byte pieces are swizzled by the row's last three bits
+    const int r8 = lane & 7, lo = lane >> 3 & 1, hi = lane >> 4;
+    const uint32_t k_row = (uint32_t)((16 * kg + lo * 8 + r8) * 128), v_row = (uint32_t)((16 * kg + hi * 8 + r8) * 128);
+    const auto piece = [&](int block_bytes, int e8) {   // of 8 elements, e8 of them in front
+        return (uint32_t)(e8 / 8 * block_bytes + ((e8 % 8) ^ r8) * 16);
+    };
+    const auto walk_of = [&](int i) {
+        mbar_wait_bounded(smem_u32(&w_full[i & 7]), (uint32_t)i >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+        return walks[i & 7];
+    };
+    const auto load_queries = [&](const Walk& v, int place) {   // a row a warp; rows that are not there come as zeros
+        const int e = lane * 8;
+        if (e >= DP) return;
+        C* to = (C*)(q_at + place * Q_PLACE + e / 64 * Q_BLOCK + kg * 128 + ((e % 64 / 8) ^ kg) * 16);
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (kg < v.rows && e < a.D) {
+            const int in = by_group(a, v.row0 + kg);
+            const long long at = (long long)(v.first + in) * a.q_row + (long long)(v.kv * a.group + v.row0 + kg - in * a.group) * a.q_head + e;
+            if (a.q_vec && a.q_shift == 1) {
+                x = *(const uint4*)((const uint16_t*)a.q + at);
+            } else if (a.q_vec) {
+                const float4 y = *(const float4*)((const float*)a.q + at), z = *(const float4*)((const float*)a.q + at + 4);
+                x = make_uint4(pack2<C>(y.x, y.y), pack2<C>(y.z, y.w), pack2<C>(z.x, z.y), pack2<C>(z.z, z.w));
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < 8; i++) to[i] = from_f32<C>(query_one<C>(a, at + i));
+                return;
+            }
+        }
+        *(uint4*)to = x;
+    };
+    // all warps have come by (a barrier whose wait ends by itself)
+    uint32_t met = 0;
+    const auto all_here = [&] {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(meet_u);
+        mbar_wait_bounded(meet_u, met & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+        met++;
+    };
+    w = walk_of(0);
+    load_queries(w, 0);
+    all_here();
+    uint32_t at = 0, wrote = 0;   // stages taken, uses of `sums`
+    for (int item = 0;; item++) {
+        int limit[2];   // keys that this lane's two rows, 2 pair and 2 pair + 1, see
+#pragma unroll
+        for (int r = 0; r < 2; r++) limit[r] = 2 * pair + r < w.rows ? max(0, w.len - w.n_new + by_group(a, w.row0 + 2 * pair + r) + 1) : w.seen;
+        const int least = least_seen(a, w);
+        uint32_t q[DP / 16][2];
+#pragma unroll
+        for (int k = 0; k < DP / 16; k += 2)
+            load_matrices<false>(q[k], smem_u32(q_at) + (uint32_t)((item & 1) * Q_PLACE) + (uint32_t)(r8 * 128) + piece(Q_BLOCK, 2 * k + (lane >> 3)));
+        float o[MT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};   // o: columns quad, quad + 8 of 16, this lane's rows; m: what is taken off, times c
+#pragma unroll
+        for (int n = 0; n < MT; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+#pragma unroll 1
+        for (int tile = w.from; tile < w.to; tile++) {
+            const int key0 = tile * KEYS + 16 * kg;
+            const bool there = key0 < w.seen, masked = key0 + 16 > least;
+            float s[2][4] = {};   // keys quad, quad + 8; in two sums
+#pragma unroll
+            for (int c = 0; c < NCH; c++, at++) {
+                const uint32_t st = at % STAGES;
+                mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                if (there) {
+#pragma unroll
+                    for (int x0 = 0; x0 < CT; x0 += 4) {   // four loads at once, then their products
+                        uint32_t k[4][4];
+#pragma unroll
+                        for (int x = 0; x < 4; x++) load_matrices<false>(k[x], ring_u + st * STAGE + k_row + piece(BLOCK_BYTES, 2 * (x0 + x) + hi));
+#pragma unroll
+                        for (int x = 0; x < 4; x++) mma_16x8x16<C>(s[x & 1], k[x], q[c * CT + x0 + x][0], q[c * CT + x0 + x][1]);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty_u + 8u * st);
+            }
+            uint32_t p[2] = {0, 0}, seen_by_any[2] = {0, 0}, seen_by_some[2] = {0, 0};   // (of values: bits of this lane's two keys, and of 8 further on)
+            if (masked)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const int key = key0 + 8 * i + 2 * pair;
+                    seen_by_any[i] = (key < w.seen ? 0xFFFFu : 0u) | (key + 1 < w.seen ? 0xFFFF0000u : 0u);
+                    seen_by_some[i] = (key >= least ? 0xFFFFu : 0u) | (key + 1 >= least ? 0xFFFF0000u : 0u);
+                }
+            if (there) {
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    s[0][x] += s[1][x];
+                    if (masked && key0 + quad + 8 * (x >> 1) >= limit[x & 1]) s[0][x] = -INFINITY;
+                }
+                float now[2];
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    float top = fmaxf(s[0][r], s[0][2 + r]);
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    top *= a.c;
+                    now[r] = m[r] == -INFINITY || top > m[r] + GROWTH ? top : m[r];
+                }
+                if (__any_sync(0xffffffffu, now[0] != m[0] || now[1] != m[1])) {
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const float by = now[r] == m[r] ? 1.0f : m[r] == -INFINITY ? 0.0f : exp2_fast(m[r] - now[r]);
+                        l[r] *= by;
+                        m[r] = now[r];
+#pragma unroll
+                        for (int n = 0; n < MT; n++) {
+                            o[n][r] *= by;
+                            o[n][2 + r] *= by;
+                        }
+                    }
+                }
+                float e[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    e[x] = exp2_fast(fmaf(s[0][x], a.c, (m[x & 1] == -INFINITY ? 0.0f : -m[x & 1]) + WEIGHT_BIAS<C>));
+                    l[x & 1] += e[x];
+                }
+                p[0] = transposed(pack2<C>(e[0], e[1]));   // row quad, keys 2 pair, 2 pair + 1 and 8 more
+                p[1] = transposed(pack2<C>(e[2], e[3]));
+            }
+#pragma unroll
+            for (int c = 0; c < NCH; c++, at++) {
+                const uint32_t st = at % STAGES;
+                mbar_wait_bounded(full_u + 8u * st, at / STAGES & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+                if (there) {
+#pragma unroll
+                    for (int x0 = 0; x0 < CT; x0 += 4) {
+                        const uint32_t v_u = ring_u + st * STAGE + v_row;
+                        uint32_t v[4][4];
+#pragma unroll
+                        for (int x = 0; x < 4; x++) load_matrices<true>(v[x], v_u + piece(BLOCK_BYTES, 2 * (x0 + x) + lo));
+                        if (masked) {
+                            // Values of keys that none of the rows sees may be anything; those that only some see, and that are no numbers, go to these rows one by one.
+                            uint32_t times0 = 0;   // a NaN for what is no number
+#pragma unroll
+                            for (int x = 0; x < 4; x++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    v[x][i] &= seen_by_any[i >> 1];
+                                    times0 = add_zero_times<C>(v[x][i] & seen_by_some[i >> 1], times0);
+                                }
+                            if (__any_sync(0xffffffffu, no_number<C>(times0) != 0)) {
+                                uint32_t odd[4][4];
+#pragma unroll
+                                for (int x = 0; x < 4; x++)
+#pragma unroll
+                                    for (int i = 0; i < 4; i++) {
+                                        odd[x][i] = v[x][i] & no_number<C>(v[x][i]) & seen_by_some[i >> 1];
+                                        v[x][i] ^= odd[x][i];
+                                    }
+#pragma unroll 1
+                                for (int j = 0; j < 16; j++) {
+                                    const int shift = j & 1 ? 16 : 0, in = (j & 7) / 2;
+                                    float weight[2];
+#pragma unroll
+                                    for (int y = 0; y < 2; y++)   // of row 2 pair + y
+                                        weight[y] = bits_as<C>(__shfl_sync(0xffffffffu, j < 8 ? p[0] : p[1], (2 * pair + y) * 4 + in) >> shift & 0xFFFFu);
+#pragma unroll
+                                    for (int x = 0; x < 4; x++)
+#pragma unroll
+                                        for (int y = 0; y < 2; y++) {   // column quad + 8 y
+                                            const uint32_t value = __shfl_sync(0xffffffffu, j < 8 ? odd[x][y] : odd[x][2 + y], (lane & ~3) + in) >> shift & 0xFFFFu;
+#pragma unroll
+                                            for (int r = 0; r < 2; r++)
+                                                if (value != 0 && key0 + j < limit[r]) o[c * CT + x0 + x][2 * y + r] = fmaf(weight[r], bits_as<C>(value), o[c * CT + x0 + x][2 * y + r]);
+                                        }
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < 4; x++) mma_16x8x16<C>(o[c * CT + x0 + x], v[x], p[0], p[1]);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty_u + 8u * st);
+            }
+        }
+        // the eight warps' sums meet; the next tile's queries come in between
+        const Walk next = walk_of(item + 1);
+        const bool more = next.to > next.from;
+        if (more) load_queries(next, (item + 1) & 1);
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
+        const bool whole = w.from == 0 && w.to == w.units;
+#pragma unroll 1
+        for (int row0 = 0; row0 < w.rows; row0 += PASS) {
+            if (wrote) mbar_wait_bounded(read_u, (wrote - 1) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
+            wrote++;
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int in = 2 * pair + r - row0;
+                if (in < 0 || in >= PASS) continue;
+                if (quad == 0) ml[8 * kg + in] = make_float2(m[r], l[r]);
+#pragma unroll
+                for (int n = 0; n < MT; n++) {
+                    float* to = sums + (PASS * kg + in) * ROW + 16 * n + quad;
+                    to[0] = o[n][r];
+                    to[8] = o[n][2 + r];
+                }
+            }
+            all_here();
+            const int rows = min(PASS, w.rows - row0);
+            for (int u = tid; u < rows * (DP / 4); u += 256) {
+                const int r = u / (DP / 4), e = u % (DP / 4) * 4, row = row0 + r;
+                float2 of[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) of[k] = ml[8 * k + r];
+                float top = of[0].x;
+#pragma unroll
+                for (int k = 1; k < 8; k++) top = fmaxf(top, of[k].x);
+                float sum = 0.0f, f[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float by = of[k].x == -INFINITY ? 0.0f : exp2_fast(of[k].x - top);
+                    const float4 x = *(const float4*)(sums + (PASS * k + r) * ROW + e);
+                    sum = fmaf(of[k].y, by, sum);
+                    f[0] = fmaf(x.x, by, f[0]);
+                    f[1] = fmaf(x.y, by, f[1]);
+                    f[2] = fmaf(x.z, by, f[2]);
+                    f[3] = fmaf(x.w, by, f[3]);
+                }
+                if (whole) {
+                    const int tok = by_group(a, w.row0 + row), head = w.kv * a.group + w.row0 + row - tok * a.group;
+                    const long long out_row = w.first + tok;
+                    const bool sees = w.len - w.n_new + tok + 1 > 0;
+                    if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (top + log2f(sum) - WEIGHT_BIAS<C>) : -INFINITY;
+                    store_four(a, out_row * a.out_row + (long long)head * a.out_head, e, f, sees ? 1.0f / sum : 0.0f, sees);
+                } else {
+                    float* to = a.slots + (long long)(2 * cta + (w.from == 0 ? 1 : 0)) * a.slot_rows * (DP + 4);
+                    *(float4*)(to + (long long)(e / 4 * a.slot_rows + row) * 4) = make_float4(f[0], f[1], f[2], f[3]);
+                    if (e == 0) *(float2*)(to + (long long)a.slot_rows * DP + 2 * row) = make_float2(top, sum);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(read_u);
+        }
+        if (!more) break;
+        w = next;
+    }
 }
 
 template <typename C, int DP, int QT, bool PAIR>
@@ -362,16 +687,12 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         spoilt[0] = spoilt[1] = -1;
-        for (int s = 0; s < STAGES; s++) {
-            mbar_init(smem_u32(&full[s]), 1);
-            mbar_init(smem_u32(&empty[s]), 1);
-        }
+        for (int s = 0; s < STAGES; s++) mbar_init(smem_u32(&full[s]), 1);
         for (int s = 0; s < 2; s++) {
             mbar_init(smem_u32(&s_full[s]), 1);
             mbar_init(smem_u32(&p_full[s]), PAIR ? 8 : 4);
             mbar_init(smem_u32(&o_done[s]), 1);
         }
-        for (int s = 0; s < 8; s++) mbar_init(smem_u32(&m_full[s]), 1);
         mbar_init(smem_u32(q_full), PAIR ? 16 : 8);
         for (int s = 0; s < 8; s++) {
             mbar_init(smem_u32(&w_full[s]), 1);
@@ -390,7 +711,16 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    const bool any = plan_work<DP, ROWS, Sh::THREADS>(a, plan, cta, PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x);   // (with barriers of the block)
+    bool few = false;
+    const bool any = plan_work<DP, ROWS, Sh::THREADS>(a, plan, cta, PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x, few);   // (with barriers of the block)
+    if (QT == 2 || PAIR) few = false;
+    if (threadIdx.x == 0) {   // how many give a stage back is known now
+        for (int s = 0; s < STAGES; s++) mbar_init(smem_u32(&empty[s]), few ? 8 : 1);
+        for (int s = 0; s < 8; s++) mbar_init(smem_u32(&m_full[s]), few ? 8 : 1);
+        mbar_fence_init();
+        fence_proxy_async();
+    }
+    __syncthreads();
     if constexpr (PAIR) cluster_sync_all();   // the other CTA's barriers are initialised
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;
@@ -409,6 +739,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         const uint32_t to[2] = {(uint32_t)(k_block * (PAIR ? BLOCK_BYTES / 2 : BLOCK_BYTES) + k_part * 128), (uint32_t)(v_block * BLOCK_BYTES + v_part * 128)};
         const uint32_t ring_u = smem_u32(ring), full_u = PAIR ? peer_smem(smem_u32(full), 0u) : smem_u32(full), empty_u = smem_u32(empty);
         const int slots = (1 << a.batch.page_shift) - 1;
+        const bool in_turn = QT == 2 || few;
         uint32_t at = 0;   // stages filled so far
         int item = 0;
         const auto publish = [&](const Walk& v) {
@@ -421,10 +752,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         do {
             publish(w);
             const int n = w.to - w.from;
-            // the steps in the order in which the tensor core takes them: keys K0 K1 V0 K2 V1 .. (QT = 1), K0 V0 K1 V1 .. (QT = 2); a step's page is looked up during the one before
+            // the steps in the order in which the tensor core takes them: keys K0 K1 V0 K2 V1 .. (QT = 1), K0 V0 K1 V1 .. (QT = 2, few rows); a step's page is looked up during the one before
             const auto tile_of = [&](int i, bool& values) {
-                values = QT == 2 ? i & 1 : i == 2 * n - 1 || (i > 0 && !(i & 1));
-                return QT == 2 ? i >> 1 : i == 2 * n - 1 ? n - 1 : values ? i / 2 - 1 : (i + 1) / 2;
+                values = in_turn ? i & 1 : i == 2 * n - 1 || (i > 0 && !(i & 1));
+                return in_turn ? i >> 1 : i == 2 * n - 1 ? n - 1 : values ? i / 2 - 1 : (i + 1) / 2;
             };
             const auto page_of = [&](int i) {   // of this lane's box; keys nobody sees come as zeros, from a page that is not there
                 bool values;
@@ -463,6 +794,9 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         } while (walk_next<ROWS>(a, w, left));
         w.to = w.from;   // no more
         publish(w);
+    } else if (few) {
+        if constexpr (QT == 1 && !PAIR)
+            if (any && warp >= 4) few_rows<C, DP>(a, w, cta, q_at, ring, full, empty, m_full, w_full, walks, (float2*)m_rows, abort_flag);
     } else if (any && warp == 1 && rank == 0) {
         // ---------------- products (of a pair: for both) ----------------
         constexpr uint32_t TYPE = std::is_same<C, __half>::value ? 0u : 1u;
@@ -983,33 +1317,20 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, f
         const bool sees = job.len - job.n_new + tok + 1 > 0;
         const float by = 1.0f / l;
         if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (m + log2f(l) - bias) : -INFINITY;
-        if (e >= a.D) continue;
-        const float f[4] = {sees ? o.x * by : 0.0f, sees ? o.y * by : 0.0f, sees ? o.z * by : 0.0f, sees ? o.w * by : 0.0f};
-        const long long to = out_row * a.out_row + (long long)head * a.out_head + e;
-        if (a.out_kind == Q38B_OUT_F32) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) ((float*)a.out)[to + i] = f[i];
-        } else {
-            const uint32_t w0 = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(f[0], f[1]) : pack2<__nv_bfloat16>(f[0], f[1]);
-            const uint32_t w1 = a.out_kind == Q38B_OUT_F16 ? pack2<__half>(f[2], f[3]) : pack2<__nv_bfloat16>(f[2], f[3]);
-            uint16_t* p = (uint16_t*)a.out + to;
-            if (a.out_vec) {
-                *(uint2*)p = make_uint2(w0, w1);
-            } else {
-                p[0] = (uint16_t)w0; p[1] = (uint16_t)(w0 >> 16); p[2] = (uint16_t)w1; p[3] = (uint16_t)(w1 >> 16);
-            }
-        }
+        const float f[4] = {o.x, o.y, o.z, o.w};
+        store_four(a, out_row * a.out_row + (long long)head * a.out_head, e, f, by, sees);
     }
 }
 
 bool encode_pages(CUtensorMap* map, const q38b_paged_kv* c, const void* base, long long page, long long slot, long long head, int box_rows) {
     const cuuint64_t dims[4] = {(cuuint64_t)c->D, (cuuint64_t)c->page_size, (cuuint64_t)c->n_heads, (cuuint64_t)c->n_pages};
-    // (the stride of one head or one page is never used: any that is allowed)
+    // (the stride of one head or one page is never used: any that is allowed.  Lines of 128 bytes: with 256, heads of 64 in [slot][head] pages fetched their neighbours', too: 64
+    // sequences of 4000 tokens, 32 + 8 heads, 142 -> 107 us; no difference for longer heads)
     const cuuint64_t strides[3] = {(cuuint64_t)slot * 2, (cuuint64_t)(c->n_heads > 1 ? head : slot) * 2, (cuuint64_t)(c->n_pages > 1 ? page : slot) * 2};
     const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
     EncodeTiledFn enc = encode_fn();
     return enc && enc(map, c->kind == Q38B_OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, box, estr,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int ctas(const q38b_ctx* ctx) { return std::min(ctx->sm_count, 256); }   // (the joining kernel counts their work with a thread each)
