@@ -15,7 +15,8 @@
 // other and every CTA takes an equal range of the units, worked out on the device from the lengths, begins and table as they are when the kernel runs.  A tile of rows that
 // two or more CTAs share leaves its sums in the work area, and a second kernel joins them, always in the same order.
 //
-// Three variants of one kernel.  Few rows: a CTA by itself; keys and values stream (32 sequences of 1600 to 32000 tokens, 24 + 4 heads of 256, a token each: 365 us = 6.6 TB/s).
+// Three variants of one kernel.  Few rows: a CTA by itself; keys and values stream (32 sequences of 1600 to 32000 tokens, 24 + 4 heads of 256, a token each: 365 us = 6.6 TB/s).  Where
+// no sequence has more than 8 rows a key head (the kernel finds out when it runs), the products are the warps' own: few_rows() below.
 // Many rows: two tiles of 128 rows in a CTA (heads of at most 128 elements), whose keys and values then cross shared memory once; for heads of 193 to 256 a pair of CTAs that
 // multiply as one (cta_group::2), each with half of the keys of a tile and half of the values' columns: one CTA by itself moves 128 KB into shared memory for 128 keys and
 // the tensor core reads 192 KB of it, 2560 clocks at 128 bytes where the products need 2048 (measured 2700), the pair moves and reads half as much (4096 tokens behind 28672:
@@ -369,7 +370,9 @@ __device__ __forceinline__ void store_four(const AttnArgs& a, long long head, in
 // The tensor core's 128 rows would be nearly empty, and what a tile of keys costs besides its bytes (scores to registers, weights back, three hand-overs) is more than these take to
 // come.  So eight warps work by themselves on warp-wide products with keys, and values' columns, as the 16 rows and the queries as the 8 columns (m16n8k16): warp kg takes
 // keys 16 kg .. 16 kg + 15 of every tile, with a maximum, a sum and outputs of its own in registers.  11 elements of the cache a clock and SM need 90 multiplications, these products have 975
-// (measured).  Nothing is waited for but the memory; at the end of a tile of rows the eight warps' sums meet in shared memory while the ring fills.
+// (measured).  Nothing is waited for but the memory; at the end of a tile of rows the eight warps' sums meet in shared memory while the ring fills.  A token each, this way and the other:
+// 64 sequences of 1000 tokens, 32 + 8 heads of 128 56 / 68 us, of 64 37 / 57; 256 of 500 98 / 140 and 69 / 117; one of 500 10.0 / 11.5 and 9.7 / 10.8; 24 + 4 heads of 256: 59 / 60, 104 / 108, 11.6 / 12.6.
+// For up to 16 rows (queries as the 16, keys as the 8, half of the columns a warp) heads of 128 gained less (59 / 68) and heads of 256 lost (86 / 60).
 template <typename C>
 __device__ __forceinline__ void mma_16x8x16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     if constexpr (std::is_same<C, __half>::value)
@@ -684,22 +687,18 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
     }
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 64) {
         *abort_flag = 0;
         spoilt[0] = spoilt[1] = -1;
-        for (int s = 0; s < STAGES; s++) mbar_init(smem_u32(&full[s]), 1);
-        for (int s = 0; s < 2; s++) {
-            mbar_init(smem_u32(&s_full[s]), 1);
-            mbar_init(smem_u32(&p_full[s]), PAIR ? 8 : 4);
-            mbar_init(smem_u32(&o_done[s]), 1);
+    }
+    {   // a barrier a thread
+        const int b = threadIdx.x;
+        const auto is = [&](const uint64_t* first, int n) { return b >= (int)(first - full) && b < (int)(first - full) + n; };
+        if (b < (int)(v_here + 8 - full)) {
+            mbar_init(smem_u32(&full[b]), is(p_full, 2) ? (PAIR ? 8 : 4) : is(q_full, 1) ? (PAIR ? 16 : 8) : 1);
+            mbar_fence_init();
+            fence_proxy_async();
         }
-        mbar_init(smem_u32(q_full), PAIR ? 16 : 8);
-        for (int s = 0; s < 8; s++) {
-            mbar_init(smem_u32(&w_full[s]), 1);
-            mbar_init(smem_u32(&v_here[s]), 1);
-        }
-        mbar_fence_init();
-        fence_proxy_async();
     }
     if (warp == 1) {
         if constexpr (PAIR) {
@@ -714,13 +713,14 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     bool few = false;
     const bool any = plan_work<DP, ROWS, Sh::THREADS>(a, plan, cta, PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x, few);   // (with barriers of the block)
     if (QT == 2 || PAIR) few = false;
-    if (threadIdx.x == 0) {   // how many give a stage back is known now
-        for (int s = 0; s < STAGES; s++) mbar_init(smem_u32(&empty[s]), few ? 8 : 1);
-        for (int s = 0; s < 8; s++) mbar_init(smem_u32(&m_full[s]), few ? 8 : 1);
-        mbar_fence_init();
-        fence_proxy_async();
+    if (few) {   // eight warps arrive there, and nothing but warps: no fences for the copies' and products' sake as above
+        if (threadIdx.x < 20) {
+            const uint32_t bar = smem_u32(threadIdx.x < 12 ? &empty[threadIdx.x] : &m_full[threadIdx.x - 12]);
+            asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+            mbar_init(bar, 8);
+        }
+        __syncthreads();
     }
-    __syncthreads();
     if constexpr (PAIR) cluster_sync_all();   // the other CTA's barriers are initialised
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *tmem_slot;

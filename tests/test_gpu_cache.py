@@ -419,3 +419,101 @@ def test_wrapper_refusals(ctx):
         with pytest.raises(api.Q38BError):
             bad()
     assert call(x=x[:0]).shape == (0, 4, 64) and append(k=k[:0], v=k[:0]) is None
+
+
+# ---- batches of at most 8 rows a key head, which warps work on by themselves ----
+@pytest.mark.parametrize("nq,nk", [(1, 1), (6, 3), (8, 1), (4, 2), (7, 7)])
+@pytest.mark.parametrize("D", [8, 64, 72, 128, 192, 256])
+@pytest.mark.parametrize("src,cache,dst", [("bf16", "bf16", "bf16"), ("f32", "f16", "f32"), ("f16", "f16", "bf16")])
+def test_few_rows(ctx, nq, nk, D, src, cache, dst):
+    """Sequences of 0 to 8 / group new tokens of none to 700, some that see nothing, cut into parts and not."""
+    most = 8 // (nq // nk)
+    run(ctx, [(1, 1), (most, 700), (0, 40), (most, most), (1, 128), (min(2, most), 0), (1, 129), (most, 16 + most), (1, 0)], nq=nq, nk=nk, D=D, dtype=cache, src=src, dst=dst)
+
+
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("page,layout", [(8, "page"), (64, "head"), (256, "both")])
+def test_few_rows_of_many_and_of_long_sequences(ctx, D, page, layout):
+    run(ctx, [(1, 1 + 7 * s % 400) for s in range(300)], nq=3, nk=1, D=D, page=page, layout=layout)
+    run(ctx, [(1, 9000), (2, 3), (1, 20011)], nq=8, nk=2, D=D, page=page, layout=layout)
+
+
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -float("inf")])
+def test_few_rows_what_a_row_does_not_see_has_no_influence(ctx, D, dtype, what):
+    plan, nq, nk = [(4, 150), (3, 10)], 4, 2
+    text, x, got = run(ctx, plan, nq=nq, nk=nk, D=D, dtype=dtype)
+    for first_spoilt in (147, 148, 149):
+        for which in ("k", "v"):
+            spoilt = Text(plan, nk, D, 16, dtype)
+            pages = spoilt.table[0].long().cpu()
+            for j in range(first_spoilt, 150):
+                (spoilt.k if which == "k" else spoilt.v)[pages[j // 16], j % 16, :, j % D] = what
+            again = ctx.attention(spoilt.cache, x, spoilt.table, spoilt.lengths, spoilt.begin)
+            ctx.check()
+            clean = first_spoilt - 146
+            assert torch.equal(again[:clean], got[:clean]) and torch.equal(again[4:], got[4:])
+            if which == "v":       # every row from there on has its weight times the infinity (or a NaN) in each spoilt column that it sees, and what it had in all others
+                for row in range(clean, 4):
+                    columns = [j % D for j in range(first_spoilt, 147 + row)]
+                    others = [c for c in range(D) if c not in columns]
+                    assert bool(torch.isnan(again[row][:, columns]).all() if math.isnan(what) else (again[row][:, columns] == what).all())
+                    assert torch.equal(again[row][:, others], got[row][:, others])
+
+
+@pytest.mark.parametrize("D", [8, 40, 72, 128, 256])
+def test_few_rows_of_any_stride_and_alignment(ctx, D):
+    text = Text([(1, 90), (2, 60), (1, 300)], 2, D, 16)
+    g = torch.Generator().manual_seed(3)
+    for src in ("bf16", "f32"):
+        for offset in (0, 1, 8):
+            room = torch.randn((4, 8, D + 11), generator=g).to(DTYPES[src]).cuda()
+            x = room[:, :, offset:offset + D]
+            back = torch.full((4, 8, D + 9), 7.0, device="cuda", dtype=DTYPES[src])
+            out = back[:, :, offset:offset + D] if offset < 9 else None
+            ctx.attention(text.cache, x, text.table, text.lengths, text.begin, out=out)
+            ctx.check()
+            check(text, x, out, D ** -0.5)
+            assert bool((back[:, :, :offset] == 7).all()) and bool((back[:, :, offset + D:] == 7).all())
+
+
+def test_few_rows_growing_scores(ctx):
+    """Maxima that grow from tile to tile and from warp to warp, by more and by less than what the running maximum may lag behind, up and down."""
+    for seed, step in enumerate((0.02, 0.3, -0.3)):
+        text = Text([(2, 900), (1, 400)], 2, 64, 16, seed=seed)
+        x = torch.randn((3, 8, 64), generator=torch.Generator().manual_seed(seed)).bfloat16().cuda()
+        for s, (_, total) in enumerate(text.plan):     # keys along the first query's direction, longer and longer
+            for kv in range(2):
+                d = x[2 * s, 4 * kv].float().cpu()
+                d = d / (d @ d)
+                grow = (torch.arange(total).float() * step if step > 0 else (torch.arange(total).float() - total) * step).unsqueeze(1) * d
+                text.keys[s][:, kv] = (text.keys[s][:, kv].float() * 0.1 + grow).bfloat16()
+            for i in range(-(-total // 16)):
+                part = slice(i * 16, min((i + 1) * 16, total))
+                text.k[text.table[s, i].long(), :part.stop - part.start] = text.keys[s][part].cuda()
+        got = ctx.attention(text.cache, x, text.table, text.lengths, text.begin, scale=1.0)
+        ctx.check()
+        check(text, x, got, 1.0)
+
+
+def test_a_captured_call_takes_few_rows_and_many(ctx):
+    """Which way a batch goes is found out when the kernel runs: twelve sequences of a token each, then one of twelve."""
+    text = Text([(1, 100 + s) for s in range(12)], 2, 128, 16)
+    x = torch.randn((12, 8, 128), generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    begin, lengths = text.begin.clone(), text.lengths.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ctx.attention(text.cache, x, text.table, lengths, begin)
+    graph.replay()
+    check(text, x, got, 128 ** -0.5)
+    begin[1:] = 12
+    graph.replay()
+    ctx.check()
+    one = Text.__new__(Text)
+    one.plan, one.keys, one.values, one.nk, one.D, one.dtype = [(12, 100)], text.keys[:1], text.values[:1], 2, 128, "bf16"
+    check(one, x, got, 128 ** -0.5)
+    begin.copy_(text.begin)
+    graph.replay()
+    ctx.check()
+    check(text, x, got, 128 ** -0.5)
