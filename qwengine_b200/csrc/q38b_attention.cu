@@ -1233,8 +1233,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     if constexpr (PAIR) cluster_sync_all();   // neither CTA leaves before both have given it back
 }
 
-// Joins the parts of tiles of rows.  A piece of work is 32 rows (the lanes: what a part left lies so) of two groups of four elements where there are many
-// parts, to each of which four warps go with every fourth part, of eight groups where there are few.  The blocks share out the pieces of all tiles that were cut.
+// Joins the parts of tiles of rows.  A piece of work is 32 rows (the lanes: what a part left lies so) of one group of four elements where there are 16 parts or more, to
+// which eight warps go with every eighth part, of two groups for four warps each from 8 parts on, of eight groups below.  The blocks share
+// out the pieces of all tiles that were cut.  (A token behind 30000, 32 + 1 heads of 128, 148 parts: four warps 19.4 us in all, eight 16.7; six or eight parts on their way at once
+// instead of four: larger tiles of rows 5 to 10 % slower.)
 template <int DP>
 __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, float bias) {
     __shared__ int upto[256], sums[8];
@@ -1243,7 +1245,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, f
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_jobs = a.ctas;
     if (a.pdl) pdl_wait_prior();
     // pieces of the jobs before and of each itself
-    const auto warps_a_group = [](int n_parts) { return n_parts >= 8 ? 4 : 1; };
+    const auto warps_a_group = [](int n_parts) { return n_parts >= 16 ? 8 : n_parts >= 8 ? 4 : 1; };
     int n = 0;
     if ((int)threadIdx.x < n_jobs) {
         const Job j = a.jobs[threadIdx.x];
@@ -1324,13 +1326,13 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, f
 
 bool encode_pages(CUtensorMap* map, const q38b_paged_kv* c, const void* base, long long page, long long slot, long long head, int box_rows) {
     const cuuint64_t dims[4] = {(cuuint64_t)c->D, (cuuint64_t)c->page_size, (cuuint64_t)c->n_heads, (cuuint64_t)c->n_pages};
-    // (the stride of one head or one page is never used: any that is allowed.  Lines of 128 bytes: with 256, heads of 64 in [slot][head] pages fetched their neighbours', too: 64
-    // sequences of 4000 tokens, 32 + 8 heads, 142 -> 107 us; no difference for longer heads)
+    // (the stride of one head or one page is never used: any that is allowed.  Heads of less than 256 bytes in [slot][head] pages: lines of 256
+    // would fetch their neighbours', too: 64 sequences of 4000 tokens, 32 + 8 heads of 64, 142 us, 107 with lines of 128; heads of 256 elements are 1 % faster with 256)
     const cuuint64_t strides[3] = {(cuuint64_t)slot * 2, (cuuint64_t)(c->n_heads > 1 ? head : slot) * 2, (cuuint64_t)(c->n_pages > 1 ? page : slot) * 2};
     const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, estr[4] = {1, 1, 1, 1};
     EncodeTiledFn enc = encode_fn();
     return enc && enc(map, c->kind == Q38B_OUT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, box, estr,
-                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, c->D < 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 int ctas(const q38b_ctx* ctx) { return std::min(ctx->sm_count, 256); }   // (the joining kernel counts their work with a thread each)
