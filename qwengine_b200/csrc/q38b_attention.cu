@@ -670,7 +670,8 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     uint64_t* q_full = m_full + 8;
     uint64_t* w_full = q_full + 1;   // [8] a tile of rows is known
     uint64_t* v_here = w_full + 8;   // [STAGES] PAIR: this CTA's values of a tile that some rows do not see all of
-    uint32_t* tmem_slot = (uint32_t*)(v_here + 8);
+    uint64_t* o_free = v_here + 8;   // QT = 1: the outputs of a tile of rows have been read, by both warpgroups
+    uint32_t* tmem_slot = (uint32_t*)(o_free + 1);
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     volatile int* spoilt = abort_flag + 1;   // [2]: the item that met values that are no numbers among keys that not all of its rows see
     Plan* plan = (Plan*)(smem + 464);
@@ -694,8 +695,8 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     {   // a barrier a thread
         const int b = threadIdx.x;
         const auto is = [&](const uint64_t* first, int n) { return b >= (int)(first - full) && b < (int)(first - full) + n; };
-        if (b < (int)(v_here + 8 - full)) {
-            mbar_init(smem_u32(&full[b]), is(p_full, 2) ? (PAIR ? 8 : 4) : is(q_full, 1) ? (PAIR ? 16 : 8) : 1);
+        if (b < (int)(o_free + 1 - full)) {
+            mbar_init(smem_u32(&full[b]), is(p_full, 2) ? (PAIR ? 8 : 4) : is(q_full, 1) || is(o_free, 1) ? (PAIR ? 16 : 8) : 1);
             mbar_fence_init();
             fence_proxy_async();
         }
@@ -837,6 +838,9 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
                     mbar_wait_bounded(smem_u32(&p_full[i & 1]), p_phase >> (i & 1) & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
                     p_phase ^= 1u << (i & 1);
+                    // A tile's first product writes over the outputs of the tile before.  QT = 2: those whose weights have just come have read them.  QT = 1: the other warpgroup
+                    // stores the other half of them, and nothing else makes this one wait for it.
+                    if (QT == 1 && i == 0 && item > 0) mbar_wait_bounded(smem_u32(o_free), (item - 1) & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
 #pragma unroll
                     for (int c = 0; c < NCH; c++) {
                         const uint32_t at = ring0 + at_values<QT, NCH>(tile, tiles) + c, st = at % STAGES;
@@ -1053,6 +1057,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                     if (row < w.rows && col0 == 0) *(float2*)(to + (long long)a.slot_rows * DP + 2 * row) = make_float2(m, l);
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                if constexpr (QT == 1) {
+                    __syncwarp();
+                    if (lane == 0) arrive(PAIR ? peer_smem(smem_u32(o_free), 0u) : smem_u32(o_free));
+                }
             }
             if (!more) break;
             w = next;
