@@ -87,6 +87,11 @@ struct Shape {
 template <int QT, int NCH> __device__ __forceinline__ uint32_t at_keys(int j) { return (uint32_t)((QT == 2 || j == 0 ? 2 * j : 2 * j - 1) * NCH); }
 template <int QT, int NCH> __device__ __forceinline__ uint32_t at_values(int j, int n) { return (uint32_t)((QT == 2 || j == n - 1 ? 2 * j + 1 : 2 * j + 2) * NCH); }
 
+// Boxes of a stage, `wide` elements of keys or values a row in pages of which a box takes box_rows slots, and the warps that load them: warp w of three takes boxes w, w + 3 ..  One
+// that has none must not follow the ring: nothing waits for it, so it could miss a stage's phase and wait for one that does not come.
+__host__ __device__ constexpr int stage_boxes(int box_rows, int wide) { return KEYS / box_rows * (wide / 64); }
+__host__ __device__ constexpr int loading_warps(int boxes) { return boxes < 3 ? boxes : 3; }
+
 // The walk of a CTA through its range of units.
 struct Walk {
     int s, first, n_new, len, kv, tile, n_tiles;   // where it is
@@ -729,12 +734,13 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     Walk w = plan->walk;
     if (any) walk_to(w, left);
 
-    if (any && (warp == 0 || warp == 2 || warp == 3)) {
+    const int boxes = stage_boxes(a.box_rows, CW);
+    if (any && (warp == 0 || (warp >= 2 && warp <= loading_warps(boxes)))) {
         // ---------------- keys and values: a lane of one of three warps a box of at most 128 slots x 64 elements ----------------
         // (A warp issues its lanes' copies one by one, some 80 clocks each: the 64 of 128 keys and values in pages of 16 took it as long as the memory does.)
         // A box of keys: block `block[0]` of 64 elements, slots `in[0]` and on of the tile; of values: [1].
         const int loader = warp == 0 ? 0 : warp - 1, box = 3 * lane + loader, k_boxes = (PAIR ? KEYS / 2 : KEYS) / a.box_rows, v_boxes = KEYS / a.box_rows;
-        const bool mine = box < v_boxes * (CW / 64);   // lanes behind the last box do nothing
+        const bool mine = box < boxes;   // lanes behind the last box do nothing
         const int k_block = box / k_boxes, k_part = box % k_boxes * a.box_rows, v_block = box / v_boxes, v_part = box % v_boxes * a.box_rows;
         const int in[2] = {k_part + (PAIR ? rank * (KEYS / 2) : 0), v_part}, x0[2] = {k_block * 64, v_block * 64 + (PAIR ? rank * 128 : 0)};
         const uint32_t to[2] = {(uint32_t)(k_block * (PAIR ? BLOCK_BYTES / 2 : BLOCK_BYTES) + k_part * 128), (uint32_t)(v_block * BLOCK_BYTES + v_part * 128)};
@@ -1448,6 +1454,14 @@ int q38b_attention(q38b_ctx* ctx, const q38b_paged_kv* c, const void* q, int q_k
     CUtensorMap kmap, vmap;
     if (!encode_pages(&kmap, c, c->k, c->k_page, c->k_slot, c->k_head, a.box_rows) || !encode_pages(&vmap, c, c->v, c->v_page, c->v_slot, c->v_head, a.box_rows)) return Q38B_ERR_ARG;
     return c->kind == Q38B_OUT_F16 ? attention_for<__half>(ctx, a, two, kmap, vmap, (cudaStream_t)stream) : attention_for<__nv_bfloat16>(ctx, a, two, kmap, vmap, (cudaStream_t)stream);
+}
+
+// Test hook (not in the public header): boxes of a stage and the warps that load them.
+int q38b_debug_attention_loading(int D, int page_size, int pair, int* boxes, int* warps) {
+    if (D < 8 || D > 256 || page_size < 8 || !boxes || !warps || (pair && padded(D) != 256)) return Q38B_ERR_ARG;
+    *boxes = stage_boxes(std::min(page_size, pair ? KEYS / 2 : KEYS), padded(D) % 128 == 0 ? 128 : 64);
+    *warps = loading_warps(*boxes);
+    return Q38B_OK;
 }
 
 // Test hook (not in the public header): two tiles of rows together never (-1), wherever there is such a variant (1), by the rule (0).
