@@ -47,7 +47,7 @@ constexpr int FEW = 8;                  // rows of a sequence and key head up to
 constexpr float GROWTH = 8.0f;           // how far, in powers of two, a row's maximum may grow before O is rescaled
 
 // A tile of rows that several CTAs share, as the one that begins it leaves it for the joining kernel
-struct Job { int n_parts, first, n_new, len, kv, row0, rows, pad; };
+struct Job { int n_parts, first, past, kv, row0, rows, pad[2]; };
 
 struct AttnArgs {
     Batch batch;
@@ -94,21 +94,22 @@ __host__ __device__ constexpr int loading_warps(int boxes) { return boxes < 3 ? 
 
 // The walk of a CTA through its range of units.
 struct Walk {
-    int s, first, n_new, len, kv, tile, n_tiles;   // where it is
+    int s, first, n_new, past, kv, tile, n_tiles;   // where it is: sequence, its rows and the tokens in front of them (negative: rows in front of the text), ..
     int row0, rows, seen, units;                   // of the tile of rows: first of the sequence's (token, head) rows, how many, keys the last of them sees, tiles of keys
     int from, to;                                  // of those, this CTA's
 };
 template <int ROWS>
 __device__ __forceinline__ void walk_sequence(const AttnArgs& a, Walk& w) {
+    const int next = a.batch.first(w.s + 1);
     w.first = a.batch.first(w.s);
-    w.n_new = max(a.batch.first(w.s + 1) - w.first, 0);
-    w.len = a.batch.length(w.s);
+    w.n_new = max(min(next, a.batch.rows) - w.first, 0);
+    w.past = a.batch.length(w.s) - max(next - w.first, 0);   // (whether the call has all of the sequence's rows or not)
     w.n_tiles = (w.n_new * a.group + ROWS - 1) / ROWS;
 }
 template <int ROWS>
 __device__ __forceinline__ int tile_seen(const AttnArgs& a, const Walk& w, int tile) {
     const int last = by_group(a, min((tile + 1) * ROWS, w.n_new * a.group) - 1);   // token
-    return max(0, w.len - w.n_new + last + 1);
+    return max(0, w.past + last + 1);
 }
 __device__ __forceinline__ int tile_units(int seen) { return max(1, (seen + KEYS - 1) / KEYS); }   // (a tile that sees nothing is one, too: its zeros are written)
 // A tile of rows costs what it sees and a start (queries, first scores, outputs: 5900 to 9900 clocks where a tile of keys takes 2200 to 3600): three tiles of keys more, which
@@ -162,7 +163,7 @@ __device__ __forceinline__ int moved_cut(const Walk& w, int in) {   // a cut `in
 }
 
 // keys that all of a tile's rows see
-__device__ __forceinline__ int least_seen(const AttnArgs& a, const Walk& w) { return max(0, w.len - w.n_new + by_group(a, w.row0) + 1); }
+__device__ __forceinline__ int least_seen(const AttnArgs& a, const Walk& w) { return max(0, w.past + by_group(a, w.row0) + 1); }
 
 // Units of one key head of a sequence, by one thread or by the lanes of a warp together
 template <int ROWS>
@@ -461,7 +462,7 @@ __device__ __forceinline__ void few_rows(const AttnArgs& a, Walk& w, int cta, ui
     for (int item = 0;; item++) {
         int limit[2];   // keys that this lane's two rows, 2 pair and 2 pair + 1, see
 #pragma unroll
-        for (int r = 0; r < 2; r++) limit[r] = 2 * pair + r < w.rows ? max(0, w.len - w.n_new + by_group(a, w.row0 + 2 * pair + r) + 1) : w.seen;
+        for (int r = 0; r < 2; r++) limit[r] = 2 * pair + r < w.rows ? max(0, w.past + by_group(a, w.row0 + 2 * pair + r) + 1) : w.seen;
         const int least = least_seen(a, w);
         uint32_t q[DP / 16][2];
 #pragma unroll
@@ -643,7 +644,7 @@ __device__ __forceinline__ void few_rows(const AttnArgs& a, Walk& w, int cta, ui
                 if (whole) {
                     const int tok = by_group(a, w.row0 + row), head = w.kv * a.group + w.row0 + row - tok * a.group;
                     const long long out_row = w.first + tok;
-                    const bool sees = w.len - w.n_new + tok + 1 > 0;
+                    const bool sees = w.past + tok + 1 > 0;
                     if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (top + log2f(sum) - WEIGHT_BIAS<C>) : -INFINITY;
                     store_four(a, out_row * a.out_row + (long long)head * a.out_head, e, f, sees ? 1.0f / sum : 0.0f, sees);
                 } else {
@@ -1073,8 +1074,8 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             tiles = w.to - w.from;
             n = QT * tiles;
             tok = by_group(a, w.row0 + row);
-            limit = row < w.rows ? max(0, w.len - w.n_new + tok + 1) : w.seen;                          // keys this row sees
-            const int least = max(0, w.len - w.n_new + by_group(a, w.row0 + min(128 * t + 32 * quad, w.rows - 1)) + 1);   // ... the warp's first row
+            limit = row < w.rows ? max(0, w.past + tok + 1) : w.seen;                          // keys this row sees
+            const int least = max(0, w.past + by_group(a, w.row0 + min(128 * t + 32 * quad, w.rows - 1)) + 1);   // ... the warp's first row
             least_item = least_seen(a, w);                                                                    // ... the item's first row
             idle = 128 * t + 32 * quad >= w.rows;   // no row of this warp's is there
             m = -INFINITY;
@@ -1225,8 +1226,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 while (c > cta && exact_cut(each, rest, plan->active, c) > last) c--;
                 job.n_parts = c - cta + 1;
                 job.first = w.first;
-                job.n_new = w.n_new;
-                job.len = w.len;
+                job.past = w.past;
                 job.kv = w.kv;
                 job.row0 = w.row0;
                 job.rows = w.rows;
@@ -1330,7 +1330,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, f
         if (part != 0 || !here) continue;
         const int tok = by_group(a, job.row0 + row), head = job.kv * a.group + job.row0 + row - tok * a.group, e = 4 * col;
         const long long out_row = job.first + tok;
-        const bool sees = job.len - job.n_new + tok + 1 > 0;
+        const bool sees = job.past + tok + 1 > 0;
         const float by = 1.0f / l;
         if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (m + log2f(l) - bias) : -INFINITY;
         const float f[4] = {o.x, o.y, o.z, o.w};

@@ -7,14 +7,15 @@
 
 namespace q38b {
 
-// The batch of a q38b_paged_kv with its lists clamped to what there is, so that no entry reaches outside the tensors.
+// The batch of a q38b_paged_kv; lengths and pages are clamped to what there is, and whoever goes through a sequence's rows to the rows there are.
 struct Batch {
     const int *table, *lengths, *begin;
     long long table_ld;
     int table_n, n_seqs, n_pages, page_shift, rows;
 
-    // first of sequence s's rows (s <= n_seqs); entries that do not ascend, or pass the rows there are, give empty sequences, never rows outside
-    __device__ __forceinline__ int first(int s) const { return min(max(begin[s], 0), rows); }
+    // first of sequence s's rows (s <= n_seqs), which may lie behind the rows there are: a call for fewer rows than the lists say takes the first of them, and each has the token
+    // that it would have with all
+    __device__ __forceinline__ int first(int s) const { return max(begin[s], 0); }
     __device__ __forceinline__ int length(int s) const {   // (whole pages of at most 2^31 - 1 slots)
         return (int)min((long long)max(lengths[s], 0), (long long)table_n << page_shift);
     }
