@@ -328,7 +328,8 @@ int q38b_cache_append(q38b_ctx* ctx, const q38b_paged_kv* cache, const void* k_d
  *   out = sum_j softmax_j(scale q . k_j) v_j    over the sequence's tokens j <= lengths[s] - new + i
  * q: q_kind, element e of head h of a row at row * q_row + h * q_head + e; out likewise in out_kind, rows outside heads or heads outside rows.  n_heads: a multiple of the cache's.  scale > 0,
  * finite; rows * n_heads below 2^30, and (rows * n_heads / 128 + n_seqs * cache->n_heads) * (table_n * page_size / 128 + 4) below 2^31.  fp32 queries are rounded to the cache's type; products and sums in fp32, weights rounded to the cache's type before they multiply values
- * (2^-8 of each at most in bf16, 2^-11 in fp16), outputs rounded once.  A row that sees no token gives zeros.  A key or value that a row does not
+ * (2^-8 of each at most in bf16, 2^-11 in fp16), outputs rounded once.  The values' sum is divided last, so the largest magnitude of a value times the tokens seen must
+ * stay below 2^127 (fp16: always).  A row that sees no token gives zeros.  A key or value that a row does not
  * see has no influence on it, whatever it holds.  lse_dev (or NULL): fp32 [rows][n_heads], the natural logarithm of sum_j exp(scale q . k_j),
  * -infinity where no token is seen.  rows: those of q and out (1 and more).  work: q38b_attention_work_bytes bytes, 16-byte aligned, the caller's, not
  * shared with a call that may run at the same time.  out must not overlap q or the cache.  The order of the sums depends on the batch and the

@@ -9,7 +9,7 @@
 //   O += P V        tcgen05.mma with P from tensor memory and V as it lies (its keys are the rows of an MN-major operand)
 // The maximum that is taken off lags behind the true one by up to 2^8: O is rescaled in tensor memory only where a row's maximum has grown by
 // more, which after the first tiles of a text is rare.  fp16 weights carry a factor of 2^7 (they end at 2^15), so that what is 2^-31 of the largest
-// still counts.
+// still counts; bf16 weights one of 2^-8 (they end at 1).
 //
 // The work is cut for all SMs whatever the batch is: tiles in the order (sequence, key head, rows), each of as many units as it sees tiles of keys, lie one behind the
 // other and every CTA takes an equal range of the units, worked out on the device from the lengths, begins and table as they are when the kernel runs.  A tile of rows that
@@ -320,7 +320,8 @@ template <typename C> __device__ __forceinline__ uint32_t pack2(float lo, float 
     else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-template <typename C> constexpr float WEIGHT_BIAS = std::is_same<C, __half>::value ? 7.0f : 0.0f;
+// fp16: weights up to 2^15.  bf16: up to 1, so that values as large as the type's, which a weight of 2^8 would take past fp32 before the division by l, stay inside.
+template <typename C> constexpr float WEIGHT_BIAS = std::is_same<C, __half>::value ? 7.0f : -GROWTH;
 // whether either 16-bit number of a word is an infinity or a NaN
 template <typename C> __device__ __forceinline__ uint32_t no_number(uint32_t w) {
     constexpr uint32_t E = std::is_same<C, __half>::value ? 0x7C00u : 0x7F80u;
@@ -645,7 +646,7 @@ __device__ __forceinline__ void few_rows(const AttnArgs& a, Walk& w, int cta, ui
                     const int tok = by_group(a, w.row0 + row), head = w.kv * a.group + w.row0 + row - tok * a.group;
                     const long long out_row = w.first + tok;
                     const bool sees = w.past + tok + 1 > 0;
-                    if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (top + log2f(sum) - WEIGHT_BIAS<C>) : -INFINITY;
+                    if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (top + (log2f(sum) - WEIGHT_BIAS<C>)) : -INFINITY;
                     store_four(a, out_row * a.out_row + (long long)head * a.out_head, e, f, sees ? 1.0f / sum : 0.0f, sees);
                 } else {
                     float* to = a.slots + (long long)(2 * cta + (w.from == 0 ? 1 : 0)) * a.slot_rows * (DP + 4);
@@ -1045,7 +1046,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                             if (row < w.rows) store_one(a, out_at + k, limit > 0 ? __uint_as_float(o) * by : 0.0f);
                         }
                     }
-                    if (a.lse && row < w.rows && col0 == 0) a.lse[out_row * a.n_heads + head] = limit > 0 ? 0.6931471805599453f * (m + log2f(l) - WEIGHT_BIAS<C>) : -INFINITY;
+                    if (a.lse && row < w.rows && col0 == 0) a.lse[out_row * a.n_heads + head] = limit > 0 ? 0.6931471805599453f * (m + (log2f(l) - WEIGHT_BIAS<C>)) : -INFINITY;
                 } else {
                     // a place in the work area: [4 columns][row] and each row's m and l behind
                     float* to = a.slots + (long long)(2 * cta + (w.from == 0 ? 1 : 0)) * a.slot_rows * (DP + 4);
@@ -1332,7 +1333,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, f
         const long long out_row = job.first + tok;
         const bool sees = job.past + tok + 1 > 0;
         const float by = 1.0f / l;
-        if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (m + log2f(l) - bias) : -INFINITY;
+        if (a.lse && e == 0) a.lse[out_row * a.n_heads + head] = sees ? 0.6931471805599453f * (m + (log2f(l) - bias)) : -INFINITY;
         const float f[4] = {o.x, o.y, o.z, o.w};
         store_four(a, out_row * a.out_row + (long long)head * a.out_head, e, f, by, sees);
     }
