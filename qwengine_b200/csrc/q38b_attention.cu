@@ -1210,7 +1210,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 named_bar_sync(1 + quad, 64);   // (the other warp of these rows; all scores of the item are there)
                 const float m2 = m_rows[(g ^ 1) * 128 + 32 * quad + lane], l2 = l_rows[(g ^ 1) * 128 + 32 * quad + lane], top = fmaxf(m, m2);
                 named_bar_sync(1 + quad, 64);   // (both have read)
-                l = (m == -INFINITY ? 0.0f : l * exp2_fast(m - top)) + (m2 == -INFINITY ? 0.0f : l2 * exp2_fast(m2 - top));
+                l = l * (m == -INFINITY ? 0.0f : exp2_fast(m - top)) + l2 * (m2 == -INFINITY ? 0.0f : exp2_fast(m2 - top));   // (times zero: a sum that is no number stays none)
                 m = top;
             }
             next = walk_of(item + 2);
