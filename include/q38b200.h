@@ -302,7 +302,7 @@ int q38b_gemm_mx4_x(q38b_ctx* ctx, const void* W_codes, long long W_ld, const vo
  * The batch: n_seqs (1..65535) sequences.  Token j of sequence s lies in slot j % page_size of page table[s * table_ld + j / page_size] (table_ld >=
  * table_n, the entries of a sequence that may be read); lengths[s]: its tokens in the cache, the chunk's new ones included; begin[s] .. begin[s + 1] - 1:
  * the chunk's rows that are its new tokens, which are its last ones (int32, n_seqs + 1 of them, ascending from 0 or more).  table, lengths and begin
- * are device arrays, read when the kernels run.  Lengths past table_n * page_size count as that many; an entry that is no page's number reads as
+ * are device arrays, read when the kernels run.  The attention counts lengths past table_n * page_size as that many; an entry that is no page's number reads as
  * zeros and is not written to; rows from begin[n_seqs] on are nobody's and left as they are.  A call for fewer rows than begin[n_seqs] does those, each for the token that
  * it is in a call for all. */
 typedef struct q38b_paged_kv {

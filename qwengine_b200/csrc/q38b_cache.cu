@@ -52,9 +52,9 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
         if (lane + 32 * n < units) load(lane + 32 * n, v[n]);
     const int s = sequence_of_row(a.batch, row), first = a.batch.first(s), next = a.batch.first(s + 1);
     if (row < first || row >= next) return;   // (nobody's row)
-    const int len = a.batch.length(s);
-    const long long j = (long long)len - (next - first) + (row - first);
-    if (j < 0) return;
+    // (of the length as it is: with one past the table, counted as the table's, the chunk would go over tokens that are there)
+    const long long j = (long long)max(a.batch.lengths[s], 0) - (next - first) + (row - first);
+    if (j < 0 || j >= (long long)a.batch.table_n << a.batch.page_shift) return;
     const int page = a.batch.page(s, (int)j);
     if (page >= a.batch.n_pages) return;
     C* dst = (C*)a.dst[what] + page * a.dst_page[what] + (j & ((1 << a.batch.page_shift) - 1)) * a.dst_slot[what];
