@@ -327,7 +327,7 @@ int q38b_cache_append(q38b_ctx* ctx, const q38b_paged_kv* cache, const void* k_d
 /* Attention of the chunk's rows over their sequences: for new token i of sequence s and query head h, which reads key head h / (n_heads / cache->n_heads),
  *   out = sum_j softmax_j(scale q . k_j) v_j    over the sequence's tokens j <= lengths[s] - new + i
  * q: q_kind, element e of head h of a row at row * q_row + h * q_head + e; out likewise in out_kind, rows outside heads or heads outside rows.  n_heads: a multiple of the cache's.  scale > 0,
- * finite; rows * n_heads below 2^30, and (rows * n_heads / 128 + n_seqs * cache->n_heads) * (table_n * page_size / 128 + 4) below 2^31.  fp32 queries are rounded to the cache's type; products and sums in fp32, weights rounded to the cache's type before they multiply values
+ * finite; table_n * page_size at most 2^31 - 128, rows * n_heads below 2^30, and (rows * n_heads / 128 + n_seqs * cache->n_heads) * (table_n * page_size / 128 + 4) below 2^31.  fp32 queries are rounded to the cache's type; products and sums in fp32, weights rounded to the cache's type before they multiply values
  * (2^-8 of each at most in bf16, 2^-11 in fp16), outputs rounded once.  The values' sum is divided last, so the largest magnitude of a value times the tokens seen must
  * stay below 2^127 (fp16: always).  A row that sees no token gives zeros.  A key or value that a row does not
  * see has no influence on it, whatever it holds.  lse_dev (or NULL): fp32 [rows][n_heads], the natural logarithm of sum_j exp(scale q . k_j),

@@ -61,9 +61,10 @@ inline int paged_kv_check(const q38b_paged_kv* c) {
     return Q38B_OK;
 }
 
-// whether the attention counts such a batch's work in 32 bits: (row, head) pairs, and tiles of 128 of them times tiles of 128 keys (and three more for a start)
+// whether the attention counts such a batch's work in 32 bits: the end of the last tile of 128 keys, (row, head) pairs, and tiles of 128 of them times tiles of keys (and three
+// more for a start)
 inline bool attention_fits(const q38b_paged_kv* c, int n_heads, int rows) {
-    return (long long)rows * n_heads <= 0x3FFFFFFF &&
+    return (long long)c->table_n * c->page_size <= 0x7FFFFFFF - 127 && (long long)rows * n_heads <= 0x3FFFFFFF &&
            ((long long)rows * n_heads / 128 + (long long)c->n_seqs * c->n_heads) * ((long long)c->table_n * c->page_size / 128 + 4) <= 0x7FFFFFFF;
 }
 
