@@ -178,6 +178,7 @@ struct Plan {             // in shared memory
     int sums[16];
     int total, cut[2];         // units of all; this CTA's first and the one behind its last
     int active;                // CTAs among which the units are divided
+    int found[2];              // whether a thread has placed the cut (begins that fall can make the units pass 32 bits: a cut then lies in several sequences, or in none)
     Walk walk;                 // the tile of rows it begins in
 };
 // where CTA c of `active` would begin if units were divided exactly: total c / active
@@ -223,7 +224,9 @@ __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p, int cta, i
     if (threadIdx.x == 0) {
         p->total = total;
         p->active = active;
-        if (end == total) p->cut[1] = total;
+        p->found[0] = p->found[1] = 0;
+        p->cut[0] = 0;
+        p->cut[1] = end == total ? total : 0;
     }
     int before = 0;            // units of the rounds before
 #pragma unroll 1
@@ -244,7 +247,7 @@ __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p, int cta, i
 #pragma unroll 1
         for (int i = 0; i < 2; i++) {
             const int cut = i ? end : begin;
-            if (!(units > 0 && cut >= at && cut < at + units)) continue;   // one thread of the block goes on, for each of the two
+            if (!(units > 0 && cut >= at && cut < at + units) || atomicExch(&p->found[i], 1)) continue;   // one thread of the block goes on, for each of the two
             Walk w;
             w.s = r * per_round + (wide ? warp : (int)threadIdx.x);
             walk_sequence<ROWS>(a, w);
@@ -257,7 +260,7 @@ __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p, int cta, i
                 if (in < START + w.units || w.tile + 1 == w.n_tiles) break;
                 in -= START + w.units;
             }
-            in = max(0, min(in, START + w.units - 1));   // (begins that do not ascend may pass what 32 bits count; whatever comes of them stays inside)
+            in = max(0, min(in, START + w.units - 1));   // (begins that fall: whatever comes of them stays inside)
             const int to = moved_cut<DP>(w, max(0, in - START));
             p->cut[i] = cut - in + (to ? START + to : 0);
             if (i == 0) {
@@ -268,7 +271,7 @@ __device__ __forceinline__ bool plan_work(const AttnArgs& a, Plan* p, int cta, i
         }
     }
     __syncthreads();
-    return p->cut[1] > p->cut[0];
+    return p->found[0] && p->cut[1] > p->cut[0];
 }
 
 __device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr) {
@@ -682,10 +685,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
     volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
     volatile int* spoilt = abort_flag + 1;   // [2]: the item that met values that are no numbers among keys that not all of its rows see
     Plan* plan = (Plan*)(smem + 464);
-    Walk* walks = (Walk*)(smem + 600);             // [8] the CTA's tiles of rows, as the first loading warp goes through them (it is at most half a ring ahead)
+    Walk* walks = (Walk*)(smem + 608);             // [8] the CTA's tiles of rows, as the first loading warp goes through them (it is at most half a ring ahead)
     float* m_rows = (float*)(smem + 1024);       // [2][128]
     float* l_rows = (float*)(smem + 2048);       // [2][128]
-    static_assert(sizeof(Plan) <= 136 && 600 + 8 * sizeof(Walk) <= 1024 && (!PAIR || STAGES <= 8), "shared memory");
+    static_assert(sizeof(Plan) <= 144 && 608 + 8 * sizeof(Walk) <= 1024 && (!PAIR || STAGES <= 8), "shared memory");
     uint8_t* q_at = smem + HEAD;
     uint8_t* ring = q_at + Sh::Q_BYTES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
