@@ -317,6 +317,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+// named_bar_sync that tells all of its threads whether each came with `yes`
+__device__ __forceinline__ bool named_bar_all(int id, int nthreads, bool yes) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.and.pred p, %2, %3, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "r"(yes ? 1u : 0u), "r"(id), "r"(nthreads) : "memory");
+    return r != 0;
+}
 template <typename C> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t r;
     if constexpr (std::is_same<C, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -426,9 +432,11 @@ __device__ __forceinline__ void few_rows(const AttnArgs& a, Walk& w, int cta, ui
     const auto piece = [&](int block_bytes, int e8) {   // of 8 elements, e8 of them in front
         return (uint32_t)(e8 / 8 * block_bytes + ((e8 % 8) ^ r8) * 16);
     };
-    const auto walk_of = [&](int i) {
-        mbar_wait_bounded(smem_u32(&w_full[i & 7]), (uint32_t)i >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
-        return walks[i & 7];
+    const auto walk_of = [&](int i) {   // (none where the wait was given up: the whole warp then ends)
+        const bool there = __all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&w_full[i & 7]), (uint32_t)i >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT));
+        Walk v = walks[i & 7];
+        if (!there) v.to = v.from;
+        return v;
     };
     const auto load_queries = [&](const Walk& v, int place) {   // a row a warp; rows that are not there come as zeros
         const int e = lane * 8;
@@ -459,7 +467,9 @@ __device__ __forceinline__ void few_rows(const AttnArgs& a, Walk& w, int cta, ui
         mbar_wait_bounded(meet_u, met & 1u, abort_flag, a.status, ST_TMEM_TIMEOUT);
         met++;
     };
-    w = walk_of(0);
+    const Walk start = walk_of(0);
+    if (start.to <= start.from) return;
+    w = start;
     load_queries(w, 0);
     all_here();
     uint32_t at = 0, wrote = 0;   // stages taken, uses of `sums`
@@ -761,7 +771,10 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             }
             item++;
         };
+        bool ended = false;   // a wait was given up: no tile of rows and no copy more, so that nobody finds a place of `walks` changed
         do {
+            ended = __any_sync(0xffffffffu, *abort_flag != 0);
+            if (ended) break;
             publish(w);
             const int n = w.to - w.from;
             // the steps in the order in which the tensor core takes them: keys K0 K1 V0 K2 V1 .. (QT = 1), K0 V0 K1 V1 .. (QT = 2, few rows); a step's page is looked up during the one before
@@ -776,7 +789,7 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             };
             int page = page_of(0);
 #pragma unroll 1
-            for (int i = 0; i < 2 * n; i++) {
+            for (int i = 0; i < 2 * n && !ended; i++) {
                 bool values;
                 const int j0 = (w.from + tile_of(i, values)) * KEYS, slot = (j0 + in[values]) & slots, next = page_of(i + 1);
                 const CUtensorMap* map = values ? &vmap : &kmap;
@@ -784,7 +797,8 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
 #pragma unroll 1
                 for (int c = 0; c < NCH; c++, at++) {
                     const uint32_t st = at % STAGES, use = at / STAGES;
-                    mbar_wait_bounded(empty_u + 8u * st, (use & 1u) ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT);
+                    ended = !__all_sync(0xffffffffu, mbar_wait_bounded(empty_u + 8u * st, (use & 1u) ^ 1u, abort_flag, a.status, ST_WAIT_EMPTY_TIMEOUT));
+                    if (ended) break;
                     if constexpr (PAIR) {
                         const uint32_t here = smem_u32(&v_here[st]);
                         if (threadIdx.x == 0) {
@@ -803,9 +817,9 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
                 }
                 page = next;
             }
-        } while (walk_next<ROWS>(a, w, left));
+        } while (!ended && walk_next<ROWS>(a, w, left));
         w.to = w.from;   // no more
-        publish(w);
+        if (!ended) publish(w);
     } else if (few) {
         if constexpr (QT == 1 && !PAIR)
             if (any && warp >= 4) few_rows<C, DP>(a, w, cta, q_at, ring, full, empty, m_full, w_full, walks, (float2*)m_rows, abort_flag);
@@ -818,9 +832,9 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         const uint32_t q_u = smem_u32(q_at), ring_u = smem_u32(ring), full_u = smem_u32(full), empty_u = smem_u32(empty);
         uint32_t ring0 = 0, p_phase = 0, item = 0;
         for (;;) {
-            mbar_wait_bounded(smem_u32(&w_full[item & 7]), item >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
+            const bool there = __all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&w_full[item & 7]), item >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT));
             const int tiles = walks[item & 7].to - walks[item & 7].from, n = QT * tiles;
-            if (tiles <= 0) break;
+            if (!there || tiles <= 0) break;
             mbar_wait_bounded(smem_u32(q_full), item & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
             const auto scores = [&](int i) {
                 const int tile = QT == 2 ? i >> 1 : i, t = QT == 2 ? i & 1 : 0;
@@ -949,17 +963,19 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
         };
         uint32_t ring0 = 0, s_use = 0, m_use = 0, looked = 0, done[2] = {0, 0};   // done: products P V from either place up to this item
         int item;   // the tile of rows in front of the one that is worked on
-        const auto walk_of = [&](int i) {
-            mbar_wait_bounded(smem_u32(&w_full[i & 7]), (uint32_t)i >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT);
-            return walks[i & 7];
+        const auto walk_there = [&](int i) {
+            return (bool)__all_sync(0xffffffffu, mbar_wait_bounded(smem_u32(&w_full[i & 7]), (uint32_t)i >> 3 & 1u, abort_flag, a.status, ST_WAIT_FULL_TIMEOUT));
         };
         // A round ends a tile of rows: the next one's queries go in place while its last products run, its outputs leave, the next one's scores become weights.
-        Walk next = walk_of(0);
+        // Where a wait was given up there may be none for one warp and still one for another: the two warps that meet at the end of a tile go on together, or neither does.
+        bool there = walk_there(0);
+        if (QT == 1) there = named_bar_all(1 + quad, 64, there);
+        Walk next = walks[0];
         float m = -INFINITY, l = 0.0f;   // m: what is taken off, times c
         int tiles = 0, n = 0, tok = 0, limit = 0, least_item = 0;
         bool idle = true;
         for (item = -1;; item++) {
-            const bool more = next.to > next.from;
+            const bool more = there && next.to > next.from;
             if (more) load_queries(next);
             if (item >= 0) {
                 {
@@ -1207,16 +1223,17 @@ attention_kernel(const AttnArgs a, const __grid_constant__ CUtensorMap kmap, con
             if constexpr (PAIR)   // the stages whose values were waited for here, by either warpgroup
                 for (int i = max(0, least_item / KEYS - w.from); i < tiles; i++) looked ^= 1u << ((ring0 + at_values<QT, NCH>(i, tiles)) % STAGES);
             ring0 += (uint32_t)(2 * tiles * NCH);
+            there = walk_there(item + 2);
             if (QT == 1) {   // both warpgroups' maxima and sums: the later of the maxima is the larger
                 m_rows[g * 128 + 32 * quad + lane] = m;
                 l_rows[g * 128 + 32 * quad + lane] = l;
                 named_bar_sync(1 + quad, 64);   // (the other warp of these rows; all scores of the item are there)
                 const float m2 = m_rows[(g ^ 1) * 128 + 32 * quad + lane], l2 = l_rows[(g ^ 1) * 128 + 32 * quad + lane], top = fmaxf(m, m2);
-                named_bar_sync(1 + quad, 64);   // (both have read)
+                there = named_bar_all(1 + quad, 64, there);   // (both have read)
                 l = l * (m == -INFINITY ? 0.0f : exp2_fast(m - top)) + l2 * (m2 == -INFINITY ? 0.0f : exp2_fast(m2 - top));   // (times zero: a sum that is no number stays none)
                 m = top;
             }
-            next = walk_of(item + 2);
+            next = walks[(item + 2) & 7];
         }
     }
     // The last tile of rows, if others go on with it, is this CTA's to announce: its parts are this CTA's and those of the CTAs up to the one with its last unit.
