@@ -15,12 +15,12 @@
 // other and every CTA takes an equal range of the units, worked out on the device from the lengths, begins and table as they are when the kernel runs.  A tile of rows that
 // two or more CTAs share leaves its sums in the work area, and a second kernel joins them, always in the same order.
 //
-// Three variants of one kernel.  Few rows: a CTA by itself; keys and values stream (32 sequences of 1600 to 32000 tokens, 24 + 4 heads of 256, a token each: 365 us = 6.6 TB/s).  Where
+// Three variants of one kernel.  Few rows: a CTA by itself; keys and values stream (32 sequences of 1600 to 32000 tokens, 24 + 4 heads of 256, a token each: 367 us = 6.5 TB/s).  Where
 // no sequence has more than 8 rows a key head (the kernel finds out when it runs), the products are the warps' own: few_rows() below.
 // Many rows: two tiles of 128 rows in a CTA (heads of at most 128 elements), whose keys and values then cross shared memory once; for heads of 193 to 256 a pair of CTAs that
 // multiply as one (cta_group::2), each with half of the keys of a tile and half of the values' columns: one CTA by itself moves 128 KB into shared memory for 128 keys and
 // the tensor core reads 192 KB of it, 2560 clocks at 128 bytes where the products need 2048 (measured 2700), the pair moves and reads half as much (4096 tokens behind 28672:
-// 2.61 -> 2.26 ms, 1370 TFLOP/s).
+// 2.61 -> 2.26 ms, 1370 TFLOP/s; in calls one behind the other, at the power limit, 2.70 ms, 1145).
 #include <cuda.h>
 #include <cuda_runtime.h>
 

@@ -98,7 +98,7 @@ template <typename T> __device__ __forceinline__ uint32_t raw8_top(const Raw8<T>
 
 // A row to a warp, or to a block, whose threads have up to four pieces of eight neighbours each; they stay in registers between the largest magnitude and the
 // codes, so that every value is read once.  What is longer than 20480 is read twice.  Bound by the issue of instructions (13 a value, 72 % of the issue slots) and memory: 17408 x
-// 5120 from bf16 53 us (5.0 TB/s), 110 with single elements read twice; 77 x 5120 from fp32 2.7 us.
+// 5120 from bf16 53 us (5.0 TB/s), 110 with single elements read twice; 77 x 5120 from fp32 2.3 us.
 constexpr int PIECES = 4;
 // VEC: whole pieces, aligned (the rest of a row's code, unused, took half of the instructions issued).  WARP: eight rows a block.
 template <typename T, bool VEC, bool WARP>
